@@ -79,6 +79,17 @@ void symm_rs(std::vector<int64_t> peer_ptrs, int64_t src_off, int64_t n, torch::
 void muon_pre(torch::Tensor g, torch::Tensor mb, torch::Tensor x, c10::optional<torch::Tensor> coef, torch::Tensor mom,
               torch::Tensor one_mom, torch::Tensor fro);
 void symm_ag_apply(std::vector<int64_t> upd_ptrs, torch::Tensor runs_i64);
+void kv_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tensor vc, torch::Tensor pos,
+                    c10::optional<torch::Tensor> count, c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs);
+std::vector<torch::Tensor> kv_cache_read(torch::Tensor kc, torch::Tensor vc, torch::Tensor lens, int64_t T,
+                                         c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs);
+void kv_cache_commit(torch::Tensor kc, torch::Tensor vc, torch::Tensor lens, torch::Tensor path, torch::Tensor count,
+                     c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs);
+torch::Tensor tree_attention(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torch::Tensor lens,
+                             c10::optional<torch::Tensor> parents, double scale, c10::optional<torch::Tensor> ks,
+                             c10::optional<torch::Tensor> vs, torch::Tensor err);
+std::vector<torch::Tensor> verify_tree(torch::Tensor tokens, torch::Tensor parents, torch::Tensor p, c10::optional<torch::Tensor> q,
+                                       torch::Tensor u);
 }  // namespace tfb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -107,6 +118,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_gemm", &tfb::decode_gemm);
   m.def("decode_gemm_trace_set", &tfb::decode_gemm_trace_set);
   m.def("kv_append", &tfb::kv_append);
+  m.def("kv_cache_write", &tfb::kv_cache_write, "rows into a KV cache at per-sequence positions (bf16, or e4m3 quantised)");
+  m.def("kv_cache_read", &tfb::kv_cache_read, "cached rows as bf16 [B, T, H, D] keys and values");
+  m.def("kv_cache_commit", &tfb::kv_cache_commit, "accepted rows of a drafted tree moved behind the context");
+  m.def("tree_attention", &tfb::tree_attention, "attention of a drafted tree over a KV cache");
+  m.def("verify_tree", &tfb::verify_tree, "drafted tokens verified against the target's probabilities");
   m.def("step_advance", &tfb::step_advance);
   m.def("argmax_rows", &tfb::argmax_rows);
   m.def("rope_norm_bwd", &tfb::rope_norm_bwd);

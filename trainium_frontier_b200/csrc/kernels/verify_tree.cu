@@ -1,0 +1,318 @@
+// Drafted tokens verified against the target's probabilities (speculative sampling over a tree).
+//
+// Node 0 is the tree's root (a token that is already part of the text); node n > 0 is a drafted
+// token, child of parents[n] < n.  Row n of p (q) holds the target's (the draft's) distribution
+// of the token after node n, and the children of a node were drawn from its row of q, each by
+// itself (q absent: a rule proposed them).  From the root on, the children of the last accepted
+// node cur are tried in order with the remainder r (at first p[cur], Z = 1):
+//     accept n      iff  u[n] q[cur][t] Z < r[t],  t = tokens[n]     (q absent: q[cur][t] = 1)
+//     reject n:     r <- max(r - Z q[cur], 0),  Z <- sum r           (q absent: r[t] <- 0)
+//                   (r / Z is the remainder's distribution; an empty one becomes p[cur], Z = 1)
+// When no child is left, the next token is the least j with r[0] + .. + r[j] > u[0] sum r.
+// The accepted tokens and that one are together distributed as if drawn from p one by one.
+//
+// Answers are whole numbers that a last bit can turn, so r, Z and every sum are in 64 bits
+// (fp32 products are then exact, and a sum's order moves it by 1e-16 only).
+//
+// What a sequence has to read whole is one row of p, and of q after a rejection: the tests
+// themselves read single entries, gathered for all nodes at once by one thread a node.  r is
+// not stored: each pass recomputes it from p, q and the Z's of the rejections so far.  A
+// cluster of CTAs shares a row, every warp a contiguous range of it, and all CTAs take the same
+// decisions from the same sums, read from each other's shared memory.  The last pass leaves the
+// warps' sums behind, so the draw re-reads only the range in which its token lies.
+// The reference has no decode path.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+
+#include "sm100_common.cuh"
+
+namespace tfb {
+
+constexpr int kVerThreads = 512;
+constexpr int kVerWarps = kVerThreads / 32;
+constexpr int kVerNodes = 64;
+constexpr int kVerCluster = 8;   // CTAs of a cluster at most
+
+struct VerArgs {
+  const int* tokens;
+  const int* parents;
+  const float* p;
+  const float* q;                // null: deterministic drafts
+  const float* u;
+  long long pb, pn, qb, qn;      // strides in elements
+  int* path;
+  int* count;
+  int* out;
+  int N, V, range;               // range: row entries a warp owns (a multiple of 128)
+};
+
+__device__ __forceinline__ double ld_dsmem_f64(uint32_t addr) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void load4(const float* row, int j, int end, float (&f)[4]) {
+  if constexpr (VEC) {
+    if (j + 4 <= end) {
+      const float4 v = *reinterpret_cast<const float4*>(row + j);
+      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = j + i < end ? row[j + i] : 0.f;
+}
+
+// VEC: rows start on 16-byte boundaries.
+template <bool VEC, bool HASQ>
+__global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(const VerArgs a) {
+  __shared__ int s_tok[kVerNodes], s_par[kVerNodes], s_path[kVerNodes];
+  __shared__ float s_u[kVerNodes], s_p[kVerNodes], s_q[kVerNodes];
+  __shared__ double s_z[kVerNodes];          // Z before each rejection at the current node
+  __shared__ int s_rej[kVerNodes];           // its rejected tokens (q absent)
+  __shared__ double s_sum[2][kVerWarps];     // the warps' sums of a pass, two passes in turn
+  __shared__ double s_all[kVerWarps * kVerCluster];
+  __shared__ double s_scan[kVerWarps];
+  __shared__ int s_pick, s_lastpos;
+
+  const int C = (int)nclusters_x() > 0 ? (int)(gridDim.x / nclusters_x()) : 1;
+  const int rank = (int)cluster_ctarank();
+  const int b = (int)(blockIdx.x / C);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int N = a.N, V = a.V;
+  const float* P = a.p + b * a.pb;
+  const float* Q = HASQ ? a.q + b * a.qb : nullptr;
+
+  if (tid < N) {
+    const int tok = a.tokens[(long long)b * N + tid], par = a.parents[(long long)b * N + tid];
+    const bool real = tid > 0 && tok >= 0 && tok < V && par >= 0 && par < tid;   // else no node's child
+    s_tok[tid] = tok;
+    s_par[tid] = real ? par : -1;
+    s_u[tid] = a.u[(long long)b * N + tid];
+    s_p[tid] = real ? P[par * a.pn + tok] : 0.f;
+    s_q[tid] = real && HASQ ? Q[par * a.qn + tok] : 1.f;
+  }
+  __syncthreads();
+
+  int cur = 0, cnt = 1, rej = 0, turn = 0;
+  double Z = 1.0;
+  bool summed = false;                       // s_all holds the sums of the present r
+  const long long w0 = (long long)(rank * kVerWarps + warp) * a.range;   // this warp's range
+  const int lo = (int)min((long long)V, w0), hi = (int)min((long long)V, w0 + a.range);
+
+  // r at one entry after the rejections so far
+  auto rest = [&](float pj, float qj, int j) -> double {
+    double r = (double)pj;
+    for (int k = 0; k < rej; ++k) {
+      if constexpr (HASQ) {
+        r = __dsub_rn(r, __dmul_rn(s_z[k], (double)qj));
+        r = r > 0.0 ? r : 0.0;
+      } else {
+        if (s_rej[k] == j) r = 0.0;
+      }
+    }
+    return r;
+  };
+  // sums of r over every warp's range, into s_all of every CTA; returns the total
+  auto pass = [&]() -> double {
+    const float* pr = P + cur * a.pn;
+    const float* qr = HASQ ? Q + cur * a.qn : nullptr;
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int j = lo + lane * 4; j < hi; j += 512) {
+      float f[4][4], g[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        load4<VEC>(pr, j + 128 * k, hi, f[k]);
+        if constexpr (HASQ) {
+          if (rej > 0) load4<VEC>(qr, j + 128 * k, hi, g[k]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] += rest(f[k][i], HASQ ? g[k][i] : 0.f, j + 128 * k + i);
+    }
+    double s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) s_sum[turn][warp] = s;
+    if (C > 1) cluster_sync(); else __syncthreads();
+    for (int i = tid; i < C * kVerWarps; i += kVerThreads)
+      s_all[i] = C > 1 ? ld_dsmem_f64(mapa_shared(smem_u32(&s_sum[turn][i % kVerWarps]), (uint32_t)(i / kVerWarps)))
+                       : s_sum[turn][i];
+    turn ^= 1;
+    __syncthreads();
+    double t = 0.0;
+    for (int i = 0; i < C * kVerWarps; ++i) t += s_all[i];
+    summed = true;
+    return t;
+  };
+
+  if (tid == 0) s_path[0] = 0;
+  for (int n = 1; n < N; ++n) {
+    if (s_par[n] != cur) continue;
+    const double qn = (double)s_q[n];
+    const double r = rest(s_p[n], s_q[n], s_tok[n]);
+    if (__dmul_rn(__dmul_rn((double)s_u[n], qn), Z) < r) {
+      __syncthreads();                       // s_path, and s_z / s_rej of the node left behind
+      cur = n;
+      if (tid == 0) s_path[cnt] = n;
+      ++cnt;
+      rej = 0;
+      Z = 1.0;
+      summed = false;
+    } else {
+      __syncthreads();
+      if (tid == 0) {
+        s_z[rej] = Z;
+        s_rej[rej] = s_tok[n];
+      }
+      ++rej;
+      __syncthreads();
+      Z = pass();
+      if (!(Z > 0.0)) {                      // nothing is left (p = q up to rounding): p itself
+        rej = 0;
+        Z = 1.0;
+        summed = false;
+      }
+    }
+  }
+  if (!summed) Z = pass();
+
+  // the draw: the warp range in which the running sum passes the target, then the entry
+  const double target = __dmul_rn((double)s_u[0], Z);
+  int at = 0;
+  double before = 0.0;
+  {
+    double run = 0.0;
+    int lastpos = 0;
+    bool found = false;
+    for (int i = 0; i < C * kVerWarps; ++i) {
+      const double s = s_all[i];
+      if (s > 0.0 && !found) {
+        lastpos = i;
+        before = run;
+        if (run + s > target) found = true;
+      }
+      run += s;
+    }
+    at = lastpos;                            // by rounding none may pass it: the last range that holds anything
+  }
+  if (rank == 0) {
+    const int r0 = (int)min((long long)V, (long long)at * a.range), r1 = (int)min((long long)V, (long long)r0 + a.range);
+    const float* pr = P + cur * a.pn;
+    const float* qr = HASQ ? Q + cur * a.qn : nullptr;
+    if (tid == 0) { s_pick = V; s_lastpos = -1; }
+    __syncthreads();
+    for (int j0 = r0; j0 < r1; j0 += kVerThreads * 4) {
+      const int j = j0 + tid * 4;
+      float f[4], g[4] = {0.f, 0.f, 0.f, 0.f};
+      load4<VEC>(pr, j, r1, f);
+      if constexpr (HASQ) {
+        if (rej > 0) load4<VEC>(qr, j, r1, g);
+      }
+      double r[4], own = 0.0;
+      int lastj = -1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        r[i] = rest(f[i], g[i], j + i);
+        own += r[i];
+        if (r[i] > 0.0 && j + i < r1) lastj = j + i;
+      }
+      double inc = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (lane == 31) s_scan[warp] = inc;
+      if (lastj >= 0) atomicMax(&s_lastpos, lastj);
+      __syncthreads();
+      double base = before;
+      for (int w = 0; w < warp; ++w) base += s_scan[w];
+      double c = base + (inc - own);
+      int pick = V;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c += r[i];
+        if (pick == V && r[i] > 0.0 && c > target) pick = j + i;
+      }
+      if (pick < V) atomicMin(&s_pick, pick);
+      double all = before;
+      for (int w = 0; w < kVerWarps; ++w) all += s_scan[w];
+      before = all;
+      __syncthreads();
+      if (s_pick < V) break;
+    }
+    const int tok = s_pick < V ? s_pick : s_lastpos >= 0 ? s_lastpos : V - 1;
+    if (tid < N) {
+      const long long o = (long long)b * N + tid;
+      a.path[o] = tid < cnt ? s_path[tid] : -1;
+      a.out[o] = tid + 1 < cnt ? s_tok[s_path[tid + 1]] : tid + 1 == cnt ? tok : -1;
+      if (tid == 0) a.count[b] = cnt;
+    }
+  }
+  if (C > 1) cluster_sync();                 // no CTA leaves while another may read its sums
+}
+
+std::vector<at::Tensor> verify_tree(at::Tensor tokens, at::Tensor parents, at::Tensor p, c10::optional<at::Tensor> q,
+                                       at::Tensor u) {
+  TORCH_CHECK(p.is_cuda() && p.dim() == 3 && p.scalar_type() == at::kFloat, "p: float32 [B, N, V]");
+  const int64_t B = p.size(0), N = p.size(1), V = p.size(2);
+  TORCH_CHECK(N >= 1 && N <= kVerNodes, "1 to 64 nodes");
+  TORCH_CHECK(V >= 1 && V <= (1 << 30), "vocabulary of 1 .. 2^30 tokens");
+  auto ints = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK(t.scalar_type() == at::kInt && t.device() == p.device() && t.dim() == 2 && t.size(0) == B && t.size(1) == N &&
+                    t.is_contiguous(), name, ": contiguous int32 [B, N] on p's device");
+    return t.data_ptr<int>();
+  };
+  VerArgs a{};
+  a.tokens = ints(tokens, "tokens");
+  a.parents = ints(parents, "parents");
+  TORCH_CHECK(u.scalar_type() == at::kFloat && u.device() == p.device() && u.dim() == 2 && u.size(0) == B && u.size(1) == N &&
+                  u.is_contiguous(), "u: contiguous float32 [B, N] on p's device");
+  auto rows = [&](const at::Tensor& t, const char* name, long long& sb, long long& sn) {
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.device() == p.device() && t.sizes() == p.sizes() && (t.size(2) == 1 || t.stride(2) == 1),
+                name, ": float32 [B, N, V] with unit inner stride on p's device");
+    sb = t.stride(0); sn = t.stride(1);
+    return (B <= 1 || sb % 4 == 0) && (N <= 1 || sn % 4 == 0) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+  };
+  bool vec = rows(p, "p", a.pb, a.pn);
+  if (q.has_value()) vec = rows(*q, "q", a.qb, a.qn) && vec;
+  a.p = p.data_ptr<float>();
+  a.q = q.has_value() ? q->data_ptr<float>() : nullptr;
+  a.u = u.data_ptr<float>();
+  c10::cuda::CUDAGuard guard(p.device());
+  auto opt = p.options().dtype(at::kInt);
+  auto path = at::empty({B, N}, opt), count = at::empty({B}, opt), out = at::empty({B, N}, opt);
+  if (B == 0) return {path, count, out};
+  a.path = path.data_ptr<int>(); a.count = count.data_ptr<int>(); a.out = out.data_ptr<int>();
+  a.N = (int)N; a.V = (int)V;
+  int C = 1;
+  a.range = (int)(((V + C * kVerWarps - 1) / (C * kVerWarps) + 127) / 128 * 128);
+  TORCH_CHECK(B <= (1LL << 31) / kVerCluster - 1, "too many sequences");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(B * C), 1, 1);
+  cfg.blockDim = dim3(kVerThreads, 1, 1);
+  cfg.stream = at::cuda::getCurrentCUDAStream();
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (vec) {
+    if (a.q) C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_tree_kernel<true, true>, a));
+    else C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_tree_kernel<true, false>, a));
+  } else {
+    if (a.q) C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_tree_kernel<false, true>, a));
+    else C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_tree_kernel<false, false>, a));
+  }
+  return {path, count, out};
+}
+
+}  // namespace tfb

@@ -187,3 +187,104 @@ def softcap_logits(x, w_lm, softcap: float, vocab: int):
         from .fused import softcap_logits as f
         return f(x, w_lm, softcap, vocab)
     return ref.softcap_logits(x, w_lm, softcap, vocab)
+
+
+def kv_cache_alloc(batch: int, heads: int, rows: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
+                   layout: str = "head", device=None):
+    """(k_cache, v_cache, k_scale, v_scale) for ``heads`` key/value heads and ``rows`` rows a
+    sequence: zeroed [B, H, T, D] views of head-major (``layout="head"``, [B, H, T, D]) or
+    token-major (``"token"``, [B, T, H, D]) storage.  ``dtype`` ``float8_e4m3fn`` makes a
+    quantised cache, whose scales are ``float8_e8m0fnu`` [B, H, T]; else the scales are None."""
+    if layout not in ("head", "token"):
+        raise ValueError("layout: 'head' or 'token'")
+    shape = (batch, heads, rows, head_dim) if layout == "head" else (batch, rows, heads, head_dim)
+    quant = dtype == torch.float8_e4m3fn
+
+    def make(sizes, dt):
+        t = torch.zeros(sizes, dtype=torch.uint8 if dt.itemsize == 1 else dt, device=device)
+        t = t.view(dt)
+        return t if layout == "head" else t.transpose(1, 2)
+    return (make(shape, dtype), make(shape, dtype),
+            make(shape[:3], torch.float8_e8m0fnu) if quant else None,
+            make(shape[:3], torch.float8_e8m0fnu) if quant else None)
+
+
+def kv_cache_write(k, v, k_cache, v_cache, pos, count=None, k_scale=None, v_scale=None) -> None:
+    """Rows k, v [B, N, H, D] into the caches [B, H, T, D] (any strides with a unit inner one):
+    row n of sequence b goes to row ``pos[b] + n`` for ``n < count[b]`` (default: all N); rows
+    that fall outside the cache are left out, and every other row stays as it is.  ``pos`` and
+    ``count`` are int32 [B] in device memory.
+
+    ``float8_e4m3fn`` caches hold each row's codes ``x * 2^-e`` rounded to nearest even and its
+    scale ``2^e`` (``float8_e8m0fnu`` [B, H, T]), ``e`` being the least integer (-117 at the
+    least) with ``max|x| <= 448 * 2^e``; a row with an infinity or a NaN reads back as NaN.
+    CUDA: k, v bfloat16 with 16-byte aligned rows, head_dim 64 / 128."""
+    if _cuda(k_cache):
+        from .speculative import kv_cache_write as f
+        return f(k, v, k_cache, v_cache, pos, count, k_scale, v_scale)
+    return ref.kv_cache_write(k, v, k_cache, v_cache, pos, count, k_scale, v_scale)
+
+
+def kv_cache_read(k_cache, v_cache, lens, T: int, k_scale=None, v_scale=None):
+    """The caches' first T rows as keys and values [B, T, H, D] (bfloat16; float32 for float32
+    caches on the CPU), zeros from row ``lens[b]`` (int32 [B]) on.  Quantised rows read back
+    exactly: every value they can hold is a bfloat16 number.  ``k.view(B * T, H * D)`` is a row
+    view as ``flash_attention.flash_fwd`` takes it."""
+    if _cuda(k_cache):
+        from .speculative import kv_cache_read as f
+        return f(k_cache, v_cache, lens, T, k_scale, v_scale)
+    return ref.kv_cache_read(k_cache, v_cache, lens, T, k_scale, v_scale)
+
+
+def kv_cache_commit(k_cache, v_cache, lens, path, count, k_scale=None, v_scale=None) -> None:
+    """Moves the accepted rows of a drafted tree up behind the context, in place: row
+    ``lens[b] + path[b, i]`` becomes row ``lens[b] + i`` for ``i < count[b]``, with its scale.
+    ``path`` int32 [B, N] is ascending over those entries, as ``verify_tree`` returns it;
+    ``lens`` and ``count`` int32 [B].  The caller advances ``lens`` by ``count``."""
+    if _cuda(k_cache):
+        from .speculative import kv_cache_commit as f
+        return f(k_cache, v_cache, lens, path, count, k_scale, v_scale)
+    return ref.kv_cache_commit(k_cache, v_cache, lens, path, count, k_scale, v_scale)
+
+
+def tree_attention(q, k_cache, v_cache, lens, parents=None, scale: float | None = None, k_scale=None, v_scale=None):
+    """Attention of N <= 64 new tokens a sequence over a cache that holds ``lens[b]`` rows of
+    context and, behind them, the N tokens' own rows (``kv_cache_write`` at ``pos = lens``).
+    q [B, N, Hq, D], caches [B, Hkv, T, D] with Hkv dividing Hq (query head h reads head
+    ``h // (Hq // Hkv)``); returns [B, N, Hq, D].
+
+    ``parents`` int32 [B, N]: node n sees the context, its ancestors and itself; -1 marks a
+    child of the context, other parents are earlier nodes.  None: a chain (node n - 1 is node
+    n's parent), so N = 1 is a plain decode step.  A node whose line of parents meets any other
+    value is unused (the padding of a smaller tree: -2), as is one whose own row lies past the
+    cache; its output is zero, and what its row holds reaches no other node.  ``scale`` defaults
+    to D^-0.5.  No gradient."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if _cuda(k_cache):
+        from .speculative import tree_attention as f
+        return f(q, k_cache, v_cache, lens, parents, scale, k_scale, v_scale)
+    return ref.tree_attention(q, k_cache, v_cache, lens, parents, scale, k_scale, v_scale)
+
+
+def verify_tree(tokens, parents, p, q, u):
+    """Speculative sampling over a tree of N <= 64 nodes: which drafted tokens are accepted, and
+    the token after them.  Returns int32 ``(path [B, N], count [B], out [B, N])``: the accepted
+    nodes in ascending order from node 0 (padded with -1), how many they are, and the tokens
+    they add to the text -- those of ``path[1:]``, then the drawn one at ``count - 1`` (padded
+    with -1).
+
+    Node 0 is the root and always accepted; ``parents`` int32 [B, N] as in ``tree_attention``.
+    p (float32 [B, N, V]) holds the target's distribution of the token after each node, q the
+    distribution from which each node's children were drawn independently, or None for drafts
+    that a rule proposed.  From the root on, the children n of the last accepted node c are
+    tried in order with a remainder r (at first p[c], its sum counted as Z = 1): n is accepted
+    iff ``u[n] * q[c, t] * Z < r[t]`` (t = tokens[n]; q None: q[c, t] = 1); otherwise ``r <-
+    max(r - Z q[c], 0)`` (q None: ``r[t] <- 0``) and ``Z <- sum r``, or r and Z start again at
+    p[c] and 1 if nothing is left.  When no child is left the next token is the least j with
+    ``r[0] + ... + r[j] > u[0] * sum r``.  u float32 [B, N] uniform in [0, 1).  Nodes with a
+    token outside the vocabulary are no node's children.  All arithmetic is in 64 bits."""
+    if _cuda(p):
+        from .speculative import verify_tree as f
+        return f(tokens, parents, p, q, u)
+    return ref.verify_tree(tokens, parents, p, q, u)
