@@ -183,6 +183,28 @@ def test_tree_attention(device, dtype, layout, case):
         run_attention(device, B, N, Hq, H, D, T, lens, dtype, layout, par, seed=len(kind))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,layout", KINDS)
+@pytest.mark.parametrize("B,N,Hq,H,D,T", [(9, 3, 6, 3, 128, 4200), (7, 40, 8, 2, 64, 4100), (12, 64, 2, 1, 128, 3900), (5, 50, 18, 6, 128, 2500)])
+def test_tree_attention_many_tiles(cuda_device, dtype, layout, B, N, Hq, H, D, T):
+    """Several key tiles and several (sequence, head) pairs a CTA, one and two row tiles; many
+    calls in a row give the same bits and no wait runs out."""
+    from trainium_frontier_b200.ops._ext import check_errors
+    g = gen(T)
+    lens = [(T - N - 1) * (b + 1) // B if b % 3 else b * 130 for b in range(B)]
+    par = make_tree(B, N, g)
+    o = run_attention("cuda", B, N, Hq, H, D, T, lens, dtype, layout, par, seed=1)
+    kc, vc, ks, vs = make_cache(B, H, T, D, dtype, layout, "cuda", gen(2))
+    q = torch.randn(B, N, Hq, D, generator=g).to(BF16).cuda()
+    args = (q, kc, vc, i32(lens, "cuda"), par.cuda(), None, ks, vs)
+    first = ops.tree_attention(*args)
+    wrong = torch.zeros((), dtype=torch.long, device="cuda")
+    for _ in range(1500):
+        wrong += (ops.tree_attention(*args) != first).any()
+    check_errors()
+    assert o.shape == first.shape and int(wrong) == 0
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
 def test_tree_attention_no_row_left(device, dtype):
@@ -228,6 +250,25 @@ def test_tree_attention_bad_drafted_rows(device, dtype, D):
     torch.testing.assert_close(torch.isinf(o) * o.sign(), torch.isinf(want) * want.sign(), equal_nan=True)
     fine = torch.isfinite(want)
     assert bool(((o - want).abs() <= bound)[fine].all()) and bool(fine[0, [0, 1, 3]].all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_every_code_and_scale_is_read_exactly(device, D):
+    """A token without context attends to itself alone: its output is its value row, each of the
+    254 finite codes times scales from the least to the greatest that stays in range."""
+    codes = torch.arange(256, dtype=torch.uint8)
+    codes = codes[(codes & 0x7f) != 0x7f]
+    exps = [10, 11, 60, 126, 127, 128, 133, 134, 135, 136, 200, 246]
+    B = -(-len(codes) // D) * len(exps)
+    kc, vc, ks, vs = ops.kv_cache_alloc(B, 1, 3, D, E4M3, device=device)
+    for i in range(B):
+        part = codes[(i // len(exps)) * D:][:D]
+        raw(vc)[i, 0, 0, :len(part)] = part.to(device)
+        raw(vs)[i, 0, 0] = exps[i % len(exps)]
+    q = torch.randn(B, 1, 1, D, generator=gen(1)).to(BF16).to(device)
+    o = ops.tree_attention(q, kc, vc, i32([0] * B, device), None, None, ks, vs)
+    assert torch.equal(o[:, 0, 0].double(), values(vc, vs)[:, 0, 0])
 
 
 @pytest.mark.parametrize("device", DEVICES)

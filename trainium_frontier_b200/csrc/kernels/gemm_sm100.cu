@@ -1267,6 +1267,25 @@ CUtensorMap make_tmap_f32(const void* ptr, uint64_t inner, uint64_t outer, uint6
   return m;
 }
 
+// Tensor map of up to five dimensions (innermost first; strides in bytes from dimension 1 on).
+// A dimension of one entry is never stepped over, so its stride is replaced by one that the
+// encoder takes.
+CUtensorMap make_tmap_nd(const void* ptr, CUtensorMapDataType type, int rank, const uint64_t* dims, const uint64_t* strides,
+                         const uint32_t* box, CUtensorMapSwizzle swizzle) {
+  bind_device_context();
+  CUtensorMap m;
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], es[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i]; bx[i] = box[i]; es[i] = 1;
+    if (i > 0) st[i - 1] = dims[i] > 1 ? strides[i - 1] : 16;
+  }
+  CUresult r = encode_fn()(&m, type, (cuuint32_t)rank, const_cast<void*>(ptr), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (rank ", rank, ") failed with code ", int(r));
+  return m;
+}
+
 int num_sms(int dev) {
   static int cache[64] = {0};
   if (!cache[dev]) {
