@@ -2,9 +2,10 @@
 // part of a drafted tree is accepted.  The format is described in kv_cache.cuh.
 //
 // All three move bytes and do nothing else that counts, so the floor is the bytes over the
-// memory rate.  A row of D = 128 (64) bf16 is 8 (4) lanes of two 16-byte loads each: the row's
-// largest magnitude is then three (two) shuffles away, and each lane's 16 codes leave as one
-// 16-byte store.
+// memory rate.  A row of D = 128 (64) bf16 is 16 (8) lanes of one 16-byte load each, whole lines
+// a warp: the row's largest magnitude is then four (three) shuffles away, and a lane's 8 codes
+// leave as one 8-byte store.  A block has one head's neighbouring rows, so that it writes (or
+// reads) one contiguous piece of a head-major cache and of its scales.
 // The reference has no decode path; these serve the cache of inference/generate.py.
 #include <cuda_fp8.h>
 
@@ -45,125 +46,140 @@ __device__ __forceinline__ uint32_t absmax8(const uint4& u) {
   return __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
 }
 
-// cache[b, :, pos[b] + n] = rows[b, n] for n < count[b]; rows outside the cache are left out.
-template <int D, bool QUANT>
+// cache[b, h, pos[b] + n] = rows[b, n, h] for n < count[b]; rows outside the cache are left out.
+// A block has one (sequence, head, keys or values) and blockDim / L * U neighbouring rows.
+template <int D, bool QUANT, int U>
 __global__ void __launch_bounds__(kKvThreads) kv_cache_write_kernel(const KvRows src, const KvView c, const int* __restrict__ pos,
                                                                     const int* __restrict__ count, int N, int H) {
-  constexpr int L = D / 16;   // lanes a row
-  const int b = blockIdx.y, kv = blockIdx.z;
-  const long long r = (long long)blockIdx.x * (kKvThreads / L) + threadIdx.x / L;
-  const int l = threadIdx.x % L;
-  const int n = (int)(r / H), h = (int)(r % H);
-  const long long t = (long long)pos[b] + n;
+  constexpr int L = D / 8;   // lanes a row
+  const int b = blockIdx.y, kv = blockIdx.z, h = blockIdx.x % H;
+  const int l = threadIdx.x % L, rows = blockDim.x / L;
+  const int n0 = (int)(blockIdx.x / H) * rows * U + threadIdx.x / L;
   const int live = count ? min(count[b], N) : N;
-  const bool on = n < live && t >= 0 && t < c.tmax;
-  uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
-  if (on) {
-    const uint4* p = reinterpret_cast<const uint4*>(src.p[kv] + b * src.b[kv] + n * src.n[kv] + h * src.h[kv]) + 2 * l;
-    u0 = p[0];
-    u1 = p[1];
-  }
-  uint8_t* dst = c.p[kv] + b * c.b + h * c.h + t * c.t;
-  if constexpr (!QUANT) {
-    if (on) {
-      reinterpret_cast<uint4*>(dst)[2 * l] = u0;
-      reinterpret_cast<uint4*>(dst)[2 * l + 1] = u1;
-    }
-  } else {
-    uint32_t m = __vmaxu2(absmax8(u0), absmax8(u1));
+  const long long t0 = pos[b];
+  uint4 u[U];
+  bool on[U];
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const int e = scale_byte(max(m & 0xffffu, m >> 16));
-    if (on) {
-      uint4 codes = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);  // a row with an inf or NaN: NaN codes too
-      if (e != kScaleNan) {
-        const float inv = __uint_as_float((uint32_t)(254 - e) << 23);   // 2^-(e - 127)
-        const uint2 a = quant8(u0, inv), d = quant8(u1, inv);
-        codes = make_uint4(a.x, a.y, d.x, d.y);
+  for (int i = 0; i < U; ++i) {
+    const int n = n0 + i * rows;
+    on[i] = n < live && t0 + n >= 0 && t0 + n < c.tmax;
+    u[i] = make_uint4(0, 0, 0, 0);
+    if (on[i]) u[i] = reinterpret_cast<const uint4*>(src.p[kv] + b * src.b[kv] + n * src.n[kv] + h * src.h[kv])[l];
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const long long t = t0 + n0 + i * rows;
+    uint8_t* dst = c.p[kv] + b * c.b + h * c.h + t * c.t;
+    if constexpr (!QUANT) {
+      if (on[i]) reinterpret_cast<uint4*>(dst)[l] = u[i];
+    } else {
+      uint32_t m = absmax8(u[i]);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const int e = scale_byte(max(m & 0xffffu, m >> 16));
+      if (on[i]) {
+        uint2 codes = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);   // a row with an inf or NaN: NaN codes too
+        if (e != kScaleNan) codes = quant8(u[i], __uint_as_float((uint32_t)(254 - e) << 23));   // times 2^-(e - 127)
+        reinterpret_cast<uint2*>(dst)[l] = codes;
+        if (l == 0) c.s[kv][b * c.sb + h * c.sh + t * c.st] = (uint8_t)e;
       }
-      reinterpret_cast<uint4*>(dst)[l] = codes;
-      if (l == 0) c.s[kv][b * c.sb + h * c.sh + t * c.st] = (uint8_t)e;
     }
   }
 }
 
 // out[b, t, h] = the cached row as bf16 for t < min(lens[b], T_max), zeros for the other t < T.
-template <int D, bool QUANT>
+// Blocks as above.
+template <int D, bool QUANT, int U>
 __global__ void __launch_bounds__(kKvThreads) kv_cache_read_kernel(const KvView c, const int* __restrict__ lens, uint8_t* __restrict__ k,
                                                                    uint8_t* __restrict__ v, int T, int H) {
-  constexpr int L = D / 16;
-  const int b = blockIdx.y, kv = blockIdx.z;
-  const long long r = (long long)blockIdx.x * (kKvThreads / L) + threadIdx.x / L;
-  const int l = threadIdx.x % L;
-  const int t = (int)(r / H), h = (int)(r % H);
-  if (t >= T) return;
-  uint4 o0 = make_uint4(0, 0, 0, 0), o1 = o0;
-  if (t < lens[b] && t < c.tmax) {
-    const uint4* p = reinterpret_cast<const uint4*>(c.p[kv] + b * c.b + h * c.h + (long long)t * c.t);
-    if constexpr (!QUANT) {
-      o0 = p[2 * l];
-      o1 = p[2 * l + 1];
-    } else {
-      const uint4 u = p[l];
-      const int e = c.s[kv][b * c.sb + h * c.sh + t * c.st];
-      const float sc = e == kScaleNan ? __int_as_float(0x7fffffff) : e == 0 ? 0x1p-127f : __uint_as_float((uint32_t)e << 23);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-      uint32_t o[8];
+  constexpr int L = D / 8;
+  const int b = blockIdx.y, kv = blockIdx.z, h = blockIdx.x % H;
+  const int l = threadIdx.x % L, rows = blockDim.x / L;
+  const int t0 = (int)(blockIdx.x / H) * rows * U + threadIdx.x / L;
+  const int live = min(min(lens[b], c.tmax), T);
+  uint4 o[U];
+  uint2 u[U];
+  int e[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
-        const float2 f = __half22float2(__half2(hr));
-        o[i] = pack_bf16x2(f.x * sc, f.y * sc);
+  for (int i = 0; i < U; ++i) {
+    const int t = t0 + i * rows;
+    o[i] = make_uint4(0, 0, 0, 0);
+    u[i] = make_uint2(0, 0);
+    e[i] = 127;
+    if (t < live) {
+      const uint8_t* p = c.p[kv] + b * c.b + h * c.h + (long long)t * c.t;
+      if constexpr (QUANT) {
+        u[i] = reinterpret_cast<const uint2*>(p)[l];
+        e[i] = c.s[kv][b * c.sb + h * c.sh + t * c.st];
+      } else {
+        o[i] = reinterpret_cast<const uint4*>(p)[l];
       }
-      o0 = make_uint4(o[0], o[1], o[2], o[3]);
-      o1 = make_uint4(o[4], o[5], o[6], o[7]);
     }
   }
-  uint4* dst = reinterpret_cast<uint4*>((kv ? v : k) + (((long long)b * T + t) * H + h) * (D * 2)) + 2 * l;
-  dst[0] = o0;
-  dst[1] = o1;
+  uint8_t* out = (kv ? v : k) + ((long long)b * T * H + h) * (D * 2);
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int t = t0 + i * rows;
+    if constexpr (QUANT) {
+      const float sc = e[i] == kScaleNan ? __int_as_float(0x7fffffff) : e[i] == 0 ? 0x1p-127f : __uint_as_float((uint32_t)e[i] << 23);
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((j < 2 ? u[i].x : u[i].y) >> (16 * (j & 1))), __NV_E4M3);
+        const float2 f = __half22float2(__half2(hr));
+        w[j] = pack_bf16x2(f.x * sc, f.y * sc);
+      }
+      o[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (t < T) reinterpret_cast<uint4*>(out + (long long)t * H * (D * 2))[l] = o[i];
+  }
 }
 
 // cache[b, h, lens[b] + i] = cache[b, h, lens[b] + path[b, i]], i < count[b], path ascending with
 // path[i] >= i.  A source is then never below its own target and never a target of an earlier
-// move, so moves in order of i are right in place; loading a batch of rows before storing any
-// of it keeps that order (every row of a batch is loaded before the batch stores).  One lane
-// owns 16 bytes of a row for all moves.
+// move, so moves in order of i are right in place -- and so are batches of moves of which all
+// rows are loaded before any is stored.  A block of 256 threads has units of min(N, 64) rows, a
+// unit being one (sequence, head, keys or values); a thread holds its 16-byte pieces of the
+// batch in registers between the two barriers.
 template <int ROW>   // bytes of a row
 __global__ void __launch_bounds__(kKvThreads) kv_cache_commit_kernel(const KvView c, const int* __restrict__ lens, const int* __restrict__ path,
-                                                                     const int* __restrict__ count, int B, int N, int H) {
-  constexpr int L = ROW / 16, U = 8;
-  const long long g = (long long)blockIdx.x * (kKvThreads / L) + threadIdx.x / L;
-  if (g >= 2LL * B * H) return;
-  const int l = threadIdx.x % L;
-  const int kv = (int)(g & 1), b = (int)((g >> 1) / H), h = (int)((g >> 1) % H);
+                                                                     const int* __restrict__ count, int B, int N, int H, int batch, int ppt) {
+  constexpr int L = ROW / 16, U = ROW / 64;   // pieces a row; pieces a thread at most (64 rows a batch)
+  const int per = batch * L;                  // pieces of a unit's batch
+  const int threads = per / ppt;              // threads of a unit, ppt <= U pieces each
+  const int slot = threadIdx.x / threads, id = threadIdx.x - slot * threads;
+  const long long unit = (long long)blockIdx.x * (kKvThreads / threads) + slot;
+  const bool real = slot < kKvThreads / threads && unit < 2LL * B * H;
+  const int kv = (int)(unit & 1), b = real ? (int)((unit >> 1) / H) : 0, h = (int)((unit >> 1) % H);
   const long long t0 = lens[b];
-  const int m = min(count[b], N);
+  const int m = real && t0 >= 0 ? min(count[b], N) : 0;
   const int* pp = path + (long long)b * N;
-  uint8_t* base = c.p[kv] + b * c.b + h * c.h + 16 * l;
+  uint8_t* base = c.p[kv] + b * c.b + h * c.h;
   uint8_t* sbase = c.s[kv] ? c.s[kv] + b * c.sb + h * c.sh : nullptr;
-  if (t0 < 0) return;
-  for (int i0 = 0; i0 < m; i0 += U) {
+  for (int i0 = 0; i0 < N; i0 += batch) {
     uint4 u[U];
     uint8_t s[U];
     bool on[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int i = i0 + j;
-      const int src = i < m ? pp[i] : -1;
+      const int piece = id + j * threads, i = i0 + piece / L, l = piece % L;
+      const int src = j < ppt && piece < per && i < m ? pp[i] : -1;
       on[j] = src > i && src < N && t0 + src < c.tmax;
       if (on[j]) {
-        u[j] = *reinterpret_cast<const uint4*>(base + (t0 + src) * c.t);
+        u[j] = *reinterpret_cast<const uint4*>(base + (t0 + src) * c.t + 16 * l);
         if (sbase && l == 0) s[j] = sbase[(t0 + src) * c.st];
       }
     }
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < U; ++j) {
+      const int piece = id + j * threads, i = i0 + piece / L, l = piece % L;
       if (on[j]) {
-        *reinterpret_cast<uint4*>(base + (t0 + i0 + j) * c.t) = u[j];
-        if (sbase && l == 0) sbase[(t0 + i0 + j) * c.st] = s[j];
+        *reinterpret_cast<uint4*>(base + (t0 + i) * c.t + 16 * l) = u[j];
+        if (sbase && l == 0) sbase[(t0 + i) * c.st] = s[j];
       }
     }
+    if (N > batch) __syncthreads();
   }
 }
 
@@ -183,6 +199,18 @@ static KvRows kv_rows(const at::Tensor& k, const at::Tensor& v, const at::Tensor
   return r;
 }
 
+// Blocks of the row kernels: up to 256 threads of D / 8 lanes a row, four rows a thread where
+// there are enough rows to fill the GPU with fewer threads.
+static dim3 kv_grid(int64_t N, int64_t H, int64_t B, int64_t D, int& threads, int& U) {
+  const int64_t L = D / 8, most = kKvThreads / L;
+  U = N >= 4 * most ? 4 : 1;
+  const int64_t rows = std::min(most, N);
+  threads = (int)((rows * L + 31) / 32 * 32);
+  const int64_t per = threads / L * U, gx = (N + per - 1) / per * H;
+  TORCH_CHECK(gx < (1LL << 31), "too many rows");
+  return dim3((unsigned)gx, (unsigned)B, 2);
+}
+
 static void check_batch(int64_t B) { TORCH_CHECK(B <= 65535, "at most 65535 sequences"); }
 
 void kv_cache_write(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor vc, at::Tensor pos,
@@ -199,10 +227,11 @@ void kv_cache_write(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor vc, at
   if (B == 0 || N == 0 || H == 0) return;
   c10::cuda::CUDAGuard guard(kc.device());
   auto s = at::cuda::getCurrentCUDAStream();
-  const int64_t per = kKvThreads / (D / 16), gx = (N * H + per - 1) / per;
-  TORCH_CHECK(gx < (1LL << 31), "too many rows");
-  const dim3 grid((unsigned)gx, (unsigned)B, 2);
-#define TFB_KV_WRITE(DD, QQ) kv_cache_write_kernel<DD, QQ><<<grid, kKvThreads, 0, s>>>(r, c, pp, cp, (int)N, (int)H)
+  int threads, U;
+  const dim3 grid = kv_grid(N, H, B, D, threads, U);
+#define TFB_KV_WRITE(DD, QQ) \
+  (U == 1 ? kv_cache_write_kernel<DD, QQ, 1><<<grid, threads, 0, s>>>(r, c, pp, cp, (int)N, (int)H) \
+          : kv_cache_write_kernel<DD, QQ, 4><<<grid, threads, 0, s>>>(r, c, pp, cp, (int)N, (int)H))
   if (D == 128) { if (quant) TFB_KV_WRITE(128, true); else TFB_KV_WRITE(128, false); }
   else { if (quant) TFB_KV_WRITE(64, true); else TFB_KV_WRITE(64, false); }
 #undef TFB_KV_WRITE
@@ -222,12 +251,13 @@ std::vector<at::Tensor> kv_cache_read(at::Tensor kc, at::Tensor vc, at::Tensor l
   auto k = at::empty({B, T, H, D}, opt), v = at::empty({B, T, H, D}, opt);
   if (k.numel() == 0) return {k, v};
   auto s = at::cuda::getCurrentCUDAStream();
-  const int64_t per = kKvThreads / (D / 16), gx = (T * H + per - 1) / per;
-  TORCH_CHECK(gx < (1LL << 31), "too many rows");
-  const dim3 grid((unsigned)gx, (unsigned)B, 2);
+  int threads, U;
+  const dim3 grid = kv_grid(T, H, B, D, threads, U);
   auto* kp = static_cast<uint8_t*>(k.data_ptr());
   auto* vp = static_cast<uint8_t*>(v.data_ptr());
-#define TFB_KV_READ(DD, QQ) kv_cache_read_kernel<DD, QQ><<<grid, kKvThreads, 0, s>>>(c, lp, kp, vp, (int)T, (int)H)
+#define TFB_KV_READ(DD, QQ) \
+  (U == 1 ? kv_cache_read_kernel<DD, QQ, 1><<<grid, threads, 0, s>>>(c, lp, kp, vp, (int)T, (int)H) \
+          : kv_cache_read_kernel<DD, QQ, 4><<<grid, threads, 0, s>>>(c, lp, kp, vp, (int)T, (int)H))
   if (D == 128) { if (quant) TFB_KV_READ(128, true); else TFB_KV_READ(128, false); }
   else { if (quant) TFB_KV_READ(64, true); else TFB_KV_READ(64, false); }
 #undef TFB_KV_READ
@@ -249,9 +279,13 @@ void kv_cache_commit(at::Tensor kc, at::Tensor vc, at::Tensor lens, at::Tensor p
   if (B == 0 || H == 0 || N == 0) return;
   c10::cuda::CUDAGuard guard(kc.device());
   auto s = at::cuda::getCurrentCUDAStream();
-  const int64_t row = D * (quant ? 1 : 2), per = kKvThreads / (row / 16), gx = (2 * B * H + per - 1) / per;
+  const int64_t row = D * (quant ? 1 : 2);
+  const int batch = (int)std::min<int64_t>(N, 64), pieces = batch * (int)(row / 16);
+  int ppt = 1;                               // pieces a thread: the least power of two that keeps a unit in one block
+  while (pieces / ppt > kKvThreads || pieces % ppt) ppt *= 2;
+  const int64_t units = kKvThreads / (pieces / ppt), gx = (2 * B * H + units - 1) / units;
   TORCH_CHECK(gx < (1LL << 31), "too many rows");
-#define TFB_KV_COMMIT(RR) kv_cache_commit_kernel<RR><<<(unsigned)gx, kKvThreads, 0, s>>>(c, lp, pp, cp, (int)B, (int)N, (int)H)
+#define TFB_KV_COMMIT(RR) kv_cache_commit_kernel<RR><<<(unsigned)gx, kKvThreads, 0, s>>>(c, lp, pp, cp, (int)B, (int)N, (int)H, batch, ppt)
   if (row == 256) TFB_KV_COMMIT(256);
   else if (row == 128) TFB_KV_COMMIT(128);
   else TFB_KV_COMMIT(64);

@@ -67,19 +67,25 @@ __device__ __forceinline__ void load4(const float* row, int j, int end, float (&
   for (int i = 0; i < 4; ++i) f[i] = j + i < end ? row[j + i] : 0.f;
 }
 
+// max(r, 0) without the 64-bit compare: the sign bit clears both words.
+__device__ __forceinline__ double clear_negative(double r) {
+  const int keep = ~(__double2hiint(r) >> 31);
+  return __hiloint2double(__double2hiint(r) & keep, __double2loint(r) & keep);
+}
+
 // VEC: rows start on 16-byte boundaries.
 template <bool VEC, bool HASQ>
-__global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(const VerArgs a) {
+__global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(const VerArgs a) {
   __shared__ int s_tok[kVerNodes], s_par[kVerNodes], s_path[kVerNodes];
   __shared__ float s_u[kVerNodes], s_p[kVerNodes], s_q[kVerNodes];
   __shared__ double s_z[kVerNodes];          // Z before each rejection at the current node
   __shared__ int s_rej[kVerNodes];           // its rejected tokens (q absent)
-  __shared__ double s_sum[2][kVerWarps];     // the warps' sums of a pass, two passes in turn
-  __shared__ double s_all[kVerWarps * kVerCluster];
+  __shared__ double s_sum[kVerWarps];        // the warps' sums of the last pass
+  __shared__ double s_tot[2];                // this CTA's sum, two passes in turn
   __shared__ double s_scan[kVerWarps];
   __shared__ int s_pick, s_lastpos;
 
-  const int C = (int)nclusters_x() > 0 ? (int)(gridDim.x / nclusters_x()) : 1;
+  const int C = (int)(gridDim.x / nclusters_x());
   const int rank = (int)cluster_ctarank();
   const int b = (int)(blockIdx.x / C);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -99,31 +105,37 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(const VerArgs 
   __syncthreads();
 
   int cur = 0, cnt = 1, rej = 0, turn = 0;
-  double Z = 1.0;
-  bool summed = false;                       // s_all holds the sums of the present r
+  double Z = 1.0, share = 0.0;               // share: lane i has CTA i's part of the last pass's total
+  bool summed = false;                       // s_sum and share belong to the present r
   const long long w0 = (long long)(rank * kVerWarps + warp) * a.range;   // this warp's range
   const int lo = (int)min((long long)V, w0), hi = (int)min((long long)V, w0 + a.range);
 
-  // r at one entry after the rejections so far
-  auto rest = [&](float pj, float qj, int j) -> double {
-    double r = (double)pj;
-    for (int k = 0; k < rej; ++k) {
-      if constexpr (HASQ) {
-        r = __dsub_rn(r, __dmul_rn(s_z[k], (double)qj));
-        r = r > 0.0 ? r : 0.0;
-      } else {
-        if (s_rej[k] == j) r = 0.0;
+  // r at M neighbouring entries from j on, after the rejections so far; f: p there, g: q there
+  auto rest = [&](auto& r, const auto& f, const auto& g, int j, int M) {
+#pragma unroll
+    for (int i = 0; i < M; ++i) r[i] = (double)f[i];
+    if (HASQ && rej > 0) {                   // Z is 1 before the first rejection
+#pragma unroll
+      for (int i = 0; i < M; ++i) r[i] = clear_negative(__dsub_rn(r[i], (double)g[i]));
+    }
+#pragma unroll 1
+    for (int k = HASQ ? 1 : 0; k < rej; ++k) {
+      const double z = s_z[k];
+      const int t = s_rej[k] - j;
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        if (HASQ) r[i] = clear_negative(__dsub_rn(r[i], __dmul_rn(z, (double)g[i])));
+        else if (t == i) r[i] = 0.0;
       }
     }
-    return r;
   };
-  // sums of r over every warp's range, into s_all of every CTA; returns the total
+  // the sum of r, and with it s_sum and share
   auto pass = [&]() -> double {
     const float* pr = P + cur * a.pn;
     const float* qr = HASQ ? Q + cur * a.qn : nullptr;
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
     for (int j = lo + lane * 4; j < hi; j += 512) {
-      float f[4][4], g[4][4];
+      float f[4][4], g[4][4] = {};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         load4<VEC>(pr, j + 128 * k, hi, f[k]);
@@ -132,22 +144,33 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(const VerArgs 
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 4; ++k) {
+        double r[4];
+        rest(r, f[k], g[k], j + 128 * k, 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] += rest(f[k][i], HASQ ? g[k][i] : 0.f, j + 128 * k + i);
+        for (int i = 0; i < 4; ++i) acc[i] += r[i];
+      }
     }
     double s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) s_sum[turn][warp] = s;
-    if (C > 1) cluster_sync(); else __syncthreads();
-    for (int i = tid; i < C * kVerWarps; i += kVerThreads)
-      s_all[i] = C > 1 ? ld_dsmem_f64(mapa_shared(smem_u32(&s_sum[turn][i % kVerWarps]), (uint32_t)(i / kVerWarps)))
-                       : s_sum[turn][i];
-    turn ^= 1;
+    __syncthreads();                         // s_sum of the pass before is no longer read
+    if (lane == 0) s_sum[warp] = s;
     __syncthreads();
-    double t = 0.0;
-    for (int i = 0; i < C * kVerWarps; ++i) t += s_all[i];
+    double t = lane < kVerWarps ? s_sum[lane] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    share = lane == 0 ? t : 0.0;
+    if (C > 1) {
+      if (tid == 0) s_tot[turn] = t;
+      cluster_sync();
+      share = lane < C ? ld_dsmem_f64(mapa_shared(smem_u32(&s_tot[turn]), (uint32_t)lane)) : 0.0;
+      t = share;
+#pragma unroll
+      for (int o = kVerCluster / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      t = __shfl_sync(0xffffffffu, t, 0);
+      turn ^= 1;
+    }
     summed = true;
     return t;
   };
@@ -155,9 +178,10 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(const VerArgs 
   if (tid == 0) s_path[0] = 0;
   for (int n = 1; n < N; ++n) {
     if (s_par[n] != cur) continue;
-    const double qn = (double)s_q[n];
-    const double r = rest(s_p[n], s_q[n], s_tok[n]);
-    if (__dmul_rn(__dmul_rn((double)s_u[n], qn), Z) < r) {
+    const float f[1] = {s_p[n]}, g[1] = {s_q[n]};
+    double r[1];
+    rest(r, f, g, s_tok[n], 1);
+    if (__dmul_rn(__dmul_rn((double)s_u[n], (double)g[0]), Z) < r[0]) {
       __syncthreads();                       // s_path, and s_z / s_rej of the node left behind
       cur = n;
       if (tid == 0) s_path[cnt] = n;
@@ -183,27 +207,30 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(const VerArgs 
   }
   if (!summed) Z = pass();
 
-  // the draw: the warp range in which the running sum passes the target, then the entry
+  // the draw: the CTA and the warp's range in which the running sum passes the target, then the
+  // entry.  By rounding none may pass it: then the last one that holds anything.
   const double target = __dmul_rn((double)s_u[0], Z);
-  int at = 0;
   double before = 0.0;
-  {
-    double run = 0.0;
-    int lastpos = 0;
+  int at = 0;
+  auto find = [&](int n, auto part) {
+    double run = before;
     bool found = false;
-    for (int i = 0; i < C * kVerWarps; ++i) {
-      const double s = s_all[i];
+    at = 0;
+    for (int i = 0; i < n; ++i) {
+      const double s = part(i);
       if (s > 0.0 && !found) {
-        lastpos = i;
+        at = i;
         before = run;
-        if (run + s > target) found = true;
+        found = run + s > target;
       }
       run += s;
     }
-    at = lastpos;                            // by rounding none may pass it: the last range that holds anything
-  }
-  if (rank == 0) {
-    const int r0 = (int)min((long long)V, (long long)at * a.range), r1 = (int)min((long long)V, (long long)r0 + a.range);
+  };
+  find(C, [&](int i) { return __shfl_sync(0xffffffffu, share, i); });
+  if (rank == at) {
+    find(kVerWarps, [&](int i) { return s_sum[i]; });
+    const long long first = (long long)(rank * kVerWarps + at) * a.range;
+    const int r0 = (int)min((long long)V, first), r1 = (int)min((long long)V, first + a.range);
     const float* pr = P + cur * a.pn;
     const float* qr = HASQ ? Q + cur * a.qn : nullptr;
     if (tid == 0) { s_pick = V; s_lastpos = -1; }
@@ -215,14 +242,13 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(const VerArgs 
       if constexpr (HASQ) {
         if (rej > 0) load4<VEC>(qr, j, r1, g);
       }
-      double r[4], own = 0.0;
+      double r[4];
+      rest(r, f, g, j, 4);
       int lastj = -1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        r[i] = rest(f[i], g[i], j + i);
-        own += r[i];
+      for (int i = 0; i < 4; ++i)
         if (r[i] > 0.0 && j + i < r1) lastj = j + i;
-      }
+      const double own = (r[0] + r[1]) + (r[2] + r[3]);
       double inc = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -232,8 +258,11 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(const VerArgs 
       if (lane == 31) s_scan[warp] = inc;
       if (lastj >= 0) atomicMax(&s_lastpos, lastj);
       __syncthreads();
-      double base = before;
-      for (int w = 0; w < warp; ++w) base += s_scan[w];
+      double base = before, all = before;
+      for (int w = 0; w < kVerWarps; ++w) {
+        if (w < warp) base += s_scan[w];
+        all += s_scan[w];
+      }
       double c = base + (inc - own);
       int pick = V;
 #pragma unroll
@@ -242,8 +271,6 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(const VerArgs 
         if (pick == V && r[i] > 0.0 && c > target) pick = j + i;
       }
       if (pick < V) atomicMin(&s_pick, pick);
-      double all = before;
-      for (int w = 0; w < kVerWarps; ++w) all += s_scan[w];
       before = all;
       __syncthreads();
       if (s_pick < V) break;
@@ -292,7 +319,11 @@ std::vector<at::Tensor> verify_tree(at::Tensor tokens, at::Tensor parents, at::T
   if (B == 0) return {path, count, out};
   a.path = path.data_ptr<int>(); a.count = count.data_ptr<int>(); a.out = out.data_ptr<int>();
   a.N = (int)N; a.V = (int)V;
+  // CTAs of a cluster: one for each 16384 entries.  Exchanging sums costs a pass about 1 us, so
+  // a row of 8192 is best left to one CTA (8 sequences x 6 nodes: 6.7 us, 7.9 with two, 8.4 with
+  // eight), and one of 131072 shared by eight (64 x 24 nodes: 46 us, 49 with four, 108 with one).
   int C = 1;
+  while (C < kVerCluster && (int64_t)C * 16384 < V) C *= 2;
   a.range = (int)(((V + C * kVerWarps - 1) / (C * kVerWarps) + 127) / 128 * 128);
   TORCH_CHECK(B <= (1LL << 31) / kVerCluster - 1, "too many sequences");
   cudaLaunchConfig_t cfg = {};
