@@ -38,6 +38,8 @@ int num_sms(int dev);
 constexpr int kTreeNodes = 64;
 constexpr uint32_t kTreePanel = 128u * 128u;   // bytes of one 64-column panel of 128 bf16 rows
 constexpr int kSegRing = 8;                    // segments whose poison masks are kept
+constexpr int kLineRing = 4;                   // segments whose ancestor masks are kept
+constexpr int kLenCache = 128;                 // context lengths kept in shared memory (of larger batches: none)
 
 struct TreeArgs {
   __nv_bfloat16* o;          // [B, N, Hq, D]
@@ -48,42 +50,47 @@ struct TreeArgs {
   int gg, rt, rg;            // head groups, row tiles and row groups (of NT tiles) a key/value head
   float scale_log2;          // |scale| log2(e), never 0
   int neg;                   // scale < 0
-  float* part;               // [2 * grid][NT * 128][D] unnormalised partial outputs
+  float4* part;              // [2 * grid][NT][D / 4][128 rows] unnormalised partial outputs
   float2* part_ml;           // [2 * grid][NT * 128] their maximum (log2 units) and sum
+  float2* pair_ml;           // [grid][128] group 1's, for group 0 (NT = 1)
   int* err;
 };
 
-__device__ __forceinline__ int tree_len(const TreeArgs& a, const KvView& c, int b) { return max(0, min(a.lens[b], c.tmax)); }
-// Key tiles of sequence b: its context and as many node rows as the cache has room for.
-__device__ __forceinline__ int tree_tiles(const TreeArgs& a, const KvView& c, int b) {
-  return (int)((min((long long)tree_len(a, c, b) + a.N, (long long)c.tmax) + 127) >> 7);
-}
+// Context lengths, from shared memory where the batch is small enough.
+struct TreeLens {
+  const int* lens;
+  const int* cache;           // null: read lens
+  int n, tmax;
+  __device__ __forceinline__ int len(int b) const { return cache ? cache[b] : max(0, min(lens[b], tmax)); }
+  // key tiles of sequence b: its context and as many node rows as the cache has room for
+  __device__ __forceinline__ int tiles(int b) const { return (int)((min((long long)len(b) + n, (long long)tmax) + 127) >> 7); }
+};
 
 // The key tiles of a CTA, in order: [pos, end) of the line of all tiles.
 struct TreeIter {
-  long long pos, end, base;   // base: first tile of sequence b on the line
+  int pos, end, base;         // base: first tile of sequence b on the line
   int b, kt, units;           // kt: key tiles of sequence b; units: (head, row group) pairs
   int h, rgi, len, k, k0, k1; // present segment: head, row group, context length, key tile and its range
   int seg;                    // segments begun so far, less one
 
   // Present tile -> next one; false at the end.
-  __device__ __forceinline__ bool next(const TreeArgs& a, const KvView& c) {
+  __device__ __forceinline__ bool next(const TreeLens& lens, int rg) {
     if (seg >= 0 && k + 1 < k1) {
       ++k;
       return true;
     }
     if (pos >= end) return false;
-    while (pos >= base + (long long)kt * units) {
-      base += (long long)kt * units;
-      kt = tree_tiles(a, c, ++b);
+    while (pos >= base + kt * units) {
+      base += kt * units;
+      kt = lens.tiles(++b);
     }
-    len = tree_len(a, c, b);
-    const long long rel = pos - base;
-    const int u = (int)(rel / kt);
-    k0 = k = (int)(rel - (long long)u * kt);
-    k1 = (int)min((long long)kt, k0 + (end - pos));
-    h = u / a.rg;
-    rgi = u - h * a.rg;
+    len = lens.len(b);
+    const unsigned rel = (unsigned)(pos - base);
+    const int u = (int)(rel / (unsigned)kt);
+    k0 = k = (int)rel - u * kt;
+    k1 = min(kt, k0 + (end - pos));
+    h = u / rg;
+    rgi = u - h * rg;
     pos += k1 - k0;
     ++seg;
     return true;
@@ -92,36 +99,34 @@ struct TreeIter {
   __device__ __forceinline__ bool last() const { return k + 1 == k1; }
 };
 
-// Start of CTA `cta` of `grid` on the line of tiles (warp-collective); total: the line's length.
-__device__ __forceinline__ TreeIter tree_begin(const TreeArgs& a, const KvView& c, int cta, int grid, long long& total) {
+// Start of CTA `cta` of `grid` on the line of tiles (warp-collective).  total * grid < 2^32.
+__device__ __forceinline__ TreeIter tree_begin(const TreeArgs& a, const TreeLens& lens, int cta, int grid) {
   const int lane = threadIdx.x & 31;
   TreeIter it;
   it.units = a.Hkv * a.rg;
-  long long sum = 0;
-  for (int b = lane; b < a.B; b += 32) sum += tree_tiles(a, c, b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  total = sum * it.units;
-  grid = (int)min((long long)grid, total);   // CTAs that have work
-  it.pos = cta < grid ? total * cta / grid : total;
-  it.end = cta < grid ? total * (cta + 1) / grid : total;
+  int sum = 0;
+  for (int b = lane; b < a.B; b += 32) sum += lens.tiles(b);
+  const int total = __reduce_add_sync(0xffffffffu, sum) * it.units;
+  grid = min(grid, total);                   // CTAs that have work
+  it.pos = cta < grid ? (int)((unsigned)total * (unsigned)cta / (unsigned)grid) : total;
+  it.end = cta < grid ? (int)((unsigned)total * (unsigned)(cta + 1) / (unsigned)grid) : total;
   it.base = 0;
   it.b = 0;
   it.seg = -1;
   it.k = it.k0 = it.k1 = 0;
   // the sequence in which pos lies
   for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const long long mine = b0 + lane < a.B ? (long long)tree_tiles(a, c, b0 + lane) * it.units : 0;
-    long long inc = mine;
+    const int mine = b0 + lane < a.B ? lens.tiles(b0 + lane) * it.units : 0;
+    int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
     const unsigned in = __ballot_sync(0xffffffffu, it.pos < it.base + inc);
     const int at = in ? __ffs(in) - 1 : 31;
-    const long long before = __shfl_sync(0xffffffffu, inc - mine, at);
-    const long long all = __shfl_sync(0xffffffffu, inc, 31);
+    const int before = __shfl_sync(0xffffffffu, inc - mine, at);
+    const int all = __shfl_sync(0xffffffffu, inc, 31);
     if (in || b0 + 32 >= a.B) {
       it.b = min(b0 + at, a.B - 1);
       it.base += before;
@@ -129,7 +134,7 @@ __device__ __forceinline__ TreeIter tree_begin(const TreeArgs& a, const KvView& 
     }
     it.base += all;
   }
-  it.kt = tree_tiles(a, c, it.b);
+  it.kt = lens.tiles(it.b);
   return it;
 }
 
@@ -206,11 +211,48 @@ __device__ __forceinline__ float tree_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint64_t tree_desc_k(uint32_t base, int kk) {   // K-major operand, 16 of D at step kk
-  return umma_desc_sw128(base + (uint32_t)(kk >> 2) * kTreePanel + (uint32_t)(kk & 3) * 32u, 16, 1024);
+// 2^v of a pair on the FMA pipe, for v <= 8 (0 below -126): v = n + f, n the nearest integer (it
+// lands in the low bits of v + 1.5 * 2^23), 2^f on [-1/2, 1/2] by a polynomial of degree 4 fitted
+// here for the least relative error (2.7e-6), n added to its exponent.  A quarter of the
+// exponentials goes this way, since the two groups' 128 a row pair are all that the MUFU unit
+// of a sub-core does in 1024 cycles.  NaN stays NaN.
+__device__ __forceinline__ float2 tree_exp2_pair(float2 v) {
+  const float2 c = make_float2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  const float2 t = __fadd2_rn(c, make_float2(12582912.f, 12582912.f));
+  const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = __fadd2_rn(c, make_float2(-n.x, -n.y));
+  float2 p = __ffma2_rn(make_float2(0.009570102207362652f, 0.009570102207362652f), f, make_float2(0.05591785907745361f, 0.05591785907745361f));
+  p = __ffma2_rn(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
+  p = __ffma2_rn(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+  p = __ffma2_rn(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  const float x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
+  const float y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
+  return make_float2(v.x >= -126.f ? x : v.x == v.x ? 0.f : v.x, v.y >= -126.f ? y : v.y == v.y ? 0.f : v.y);
 }
-__device__ __forceinline__ uint64_t tree_desc_mn(uint32_t base, int kk) {  // MN-major operand, 16 keys at step kk
-  return umma_desc_sw128(base + (uint32_t)kk * 2048u, kTreePanel, 1024);
+
+// Low word of an operand's descriptor (128-byte swizzle; the high word is the same for all), and
+// what a step of 16 along the contraction adds to it: 32 bytes within a 64-column panel of a
+// K-major operand, 16 rows of 128 bytes of an MN-major one.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t tree_desc_k(uint32_t addr) { return ((addr >> 4) & 0x3fffu) | (1u << 16); }
+__device__ __forceinline__ uint32_t tree_desc_mn(uint32_t addr) { return ((addr >> 4) & 0x3fffu) | ((kTreePanel >> 4) << 16); }
+__host__ __device__ constexpr uint32_t tree_step_k(int kk) { return (uint32_t)(kk >> 2) * (kTreePanel >> 4) + (uint32_t)(kk & 3) * 2u; }
+__host__ __device__ constexpr uint32_t tree_step_mn(int kk) { return (uint32_t)kk * 128u; }
+__device__ __forceinline__ void tree_mma(uint32_t d, uint32_t alo, uint32_t blo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d), "r"(alo), "r"(blo), "r"(idesc), "r"(accumulate),
+      "r"(kDescHi));
+}
+__device__ __forceinline__ void tree_mma_p(uint32_t d, uint32_t a_tmem, uint32_t blo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d), "r"(a_tmem), "r"(blo), "r"(idesc), "r"(accumulate),
+      "r"(kDescHi));
 }
 
 // 4 e4m3 codes -> 4 bf16 (two words), times m1 (and m2 unless it is 1).  The code's exponent and
@@ -230,82 +272,129 @@ __device__ __forceinline__ __nv_bfloat162 bf16x2_bits(uint32_t h) {
   return *reinterpret_cast<const __nv_bfloat162*>(&w);
 }
 
+__device__ __forceinline__ void tree_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// Adds what is not finite in the drafted value rows `bad` (nodes that the query sees) to 16
+// columns from `col` on; those entries were zeroed for the product.
+template <bool QUANT>
+__device__ __noinline__ void tree_add_bad(float (&f)[16], unsigned long long bad, const KvView& c, int b, int h, int len, int col) {
+  for (; bad; bad &= bad - 1) {
+    const int j = __ffsll((long long)bad) - 1;
+    if (QUANT) {                             // the row's scale is NaN
+      for (int k = 0; k < 16; ++k) f[k] = __int_as_float(0x7fffffff);
+    } else {
+      const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(c.p[1] + b * c.b + h * c.h + ((long long)len + j) * c.t) + col;
+      for (int k = 0; k < 16; ++k) {
+        const float v = __bfloat162float(row[k]);
+        if (!(fabsf(v) < INFINITY)) f[k] += v;
+      }
+    }
+  }
+}
+
 template <int D, bool QUANT, int NT>
 struct TreeCfg {
   static constexpr uint32_t TILE = 128u * D * 2u;
   static constexpr uint32_t RAW = 128u * D;
-  static constexpr int QS = 2 / NT;            // stages of NT query tiles
-  static constexpr int NS = QUANT ? 3 : 5;     // bf16 key / value tiles
-  static constexpr int RS = QUANT ? 4 : 0;     // e4m3 key / value tiles
-  static constexpr int AUX = QUANT ? 4 : 1;    // warps that convert, or clear unused rows
-  static constexpr int THREADS = 32 * (2 + 4 * NT + AUX);
-  static constexpr size_t SMEM = 1024 + 2 * TILE + NS * TILE + RS * RAW + 40 * 8 + kSegRing * 8 + 16;
-  static constexpr int LEAD = NT == 1 ? 2 : 1; // key tiles ahead of the first value tile
+  static constexpr int NK = QUANT ? 2 : 3;                      // bf16 key tiles
+  static constexpr int NV = QUANT ? 3 - NT : 4 - NT;            // bf16 value tiles
+  static constexpr int NR = QUANT ? 2 : 0;                      // e4m3 tiles of either kind
+  static constexpr int AUX = QUANT ? 8 : 1;                     // warps that convert, or clear unused rows
+  static constexpr int THREADS = 32 * (3 + 8 + AUX);
+  static constexpr int BARS = 48;
+  static constexpr size_t SMEM = (NT + NK + NV) * TILE + 2 * NR * RAW + BARS * 8 + kSegRing * 8 + kLineRing * kTreeNodes * 8 + kLenCache * 4 + 16;
 };
-static_assert(TreeCfg<128, false, 1>::SMEM <= 232448 && TreeCfg<128, true, 1>::SMEM <= 232448, "shared memory");
+static_assert(TreeCfg<128, false, 1>::SMEM <= 232448 && TreeCfg<128, true, 1>::SMEM <= 232448 && TreeCfg<128, false, 2>::SMEM <= 232448 &&
+              TreeCfg<128, true, 2>::SMEM <= 232448, "shared memory");
 
-// Roles: warp 0 loads (TMA), warp 1 issues the products, NT groups of four warps run the softmax
-// of a row tile each, the rest converts quantised tiles or clears unused rows of value tiles.
-// Key and value tiles share one ring in the order in which the products take them.
-//   NT = 1: S is double-buffered in TMEM (S(g + 2) is issued behind P(g) V(g)), so the softmax
-//           never waits for a product.  TMEM: S 2 x 128 | O 128.
-//   NT = 2: one S a row tile; the tiles alternate.  TMEM: S 2 x 128 | O 2 x 128.
-// P overwrites the first 64 columns of its S as packed bf16 pairs.
+// Roles: warp 0 loads (TMA: one lane keys and queries, one values), warps 1 and 2 issue the products of a group each, two groups of four warps run the
+// softmax, the rest converts quantised tiles or clears unused rows of value tiles.  A group works
+// through half tiles of 64 keys:
+//   NT = 2: group t has row tile t and takes both halves of every key tile in turn;
+//   NT = 1: both groups have the one row tile, group t half t of every key tile, each with a
+//           maximum, sum and O of its own; at the end of a segment group 0 adds group 1's.
+// A group's S is double-buffered in TMEM: S(i + 2) is issued behind P(i) V(i), so the softmax never
+// waits for a product, and its 64 scores a row stay in registers from the maximum to the
+// exponentials.  (With 128-key tiles and one S a group, each tile's chain S -> softmax -> P V ran
+// serially, 4300 cycles for what the softmax needs 2300 of.)
+// TMEM: group t's S at 128 t + 64 (i & 1), P over its first 32 columns; O at 256 + 128 t.
 template <int D, bool QUANT, int NT>
 __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                          const __grid_constant__ CUtensorMap tmV, const TreeArgs a, const KvView c) {
+                          const __grid_constant__ CUtensorMap tmV, const TreeArgs a, const __grid_constant__ KvView c) {
   using Cfg = TreeCfg<D, QUANT, NT>;
   constexpr uint32_t TILE = Cfg::TILE, RAW = Cfg::RAW;
-  constexpr int NS = Cfg::NS, RS = Cfg::RS, QS = Cfg::QS, LEAD = Cfg::LEAD;
+  constexpr int NK = Cfg::NK, NV = Cfg::NV, NR = Cfg::NR;
   constexpr int PANELS = D / 64;
-  constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, false, false);
+  constexpr int NH = NT;                       // half tiles of a key tile that a group takes
+  constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 64, false, false);
   constexpr uint32_t IDESC_O = umma_idesc_bf16(128, D, false, true);
 
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                          // [2] tiles: QS stages of NT
-  uint8_t* sKV = sQ + 2 * TILE;                // [NS] tiles
-  uint8_t* sRaw = sKV + NS * TILE;             // [RS] tiles
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + RS * RAW);
-  uint64_t* q_full = bars;                     // [2]
-  uint64_t* q_empty = bars + 2;                // [2]
-  uint64_t* kv_full = bars + 4;                // [NS <= 5]
-  uint64_t* kv_empty = bars + 9;               // [NS]
-  uint64_t* v_ready = bars + 14;               // [NS] value tiles whose unused rows are cleared (not QUANT)
-  uint64_t* raw_full = bars + 19;              // [RS <= 4]
-  uint64_t* raw_empty = bars + 23;             // [RS]
-  uint64_t* s_full = bars + 27;                // [2]
-  uint64_t* p_full = bars + 29;                // [2]
-  uint64_t* pv_done = bars + 31;               // [2]
-  uint64_t* drain = bars + 33;
-  // value tiles land on a barrier of their own (not QUANT): the warp that waits for them waits for
-  // no key tile, and a wait by parity must see every phase of its barrier
-  uint64_t* v_full = bars + 34;                // [NS]
-  unsigned long long* s_poison = reinterpret_cast<unsigned long long*>(bars + 40);   // [kSegRing] drafted rows not finite
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_poison + kSegRing);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0) {         // the swizzled tiles need it
+    if (threadIdx.x == 0) atomicOr(a.err, ERR_BAD_ARG);
+    return;
+  }
+  uint8_t* sQ = smem;                          // [NT] tiles
+  uint8_t* sK = sQ + NT * TILE;                // [NK]
+  uint8_t* sV = sK + NK * TILE;                // [NV]
+  uint8_t* sRaw = sV + NV * TILE;              // [2][NR]: keys, values
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + 2 * NR * RAW);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;                 // [NK <= 3]
+  uint64_t* k_empty = bars + 5;                // [NK]
+  uint64_t* v_full = bars + 8;                 // [NV <= 3]
+  uint64_t* v_empty = bars + 11;               // [NV]
+  uint64_t* v_ready = bars + 14;               // [NV] value tiles whose unused rows are cleared (not QUANT)
+  uint64_t* raw_full = bars + 17;              // [2][NR]
+  uint64_t* raw_empty = bars + 21;             // [2][NR]
+  uint64_t* s_full = bars + 25;                // [2 groups][2 buffers]
+  uint64_t* p_full = bars + 29;                // [2][2]
+  uint64_t* pv_done = bars + 33;               // [2][2]
+  uint64_t* line_full = bars + 37;             // [kLineRing]
+  uint64_t* ml_full = bars + 41;               // group 1's maximum and sum are written, its O is done (NT = 1)
+  uint64_t* o_free = bars + 42;                // group 0 has read them (NT = 1)
+  uint64_t* drain = bars + 43;                 // [2]
+  unsigned long long* s_poison = reinterpret_cast<unsigned long long*>(bars + Cfg::BARS);   // [kSegRing] drafted rows not finite
+  unsigned long long* s_line = s_poison + kSegRing;                                         // [kLineRing][kTreeNodes]
+  int* s_len = reinterpret_cast<int*>(s_line + kLineRing * kTreeNodes);                     // [kLenCache]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_len + kLenCache);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 2);
+    for (int i = 0; i < NK; ++i) {
+      mbar_init(&k_full[i], QUANT ? 128 : 1);
+      mbar_init(&k_empty[i], 2);
+    }
+    for (int i = 0; i < NV; ++i) {
+      mbar_init(&v_full[i], QUANT ? 128 : 1);
+      mbar_init(&v_empty[i], 2);
+      mbar_init(&v_ready[i], 32);
+    }
+    for (int i = 0; i < 2 * NR; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 128);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
       mbar_init(&pv_done[i], 1);
     }
-    for (int i = 0; i < NS; ++i) {
-      mbar_init(&kv_full[i], QUANT ? 128 : 1);
-      mbar_init(&kv_empty[i], 1);
-      mbar_init(&v_ready[i], 32);
-      mbar_init(&v_full[i], 1);
-    }
-    for (int i = 0; i < RS; ++i) {
-      mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 128);
-    }
-    mbar_init(drain, 1);
+    for (int i = 0; i < kLineRing; ++i) mbar_init(&line_full[i], 32);
+    mbar_init(ml_full, 128);
+    mbar_init(o_free, 128);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     for (int i = 0; i < kSegRing; ++i) s_poison[i] = 0;
     *abort_flag = 0;
     fence_barrier_init();
@@ -317,449 +406,443 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  long long total;
-  TreeIter it = tree_begin(a, c, (int)blockIdx.x, (int)gridDim.x, total);
-  const int tiles = (int)(it.end - it.pos);    // of this CTA
+  const TreeLens lens{a.lens, a.B <= kLenCache ? s_len : nullptr, a.N, c.tmax};
+  if (threadIdx.x >= 64)
+    for (int i = (int)threadIdx.x - 64; i < a.B && i < kLenCache; i += (int)blockDim.x - 64) s_len[i] = max(0, min(a.lens[i], c.tmax));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   griddep_launch_dependents();
+  TreeIter it = tree_begin(a, lens, (int)blockIdx.x, (int)gridDim.x);
+  const int tiles = it.end - it.pos;           // of this CTA
   const uint32_t tmem = *tmem_slot;
-  constexpr uint32_t O_COL = 256;
-  // position in the ring of the value tile of tile g
-  auto v_item = [&](int g) { return NT == 1 ? min(2 * g + 2, 2 * tiles - 1) : 2 * g + 1; };
 
   if (warp == 0) {
-    // ------------------------------------------------------------------ loads
-    if (lane == 0 && tiles > 0) {
+    // ------------------------------------------------------------------ loads: lane 0 keys and queries, lane 1 values
+    if (lane < 2 && tiles > 0) {
+      const int v = lane, R = QUANT ? NR : v ? NV : NK;
+      const CUtensorMap* map = v ? &tmV : &tmK;
+      uint64_t* const full = QUANT ? raw_full + v * NR : v ? v_full : k_full;
+      uint64_t* const empty = QUANT ? raw_empty + v * NR : v ? v_empty : k_empty;
+      uint8_t* const dst = QUANT ? sRaw + v * NR * RAW : v ? sV : sK;
       bool ok = true;
-      int item = 0, q_segs = 0;
-      uint64_t* const empty = QUANT ? raw_empty : kv_empty;
-      constexpr int R = QUANT ? RS : NS;
-      uint32_t is_v = 0, phase[2] = {0, 0};     // per slot: what it holds, and the parities of its barriers
-      auto full = [&](int slot, int v) { return QUANT ? &raw_full[slot] : v ? &v_full[slot] : &kv_full[slot]; };
-      auto tile = [&](const TreeIter& t, int v) -> bool {
-        const int slot = item % R;
-        if (item >= R && !mbar_wait(&empty[slot], ((item / R) + 1) & 1, abort_flag, a.err, ERR_TIMEOUT_PRODUCER)) return false;
-        uint64_t* bar = full(slot, v);
-        const CUtensorMap* map = v ? &tmV : &tmK;
-        mbar_arrive_expect_tx(bar, QUANT ? RAW : TILE);
-        is_v = (is_v & ~(1u << slot)) | ((uint32_t)v << slot);
-        phase[QUANT ? 0 : v] ^= 1u << slot;
-        if constexpr (QUANT) {
-          tma_load_4d(sRaw + slot * RAW, map, bar, 0, t.k * 128, t.h, t.b);
-        } else {
-#pragma unroll
-          for (int p = 0; p < PANELS; ++p)
-            tma_load_4d(sKV + slot * TILE + p * kTreePanel, map, bar, p * 64, t.k * 128, t.h, t.b);
-        }
-        ++item;
-        return true;
-      };
+      int g = 0, segs = 0;                     // tiles begun, query tiles begun
       auto queries = [&](const TreeIter& t) -> bool {
-        const int st = t.seg % QS;
-        if (t.seg >= QS && !mbar_wait(&q_empty[st], ((t.seg / QS) + 1) & 1, abort_flag, a.err, ERR_TIMEOUT_PRODUCER)) return false;
-        mbar_arrive_expect_tx(&q_full[st], (uint32_t)(NT * PANELS * a.gb * a.nb) * 128u);
+        if (segs > 0 && !mbar_wait(q_empty, (segs + 1) & 1, abort_flag, a.err, ERR_TIMEOUT_PRODUCER)) return false;
+        mbar_arrive_expect_tx(q_full, (uint32_t)(NT * PANELS * a.gb * a.nb) * 128u);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           const int rt = t.rgi * NT + i;
           const int ng = rt / a.gg, hg = rt - ng * a.gg;
 #pragma unroll
           for (int p = 0; p < PANELS; ++p)
-            tma_load_5d(sQ + (st * NT + i) * TILE + p * kTreePanel, &tmQ, &q_full[st], p * 64, hg * a.gb, ng * a.nb, t.h, t.b);
+            tma_load_5d(sQ + i * TILE + p * kTreePanel, &tmQ, q_full, p * 64, hg * a.gb, ng * a.nb, t.h, t.b);
         }
-        q_segs = t.seg + 1;
+        ++segs;
         return true;
       };
-      TreeIter ki = it, vi = it;
-      auto key = [&]() -> bool {   // the next key tile, behind its queries; true also at the end
-        if (!ki.next(a, c)) return true;
-        if (ki.first() && !queries(ki)) return false;
-        return tile(ki, 0);
-      };
-      for (int i = 0; i < LEAD && ok; ++i) ok = key();
-      while (ok && vi.next(a, c)) ok = tile(vi, 1) && key();
+      while (it.next(lens, a.rg)) {
+        if (v == 0 && it.first() && !queries(it)) { ok = false; break; }
+        const int slot = g % R;
+        if (g >= R && !mbar_wait(&empty[slot], ((g / R) + 1) & 1, abort_flag, a.err, ERR_TIMEOUT_PRODUCER)) { ok = false; break; }
+        mbar_arrive_expect_tx(&full[slot], QUANT ? RAW : TILE);
+        if constexpr (QUANT) {
+          tma_load_4d(dst + slot * RAW, map, &full[slot], 0, it.k * 128, it.h, it.b);
+        } else {
+#pragma unroll
+          for (int p = 0; p < PANELS; ++p)
+            tma_load_4d(dst + slot * TILE + p * kTreePanel, map, &full[slot], p * 64, it.k * 128, it.h, it.b);
+        }
+        ++g;
+      }
       if (!ok) {   // let the copies in flight land before the CTA ends
         const unsigned long long t0 = globaltimer_ns();
-        for (int i = max(0, item - R); i < item; ++i) {
-          const int slot = i % R, v = (is_v >> slot) & 1;
-          while (!mbar_try_wait(full(slot, v), ((phase[QUANT ? 0 : v] >> slot) & 1) ^ 1))
+        for (int i = max(0, g - R); i < g; ++i)
+          while (!mbar_try_wait(&full[i % R], (i / R) & 1))
             if (globaltimer_ns() - t0 > 100000000ull) break;
-        }
-        for (int i = max(0, q_segs - QS); i < q_segs; ++i)
-          while (!mbar_try_wait(&q_full[i % QS], (i / QS) & 1))
+        if (segs > 0)
+          while (!mbar_try_wait(q_full, (segs - 1) & 1))
             if (globaltimer_ns() - t0 > 100000000ull) break;
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ products
-    if (lane == 0 && tiles > 0) {
-      bool ok = true;
-      uint32_t vphase = 0, kphase = 0;          // per slot (not QUANT: keys and values land on separate barriers)
-      TreeIter si[NT], pi[NT];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) si[i] = pi[i] = it;
-      int sg[NT] = {}, pg[NT] = {};
-      auto k_item = [&](int g) { return NT == 1 ? (g < 2 ? g : 2 * g - 1) : 2 * g; };
-      // S of the next tile of row tile t; true also at the end
-      auto scores = [&](int t) -> bool {
-        if (!si[t].next(a, c)) return true;
-        const int g = sg[t]++, kit = k_item(g), st = si[t].seg % QS;
-        if (si[t].first() && !mbar_wait(&q_full[st], (si[t].seg / QS) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
-        if (!mbar_wait(&kv_full[kit % NS], QUANT ? (kit / NS) & 1 : (kphase >> (kit % NS)) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA))
-          return false;
-        tc_fence_after();
-        const uint32_t q_addr = smem_u32(sQ + (st * NT + t) * TILE), k_addr = smem_u32(sKV + (kit % NS) * TILE);
-        const int buf = NT == 1 ? g & 1 : t;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tmem + buf * 128, tree_desc_k(q_addr, kk), tree_desc_k(k_addr, kk), IDESC_S, kk > 0 ? 1u : 0u);
-        umma_commit(&s_full[buf]);
-        if (t == NT - 1) {
-          kphase ^= 1u << (kit % NS);
-          umma_commit(&kv_empty[kit % NS]);
-          if (si[t].last()) umma_commit(&q_empty[st]);
-        }
-        return true;
-      };
-      auto outputs = [&](int t) -> bool {
-        pi[t].next(a, c);
-        const int g = pg[t]++, vit = v_item(g), slot = vit % NS, buf = NT == 1 ? g & 1 : t;
-        if (t == 0) {
-          if constexpr (QUANT) {
-            if (!mbar_wait(&kv_full[slot], (vit / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
-          } else {
-            if (!mbar_wait(&v_ready[slot], (vphase >> slot) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
-            vphase ^= 1u << slot;
+  } else if (warp <= 2) {
+    // ------------------------------------------------------------------ products of group t
+    if (tiles > 0) {   // the whole warp keeps the schedule (in uniform registers), one lane issues
+      const int t = warp - 1;
+      bool ok = true, more = true;
+      TreeIter si = it, pi = it;               // tiles of the scores and of the outputs
+      int ks = NK - 1, vs = NV - 1;            // their places in the rings, and the phases of those
+      uint32_t kph = 1, vph = 1;
+      const uint32_t qd = tree_desc_k(smem_u32(sQ)) + (NT == 1 ? 0u : (uint32_t)t * (TILE >> 4));
+      const uint32_t kd0 = tree_desc_k(smem_u32(sK)), vd0 = tree_desc_mn(smem_u32(sV));
+      const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
+      uint64_t* const in_v = QUANT ? v_full : v_ready;
+      // the scores of the group's half tile i; true also at the end
+      auto scores = [&](int i) -> bool {
+        const int half = NT == 1 ? t : i & 1, buf = i & 1;
+        if (NH == 1 || half == 0) {
+          more = more && si.next(lens, a.rg);
+          if (more) {
+            if (++ks == NK) { ks = 0; kph ^= 1; }
+            if (si.first() && !mbar_wait_warp(q_full, si.seg & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+            if (!mbar_wait_warp(&k_full[ks], kph, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+            tc_fence_after();
           }
         }
-        if (!mbar_wait(&p_full[buf], NT == 1 ? (g >> 1) & 1 : g & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
-        tc_fence_after();
-        const uint32_t v_addr = smem_u32(sKV + slot * TILE);
+        if (!more) return true;
+        const uint32_t kd = kd0 + (uint32_t)ks * (TILE >> 4) + (uint32_t)half * (8192u >> 4);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_bf16_tmem_a(tmem + O_COL + t * 128, tmem + buf * 128 + kk * 8, tree_desc_mn(v_addr, kk), IDESC_O,
-                           (!pi[t].first() || kk > 0) ? 1u : 0u);
-        if (t == NT - 1) umma_commit(&kv_empty[slot]);
-        umma_commit(&pv_done[buf]);
+          for (int kk = 0; kk < D / 16; ++kk)
+            tree_mma(tS + buf * 64, qd + tree_step_k(kk), kd + tree_step_k(kk), IDESC_S, kk > 0 ? 1u : 0u);
+          umma_commit(&s_full[t * 2 + buf]);
+          if (NH == 1 || half == 1) {
+            umma_commit(&k_empty[ks]);
+            if (si.last()) umma_commit(q_empty);
+          }
+        }
+        __syncwarp();
         return true;
       };
-      for (int i = 0; i < LEAD && ok; ++i)
+      auto outputs = [&](int i) -> bool {
+        const int half = NT == 1 ? t : i & 1, buf = i & 1;
+        if (NH == 1 || half == 0) {
+          pi.next(lens, a.rg);
+          if (++vs == NV) { vs = 0; vph ^= 1; }
+          if (!mbar_wait_warp(&in_v[vs], vph, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+        }
+        if (!mbar_wait_warp(&p_full[t * 2 + buf], (i >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+        tc_fence_after();
+        const uint32_t vd = vd0 + (uint32_t)vs * (TILE >> 4) + (uint32_t)half * tree_step_mn(4);
+        const uint32_t add = pi.first() && (NH == 1 || half == 0) ? 0u : 1u;
+        if (elect_one()) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) ok = ok && scores(t);
-      for (int g = 0; g < tiles && ok; ++g)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) ok = ok && outputs(t) && scores(t);
+          for (int kk = 0; kk < 4; ++kk) tree_mma_p(tO, tS + buf * 64 + kk * 8, vd + tree_step_mn(kk), IDESC_O, kk > 0 ? 1u : add);
+          if (NH == 1 || half == 1) umma_commit(&v_empty[vs]);
+          umma_commit(&pv_done[t * 2 + buf]);
+        }
+        __syncwarp();
+        return true;
+      };
+      ok = scores(0) && scores(1);
+      for (int i = 0; i < tiles * NH && ok; ++i) ok = outputs(i) && scores(i + 2);
       if (!ok) {
         *abort_flag = 1;
-        umma_commit(drain);
+        if (elect_one()) umma_commit(&drain[t]);
+        __syncwarp();
         const unsigned long long t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain, 0))
+        while (!mbar_try_wait(&drain[t], 0))
           if (globaltimer_ns() - t0 > 100000000ull) break;
       }
     }
-  } else if (warp < 2 + 4 * NT) {
-    // ------------------------------------------------------------------ softmax of row tile t
-    const int t = (warp - 2) >> 2, q4 = warp & 3, r = q4 * 32 + lane;
+  } else if (warp < 11) {
+    // ------------------------------------------------------------------ softmax, group t
+    const int t = (warp - 3) >> 2, q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
-    const uint32_t tO = tmem + O_COL + t * 128 + lane_off;
+    const uint32_t tO = tmem + 256 + t * 128 + lane_off;
     const float cl = a.scale_log2;
     const int rn = r / a.gb, rh = r - rn * a.gb;
     float m_run = -INFINITY, l = 0.f;
     unsigned long long line = 0;
-    int n = 0, head = 0, g = 0;
+    int n = 0, head = 0, i = 0;                // i: half tile of the group
     bool live = false, warp_live = false, ok = true;
-    while (ok && it.next(a, c)) {
+    while (ok && it.next(lens, a.rg)) {
       if (it.first()) {
-        const int rt = it.rgi * NT + t;
+        const int rt = it.rgi * NT + (NT == 1 ? 0 : t);
         const int ng = rt / a.gg, hg = rt - ng * a.gg;
         n = ng * a.nb + rn;
         head = hg * a.gb + rh;
         live = rn < a.nb && n < a.N && head < a.G && rt < a.rt;
         warp_live = __any_sync(0xffffffffu, live);
-        unsigned long long m0, m1;
-        tree_lines(a.parents ? a.parents + (long long)it.b * a.N : nullptr, a.N, c.tmax - it.len, m0, m1);
-        const unsigned long long x0 = __shfl_sync(0xffffffffu, m0, n & 31), x1 = __shfl_sync(0xffffffffu, m1, n & 31);
-        line = !live ? 0 : n >= 32 ? x1 : x0;
+        const int lr = it.seg & (kLineRing - 1);
+        if (!mbar_wait_warp(&line_full[lr], (it.seg / kLineRing) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+        line = live ? s_line[lr * kTreeNodes + n] : 0;
         m_run = -INFINITY;
         l = 0.f;
       }
-      const int buf = NT == 1 ? g & 1 : t, sph = NT == 1 ? (g >> 1) & 1 : g & 1;
-      const uint32_t tS = tmem + buf * 128 + lane_off;
-      if (!mbar_wait_warp(&s_full[buf], sph, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
-      // products into O up to tile g - 2 (NT = 1) or g - 1 were issued before S(g): these waits
-      // only keep count of the barrier's phases
-      if (NT == 1 ? g >= 2 : g >= 1) {
-        if (!mbar_wait_warp(&pv_done[buf], sph ^ 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
-      }
-      tc_fence_after();
-      if (warp_live) {
-        const int off = it.k * 128 - it.len;          // of the tile's first key from the first node's row
-        const bool masked = off + 128 > 0;
-        float x[64];
-        // half hf of the row of S: scaled by the sign, masked columns -inf
-        auto half_row = [&](int hf) {
-          uint32_t* xr = reinterpret_cast<uint32_t*>(x);
-          __syncwarp();
-          tmem_ld_32x32b_x32(tS + hf * 64, *reinterpret_cast<uint32_t(*)[32]>(xr));
-          tmem_ld_32x32b_x32(tS + hf * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(xr + 32));
-          tmem_ld_wait();
-          if (a.neg) {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) x[i] = -x[i];
-          }
-          if (masked) {
-            const uint32_t w0 = tree_word(line, off + hf * 64), w1 = tree_word(line, off + hf * 64 + 32);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (!((w0 >> i) & 1u)) x[i] = -INFINITY;
-              if (!((w1 >> i) & 1u)) x[32 + i] = -INFINITY;
-            }
-          }
-        };
-        auto half_max = [&](float mx) -> float {
-          float m4[4] = {mx, x[0], x[1], x[2]};
-#pragma unroll
-          for (int i = 3; i < 63; i += 4)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], x[i + k]);
-          return fmaxf(fmaxf(fmaxf(m4[0], x[63]), m4[1]), fmaxf(m4[2], m4[3]));
-        };
-        half_row(0);
-        float mx = half_max(-INFINITY);
-        half_row(1);
-        mx = half_max(mx) * cl;
-        // the exponents' reference moves only when the maximum grows by more than 8 (p stays below 2^8)
-        float alpha = 1.f;
-        const bool grow = live && mx > m_run + 8.f;
-        if (grow) {
-          alpha = tree_ex2(m_run - mx);
-          m_run = mx;
-        }
-        const float mref = m_run == -INFINITY ? 0.f : m_run;   // nothing seen so far: every p is 2^-inf = 0
-        const float2 c2 = make_float2(cl, cl), nm2 = make_float2(-mref, -mref);
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint32_t pk[2][32];
-        auto half_exp = [&](uint32_t (&p)[32]) {
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            const float2 v = __ffma2_rn(make_float2(x[i], x[i + 1]), c2, nm2);
-            const float2 e = make_float2(tree_ex2(v.x), tree_ex2(v.y));
-            p[i >> 1] = pack_bf16x2(e.x, e.y);
-            sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], e);
-          }
-        };
-        half_exp(pk[1]);
-        half_row(0);
-        half_exp(pk[0]);
-        const float2 s2 = __fadd2_rn(sum[0], sum[1]);
-        l = l * alpha + (s2.x + s2.y);
-        if (!it.first() && __any_sync(0xffffffffu, grow)) {
-          if (NT == 1 && !mbar_wait_warp(&pv_done[buf ^ 1], ((g - 1) >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
-          tc_fence_after();
 #pragma unroll 1
-          for (int cc = 0; cc < D / 32; ++cc) {
-            uint32_t o[32];
-            __syncwarp();
-            tmem_ld_32x32b_x32(tO + cc * 32, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st_32x32b_x32(tO + cc * 32, o);
-          }
-        }
-        __syncwarp();
-        tmem_st_32x32b_x32(tS, pk[0]);
-        tmem_st_32x32b_x32(tS + 32, pk[1]);
-        tmem_st_wait();
-        tc_fence_before();
-      }
-      mbar_arrive(&p_full[buf]);
-      if (it.last()) {
-        if (!mbar_wait_warp(&pv_done[buf], sph, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      for (int hf = 0; hf < NH; ++hf, ++i) {
+        const int half = NT == 1 ? t : hf, buf = i & 1, ph = (i >> 1) & 1;
+        const uint32_t tS = tmem + t * 128 + buf * 64 + lane_off;
+        // P(i - 2) V was issued before S(i): the second wait only keeps count of its barrier's phases
+        ok = mbar_wait(&s_full[t * 2 + buf], ph, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE) &&
+             (i < 2 || mbar_wait(&pv_done[t * 2 + buf], ph ^ 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE));
+        ok = __all_sync(0xffffffffu, ok) != 0;
+        if (!ok) break;
         tc_fence_after();
         if (warp_live) {
-          const bool whole = it.k0 == 0 && it.k1 == it.kt;
-          const long long slot = 2LL * blockIdx.x + (it.k0 == 0 ? 1 : 0);
-          const float inv = line == 0 || l == 0.f ? 0.f : 1.f / l;
-          unsigned long long bad = s_poison[it.seg & (kSegRing - 1)] & line;
-          __nv_bfloat16* dst = a.o + (((long long)it.b * a.N + n) * a.Hq + it.h * a.G + head) * D;
-          float* pd = a.part + ((slot * NT + t) * 128 + r) * D;
-#pragma unroll 1
-          for (int cc = 0; cc < D / 32; ++cc) {
-            uint32_t o[32];
+          const int off = it.k * 128 + half * 64 - it.len;   // of the first key from the first node's row
+          float x[64];
+          {
+            uint32_t* xr = reinterpret_cast<uint32_t*>(x);
             __syncwarp();
-            tmem_ld_32x32b_x32(tO + cc * 32, o);
+            tmem_ld_32x32b_x32(tS, *reinterpret_cast<uint32_t(*)[32]>(xr));
+            tmem_ld_32x32b_x32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(xr + 32));
             tmem_ld_wait();
-            float f[32];
+          }
+          if (a.neg) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = line != 0 && l != 0.f ? __uint_as_float(o[i]) : 0.f;
-            for (unsigned long long w = bad; w; w &= w - 1) {   // rows with an infinity or a NaN: those entries
-              const int j = __ffsll((long long)w) - 1;
-              if constexpr (QUANT) {
+            for (int k = 0; k < 64; ++k) x[k] = -x[k];
+          }
+          if (off + 64 > 0) {
+            const uint32_t w0 = tree_word(line, off), w1 = tree_word(line, off + 32);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) f[i] = __int_as_float(0x7fffffff);
-              } else {
-                const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(c.p[1] + it.b * c.b + it.h * c.h +
-                                                                                  ((long long)it.len + j) * c.t) + cc * 32;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  const float v = __bfloat162float(row[i]);
-                  if (!(fabsf(v) < INFINITY)) f[i] += v;
-                }
-              }
-            }
-            if (live) {
-              if (whole) {
-#pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                  uint4 u;
-                  u.x = pack_bf16x2(f[i] * inv, f[i + 1] * inv);
-                  u.y = pack_bf16x2(f[i + 2] * inv, f[i + 3] * inv);
-                  u.z = pack_bf16x2(f[i + 4] * inv, f[i + 5] * inv);
-                  u.w = pack_bf16x2(f[i + 6] * inv, f[i + 7] * inv);
-                  *reinterpret_cast<uint4*>(dst + cc * 32 + i) = u;
-                }
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; i += 4)
-                  *reinterpret_cast<float4*>(pd + cc * 32 + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-              }
+            for (int k = 0; k < 32; ++k) {
+              if (!((w0 >> k) & 1u)) x[k] = -INFINITY;
+              if (!((w1 >> k) & 1u)) x[32 + k] = -INFINITY;
             }
           }
-          if (live && !whole) a.part_ml[(slot * NT + t) * 128 + r] = line != 0 ? make_float2(m_run, l) : make_float2(-INFINITY, 0.f);
+          float m4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int k = 4; k < 64; k += 8)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m4[j] = fmaxf(fmaxf(m4[j], x[k + j]), k + 4 < 64 ? x[k + 4 + j] : x[k + j]);
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * cl;
+          // the exponents' reference moves only when the maximum grows by more than 8 (p stays below 2^8)
+          float alpha = 1.f;
+          const bool grow = live && mx > m_run + 8.f;
+          if (grow) {
+            alpha = tree_ex2(m_run - mx);
+            m_run = mx;
+          }
+          const float mref = m_run == -INFINITY ? 0.f : m_run;   // nothing seen so far: every p is 2^-inf = 0
+          const float2 c2 = make_float2(cl, cl), nm2 = make_float2(-mref, -mref);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t p[32];
+#pragma unroll
+          for (int k = 0; k < 64; k += 2) {
+            const float2 v = __ffma2_rn(make_float2(x[k], x[k + 1]), c2, nm2);
+            const float2 e = k < 48 ? make_float2(tree_ex2(v.x), tree_ex2(v.y)) : tree_exp2_pair(v);
+            p[k >> 1] = pack_bf16x2(e.x, e.y);   // P in 8 bits of significand for the product, its sum in 32 bits
+            sum[(k >> 1) & 1] = __fadd2_rn(sum[(k >> 1) & 1], e);
+          }
+          __syncwarp();
+          tmem_st_32x32b_x32(tS, p);
+          const float2 s2 = __fadd2_rn(sum[0], sum[1]);
+          l = l * alpha + (s2.x + s2.y);
+          if (!(it.first() && hf == 0) && __any_sync(0xffffffffu, grow)) {
+            if (!mbar_wait_warp(&pv_done[t * 2 + (buf ^ 1)], ((i - 1) >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll 1
+            for (int cc = 0; cc < D / 32; ++cc) {
+              uint32_t o[32];
+              __syncwarp();
+              tmem_ld_32x32b_x32(tO + cc * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              tmem_st_32x32b_x32(tO + cc * 32, o);
+            }
+          }
+          tmem_st_wait();
+          tc_fence_before();
         }
-        tc_fence_before();
+        // group 1's O of the segment before is still to be read
+        if (NT == 1 && t == 1 && it.first() && it.seg > 0 &&
+            !mbar_wait_warp(o_free, (it.seg - 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+        mbar_arrive(&p_full[t * 2 + buf]);
       }
-      ++g;
+      if (!ok || !it.last()) continue;
+      // end of the segment: O is complete
+      if (!mbar_wait_warp(&pv_done[t * 2 + ((i - 1) & 1)], ((i - 1) >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      tc_fence_after();
+      float2* other = a.pair_ml + (long long)blockIdx.x * 128 + r;
+      if (NT == 1 && t == 1) {
+        *other = make_float2(m_run, l);
+        tc_fence_before();
+        mbar_arrive(ml_full);
+        continue;
+      }
+      float f0 = 1.f, f1 = 0.f;
+      if constexpr (NT == 1) {
+        if (!mbar_wait_warp(ml_full, it.seg & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+        tc_fence_after();
+        const volatile float2* ov = other;
+        const float2 ml = make_float2(ov->x, ov->y);
+        // the two halves at the larger of their references; one that saw nothing counts nothing
+        const float mm = l == 0.f ? ml.x : ml.y == 0.f ? m_run : fmaxf(m_run, ml.x);
+        f0 = l == 0.f ? 0.f : tree_ex2(m_run - mm);
+        f1 = ml.y == 0.f ? 0.f : tree_ex2(ml.x - mm);
+        l = (l == 0.f ? 0.f : l * f0) + (ml.y == 0.f ? 0.f : ml.y * f1);
+        m_run = mm;
+      }
+      if (warp_live) {
+        const bool whole = it.k0 == 0 && it.k1 == it.kt;
+        const long long slot = 2LL * blockIdx.x + (it.k0 == 0 ? 1 : 0);
+        const float inv = line != 0 && l != 0.f ? 1.f / l : 0.f;
+        if (line == 0 || l == 0.f) f0 = f1 = 0.f;   // an unused node, or nothing seen
+        const unsigned long long bad = s_poison[it.seg & (kSegRing - 1)] & line;
+        __nv_bfloat16* dst = a.o + (((long long)it.b * a.N + n) * a.Hq + it.h * a.G + head) * D;
+        float4* pd = a.part + (slot * NT + (NT == 1 ? 0 : t)) * (D / 4) * 128 + r;
+        // a short loop: this code runs once a segment, and fetching it costs more than running it
+#pragma unroll 1
+        for (int cc = 0; cc < D / 16; ++cc) {
+          uint32_t o[16], o1[16];
+          float f[16];
+          __syncwarp();
+          tree_ld16(tO + cc * 16, o);
+          if constexpr (NT == 1) tree_ld16(tO + 128 + cc * 16, o1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            f[k] = f0 != 0.f ? __uint_as_float(o[k]) * f0 : 0.f;
+            if constexpr (NT == 1) f[k] += f1 != 0.f ? __uint_as_float(o1[k]) * f1 : 0.f;
+          }
+          if (bad) tree_add_bad<QUANT>(f, bad, c, it.b, it.h, it.len, cc * 16);
+          if (!live) continue;
+          if (whole) {
+            uint4* d4 = reinterpret_cast<uint4*>(dst + cc * 16);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              d4[k] = make_uint4(pack_bf16x2(f[8 * k] * inv, f[8 * k + 1] * inv), pack_bf16x2(f[8 * k + 2] * inv, f[8 * k + 3] * inv),
+                                 pack_bf16x2(f[8 * k + 4] * inv, f[8 * k + 5] * inv), pack_bf16x2(f[8 * k + 6] * inv, f[8 * k + 7] * inv));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) pd[(cc * 4 + k) * 128] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+          }
+        }
+        if (live && !whole) a.part_ml[(slot * NT + (NT == 1 ? 0 : t)) * 128 + r] = line != 0 ? make_float2(m_run, l) : make_float2(-INFINITY, 0.f);
+      }
+      tc_fence_before();
+      if (NT == 1) mbar_arrive(o_free);
     }
   } else {
     // ------------------------------------------------------------------ e4m3 -> bf16, unused rows
-    const int tid = (int)threadIdx.x - 32 * (2 + 4 * NT);
+    const int tid = (int)threadIdx.x - 352;
     unsigned long long used = 0;
-    int used_seg = -1;
-    auto enter = [&](const TreeIter& v) {       // a value tile's segment (warp-collective)
-      if (v.seg == used_seg) return;
-      used_seg = v.seg;
+    // a value tile's segment (warp-collective): which drafted rows are used, and the lines for the softmax
+    auto enter = [&](const TreeIter& v, bool publish) {
       unsigned long long m0, m1;
       tree_lines(a.parents ? a.parents + (long long)v.b * a.N : nullptr, a.N, c.tmax - v.len, m0, m1);
       used = used_nodes(m0, m1);
-      if (tid == 0) s_poison[(v.seg + 3) & (kSegRing - 1)] = 0;   // last used five segments ago
+      if (publish) {
+        const int lr = v.seg & (kLineRing - 1);
+        s_line[lr * kTreeNodes + lane] = m0;
+        s_line[lr * kTreeNodes + 32 + lane] = m1;
+        if (lane == 0) s_poison[(v.seg + 3) & (kSegRing - 1)] = 0;   // last used five segments ago
+        mbar_arrive(&line_full[lr]);
+      }
     };
     if constexpr (!QUANT) {
       constexpr int CH = D / 8;                 // 16-byte chunks a row
-      int g = 0;
-      uint32_t vphase = 0;
-      while (it.next(a, c)) {
-        enter(it);
-        const int slot = v_item(g++) % NS;
-        if (!mbar_wait_warp(&v_full[slot], (vphase >> slot) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) break;
-        vphase ^= 1u << slot;
+      for (int g = 0; it.next(lens, a.rg); ++g) {
+        if (it.first()) enter(it, true);
+        const int slot = g % NV;
+        if (!mbar_wait_warp(&v_full[slot], (g / NV) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) break;
         const int off = it.k * 128 - it.len;
         if (off + 128 > 0) {
-          uint8_t* tile = sKV + slot * TILE;
+          uint8_t* tile = sV + slot * TILE;
           unsigned long long bad = 0;
-          for (int row = max(0, -off) + lane / CH; row < 128; row += 32 / CH) {
-            const int j = row + off, ch = lane % CH;
-            uint4* p = reinterpret_cast<uint4*>(tile + (ch >> 3) * kTreePanel + sw128_chunk_offset(row, ch & 7));
-            if (j >= kTreeNodes || !((used >> j) & 1)) {
-              *p = make_uint4(0, 0, 0, 0);
-            } else {
-              uint4 u = *p;
-              uint32_t* w = reinterpret_cast<uint32_t*>(&u);
-              bool hit = false;
+          const int ch = lane % CH, r0 = max(0, -off);
+          const int nodes = min(128, max(r0, a.N - off));      // rows from r0 to here are nodes', those behind nobody's
+          auto at = [&](int row) { return reinterpret_cast<uint4*>(tile + (ch >> 3) * kTreePanel + sw128_chunk_offset(row, ch & 7)); };
+#pragma unroll 8
+          for (int row = nodes + lane / CH; row < 128; row += 32 / CH) *at(row) = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+          for (int row = r0 + lane / CH; row < nodes; row += 32 / CH) {
+            const int j = row + off;
+            uint4 u = *at(row);
+            uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+            bool hit = false;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                if ((w[i] & 0x7f80u) == 0x7f80u) { w[i] &= 0xffff0000u; hit = true; }
-                if ((w[i] & 0x7f800000u) == 0x7f800000u) { w[i] &= 0xffffu; hit = true; }
-              }
-              if (hit) {
-                *p = u;
-                bad |= 1ull << j;
-              }
+            for (int i = 0; i < 4; ++i) {
+              if ((w[i] & 0x7f80u) == 0x7f80u) { w[i] &= 0xffff0000u; hit = true; }
+              if ((w[i] & 0x7f800000u) == 0x7f800000u) { w[i] &= 0xffffu; hit = true; }
             }
+            if (!((used >> j) & 1)) u = make_uint4(0, 0, 0, 0);
+            else if (hit) bad |= 1ull << j;
+            if (hit || !((used >> j) & 1)) *at(row) = u;
           }
-          uint32_t lo = __reduce_or_sync(0xffffffffu, (uint32_t)bad), hi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32));
+          const uint32_t lo = __reduce_or_sync(0xffffffffu, (uint32_t)bad), hi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32));
           if (lane == 0 && (lo | hi)) s_poison[it.seg & (kSegRing - 1)] |= ((unsigned long long)hi << 32) | lo;
           fence_proxy_async_smem();
         }
         mbar_arrive(&v_ready[slot]);
       }
     } else {
-      // chunk q of a tile: 16 codes of row q / CH; a thread's rows are tid / CH + i * (128 / CH)
-      constexpr int CH = D / 16, RPT = CH;      // chunks a row = rows a thread
-      const int ch = tid % CH, row0 = tid / CH;
-      constexpr int STEP = 128 / CH;
-      TreeIter ki = it, vi = it;
-      int item = 0;
-      uint32_t sc[RPT];
-      auto scales = [&](const TreeIter& x, int kv) {
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-          const long long tt = (long long)x.k * 128 + row0 + i * STEP;
-          sc[i] = tt < c.tmax ? c.s[kv][x.b * c.sb + x.h * c.sh + tt * c.st] : 127u;
-        }
-      };
-      auto convert = [&](const TreeIter& x, int kv) -> bool {
-        const int rslot = item % RS, slot = item % NS;
-        if (!mbar_wait_warp(&raw_full[rslot], (item / RS) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) return false;
-        if (item >= NS && !mbar_wait_warp(&kv_empty[slot], ((item / NS) + 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) return false;
-        const uint8_t* src = sRaw + rslot * RAW;
-        uint8_t* dst = sKV + slot * TILE + (ch >> 2) * kTreePanel;
-        const int off = x.k * 128 - x.len;
+      // four warps convert the keys, four the values; a thread has 16 codes of each of its rows,
+      // row0 + i * STEP, whose scales are fetched while the tile before is converted
+      constexpr int CH = D / 16, STEP = 128 / CH, RPT = CH;
+      const int v = tid >> 7, ch = tid % CH, row0 = (tid & 127) / CH;
+      const int R = v ? NV : NK;
+      uint64_t* const out_full = v ? v_full : k_full;
+      uint64_t* const out_empty = v ? v_empty : k_empty;
+      const uint8_t* sb = c.s[v];
+      uint32_t ahead[RPT];
+      TreeIter nx = it;                         // one tile ahead of `it`
+      auto scales = [&]() {
+        const uint8_t* p = sb + nx.b * c.sb + nx.h * c.sh + (long long)nx.k * 128 * c.st;
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
           const int row = row0 + i * STEP;
-          const uint4 u = *reinterpret_cast<const uint4*>(src + row * D + ch * 16);
-          uint32_t e = sc[i];
-          bool clear = false;
-          if (kv == 1 && row + off >= 0) {      // behind the context
-            const int j = row + off;
-            clear = j >= kTreeNodes || !((used >> j) & 1);
-            if (!clear && e == (uint32_t)kScaleNan) {
-              clear = true;
-              if (ch == 0) atomicOr(&s_poison[x.seg & (kSegRing - 1)], 1ull << j);
-            }
-          }
-          const __nv_bfloat162 m1 = bf16x2_bits(e == (uint32_t)kScaleNan ? 0x7fffu : min(e + 120u, 254u) << 7);
-          const uint2 p0 = codes4(u.x, m1), p1 = codes4(u.y, m1), p2 = codes4(u.z, m1), p3 = codes4(u.w, m1);
-          uint4 o0 = make_uint4(p0.x, p0.y, p1.x, p1.y), o1 = make_uint4(p2.x, p2.y, p3.x, p3.y);
-          if (e > 134u && e != (uint32_t)kScaleNan) {   // scales above 2^7
-            const __nv_bfloat162 m2 = bf16x2_bits((e - 7u) << 7);
-            uint32_t* w0 = reinterpret_cast<uint32_t*>(&o0);
-            uint32_t* w1 = reinterpret_cast<uint32_t*>(&o1);
+          ahead[i] = nx.k * 128 + row < c.tmax ? p[row * c.st] : 127u;
+        }
+      };
+      if (nx.next(lens, a.rg)) scales();
+      for (int g = 0; it.next(lens, a.rg); ++g) {
+        if (it.first() && v) enter(it, tid == 128 + lane);
+        const int off = it.k * 128 - it.len;
+        // factors of the rows: 2^120 times the scale (0 for a row that nothing may see); scales above
+        // 2^7 take a second one
+        uint32_t e[RPT];
+        bool wide = false;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const __nv_bfloat162 y0 = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&w0[k]), m2);
-              const __nv_bfloat162 y1 = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&w1[k]), m2);
-              w0[k] = *reinterpret_cast<const uint32_t*>(&y0);
-              w1[k] = *reinterpret_cast<const uint32_t*>(&y1);
+        for (int i = 0; i < RPT; ++i) {
+          e[i] = ahead[i];
+          wide |= e[i] > 134u && e[i] != (uint32_t)kScaleNan;
+        }
+        uint32_t m1[RPT];
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) m1[i] = e[i] == (uint32_t)kScaleNan ? 0x7fffu : min(e[i] + 120u, 254u) << 7;
+        if (v && off + 128 > 0) {
+#pragma unroll
+          for (int i = 0; i < RPT; ++i) {
+            const int j = row0 + i * STEP + off;
+            if (j < 0) continue;
+            const bool seen = j < kTreeNodes && ((used >> j) & 1);
+            if (seen && e[i] == (uint32_t)kScaleNan && ch == 0) atomicOr(&s_poison[it.seg & (kSegRing - 1)], 1ull << j);
+            if (!seen || e[i] == (uint32_t)kScaleNan) m1[i] = 0;
+          }
+        }
+        if (nx.next(lens, a.rg)) scales();
+        const int rslot = g % NR, slot = g % R;
+        if (!mbar_wait_warp(&raw_full[v * NR + rslot], (g / NR) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) break;
+        const uint8_t* src = sRaw + (v * NR + rslot) * RAW + row0 * D + ch * 16;
+        if (g >= R && !mbar_wait_warp(&out_empty[slot], ((g / R) + 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) break;
+        uint8_t* dst = (v ? sV : sK) + slot * TILE + (ch >> 2) * kTreePanel;
+        // the two panels' lanes store their two chunks in opposite order: no bank is hit twice
+        const bool swap = ch >= 4;
+        const int c0 = 2 * (ch & 3) + (swap ? 1 : 0);
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src + i * STEP * D);
+          const __nv_bfloat162 f = bf16x2_bits(m1[i]);
+          const uint2 p0 = codes4(u.x, f), p1 = codes4(u.y, f), p2 = codes4(u.z, f), p3 = codes4(u.w, f);
+          const uint4 o0 = make_uint4(p0.x, p0.y, p1.x, p1.y), o1 = make_uint4(p2.x, p2.y, p3.x, p3.y);
+          const int row = row0 + i * STEP;
+          *reinterpret_cast<uint4*>(dst + sw128_chunk_offset(row, c0)) = swap ? o1 : o0;
+          *reinterpret_cast<uint4*>(dst + sw128_chunk_offset(row, c0 ^ 1)) = swap ? o0 : o1;
+        }
+        if (__any_sync(0xffffffffu, wide)) {
+#pragma unroll 1
+          for (int i = 0; i < RPT; ++i) {
+            uint32_t ei = 127u;
+#pragma unroll
+            for (int k = 0; k < RPT; ++k) ei = k == i ? e[k] : ei;
+            if (ei <= 134u || ei == (uint32_t)kScaleNan) continue;
+            const __nv_bfloat162 f = bf16x2_bits((ei - 7u) << 7);
+            for (int k = 0; k < 2; ++k) {
+              uint32_t* w = reinterpret_cast<uint32_t*>(dst + sw128_chunk_offset(row0 + i * STEP, c0 ^ k));
+              for (int q = 0; q < 4; ++q) {
+                const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[q]), f);
+                w[q] = *reinterpret_cast<const uint32_t*>(&y);
+              }
             }
           }
-          if (clear) o0 = o1 = make_uint4(0, 0, 0, 0);
-          const int c0 = 2 * (ch & 3);
-          // the two panels' lanes store their chunks in opposite order: no bank is hit twice
-          const bool swap = ch >= 4;
-          *reinterpret_cast<uint4*>(dst + sw128_chunk_offset(row, swap ? c0 + 1 : c0)) = swap ? o1 : o0;
-          *reinterpret_cast<uint4*>(dst + sw128_chunk_offset(row, swap ? c0 : c0 + 1)) = swap ? o0 : o1;
         }
         fence_proxy_async_smem();
-        mbar_arrive(&kv_full[slot]);
-        mbar_arrive(&raw_empty[rslot]);
-        ++item;
-        return true;
-      };
-      bool ok = true;
-      auto key = [&]() -> bool {
-        if (!ki.next(a, c)) return true;
-        scales(ki, 0);
-        return convert(ki, 0);
-      };
-      for (int i = 0; i < LEAD && ok; ++i) ok = key();
-      while (ok && vi.next(a, c)) {
-        enter(vi);
-        scales(vi, 1);
-        ok = convert(vi, 1) && key();
+        mbar_arrive(&out_full[slot]);
+        mbar_arrive(&raw_empty[v * NR + rslot]);
       }
     }
   }
@@ -771,60 +854,89 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
   }
 }
 
-// Adds the parts of the units that more than one CTA worked on: one warp a query row.
+// Adds the parts of the units that more than one CTA worked on.  A CTA has RP neighbouring rows
+// of a row tile (RP: the rows of the tile, at most 32, rounded up to a power of two); the lanes of
+// a warp are RP rows x 32 / RP parts, its warps share the D / 4 columns of four.  Parts are added
+// lane by lane and then by a fixed tree over the lanes, so the order never changes.
 template <int D>
-__global__ void __launch_bounds__(128) tree_combine_kernel(const TreeArgs a, const KvView c, int grid, int NT) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const bool on = w < (long long)a.B * a.N * a.Hq;
-  long long c0 = 0, c1 = 0;
-  int row = 0;
-  if (on) {
-    const int hq = (int)(w % a.Hq), n = (int)(w / a.Hq % a.N), b = (int)(w / a.Hq / a.N);
-    const int h = hq / a.G, hd = hq - h * a.G, units = a.Hkv * a.rg;
-    long long all = 0, before = 0;
-    for (int i = lane; i < a.B; i += 32) {
-      const long long k = tree_tiles(a, c, i);
-      all += k;
-      if (i < b) before += k;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      all += __shfl_xor_sync(0xffffffffu, all, o);
-      before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    const int rt = (n / a.nb) * a.gg + hd / a.gb;
-    row = (rt % NT) * 128 + (n % a.nb) * a.gb + hd % a.gb;
-    const long long W = all * units, kt = tree_tiles(a, c, b);
-    grid = (int)min((long long)grid, W);
-    const long long p0 = before * units + (long long)(h * a.rg + rt / NT) * kt;
-    c0 = ((p0 + 1) * grid - 1) / W;          // the CTA that owns a position of the line
-    c1 = ((p0 + kt) * grid - 1) / W;
+__global__ void __launch_bounds__(128) tree_combine_kernel(const TreeArgs a, const KvView c, int grid, int NT, int RP, int blocks) {
+  constexpr int Q = D / 16;                  // columns of four a warp
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int blk = (int)(blockIdx.x % blocks);
+  long long u = blockIdx.x / blocks;
+  const int rt = (int)(u % a.rt);
+  u /= a.rt;
+  const int h = (int)(u % a.Hkv), b = (int)(u / a.Hkv), units = a.Hkv * a.rg;
+  const TreeLens lens{a.lens, nullptr, a.N, c.tmax};
+  int all = 0, before = 0;
+  for (int i = lane; i < a.B; i += 32) {
+    const int k = lens.tiles(i);
+    all += k;
+    if (i < b) before += k;
   }
+  all = __reduce_add_sync(0xffffffffu, all);
+  before = __reduce_add_sync(0xffffffffu, before);
+  const unsigned W = (unsigned)(all * units), kt = (unsigned)lens.tiles(b), G = min((unsigned)grid, W);
+  const unsigned p0 = (unsigned)(before * units) + (unsigned)(h * a.rg + rt / NT) * kt;
+  const int c0 = (int)(((p0 + 1) * G - 1) / W), c1 = (int)(((p0 + kt) * G - 1) / W);   // CTAs that own the unit's ends
   griddep_wait();                            // every thread: this grid ends after the one before it
-  if (!on || c0 == c1) return;               // one CTA had the whole unit and wrote it
+  if (c0 == c1) return;                      // one CTA had the whole unit and wrote it
+  const int PS = 32 / RP, ps = lane / RP, r = blk * RP + lane % RP;
+  const int ng = rt / a.gg, hg = rt - ng * a.gg, rn = r / a.gb, rh = r - rn * a.gb;
+  const int n = ng * a.nb + rn, head = hg * a.gb + rh;
+  const bool live = r < 128 && rn < a.nb && n < a.N && head < a.G;
   // CTA c0 ends with this unit's first part (slot 1), the others begin with theirs (slot 0)
+  auto place = [&](int i) { return (2LL * i + (i == c0 ? 1 : 0)) * NT + rt % NT; };
   float M = -INFINITY;
-  for (long long i = c0; i <= c1; ++i) {
-    const float2 ml = __ldcg(&a.part_ml[(2 * i + (i == c0 ? 1 : 0)) * NT * 128 + row]);
-    if (ml.y != 0.f) M = fmaxf(M, ml.x);
-  }
-  float acc[E] = {}, L = 0.f;
-  for (long long i = c0; i <= c1; ++i) {
-    const long long at = (2 * i + (i == c0 ? 1 : 0)) * NT * 128 + row;
-    const float2 ml = __ldcg(&a.part_ml[at]);
-    if (ml.y == 0.f) continue;
-    const float f = tree_ex2(ml.x - M);
-    L += f * ml.y;
-    const float* p = a.part + at * D + lane * E;
+  if (live)
+    for (int i = c0 + ps; i <= c1; i += PS) {
+      const float2 ml = __ldcg(&a.part_ml[place(i) * 128 + r]);
+      if (ml.y != 0.f) M = fmaxf(M, ml.x);
+    }
+  for (int o = RP; o < 32; o *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float4 acc[Q];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += f * __ldcg(p + e);
+  for (int q = 0; q < Q; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float L = 0.f;
+  if (live) {
+#pragma unroll 2
+    for (int i = c0 + ps; i <= c1; i += PS) {
+      const float2 ml = __ldcg(&a.part_ml[place(i) * 128 + r]);
+      const float4* p = a.part + (place(i) * (D / 4) + warp * Q) * 128 + r;
+      float4 v[Q];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) v[q] = __ldcg(p + q * 128);
+      if (ml.y == 0.f) continue;             // the row saw nothing there
+      const float f = tree_ex2(ml.x - M);
+      L += f * ml.y;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        acc[q].x += f * v[q].x; acc[q].y += f * v[q].y; acc[q].z += f * v[q].z; acc[q].w += f * v[q].w;
+      }
+    }
   }
+  for (int o = RP; o < 32; o *= 2) {
+    L += __shfl_xor_sync(0xffffffffu, L, o);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      acc[q].x += __shfl_xor_sync(0xffffffffu, acc[q].x, o);
+      acc[q].y += __shfl_xor_sync(0xffffffffu, acc[q].y, o);
+      acc[q].z += __shfl_xor_sync(0xffffffffu, acc[q].z, o);
+      acc[q].w += __shfl_xor_sync(0xffffffffu, acc[q].w, o);
+    }
+  }
+  if (!live || ps != 0) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  __nv_bfloat16* dst = a.o + w * D + lane * E;
+  __nv_bfloat16* dst = a.o + (((long long)b * a.N + n) * a.Hq + h * a.G + head) * D + warp * Q * 4;
 #pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+  for (int q = 0; q < Q; q += 2) {
+    uint4 w;
+    w.x = pack_bf16x2(acc[q].x * inv, acc[q].y * inv);
+    w.y = pack_bf16x2(acc[q].z * inv, acc[q].w * inv);
+    w.z = pack_bf16x2(acc[q + 1].x * inv, acc[q + 1].y * inv);
+    w.w = pack_bf16x2(acc[q + 1].z * inv, acc[q + 1].w * inv);
+    *reinterpret_cast<uint4*>(dst + 4 * q) = w;
+  }
 }
 
 template <int D, bool QUANT, int NT>
@@ -844,12 +956,16 @@ static void tree_launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)(((long long)a.B * a.N * a.Hq + 3) / 4), 1, 1);
+  const int rows = a.nb * a.gb;              // of a row tile
+  int RP = 1;
+  while (RP < 32 && RP < rows) RP *= 2;
+  const int blocks = (rows + RP - 1) / RP;
+  cfg.gridDim = dim3((unsigned)((long long)a.B * a.Hkv * a.rt * blocks), 1, 1);
   cfg.blockDim = dim3(128, 1, 1);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, tree_combine_kernel<D>, a, c, grid, NT));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, tree_combine_kernel<D>, a, c, grid, NT, RP, blocks));
 }
 
 at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor lens,
@@ -888,11 +1004,12 @@ at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor
   a.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
   a.err = err.data_ptr<int>();
   const int64_t most = B * H * a.rg * ((T + 127) / 128);
-  TORCH_CHECK(most < (1LL << 36), "too much work for one call");
   const int grid = (int)std::min<int64_t>(num_sms(kc.device().index()), most);
-  auto part = at::empty({(int64_t)2 * grid * NT * 128 * (D + 2)}, q.options().dtype(at::kFloat));
-  a.part = part.data_ptr<float>();
-  a.part_ml = reinterpret_cast<float2*>(a.part + (int64_t)2 * grid * NT * 128 * D);
+  TORCH_CHECK(most * (grid + 1) < (1LL << 31), "too many key tiles for one call");   // the kernels count in 32 bits
+  auto part = at::empty({(int64_t)2 * grid * NT * 128 * (D + 2) + (int64_t)grid * 256}, q.options().dtype(at::kFloat));
+  a.part = reinterpret_cast<float4*>(part.data_ptr<float>());
+  a.part_ml = reinterpret_cast<float2*>(part.data_ptr<float>() + (int64_t)2 * grid * NT * 128 * D);
+  a.pair_ml = a.part_ml + (int64_t)2 * grid * NT * 128;
 
   const uint64_t u = 2;
   const uint64_t qd[5] = {(uint64_t)D, (uint64_t)G, (uint64_t)N, (uint64_t)H, (uint64_t)B};
