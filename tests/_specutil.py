@@ -50,7 +50,9 @@ def attention64(q, kc, vc, lens, parents, scale, ks, vs):
     sum p|v| / l from the first and 2^-8 |o| from the second.  The 32-bit scores are off by at
     most 2^-20 sum |q k| scale (128 products and additions of 2^-24 each, truncation in the
     tensor core included), which enters p as a relative error twice (p and l); exponentials
-    and sums add 2^-18 of sum p|v| / l."""
+    and sums add 2^-18 of sum p|v| / l.  Over a quantised cache the weights p * scale may be held
+    in f16 instead of bf16: 2^-11 of their value, or half a subnormal step, 2^-25 of the largest
+    one, against each code."""
     B, N, Hq, D = q.shape
     H, T = kc.shape[1:3]
     G = Hq // H
@@ -70,7 +72,11 @@ def attention64(q, kc, vc, lens, parents, scale, ks, vs):
                 o[b, n, h] = (p[:, None] * vv).sum(0)
                 a = (p[:, None] * vv.abs()).sum(0)
                 ds = 2.0 ** -20 * float((kk.abs() @ q[b, n, h].abs()).max()) * abs(scale)
-                bound[b, n, h] = 2.0 ** -8 * o[b, n, h].abs() + (2.0 ** -8 * 1.01 + 2 * ds + 2.0 ** -18) * a + 2.0 ** -126
+                sub = 0.0
+                if vs is not None:
+                    sv = vs.cpu()[b, h // G][rows].double()
+                    sub = 2.0 ** -25 * float((p * sv).max()) * vc.cpu()[b, h // G][rows].double().abs().sum(0)
+                bound[b, n, h] = sub + 2.0 ** -8 * o[b, n, h].abs() + (2.0 ** -8 * 1.01 + 2 * ds + 2.0 ** -18) * a + 2.0 ** -126
     return o, bound
 
 

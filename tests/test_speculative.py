@@ -70,7 +70,9 @@ def test_cache_write_and_read(device, dtype, layout, B, N, H, D, T):
                 for h in range(H):
                     if dtype == E4M3:
                         codes, scale = quant_row(x[b, n, h])
-                        want[i][b, h, t] = raw(torch.tensor(codes, dtype=torch.float64).to(E4M3))
+                        codes = torch.tensor(codes, dtype=torch.float64)
+                        # a row that is not finite has the scale NaN and codes 0
+                        want[i][b, h, t] = raw(torch.where(codes.isnan(), 0.0, codes).to(E4M3))
                         want[2 + i][b, h, t] = 255 if math.isnan(scale) else 127 + int(math.log2(scale))
                     else:
                         want[i][b, h, t] = x[b, n, h]
@@ -250,6 +252,28 @@ def test_tree_attention_bad_drafted_rows(device, dtype, D):
     torch.testing.assert_close(torch.isinf(o) * o.sign(), torch.isinf(want) * want.sign(), equal_nan=True)
     fine = torch.isfinite(want)
     assert bool(((o - want).abs() <= bound)[fine].all()) and bool(fine[0, [0, 1, 3]].all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("N,Hq,H", [(3, 2, 1), (6, 8, 2), (40, 4, 1)])
+def test_scales_of_any_size(device, N, Hq, H):
+    """Value rows from 2^-100 to 2^100, zero rows among them (the least scale), key rows from 2^-20 on."""
+    B, T, D, ln = 2, 420, 128, [370, 5]
+    g = gen(N)
+    x = torch.randn(2, B, T, H, D, generator=g)
+    x[0] *= torch.exp2(torch.randint(-20, 2, (B, T, H, 1), generator=g).float())
+    x[1] *= torch.exp2(torch.randint(-100, 100, (B, T, H, 1), generator=g).float())
+    x[1, :, ::3] = 0
+    x[1, 0] *= 2.0 ** -24
+    cache = ops.kv_cache_alloc(B, H, T, D, E4M3, device=device)
+    kc, vc, ks, vs = cache
+    x = x.to(BF16).to(device)
+    ops.kv_cache_write(x[0], x[1], kc, vc, i32([0, 0], device), None, ks, vs)
+    par = make_tree(B, N, g)
+    q = torch.randn(B, N, Hq, D, generator=g).to(BF16).to(device)
+    o = ops.tree_attention(q, kc, vc, i32(ln, device), par.to(device), None, ks, vs)
+    want, bound = attention64(q, kc, vc, ln, par, D ** -0.5, ks, vs)
+    assert bool(((o.double().cpu() - want).abs() <= bound).all())
 
 
 @pytest.mark.parametrize("device", DEVICES)

@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_cache_write_kernel(const KvRows
       for (int o = L / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
       const int e = scale_byte(max(m & 0xffffu, m >> 16));
       if (on[i]) {
-        uint2 codes = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);   // a row with an inf or NaN: NaN codes too
+        uint2 codes = make_uint2(0, 0);        // a row with an inf or NaN: its scale says so
         if (e != kScaleNan) codes = quant8(u[i], __uint_as_float((uint32_t)(254 - e) << 23));   // times 2^-(e - 127)
         reinterpret_cast<uint2*>(dst)[l] = codes;
         if (l == 0) c.s[kv][b * c.sb + h * c.sh + t * c.st] = (uint8_t)e;

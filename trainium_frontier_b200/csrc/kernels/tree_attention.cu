@@ -854,6 +854,12 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
   }
 }
 
+}  // namespace tfb
+
+#include "tree_attention_few.cuh"
+
+namespace tfb {
+
 // Adds the parts of the units that more than one CTA worked on.  A CTA has RP neighbouring rows
 // of a row tile (RP: the rows of the tile, at most 32, rounded up to a power of two); the lanes of
 // a warp are RP rows x 32 / RP parts, its warps share the D / 4 columns of four.  Parts are added
@@ -939,19 +945,8 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeArgs a, con
   }
 }
 
-template <int D, bool QUANT, int NT>
-static void tree_launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TreeArgs& a, const KvView& c,
-                        int grid, cudaStream_t s) {
-  using Cfg = TreeCfg<D, QUANT, NT>;
-  static bool set[64] = {};                  // a function's attributes are kept by device
-  int dev = 0;
-  C10_CUDA_CHECK(cudaGetDevice(&dev));
-  if (dev >= 64 || !set[dev]) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(tree_attention_kernel<D, QUANT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::SMEM));
-    if (dev < 64) set[dev] = true;
-  }
-  tree_attention_kernel<D, QUANT, NT><<<grid, Cfg::THREADS, Cfg::SMEM, s>>>(tq, tk, tv, a, c);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+template <int D>
+static void combine_launch(const TreeArgs& a, const KvView& c, int grid, int NT, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -966,6 +961,39 @@ static void tree_launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, tree_combine_kernel<D>, a, c, grid, NT, RP, blocks));
+}
+
+template <typename K>
+static void tree_smem(K kernel, size_t bytes, bool (&set)[64]) {   // a function's attributes are kept by device
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev >= 64 || !set[dev]) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) set[dev] = true;
+  }
+}
+
+template <int D, bool QUANT, int EH>
+static void few_launch(const CUtensorMap& tk, const CUtensorMap& tv, const at::Tensor& q, const TreeArgs& a, const KvView& c, int grid,
+                       cudaStream_t s) {
+  using Cfg = FewCfg<D, QUANT, EH>;
+  static bool set[64] = {};
+  tree_smem(tree_few_kernel<D, QUANT, EH>, Cfg::SMEM, set);
+  tree_few_kernel<D, QUANT, EH><<<grid, kFewThreads, Cfg::SMEM, s>>>(tk, tv, reinterpret_cast<const __nv_bfloat16*>(q.data_ptr()), q.stride(0),
+                                                                     q.stride(1), q.stride(2), a, c);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  combine_launch<D>(a, c, grid, 1, s);
+}
+
+template <int D, bool QUANT, int NT>
+static void tree_launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TreeArgs& a, const KvView& c,
+                        int grid, cudaStream_t s) {
+  using Cfg = TreeCfg<D, QUANT, NT>;
+  static bool set[64] = {};
+  tree_smem(tree_attention_kernel<D, QUANT, NT>, Cfg::SMEM, set);
+  tree_attention_kernel<D, QUANT, NT><<<grid, Cfg::THREADS, Cfg::SMEM, s>>>(tq, tk, tv, a, c);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  combine_launch<D>(a, c, grid, NT, s);
 }
 
 at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor lens,
@@ -989,12 +1017,14 @@ at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor
   TORCH_CHECK(B * N * Hq < (1LL << 31), "too many query rows");
   const int G = (int)(Hq / H);
   a.B = (int)B; a.N = (int)N; a.Hq = (int)Hq; a.Hkv = (int)H; a.G = G;
+  // up to 32 rows a key/value head: the register kernel, with 8, 16 or 32 rows
+  const int rows = (int)std::min<int64_t>(N * G, 1 << 20), EH = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 0;
   // rows of a tile: nb nodes of gb heads each
   a.gb = std::min(G, 128);
   a.nb = std::min((int)N, 128 / a.gb);
   a.gg = (G + a.gb - 1) / a.gb;
   a.rt = (((int)N + a.nb - 1) / a.nb) * a.gg;
-  const int NT = a.rt > 1 ? 2 : 1;           // two row tiles share each key / value tile
+  const int NT = a.rt > 1 ? 2 : 1;           // two row tiles share each key / value tile (none with EH)
   a.rg = (a.rt + NT - 1) / NT;
   a.scale_log2 = std::max((float)(std::abs(scale) * 1.4426950408889634), 1e-30f);   // -inf * 0 is NaN
   a.neg = scale < 0;
@@ -1011,18 +1041,28 @@ at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor
   a.part_ml = reinterpret_cast<float2*>(part.data_ptr<float>() + (int64_t)2 * grid * NT * 128 * D);
   a.pair_ml = a.part_ml + (int64_t)2 * grid * NT * 128;
 
+  const uint64_t kd[4] = {(uint64_t)D, (uint64_t)T, (uint64_t)H, (uint64_t)B};
+  const uint64_t kst[3] = {(uint64_t)c.t, (uint64_t)c.h, (uint64_t)c.b};
+  const uint32_t kb[4] = {quant ? (uint32_t)D : 64u, 128, 1, 1};
+  const auto type = quant ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const auto sw = quant && !EH ? CU_TENSOR_MAP_SWIZZLE_NONE : quant && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  const CUtensorMap tk = make_tmap_nd(c.p[0], type, 4, kd, kst, kb, sw), tv = make_tmap_nd(c.p[1], type, 4, kd, kst, kb, sw);
+  auto s = at::cuda::getCurrentCUDAStream();
+  if (EH) {
+#define TFB_FEW(DD, QQ)                                               \
+  (EH == 1   ? few_launch<DD, QQ, 1>(tk, tv, q, a, c, grid, s)        \
+   : EH == 2 ? few_launch<DD, QQ, 2>(tk, tv, q, a, c, grid, s)        \
+             : few_launch<DD, QQ, 4>(tk, tv, q, a, c, grid, s))
+    if (D == 128) { if (quant) TFB_FEW(128, true); else TFB_FEW(128, false); }
+    else { if (quant) TFB_FEW(64, true); else TFB_FEW(64, false); }
+#undef TFB_FEW
+    return o;
+  }
   const uint64_t u = 2;
   const uint64_t qd[5] = {(uint64_t)D, (uint64_t)G, (uint64_t)N, (uint64_t)H, (uint64_t)B};
   const uint64_t qs[4] = {q.stride(2) * u, q.stride(1) * u, (uint64_t)G * q.stride(2) * u, q.stride(0) * u};
   const uint32_t qb[5] = {64, (uint32_t)a.gb, (uint32_t)a.nb, 1, 1};
   const CUtensorMap tq = make_tmap_nd(q.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, qd, qs, qb, CU_TENSOR_MAP_SWIZZLE_128B);
-  const uint64_t kd[4] = {(uint64_t)D, (uint64_t)T, (uint64_t)H, (uint64_t)B};
-  const uint64_t kst[3] = {(uint64_t)c.t, (uint64_t)c.h, (uint64_t)c.b};
-  const uint32_t kb[4] = {quant ? (uint32_t)D : 64u, 128, 1, 1};
-  const auto type = quant ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const auto sw = quant ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
-  const CUtensorMap tk = make_tmap_nd(c.p[0], type, 4, kd, kst, kb, sw), tv = make_tmap_nd(c.p[1], type, 4, kd, kst, kb, sw);
-  auto s = at::cuda::getCurrentCUDAStream();
 #define TFB_TREE(DD, QQ) (NT == 1 ? tree_launch<DD, QQ, 1>(tq, tk, tv, a, c, grid, s) : tree_launch<DD, QQ, 2>(tq, tk, tv, a, c, grid, s))
   if (D == 128) { if (quant) TFB_TREE(128, true); else TFB_TREE(128, false); }
   else { if (quant) TFB_TREE(64, true); else TFB_TREE(64, false); }
