@@ -20,6 +20,10 @@ struct KvRows {                  // rows [B, N, H, D] outside the cache
   long long b[2], n[2], h[2];    // strides in bytes
 };
 
+// Keys' or values' entry of a parameter array; by an index, the array would be copied to local memory.
+template <typename T>
+__device__ __forceinline__ T pick(const T (&a)[2], int kv) { return kv ? a[1] : a[0]; }
+
 // Exponent byte of the least power-of-two scale (2^-117 at the least) under which a row whose
 // largest magnitude has the bf16 bits `amax` fits +-448 = 1.75 * 2^8; 255 if it is not finite.
 __device__ __forceinline__ int scale_byte(uint32_t amax) {
@@ -47,43 +51,74 @@ __device__ __forceinline__ uint32_t absmax8(const uint4& u) {
 }
 
 // cache[b, h, pos[b] + n] = rows[b, n, h] for n < count[b]; rows outside the cache are left out.
-// A block has one (sequence, head, keys or values) and blockDim / L * U neighbouring rows.
+// A block has one (sequence, head, keys or values) and blockDim / L * U neighbouring rows, a
+// thread U of them in a row.  With U = 4 the four rows' maxima are found together: two 16-bit
+// maxima a word, and the two words of a thread are halved between its lanes in the first step
+// (5 shuffles instead of 16, which with the loads kept the L1 pipe 84 % busy: 114 us for 16 x 4096
+// rows of 8 heads).
 template <int D, bool QUANT, int U>
 __global__ void __launch_bounds__(kKvThreads) kv_cache_write_kernel(const KvRows src, const KvView c, const int* __restrict__ pos,
                                                                     const int* __restrict__ count, int N, int H) {
+  static_assert(U == 1 || U == 4, "rows a thread");
   constexpr int L = D / 8;   // lanes a row
   const int b = blockIdx.y, kv = blockIdx.z, h = blockIdx.x % H;
   const int l = threadIdx.x % L, rows = blockDim.x / L;
-  const int n0 = (int)(blockIdx.x / H) * rows * U + threadIdx.x / L;
+  const int n0 = ((int)(blockIdx.x / H) * rows + threadIdx.x / L) * U;
   const int live = count ? min(count[b], N) : N;
   const long long t0 = pos[b];
+  const uint8_t* sp = pick(src.p, kv) + b * pick(src.b, kv) + h * pick(src.h, kv) + n0 * pick(src.n, kv) + 16 * l;
+  uint8_t* dp = pick(c.p, kv) + b * c.b + h * c.h + (t0 + n0) * c.t;
   uint4 u[U];
   bool on[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    const int n = n0 + i * rows;
-    on[i] = n < live && t0 + n >= 0 && t0 + n < c.tmax;
+    on[i] = n0 + i < live && t0 + n0 + i >= 0 && t0 + n0 + i < c.tmax;
     u[i] = make_uint4(0, 0, 0, 0);
-    if (on[i]) u[i] = reinterpret_cast<const uint4*>(src.p[kv] + b * src.b[kv] + n * src.n[kv] + h * src.h[kv])[l];
+    if (on[i]) u[i] = *reinterpret_cast<const uint4*>(sp + i * pick(src.n, kv));
   }
+  if constexpr (!QUANT) {
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const long long t = t0 + n0 + i * rows;
-    uint8_t* dst = c.p[kv] + b * c.b + h * c.h + t * c.t;
-    if constexpr (!QUANT) {
-      if (on[i]) reinterpret_cast<uint4*>(dst)[l] = u[i];
+    for (int i = 0; i < U; ++i)
+      if (on[i]) reinterpret_cast<uint4*>(dp + i * c.t)[l] = u[i];
+  } else {
+    uint32_t top[U];                           // the rows' largest magnitudes, as bf16 bits
+    uint32_t m[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      m[i] = absmax8(u[i]);
+      m[i] = max(m[i] & 0xffffu, m[i] >> 16);
+    }
+    if constexpr (U == 4) {
+      const uint32_t w0 = m[0] | (m[1] << 16), w1 = m[2] | (m[3] << 16);
+      const bool up = (l & (L / 2)) != 0;      // the upper lanes go on with rows 2 and 3
+      uint32_t w = __vmaxu2(up ? w1 : w0, __shfl_xor_sync(0xffffffffu, up ? w0 : w1, L / 2));
+#pragma unroll
+      for (int o = L / 4; o > 0; o >>= 1) w = __vmaxu2(w, __shfl_xor_sync(0xffffffffu, w, o));
+      const uint32_t x = __shfl_xor_sync(0xffffffffu, w, L / 2);
+      const uint32_t a = up ? x : w, d = up ? w : x;
+      top[0] = a & 0xffffu; top[1] = a >> 16; top[2] = d & 0xffffu; top[3] = d >> 16;
     } else {
-      uint32_t m = absmax8(u[i]);
+      uint32_t w = m[0];
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const int e = scale_byte(max(m & 0xffffu, m >> 16));
+      for (int o = L / 2; o > 0; o >>= 1) w = max(w, __shfl_xor_sync(0xffffffffu, w, o));
+      top[0] = w;
+    }
+    uint32_t byte = 0;
+    bool byte_on = false;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int e = scale_byte(top[i]);
       if (on[i]) {
         uint2 codes = make_uint2(0, 0);        // a row with an inf or NaN: its scale says so
         if (e != kScaleNan) codes = quant8(u[i], __uint_as_float((uint32_t)(254 - e) << 23));   // times 2^-(e - 127)
-        reinterpret_cast<uint2*>(dst)[l] = codes;
-        if (l == 0) c.s[kv][b * c.sb + h * c.sh + t * c.st] = (uint8_t)e;
+        reinterpret_cast<uint2*>(dp + i * c.t)[l] = codes;
+      }
+      if (l == i) {                            // lane i stores row i's scale
+        byte = (uint32_t)e;
+        byte_on = on[i];
       }
     }
+    if (byte_on) pick(c.s, kv)[b * c.sb + h * c.sh + (t0 + n0 + l) * c.st] = (uint8_t)byte;
   }
 }
 
@@ -107,10 +142,10 @@ __global__ void __launch_bounds__(kKvThreads) kv_cache_read_kernel(const KvView 
     u[i] = make_uint2(0, 0);
     e[i] = 127;
     if (t < live) {
-      const uint8_t* p = c.p[kv] + b * c.b + h * c.h + (long long)t * c.t;
+      const uint8_t* p = pick(c.p, kv) + b * c.b + h * c.h + (long long)t * c.t;
       if constexpr (QUANT) {
         u[i] = reinterpret_cast<const uint2*>(p)[l];
-        e[i] = c.s[kv][b * c.sb + h * c.sh + t * c.st];
+        e[i] = pick(c.s, kv)[b * c.sb + h * c.sh + t * c.st];
       } else {
         o[i] = reinterpret_cast<const uint4*>(p)[l];
       }
@@ -138,48 +173,51 @@ __global__ void __launch_bounds__(kKvThreads) kv_cache_read_kernel(const KvView 
 // cache[b, h, lens[b] + i] = cache[b, h, lens[b] + path[b, i]], i < count[b], path ascending with
 // path[i] >= i.  A source is then never below its own target and never a target of an earlier
 // move, so moves in order of i are right in place -- and so are batches of moves of which all
-// rows are loaded before any is stored.  A block of 256 threads has units of min(N, 64) rows, a
-// unit being one (sequence, head, keys or values); a thread holds its 16-byte pieces of the
-// batch in registers between the two barriers.
+// rows are loaded before any is stored.  A block of 256 threads has units of at most 64 rows, a unit
+// being one (sequence, head, keys or values): `rows` rows of L lanes at a time, U times, held in
+// registers between the two barriers.
 template <int ROW>   // bytes of a row
-__global__ void __launch_bounds__(kKvThreads) kv_cache_commit_kernel(const KvView c, const int* __restrict__ lens, const int* __restrict__ path,
-                                                                     const int* __restrict__ count, int B, int N, int H, int batch, int ppt) {
-  constexpr int L = ROW / 16, U = ROW / 64;   // pieces a row; pieces a thread at most (64 rows a batch)
-  const int per = batch * L;                  // pieces of a unit's batch
-  const int threads = per / ppt;              // threads of a unit, ppt <= U pieces each
+__global__ void __launch_bounds__(kKvThreads, 6) kv_cache_commit_kernel(const KvView c, const int* __restrict__ lens, const int* __restrict__ path,
+                                                                        const int* __restrict__ count, int B, int N, int H, int rows) {
+  constexpr int L = ROW / 16, U = ROW / 64;   // 64 rows a batch: U * 256 / L
+  const int threads = rows * L;
   const int slot = threadIdx.x / threads, id = threadIdx.x - slot * threads;
-  const long long unit = (long long)blockIdx.x * (kKvThreads / threads) + slot;
-  const bool real = slot < kKvThreads / threads && unit < 2LL * B * H;
+  const int units = kKvThreads / threads;
+  const long long unit = (long long)blockIdx.x * units + slot;
+  const bool real = slot < units && unit < 2LL * B * H;
   const int kv = (int)(unit & 1), b = real ? (int)((unit >> 1) / H) : 0, h = (int)((unit >> 1) % H);
   const long long t0 = lens[b];
   const int m = real && t0 >= 0 ? min(count[b], N) : 0;
   const int* pp = path + (long long)b * N;
-  uint8_t* base = c.p[kv] + b * c.b + h * c.h;
-  uint8_t* sbase = c.s[kv] ? c.s[kv] + b * c.sb + h * c.sh : nullptr;
-  for (int i0 = 0; i0 < N; i0 += batch) {
+  const int l = id % L, i1 = id / L;
+  uint8_t* base = pick(c.p, kv) + b * c.b + h * c.h + t0 * c.t + 16 * l;
+  uint8_t* sbase = pick(c.s, kv) && l == 0 ? pick(c.s, kv) + b * c.sb + h * c.sh + t0 * c.st : nullptr;
+  const int room = (int)min((long long)N, c.tmax - t0);   // rows behind the context
+  for (int i0 = i1; i0 - i1 < N; i0 += U * rows) {
     uint4 u[U];
     uint8_t s[U];
-    bool on[U];
+    int src[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int piece = id + j * threads, i = i0 + piece / L, l = piece % L;
-      const int src = j < ppt && piece < per && i < m ? pp[i] : -1;
-      on[j] = src > i && src < N && t0 + src < c.tmax;
-      if (on[j]) {
-        u[j] = *reinterpret_cast<const uint4*>(base + (t0 + src) * c.t + 16 * l);
-        if (sbase && l == 0) s[j] = sbase[(t0 + src) * c.st];
-      }
+      const int i = i0 + j * rows;
+      src[j] = i < m ? pp[i] : -1;
+      if (src[j] <= i || src[j] >= room) src[j] = -1;
     }
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (src[j] >= 0) {
+        u[j] = *reinterpret_cast<const uint4*>(base + src[j] * c.t);
+        if (sbase) s[j] = sbase[src[j] * c.st];
+      }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int piece = id + j * threads, i = i0 + piece / L, l = piece % L;
-      if (on[j]) {
-        *reinterpret_cast<uint4*>(base + (t0 + i) * c.t + 16 * l) = u[j];
-        if (sbase && l == 0) sbase[(t0 + i) * c.st] = s[j];
+    for (int j = 0; j < U; ++j)
+      if (src[j] >= 0) {
+        const int i = i0 + j * rows;
+        *reinterpret_cast<uint4*>(base + i * c.t) = u[j];
+        if (sbase) sbase[i * c.st] = s[j];
       }
-    }
-    if (N > batch) __syncthreads();
+    if (N > U * rows) __syncthreads();
   }
 }
 
@@ -280,12 +318,10 @@ void kv_cache_commit(at::Tensor kc, at::Tensor vc, at::Tensor lens, at::Tensor p
   c10::cuda::CUDAGuard guard(kc.device());
   auto s = at::cuda::getCurrentCUDAStream();
   const int64_t row = D * (quant ? 1 : 2);
-  const int batch = (int)std::min<int64_t>(N, 64), pieces = batch * (int)(row / 16);
-  int ppt = 1;                               // pieces a thread: the least power of two that keeps a unit in one block
-  while (pieces / ppt > kKvThreads || pieces % ppt) ppt *= 2;
-  const int64_t units = kKvThreads / (pieces / ppt), gx = (2 * B * H + units - 1) / units;
+  const int rows = (int)std::min<int64_t>(N, kKvThreads / (row / 16));
+  const int64_t units = kKvThreads / (rows * (row / 16)), gx = (2 * B * H + units - 1) / units;
   TORCH_CHECK(gx < (1LL << 31), "too many rows");
-#define TFB_KV_COMMIT(RR) kv_cache_commit_kernel<RR><<<(unsigned)gx, kKvThreads, 0, s>>>(c, lp, pp, cp, (int)B, (int)N, (int)H, batch, ppt)
+#define TFB_KV_COMMIT(RR) kv_cache_commit_kernel<RR><<<(unsigned)gx, kKvThreads, 0, s>>>(c, lp, pp, cp, (int)B, (int)N, (int)H, rows)
   if (row == 256) TFB_KV_COMMIT(256);
   else if (row == 128) TFB_KV_COMMIT(128);
   else TFB_KV_COMMIT(64);
