@@ -15,3 +15,101 @@ def test_generate_reference_shapes_and_determinism():
     a = generate_reference(m, p, 5)
     b = generate_reference(m, p, 5)
     assert a.shape == (2, 5) and torch.equal(a, b)
+
+
+def _small_model(seed=0):
+    cfg = preset("tiny", depth=2)
+    torch.manual_seed(seed)
+    m = GPT(cfg.model_config(), cfg)
+    m.init_weights()
+    with torch.no_grad():   # a non-degenerate random model (zero-init projections otherwise)
+        for b in m.transformer.h:
+            b.mlp.c_proj.weight.normal_(0, 0.02)
+        m.lm_head.weight.normal_(0, 0.05)
+    return m.eval()
+
+
+def test_speculative_greedy_is_greedy():
+    """Whatever the draft proposes -- the right tokens, wrong ones, a tree of both, nothing --
+    greedy speculative decoding gives plain greedy decoding's tokens."""
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator, ngram_draft
+    m = _small_model()
+    p = torch.randint(1, 8192, (3, 16))
+    n = 12
+    want = generate_reference(m, p, n)
+
+    def oracle(text, lens):     # right tokens on one branch (node 2, 3, 5), wrong ones beside it
+        full = torch.cat([p, want], 1)
+        tok = torch.randint(0, 8192, (3, 5), dtype=torch.int32)
+        for b in range(3):
+            rest = full[b, int(lens[b]):][:3].tolist()
+            for k, node in enumerate((2, 3, 5)):
+                if k < len(rest):
+                    tok[b, node - 1] = rest[k]
+        return tok, torch.tensor([[0, 0, 2, 2, 3]] * 3, dtype=torch.int32), None
+
+    def nothing(text, lens):
+        return torch.full((3, 2), -1, dtype=torch.int32), torch.full((3, 2), -2, dtype=torch.int32), None
+    for draft, most in ((oracle, 4), (nothing, n - 1), (ngram_draft(4), n - 1)):
+        g = SpeculativeGenerator(m, 3, 64, draft)
+        assert torch.equal(g.generate(p, n).long(), want.long())
+        assert g.rounds <= most
+
+
+def test_speculative_sampling_draws_from_the_target():
+    """Sampled with a draft distribution that is not the target's: the first two tokens'
+    frequencies over many sequences follow the target's within 5 standard deviations."""
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    m = _small_model(1)
+    M = 600
+    p = torch.randint(1, 8192, (1, 4)).expand(M, 4).contiguous()
+    with torch.no_grad():
+        law = torch.softmax(m(p[:1])[0, -1] / 0.1, -1)
+    g = torch.Generator().manual_seed(3)
+
+    def draft(text, lens):
+        q = torch.softmax(torch.randn(1, 1, 8192, generator=g), -1).expand(M, 3, 8192).contiguous()
+        tok = torch.multinomial(q[:, :2].reshape(-1, 8192), 1, generator=g).view(M, 2).to(torch.int32)
+        return tok, torch.tensor([[0, 1]] * M, dtype=torch.int32), q
+    out = SpeculativeGenerator(m, M, 16, draft).generate(p, 3, 0.1, g)
+    top = law.argmax()
+    share, want = (out[:, 0] == top).double().mean(), law[top].double()
+    assert abs(share - want) <= 5 * (want * (1 - want) / M).sqrt()
+
+
+def test_speculative_quantised_cache_runs():
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    m = _small_model()
+    p = torch.randint(1, 8192, (2, 9))
+    out = SpeculativeGenerator(m, 2, 40, kv_dtype=torch.float8_e4m3fn).generate(p, 10)
+    assert out.shape == (2, 10) and int(out.min()) >= 0
+
+
+def test_speculative_refusals():
+    import pytest
+
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    m = _small_model()
+    with pytest.raises(ValueError):
+        SpeculativeGenerator(m, 2, m.config.sequence_len + 1)
+    g = SpeculativeGenerator(m, 2, 32)
+    with pytest.raises(ValueError):
+        g.generate(torch.ones(1, 4, dtype=torch.long), 2)
+    with pytest.raises(ValueError):
+        g.generate(torch.ones(2, 30, dtype=torch.long), 8)
+    with pytest.raises(ValueError):
+        g.generate(torch.ones(2, 3, dtype=torch.long), 0)
+
+
+def test_ngram_draft():
+    from trainium_frontier_b200.inference.speculative import ngram_draft
+    text = torch.zeros(4, 12, dtype=torch.long)
+    text[0, :8] = torch.tensor([5, 6, 7, 8, 5, 6, 9, 9])     # ends in a pair never seen before
+    text[1, :9] = torch.tensor([1, 2, 3, 4, 1, 2, 7, 1, 2])  # latest earlier "1 2" is at 4
+    text[2, :1] = 3                                          # shorter than the order
+    text[3, :12] = 4                                         # one token over and over, to the end of the row
+    lens = torch.tensor([8, 9, 1, 12], dtype=torch.int32)
+    tok, par, q = ngram_draft(3)(text, lens)
+    assert q is None
+    assert tok.tolist() == [[-1] * 3, [7, 1, 2], [-1] * 3, [4, -1, -1]]
+    assert par.tolist() == [[-2] * 3, [0, 1, 2], [-2] * 3, [0, -2, -2]]

@@ -83,3 +83,38 @@ def test_split_decode_attention_kernel(cuda_device, layout):
         ref = torch.softmax(qf @ kf.transpose(-1, -2) * D ** -0.5, -1) @ vf
         assert (out.float().view(B, H, D) - ref.squeeze(2)).abs().max().item() < 2e-2, L
         assert int(cnt.abs().sum()) == 0
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float8_e4m3fn])
+def test_speculative_greedy_decoding(cuda_device, kv, head_dim):
+    """Speculative greedy decoding against plain greedy decoding by recomputation: a draft that
+    knows the answer on one branch of its tree, and the draft by rule."""
+    from trainium_frontier_b200.inference.generate import generate_reference
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    from trainium_frontier_b200.ops._ext import check_errors
+    m = _model(cuda_device, head_dim=head_dim)
+    B, T, N = 4, 128, 24
+    prompts = torch.randint(1, 8192, (B, T), device=cuda_device, dtype=torch.int32)
+    ref = generate_reference(m, prompts, N)
+    full = torch.cat([prompts.long(), ref.long(), torch.zeros(B, 8, device=cuda_device, dtype=torch.long)], 1)
+
+    def oracle(text, lens):
+        tok = torch.randint(0, 8192, (B, 5), device=cuda_device).to(torch.int32)
+        for k, node in enumerate((2, 3, 5)):
+            tok[:, node - 1] = full.gather(1, (lens.long() + k).clamp_max(full.shape[1] - 1)[:, None])[:, 0].to(torch.int32)
+        return tok, torch.tensor([[0, 0, 2, 2, 3]] * B, dtype=torch.int32, device=cuda_device), None
+    for draft in (oracle, None):
+        g = SpeculativeGenerator(m, B, 256, draft, kv)
+        out = g.generate(prompts, N)
+        check_errors()
+        assert out.shape == (B, N)
+        if kv == torch.bfloat16:
+            # bf16 logits of two kernel paths may break near-ties differently late in the sequence
+            assert torch.equal(out[:, :4].long(), ref[:, :4].long())
+            agree = (out.long() == ref.long()).float().mean().item()
+            assert agree > 0.9, agree
+            assert draft is None or g.rounds < N // 2
+    sampled = SpeculativeGenerator(m, B, 256, None, kv).generate(prompts, 8, 1.0)
+    check_errors()
+    assert int(sampled.min()) >= 0 and int(sampled.max()) < 8192
