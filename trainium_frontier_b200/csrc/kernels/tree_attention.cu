@@ -760,83 +760,67 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
         mbar_arrive(&v_ready[slot]);
       }
     } else {
-      // four warps convert the keys, four the values; a thread has 16 codes of each of its rows,
-      // row0 + i * STEP, whose scales are fetched while the tile before is converted
-      constexpr int CH = D / 16, STEP = 128 / CH, RPT = CH;
-      const int v = tid >> 7, ch = tid % CH, row0 = (tid & 127) / CH;
+      // four warps convert the keys, four the values, 32 neighbouring rows of a tile each: a lane
+      // looks after one row's scale, fetched while the tile before is converted, and has 16 codes of
+      // every RPI-th row.  The loop stays short on purpose: unrolled over all rows it ran out of the
+      // instruction caches (the first cause of stalls, 3.3 warps of 11.7).
+      constexpr int CH = D / 16, RPI = 32 / CH;             // 16-code chunks a row, rows an iteration
+      const int v = tid >> 7, cw = (tid >> 5) & 3, ch = lane % CH, own = cw * 32 + lane;
       const int R = v ? NV : NK;
       uint64_t* const out_full = v ? v_full : k_full;
       uint64_t* const out_empty = v ? v_empty : k_empty;
-      const uint8_t* sb = c.s[v];
-      uint32_t ahead[RPT];
+      const uint8_t* sb = v ? c.s[1] : c.s[0];
+      uint32_t ahead = 127u;
       TreeIter nx = it;                         // one tile ahead of `it`
-      auto scales = [&]() {
-        const uint8_t* p = sb + nx.b * c.sb + nx.h * c.sh + (long long)nx.k * 128 * c.st;
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-          const int row = row0 + i * STEP;
-          ahead[i] = nx.k * 128 + row < c.tmax ? p[row * c.st] : 127u;
-        }
+      auto scale = [&]() {
+        const int row = nx.k * 128 + own;
+        ahead = row < c.tmax ? sb[nx.b * c.sb + nx.h * c.sh + (long long)row * c.st] : 127u;
       };
-      if (nx.next(lens, a.rg)) scales();
+      if (nx.next(lens, a.rg)) scale();
+      int rslot = NR - 1, slot = R - 1;
+      uint32_t rph = 1, ph = 0;
       for (int g = 0; it.next(lens, a.rg); ++g) {
         if (it.first() && v) enter(it, tid == 128 + lane);
-        const int off = it.k * 128 - it.len;
-        // factors of the rows: 2^120 times the scale (0 for a row that nothing may see); scales above
-        // 2^7 take a second one
-        uint32_t e[RPT];
-        bool wide = false;
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-          e[i] = ahead[i];
-          wide |= e[i] > 134u && e[i] != (uint32_t)kScaleNan;
+        const int j = it.k * 128 - it.len + own;            // the lane's row from the first node's
+        const uint32_t e = ahead;
+        // the row's factor: 2^120 times its scale; scales above 2^7 take a second one
+        uint32_t mine = e == (uint32_t)kScaleNan ? 0x7fffu : min(e + 120u, 254u) << 7;
+        if (v && j >= 0) {                                  // behind the context: 0 for a row that nothing may see
+          const bool seen = j < kTreeNodes && ((used >> j) & 1);
+          if (seen && e == (uint32_t)kScaleNan) atomicOr(&s_poison[it.seg & (kSegRing - 1)], 1ull << j);
+          if (!seen || e == (uint32_t)kScaleNan) mine = 0;
         }
-        uint32_t m1[RPT];
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) m1[i] = e[i] == (uint32_t)kScaleNan ? 0x7fffu : min(e[i] + 120u, 254u) << 7;
-        if (v && off + 128 > 0) {
-#pragma unroll
-          for (int i = 0; i < RPT; ++i) {
-            const int j = row0 + i * STEP + off;
-            if (j < 0) continue;
-            const bool seen = j < kTreeNodes && ((used >> j) & 1);
-            if (seen && e[i] == (uint32_t)kScaleNan && ch == 0) atomicOr(&s_poison[it.seg & (kSegRing - 1)], 1ull << j);
-            if (!seen || e[i] == (uint32_t)kScaleNan) m1[i] = 0;
-          }
-        }
-        if (nx.next(lens, a.rg)) scales();
-        const int rslot = g % NR, slot = g % R;
-        if (!mbar_wait_warp(&raw_full[v * NR + rslot], (g / NR) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) break;
-        const uint8_t* src = sRaw + (v * NR + rslot) * RAW + row0 * D + ch * 16;
-        if (g >= R && !mbar_wait_warp(&out_empty[slot], ((g / R) + 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) break;
+        const uint32_t second = e > 134u && e != (uint32_t)kScaleNan ? (e - 7u) << 7 : 0x3f80u;
+        if (nx.next(lens, a.rg)) scale();
+        if (++rslot == NR) { rslot = 0; rph ^= 1; }
+        if (++slot == R) { slot = 0; ph ^= 1; }
+        if (!mbar_wait_warp(&raw_full[v * NR + rslot], rph, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) break;
+        if (g >= R && !mbar_wait_warp(&out_empty[slot], ph, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) break;
+        const uint8_t* src = sRaw + (v * NR + rslot) * RAW + (cw * 32 + lane / CH) * D + ch * 16;
         uint8_t* dst = (v ? sV : sK) + slot * TILE + (ch >> 2) * kTreePanel;
         // the two panels' lanes store their two chunks in opposite order: no bank is hit twice
         const bool swap = ch >= 4;
         const int c0 = 2 * (ch & 3) + (swap ? 1 : 0);
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-          const uint4 u = *reinterpret_cast<const uint4*>(src + i * STEP * D);
-          const __nv_bfloat162 f = bf16x2_bits(m1[i]);
+        const bool wide = __any_sync(0xffffffffu, second != 0x3f80u);
+#pragma unroll 2
+        for (int i = 0; i < CH; ++i) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src + i * RPI * D);
+          const __nv_bfloat162 f = bf16x2_bits(__shfl_sync(0xffffffffu, mine, i * RPI + lane / CH));
           const uint2 p0 = codes4(u.x, f), p1 = codes4(u.y, f), p2 = codes4(u.z, f), p3 = codes4(u.w, f);
           const uint4 o0 = make_uint4(p0.x, p0.y, p1.x, p1.y), o1 = make_uint4(p2.x, p2.y, p3.x, p3.y);
-          const int row = row0 + i * STEP;
+          const int row = cw * 32 + i * RPI + lane / CH;
           *reinterpret_cast<uint4*>(dst + sw128_chunk_offset(row, c0)) = swap ? o1 : o0;
           *reinterpret_cast<uint4*>(dst + sw128_chunk_offset(row, c0 ^ 1)) = swap ? o0 : o1;
         }
-        if (__any_sync(0xffffffffu, wide)) {
+        if (wide) {
 #pragma unroll 1
-          for (int i = 0; i < RPT; ++i) {
-            uint32_t ei = 127u;
+          for (int i = 0; i < 2 * CH; ++i) {
+            const __nv_bfloat162 f = bf16x2_bits(__shfl_sync(0xffffffffu, second, (i >> 1) * RPI + lane / CH));
+            uint32_t* w = reinterpret_cast<uint32_t*>(dst + sw128_chunk_offset(cw * 32 + (i >> 1) * RPI + lane / CH, c0 ^ (i & 1)));
 #pragma unroll
-            for (int k = 0; k < RPT; ++k) ei = k == i ? e[k] : ei;
-            if (ei <= 134u || ei == (uint32_t)kScaleNan) continue;
-            const __nv_bfloat162 f = bf16x2_bits((ei - 7u) << 7);
-            for (int k = 0; k < 2; ++k) {
-              uint32_t* w = reinterpret_cast<uint32_t*>(dst + sw128_chunk_offset(row0 + i * STEP, c0 ^ k));
-              for (int q = 0; q < 4; ++q) {
-                const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[q]), f);
-                w[q] = *reinterpret_cast<const uint32_t*>(&y);
-              }
+            for (int q = 0; q < 4; ++q) {
+              const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[q]), f);
+              w[q] = *reinterpret_cast<const uint32_t*>(&y);
             }
           }
         }
