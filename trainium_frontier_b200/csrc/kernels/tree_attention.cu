@@ -215,7 +215,9 @@ __device__ __forceinline__ float tree_ex2(float x) {
 // lands in the low bits of v + 1.5 * 2^23), 2^f on [-1/2, 1/2] by a polynomial of degree 4 fitted
 // here for the least relative error (2.7e-6), n added to its exponent.  A quarter of the
 // exponentials goes this way, since the two groups' 128 a row pair are all that the MUFU unit
-// of a sub-core does in 1024 cycles.  NaN stays NaN.
+// of a sub-core does in 1024 cycles (bf16 caches: 126 instead of 138 us without any exponentials at
+// all, so little is left; beside the conversion of quantised tiles the extra instructions cost
+// more than they save, 376 against 350 us).  NaN stays NaN.
 __device__ __forceinline__ float2 tree_exp2_pair(float2 v) {
   const float2 c = make_float2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
   const float2 t = __fadd2_rn(c, make_float2(12582912.f, 12582912.f));
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
 #pragma unroll
           for (int k = 0; k < 64; k += 2) {
             const float2 v = __ffma2_rn(make_float2(x[k], x[k + 1]), c2, nm2);
-            const float2 e = k < 48 ? make_float2(tree_ex2(v.x), tree_ex2(v.y)) : tree_exp2_pair(v);
+            const float2 e = QUANT || k < 48 ? make_float2(tree_ex2(v.x), tree_ex2(v.y)) : tree_exp2_pair(v);
             p[k >> 1] = pack_bf16x2(e.x, e.y);   // P in 8 bits of significand for the product, its sum in 32 bits
             sum[(k >> 1) & 1] = __fadd2_rn(sum[(k >> 1) & 1], e);
           }
@@ -1002,7 +1004,7 @@ at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor
   const int G = (int)(Hq / H);
   a.B = (int)B; a.N = (int)N; a.Hq = (int)Hq; a.Hkv = (int)H; a.G = G;
   // up to 32 rows a key/value head: the register kernel, with 8, 16 or 32 rows
-  const int rows = (int)std::min<int64_t>(N * G, 1 << 20), EH = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 0;
+  const int rows = (int)std::min<int64_t>(N * G, 1 << 20), EH = rows <= 8 ? 1 : rows <= 16 ? 2 : 0;
   // rows of a tile: nb nodes of gb heads each
   a.gb = std::min(G, 128);
   a.nb = std::min((int)N, 128 / a.gb);
@@ -1033,10 +1035,8 @@ at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor
   const CUtensorMap tk = make_tmap_nd(c.p[0], type, 4, kd, kst, kb, sw), tv = make_tmap_nd(c.p[1], type, 4, kd, kst, kb, sw);
   auto s = at::cuda::getCurrentCUDAStream();
   if (EH) {
-#define TFB_FEW(DD, QQ)                                               \
-  (EH == 1   ? few_launch<DD, QQ, 1>(tk, tv, q, a, c, grid, s)        \
-   : EH == 2 ? few_launch<DD, QQ, 2>(tk, tv, q, a, c, grid, s)        \
-             : few_launch<DD, QQ, 4>(tk, tv, q, a, c, grid, s))
+#define TFB_FEW(DD, QQ) \
+  (EH == 1 ? few_launch<DD, QQ, 1>(tk, tv, q, a, c, grid, s) : few_launch<DD, QQ, 2>(tk, tv, q, a, c, grid, s))
     if (D == 128) { if (quant) TFB_FEW(128, true); else TFB_FEW(128, false); }
     else { if (quant) TFB_FEW(64, true); else TFB_FEW(64, false); }
 #undef TFB_FEW

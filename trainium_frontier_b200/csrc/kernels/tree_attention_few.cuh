@@ -25,12 +25,13 @@ struct FewCfg {
   static constexpr int MT = (EH + 1) / 2;                          // 16-row tiles
   static constexpr uint32_t TILE = 128u * D * (QUANT ? 1u : 2u);   // a key or value tile
   static constexpr int NS = QUANT ? 6 : D == 128 ? 3 : 6;          // stages of one of each (at most a warp's worth)
-  static constexpr uint32_t OUT = kFewWarps * (512 + 4 * 16) * 4;  // outputs added at a time: 512 of each warp, rows padded
+  static constexpr int OUTF = 512;                                 // output values of a warp added at a time
+  static constexpr uint32_t OUT = kFewWarps * (OUTF + 4 * 16) * 4; // rows padded
   static constexpr uint32_t QF = MT * (D / 16) * 512u;             // query fragments
   static constexpr size_t SMEM = 2 * NS * TILE + QF + OUT + kFewWarps * 16 * MT * 8 + 2 * NS * 8 + 16 + 16 * MT * 8 + kLenCache * 4 + 16;
 };
-static_assert(FewCfg<128, true, 4>::NS <= kFewWarps && FewCfg<64, true, 4>::NS <= kFewWarps, "a warp a stage");
-static_assert(FewCfg<128, false, 4>::SMEM <= 232448 && FewCfg<128, true, 4>::SMEM <= 232448 && FewCfg<64, false, 4>::SMEM <= 232448,
+static_assert(FewCfg<128, true, 2>::NS <= kFewWarps && FewCfg<64, true, 2>::NS <= kFewWarps, "a warp a stage");
+static_assert(FewCfg<128, false, 2>::SMEM <= 232448 && FewCfg<128, true, 2>::SMEM <= 232448 && FewCfg<64, false, 2>::SMEM <= 232448,
               "shared memory");
 
 template <bool F16>
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   float o[MT][NTILE][4], m[MT][2], l[MT][2], cr[MT][2];
   float mw[MT][2];                             // reference of the weights (QUANT; else m)
   unsigned long long line[MT][2], used = 0;
-  uint32_t sc[4], se[4];                       // scale bytes of this lane's four keys: keys, values
+  uint32_t ahead = 127u;                       // scale byte of the next tile: keys (lanes 0-15) and values of the warp's keys
   int g = 0, seg = 0;
   // row of fragment half e of row tile mt
   auto row_of = [&](int mt, int e) { return mt * 16 + e * 8 + gq; };
@@ -175,16 +176,11 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     }
   // this lane's keys 2j, 2j + 1, 8 + 2j, 9 + 2j of the warp's 16
   auto key_of = [&](int i) { return warp * 16 + (i >> 1) * 8 + 2 * j + (i & 1); };
+  const uint8_t* const sbase = QUANT ? (lane < 16 ? c.s[0] : c.s[1]) : nullptr;
   auto fetch_scales = [&](const TreeIter& t) {
     if constexpr (QUANT) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const long long tt = (long long)t.k * 128 + key_of(i);
-        const long long at = t.b * c.sb + t.h * c.sh + tt * c.st;
-        const bool in = tt < c.tmax;
-        sc[i] = in ? c.s[0][at] : 127u;
-        se[i] = in ? c.s[1][at] : 127u;
-      }
+      const int row = t.k * 128 + warp * 16 + (lane & 15);
+      ahead = row < c.tmax ? sbase[t.b * c.sb + t.h * c.sh + (long long)row * c.st] : 127u;
     }
   };
   TreeIter nx = it;                            // one tile ahead
@@ -265,9 +261,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           for (int k = 0; k < 4; ++k) o[mt][i][k] = 0.f;
       __syncthreads();
     }
-    uint32_t ck[4], cv[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { ck[i] = sc[i]; cv[i] = se[i]; }
+    const uint32_t bytes = ahead;
     if (nx.next(lens, a.rg)) fetch_scales(nx);
     const int slot = g % NS;
     mbar_wait(&full[slot], (g / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
@@ -331,21 +325,24 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       alive[i] = !masked || at < 0 || (at < kTreeNodes && ((used >> at) & 1));
       if constexpr (QUANT) {
         const float nan = __int_as_float(0x7fffffff);
-        fk[i] = ck[i] == (uint32_t)kScaleNan ? nan : __uint_as_float(max(ck[i], 1u) << 23);
-        ev[i] = cv[i] == (uint32_t)kScaleNan ? nan : (float)((int)cv[i] - 127);
-        alive[i] = alive[i] && cv[i] != (uint32_t)kScaleNan;   // such a row's weight is NaN already
+        const uint32_t ck = __shfl_sync(0xffffffffu, bytes, key_of(i) - warp * 16), cv = __shfl_sync(0xffffffffu, bytes, 16 + key_of(i) - warp * 16);
+        fk[i] = ck == (uint32_t)kScaleNan ? nan : __uint_as_float(max(ck, 1u) << 23);
+        ev[i] = cv == (uint32_t)kScaleNan ? nan : (float)((int)cv - 127);
+        alive[i] = alive[i] && cv != (uint32_t)kScaleNan;   // such a row's weight is NaN already
       }
     }
     uint32_t pa[MT][4];
     bool grow = false;
     float alpha[MT][2];
-    // the larger of the quad's maximum and the reference, which moves only by more than 8
-    auto refer = [&](float mx, float& ref) -> float {
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      if (!(mx > ref + 8.f)) return 1.f;
-      const float al = tree_ex2(ref - mx);
-      ref = mx;
+    auto quad_max = [](float x) {
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+      return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+    };
+    // moves a reference to a maximum that is larger by more than 8; the factor for what stands at the old one
+    auto refer = [](float mx, float& ref) -> float {
+      const bool up = mx > ref + 8.f;
+      const float al = up ? tree_ex2(ref - mx) : 1.f;
+      ref = up ? mx : ref;
       return al;
     };
 #pragma unroll
@@ -370,17 +367,23 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float x[4] = {s[mt][0][2 * e], s[mt][0][2 * e + 1], s[mt][1][2 * e], s[mt][1][2 * e + 1]};
-        const float al = refer(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), m[mt][e]);
+        float y[4];
+        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), my = mx;
+        if constexpr (QUANT) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = x[i] == -INFINITY ? -INFINITY : x[i] + ev[i];
+          my = quad_max(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+        }
+        mx = quad_max(mx);
+        const float al = refer(mx, m[mt][e]);
         const float ref = m[mt][e] == -INFINITY ? 0.f : m[mt][e];
         float p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = tree_ex2(x[i] - ref);
         l[mt][e] = l[mt][e] * al + ((p[0] + p[1]) + (p[2] + p[3]));
         if constexpr (QUANT) {
-          float y[4], w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = x[i] == -INFINITY ? -INFINITY : x[i] + ev[i];
-          alpha[mt][e] = refer(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), mw[mt][e]);
+          float w[4];
+          alpha[mt][e] = refer(my, mw[mt][e]);
           const float rw = mw[mt][e] == -INFINITY ? 0.f : mw[mt][e];
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[i] = tree_ex2(y[i] - rw);
@@ -508,7 +511,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       return M;
     };
     const int rp = EH > 1 ? 16 : R <= 4 ? 4 : 8;          // rows added at a time, and the columns that fit
-    const int hc = min(512 / rp, D);
+    const int hc = min(Cfg::OUTF / rp, D);
 #pragma unroll 1
     for (int mt = 0; mt < MT; ++mt) {
       float f[2] = {0.f, 0.f};
