@@ -77,6 +77,54 @@ def test_speculative_sampling_draws_from_the_target():
     assert abs(share - want) <= 5 * (want * (1 - want) / M).sqrt()
 
 
+def _attending_model():
+    m = _small_model()
+    with torch.no_grad():   # the tokens depend on the attention
+        for b in m.transformer.h:
+            b.attn.c_proj.weight.normal_(0, 0.2)
+    return m
+
+
+def test_speculative_greedy_depends_on_the_cache():
+    """Plain greedy tokens where the attention decides them, with drafts by rule and with right
+    and wrong branches."""
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator, ngram_draft
+    m = _attending_model()
+    p = torch.randint(1, 8192, (2, 10))
+    full = torch.cat([p, generate_reference(m, p, 12)], 1)
+    other = p.clone()
+    other[:, :9] = torch.randint(1, 8192, (2, 9))   # the same last token: only attention tells the texts apart
+    assert not torch.equal(generate_reference(m, other, 4), full[:, 10:14])
+
+    def draft(text, lens):
+        tok = torch.full((2, 5), 3, dtype=torch.int32)
+        for b in range(2):
+            for k, t in enumerate(full[b, int(lens[b]):][:3].tolist()):
+                tok[b, (1, 2, 4)[k]] = t
+        return tok, torch.tensor([[0, 0, 2, 2, 3]] * 2, dtype=torch.int32), None
+    for d in (draft, ngram_draft(4)):
+        assert torch.equal(SpeculativeGenerator(m, 2, 40, d).generate(p, 12).long(), full[:, 10:].long())
+
+
+def test_speculative_tree_reaches_past_the_end():
+    """The right tokens on the last nodes of a wide tree, and no room beyond the text's end: the
+    tree's rows go past it, and greedy decoding still gives plain greedy decoding's tokens."""
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    m = _attending_model()
+    p = torch.randint(1, 8192, (2, 10))
+    for n in (2, 3, 4, 9):
+        full = torch.cat([p, generate_reference(m, p, n)], 1)
+
+        def draft(text, lens):
+            tok = torch.full((2, 63), 3, dtype=torch.int32)
+            for b in range(2):
+                rest = full[b, int(lens[b]):][:2].tolist()
+                for k, t in enumerate(rest):
+                    tok[b, 61 + k] = t
+            return tok, torch.tensor([[0] * 62 + [62]] * 2, dtype=torch.int32), None
+        assert torch.equal(SpeculativeGenerator(m, 2, 10 + n, draft).generate(p, n).long(), full[:, 10:].long())
+
+
 def test_speculative_quantised_cache_runs():
     from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
     m = _small_model()

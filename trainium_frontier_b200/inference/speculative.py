@@ -63,7 +63,8 @@ class SpeculativeGenerator:
         self.B, self.max_len = max_batch, max_len
         self.draft = draft or ngram_draft(7)
         dt = kv_dtype or model.compute_dtype
-        self.caches = [ops.kv_cache_alloc(max_batch, self.H, max_len, self.D, dt, device=self.dev)
+        rows = max_len + 64   # a tree begins before max_len, and its last nodes may be the accepted ones
+        self.caches = [ops.kv_cache_alloc(max_batch, self.H, rows, self.D, dt, device=self.dev)
                        for _ in range(cfg.n_layer)]
         self.rounds = 0
 
