@@ -125,6 +125,17 @@ def test_speculative_tree_reaches_past_the_end():
         assert torch.equal(SpeculativeGenerator(m, 2, 10 + n, draft).generate(p, n).long(), full[:, 10:].long())
 
 
+def test_speculative_tokens_outside_the_vocabulary():
+    """A draft's tokens outside the vocabulary are read nowhere and never accepted."""
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    m = _attending_model()
+    p = torch.randint(1, 8192, (2, 10))
+    for bad in (8192, 2 ** 31 - 1, -5):
+        draft = lambda text, lens: (torch.full((2, 2), bad, dtype=torch.int32),  # noqa: E731
+                                    torch.tensor([[0, 1]] * 2, dtype=torch.int32), None)
+        assert torch.equal(SpeculativeGenerator(m, 2, 32, draft).generate(p, 4).long(), generate_reference(m, p, 4).long())
+
+
 def test_speculative_quantised_cache_runs():
     from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
     m = _small_model()

@@ -45,7 +45,8 @@ def ngram_draft(n: int, order: int = 2):
 class SpeculativeGenerator:
     """``draft(text [B, max_len] int64, lens [B] int32) -> (tokens [B, n] int32, parents [B, n]
     int32, q)`` proposes n < 64 nodes: node i of the draft is node i + 1 of the tree, whose node
-    0 is the text's last token, and ``parents`` are tree nodes (-2: unused).  ``q`` [B, n + 1, V]
+    0 is the text's last token, and ``parents`` are tree nodes (-2: unused).  A token outside the
+    vocabulary is never accepted.  ``q`` [B, n + 1, V]
     holds the distributions that the children of each tree node were drawn from, or is None for
     a rule (``ops.verify_tree``)."""
 
@@ -129,7 +130,7 @@ class SpeculativeGenerator:
             parents = torch.cat([root, par], 1).contiguous()
             depth = ops.ref.tree_lines(parents, B, N, dev).sum(-1) - 1
             pos = (cached.long()[:, None] + depth).clamp(0, self.max_len - 1)
-            hidden = self._hidden(tokens.clamp_min(0), pos, cached, parents, False)
+            hidden = self._hidden(tokens.clamp(0, self.V - 1), pos, cached, parents, False)
             path, count, out = ops.verify_tree(tokens, parents, self._probabilities(hidden, temperature), q, uniform(B, N))
             count = torch.minimum(count, (end - 1 - cached).clamp_min(0))   # a finished sequence stays as it is
             for kc, vc, ks, vs in self.caches:
