@@ -118,3 +118,40 @@ def test_speculative_greedy_decoding(cuda_device, kv, head_dim):
     sampled = SpeculativeGenerator(m, B, 256, None, kv).generate(prompts, 8, 1.0)
     check_errors()
     assert int(sampled.min()) >= 0 and int(sampled.max()) < 8192
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_speculative_decoding_where_attention_decides(cuda_device, head_dim):
+    """Attention projections that are not zero, a wide tree whose last nodes hold the right tokens
+    and a cache that ends with the text.  The new tokens against the same model's probabilities by
+    recomputation: each is the largest or nearer to it than the two paths' bf16 rounding."""
+    from trainium_frontier_b200.inference.generate import generate_reference
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    from trainium_frontier_b200.ops._ext import check_errors
+    m = _model(cuda_device, head_dim=head_dim)
+    with torch.no_grad():
+        for b in m.transformer.h:
+            b.attn.c_proj.weight.normal_(0, 0.2)
+    B, T, N = 3, 128, 10
+    prompts = torch.randint(1, 8192, (B, T), device=cuda_device, dtype=torch.int32)
+    other = prompts.clone()
+    other[:, :T - 1] = torch.randint(1, 8192, (B, T - 1), device=cuda_device, dtype=torch.int32)
+    ref = generate_reference(m, prompts, N)
+    assert not torch.equal(generate_reference(m, other, N), ref)
+    full = torch.cat([prompts.long(), ref.long(), torch.zeros(B, 8, device=cuda_device, dtype=torch.long)], 1)
+
+    def draft(text, lens):
+        tok = torch.full((B, 63), 3, dtype=torch.int32, device=cuda_device)
+        for k in range(2):
+            tok[:, 61 + k] = full.gather(1, (lens.long() + k).clamp_max(full.shape[1] - 1)[:, None])[:, 0].to(torch.int32)
+        return tok, torch.tensor([[0] * 62 + [62]] * B, dtype=torch.int32, device=cuda_device), None
+    g = SpeculativeGenerator(m, B, T + N, draft)
+    out = g.generate(prompts, N).long()
+    check_errors()
+    text = torch.cat([prompts.long(), out], 1)
+    with torch.no_grad():
+        z = m(torch.nn.functional.pad(text, (0, 256 - T - N)).to(torch.int32))[:, T - 1:T + N - 1].double()
+    gap = z.amax(-1) - z.gather(-1, out[..., None])[..., 0]
+    # a logit is a product of n_embd terms of a normed state and weights of 0.05, each state off by
+    # some roundings of 2^-8 in either path: sqrt(256) * 0.05 * 2^-8 * 8 roundings * 2 paths, four times over
+    assert float(gap.max()) <= 4 * 256 ** 0.5 * 0.05 * 2 ** -8 * 16, gap
