@@ -6,6 +6,11 @@
 // a warp: the row's largest magnitude is then four (three) shuffles away, and a lane's 8 codes
 // leave as one 8-byte store.  A block has one head's neighbouring rows, so that it writes (or
 // reads) one contiguous piece of a head-major cache and of its scales.
+//
+// Measured on a B200 (calls replayed from a graph; floors at 6.54 TB/s): one e4m3 row for 32 sequences
+// of 10 heads 1.9 us; 16 x 4096 rows of 8 heads 70 us of 62; read of 8 x 16384 rows 119 us of 118;
+// commit of 256 trees of 64 nodes, 8 bf16 heads, 21.6 us of 10 (rows of 256 bytes, two dependent
+// loads and a barrier apart).
 // The reference has no decode path; these serve the cache of inference/generate.py.
 #include <cuda_fp8.h>
 
@@ -20,7 +25,8 @@ struct KvRows {                  // rows [B, N, H, D] outside the cache
   long long b[2], n[2], h[2];    // strides in bytes
 };
 
-// Keys' or values' entry of a parameter array; by an index, the array would be copied to local memory.
+// Keys' or values' entry of a parameter array.  Indexed, the array is copied to local memory by every
+// thread: 109 instead of 70 us for 16 x 4096 written rows of 8 heads, 159 instead of 119 for 8 x 16384 read.
 template <typename T>
 __device__ __forceinline__ T pick(const T (&a)[2], int kv) { return kv ? a[1] : a[0]; }
 
@@ -54,8 +60,8 @@ __device__ __forceinline__ uint32_t absmax8(const uint4& u) {
 // A block has one (sequence, head, keys or values) and blockDim / L * U neighbouring rows, a
 // thread U of them in a row.  With U = 4 the four rows' maxima are found together: two 16-bit
 // maxima a word, and the two words of a thread are halved between its lanes in the first step
-// (5 shuffles instead of 16, which with the loads kept the L1 pipe 84 % busy: 114 us for 16 x 4096
-// rows of 8 heads).
+// (5 shuffles instead of 16: 109 instead of 114 us for 16 x 4096
+// rows of 8 heads, when the parameters still were copied to local memory).
 template <int D, bool QUANT, int U>
 __global__ void __launch_bounds__(kKvThreads) kv_cache_write_kernel(const KvRows src, const KvView c, const int* __restrict__ pos,
                                                                     const int* __restrict__ count, int N, int H) {

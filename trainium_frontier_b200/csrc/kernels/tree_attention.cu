@@ -18,9 +18,22 @@
 // output with its maximum and sum in a workspace, and a second, small kernel adds the parts of
 // such a unit in order; results do not depend on timing.
 //
-// Quantised caches: four warps turn the e4m3 tiles into bf16 ones in shared memory, the
+// Quantised caches: eight warps turn the e4m3 tiles into bf16 ones in shared memory, the
 // row's power-of-two scale included (exactly, see kv_cache.cuh), since a product of a 16-bit
-// and an 8-bit operand does not exist and q in 8 bits would lose half its significand.
+// and an 8-bit operand does not exist and q in 8 bits would lose half its significand.  (f16 tiles
+// brought to the largest scale of 32 rows convert in a fifth of the instructions, but a small row
+// beside a large one that the query does not see then loses its bits.)
+//
+// Up to 16 query rows a key/value head take the kernel of tree_attention_few.cuh.
+//
+// Measured on a B200 (calls replayed from a graph; the floor is the bytes at 6.54 TB/s or the
+// products at 1.68 PFLOP/s): 64-node trees, 32 / 8 heads, 16 sequences of 4096 .. 8191 bf16 rows: 137 us
+// of 65; 24-node trees, 32 / 8 heads, 8 sequences of 32768 .. 65535 e4m3 rows: 352 us of 125.  What is
+// left there is mostly the softmax and conversion warps' latency.  Parts left out in a copy: the first
+// case, 138 us whole, took 126 without exponentials and 113 with an eighth of the products besides;
+// the second, 527 us before the conversion loop was shortened, 392 without conversion, 454 without
+// exponentials and 318 without either (376 after it, 350 without polynomial exponentials
+// as well).  Tiles of 64 keys with deeper rings were slower (145 and 705 us).
 //
 // A row behind the context that no node uses may hold anything: its scores are masked, and its
 // values are zeroed in shared memory before the product (0 * NaN is NaN).  A drafted row that is
@@ -315,8 +328,10 @@ struct TreeCfg {
 static_assert(TreeCfg<128, false, 1>::SMEM <= 232448 && TreeCfg<128, true, 1>::SMEM <= 232448 && TreeCfg<128, false, 2>::SMEM <= 232448 &&
               TreeCfg<128, true, 2>::SMEM <= 232448, "shared memory");
 
-// Roles: warp 0 loads (TMA: one lane keys and queries, one values), warps 1 and 2 issue the products of a group each, two groups of four warps run the
-// softmax, the rest converts quantised tiles or clears unused rows of value tiles.  A group works
+// Roles: warp 0 loads (TMA: one lane keys and queries, one lane values), warps 1 and 2 issue the
+// products of a group each (one warp for both was busy with nothing else: 158 against 143 us), two
+// groups of four warps run the softmax, the rest converts quantised tiles or clears unused rows of
+// value tiles.  A group works
 // through half tiles of 64 keys:
 //   NT = 2: group t has row tile t and takes both halves of every key tile in turn;
 //   NT = 1: both groups have the one row tile, group t half t of every key tile, each with a
@@ -765,7 +780,7 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
       // four warps convert the keys, four the values, 32 neighbouring rows of a tile each: a lane
       // looks after one row's scale, fetched while the tile before is converted, and has 16 codes of
       // every RPI-th row.  The loop stays short on purpose: unrolled over all rows it ran out of the
-      // instruction caches (the first cause of stalls, 3.3 warps of 11.7).
+      // instruction caches (3.3 of 11.7 warps stalled on that; 525 against 375 us).
       constexpr int CH = D / 16, RPI = 32 / CH;             // 16-code chunks a row, rows an iteration
       const int v = tid >> 7, cw = (tid >> 5) & 3, ch = lane % CH, own = cw * 32 + lane;
       const int R = v ? NV : NK;
@@ -1003,7 +1018,10 @@ at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor
   TORCH_CHECK(B * N * Hq < (1LL << 31), "too many query rows");
   const int G = (int)(Hq / H);
   a.B = (int)B; a.N = (int)N; a.Hq = (int)Hq; a.Hkv = (int)H; a.G = G;
-  // up to 32 rows a key/value head: the register kernel, with 8, 16 or 32 rows
+  // up to 16 rows a key/value head: the register kernel.  16 sequences of 8191 rows, 8 heads of 128:
+  // bf16 76 us against 79 for the tensor-core tiles at 1 .. 8 rows, 85 against 81 at 16; e4m3 82 against
+  // 110 and 96 against 112; 32 sequences of 575 bf16 rows 25 against 33.  With 32 rows it spilled: 180
+  // against 83.
   const int rows = (int)std::min<int64_t>(N * G, 1 << 20), EH = rows <= 8 ? 1 : rows <= 16 ? 2 : 0;
   // rows of a tile: nb nodes of gb heads each
   a.gb = std::min(G, 128);
