@@ -23,8 +23,9 @@
 // warps' sums behind, so the draw re-reads only the range in which its token lies.
 //
 // Measured on a B200 (calls replayed from a graph): 8 sequences x 6 nodes, vocabulary 8192: 6.2 us;
-// 64 x 24 nodes, 131072: 39 us (47 with one subtraction a rejection), where the last rows alone are 10 us at the memory's rate.  The bound
-// is the slowest sequence's chain of passes (each waits for the one before), not the bytes.
+// 64 x 24 nodes, 131072: 36 us (47 with one subtraction a rejection and eight CTAs a row), where the
+// last rows alone are 10 us at the memory's rate.  The bound is the slowest sequence's chain of
+// passes, up to four there, each of which waits for the one before.
 // The reference has no decode path.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -34,6 +35,8 @@
 #include "sm100_common.cuh"
 
 namespace tfb {
+
+int num_sms(int dev);
 
 constexpr int kVerThreads = 512;
 constexpr int kVerWarps = kVerThreads / 32;
@@ -323,13 +326,18 @@ std::vector<at::Tensor> verify_tree(at::Tensor tokens, at::Tensor parents, at::T
   if (B == 0) return {path, count, out};
   a.path = path.data_ptr<int>(); a.count = count.data_ptr<int>(); a.out = out.data_ptr<int>();
   a.N = (int)N; a.V = (int)V;
-  // CTAs of a cluster: one for each 16384 entries.  Exchanging sums costs a pass about 1 us, so
-  // a row of 8192 is best left to one CTA (8 sequences x 6 nodes: 6.7 us, 7.9 with two, 8.4 with
-  // eight), and one of 131072 shared by eight (64 x 24 nodes: 39 us).
-  int C = 1;
-  while (C < kVerCluster && (int64_t)C * 16384 < V) C *= 2;
-  a.range = (int)(((V + C * kVerWarps - 1) / (C * kVerWarps) + 127) / 128 * 128);
   TORCH_CHECK(B <= (1LL << 31) / kVerCluster - 1, "too many sequences");
+  // CTAs of a cluster: at most one for each 16384 entries, since exchanging sums costs a pass about
+  // 1 us (8 sequences x 6 nodes, 8192 entries: 6.7 us with one, 7.9 with two, 8.4 with eight,
+  // when a pass still took one subtraction a rejection).  Two CTAs
+  // fit on a SM; more than that wait their turn, which pays only while a CTA's range is long: turns
+  // at most as many as times 16384 entries a CTA.  131072 entries, 24 nodes, with 1 / 2 / 4 / 8 CTAs:
+  // 32 sequences 60 / 38 / 25 / 22 us, 64: 65 / 42 / 34 / 40, 128: 92 / 65 / 57 / 70, 256: 113 / 87 / 89 / 125;
+  // 32768 entries: 128 sequences 30 / 27 / 31 / 56, 512: 53 / 64 / 94 / 191.
+  const int64_t slots = 2 * num_sms(p.device().index());
+  int C = 1;
+  while (C < kVerCluster && (int64_t)C * 16384 < V && B * (2 * C) * (2 * C) * 16384 <= slots * V) C *= 2;
+  a.range = (int)(((V + C * kVerWarps - 1) / (C * kVerWarps) + 127) / 128 * 128);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
