@@ -636,3 +636,28 @@ def test_refusals(device):
             call()
     with pytest.raises(ValueError):
         ops.kv_cache_alloc(1, 1, 1, 64, layout="row")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("V", [64, 20000, 131072])
+@pytest.mark.parametrize("sharp", [0.5, 0.99, 0.9999])
+def test_verify_remainder_far_below_one(device, V, sharp):
+    """Many rejections of tokens that the target wants less than the draft, where one token keeps a
+    remainder: it falls by 1 - q[t] at each (down to 1e-4 ** 23 here), and stays the only one left,
+    so that the next token is t whatever the numbers are."""
+    B, N, t = 4, 24, V // 3
+    q = torch.full((B, N, V), (1 - sharp) / (V - 1))
+    p = torch.full((B, N, V), (1 - sharp) / (V - 1) / 2)
+    q[..., t], p[..., t] = sharp, (1 + sharp) / 2
+    g = torch.Generator().manual_seed(V)
+    tokens = torch.randint(0, V - 1, (B, N), generator=g, dtype=torch.int32)
+    tokens += (tokens >= t).to(torch.int32)
+    parents = torch.zeros(B, N, dtype=torch.int32)
+    parents[:, 0] = -1
+    u = torch.rand(B, N, generator=g)
+    u[:, 1] = 0.75                        # 2 u q > 2 p; later ones have no remainder, whatever u
+    u[1:, 2:] = u[1:, 2:] / 4
+    args = [x.to(device) for x in (tokens, parents, p, q, u)]
+    path, count, out = ops.verify_tree(*args)
+    assert count.tolist() == [1] * B
+    assert path[:, 0].tolist() == [0] * B and out[:, 0].tolist() == [t] * B

@@ -17,7 +17,9 @@
 // What a sequence has to read whole is one row of p, and of q after a rejection: the tests
 // themselves read single entries, gathered for all nodes at once by one thread a node.  r is
 // not stored: each pass recomputes it from p and q as max(p - S q, 0), S the sum of the Z's of the
-// rejections so far, which is all of them in one step, since q and Z are not negative.  A
+// rejections so far, which is all of them in one step, since q and Z are not negative.  Its error is
+// 2^-53 of p, the same as a single step's, but the steps one by one keep a remainder that has become
+// small exact to 2^-53 of itself: below Z = 2^-20 they are taken one by one.  A
 // cluster of CTAs shares a row, every warp a contiguous range of it, and all CTAs take the same
 // decisions from the same sums, read from each other's shared memory.  The last pass leaves the
 // warps' sums behind, so the draw re-reads only the range in which its token lies.
@@ -86,6 +88,7 @@ template <bool VEC, bool HASQ>
 __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(const VerArgs a) {
   __shared__ int s_tok[kVerNodes], s_par[kVerNodes], s_path[kVerNodes];
   __shared__ float s_u[kVerNodes], s_p[kVerNodes], s_q[kVerNodes];
+  __shared__ double s_z[kVerNodes];          // Z before each rejection at the current node
   __shared__ int s_rej[kVerNodes];           // the rejected tokens (q absent)
   __shared__ double s_sum[kVerWarps];        // the warps' sums of the last pass
   __shared__ double s_tot[2];                // this CTA's sum, two passes in turn
@@ -113,6 +116,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(const VerAr
 
   int cur = 0, cnt = 1, rej = 0, turn = 0;
   double Z = 1.0, S = 0.0, share = 0.0;      // S: sum of Z over the rejections; share: lane i has CTA i's part of the last pass's total
+  bool deep = false;                         // Z is small: rejections one by one (q given)
   bool summed = false;                       // s_sum and share belong to the present r
   const long long w0 = (long long)(rank * kVerWarps + warp) * a.range;   // this warp's range
   const int lo = (int)min((long long)V, w0), hi = (int)min((long long)V, w0 + a.range);
@@ -122,7 +126,14 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(const VerAr
 #pragma unroll
     for (int i = 0; i < M; ++i) r[i] = (double)f[i];
     if constexpr (HASQ) {
-      if (rej > 0) {
+      if (deep) {
+#pragma unroll 1
+        for (int k = 0; k < rej; ++k) {
+          const double z = s_z[k];
+#pragma unroll
+          for (int i = 0; i < M; ++i) r[i] = clear_negative(__dsub_rn(r[i], __dmul_rn(z, (double)g[i])));
+        }
+      } else if (rej > 0) {
 #pragma unroll
         for (int i = 0; i < M; ++i) r[i] = clear_negative(__fma_rn(-S, (double)g[i], r[i]));
       }
@@ -189,25 +200,34 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(const VerAr
     double r[1];
     rest(r, f, g, s_tok[n], 1);
     if (__dmul_rn(__dmul_rn((double)s_u[n], (double)g[0]), Z) < r[0]) {
-      __syncthreads();                       // s_path, and s_rej of the node left behind
+      __syncthreads();                       // s_path, and s_z / s_rej of the node left behind
       cur = n;
       if (tid == 0) s_path[cnt] = n;
       ++cnt;
       rej = 0;
       Z = 1.0;
       S = 0.0;
+      deep = false;
       summed = false;
     } else {
       __syncthreads();
-      if (tid == 0) s_rej[rej] = s_tok[n];
+      if (tid == 0) {
+        s_z[rej] = Z;
+        s_rej[rej] = s_tok[n];
+      }
       ++rej;
       S += Z;
       __syncthreads();
       Z = pass();
+      if (HASQ && !deep && Z < 0x1p-20) {
+        deep = true;
+        if (rej > 1) Z = pass();             // the first rejection is one step in any case
+      }
       if (!(Z > 0.0)) {                      // nothing is left (p = q up to rounding): p itself
         rej = 0;
         Z = 1.0;
         S = 0.0;
+        deep = false;
         summed = false;
       }
     }
