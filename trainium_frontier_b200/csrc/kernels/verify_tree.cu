@@ -24,8 +24,8 @@
 // decisions from the same sums, read from each other's shared memory.  The last pass leaves the
 // warps' sums behind, so the draw re-reads only the range in which its token lies.
 //
-// Measured on a B200 (calls replayed from a graph): 8 sequences x 6 nodes, vocabulary 8192: 6.2 us;
-// 64 x 24 nodes, 131072: 36 us (47 with one subtraction a rejection and eight CTAs a row), where the
+// Measured on a B200 (calls replayed from a graph): 8 sequences x 6 nodes, vocabulary 8192: 6.7 us;
+// 64 x 24 nodes, 131072: 38 us (47 with one subtraction a rejection and eight CTAs a row), where the
 // last rows alone are 10 us at the memory's rate.  The bound is the slowest sequence's chain of
 // passes, up to four there, each of which waits for the one before.
 // The reference has no decode path.
@@ -152,21 +152,36 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(const VerAr
     const float* pr = P + cur * a.pn;
     const float* qr = HASQ ? Q + cur * a.qn : nullptr;
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int j = lo + lane * 4; j < hi; j += 512) {
-      float f[4][4], g[4][4] = {};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        load4<VEC>(pr, j + 128 * k, hi, f[k]);
-        if constexpr (HASQ) {
-          if (rej > 0) load4<VEC>(qr, j + 128 * k, hi, g[k]);
-        }
+    if (HASQ && deep) {                      // in a loop of its own: 38 against 42 us
+#pragma unroll 1
+      for (int j = lo + lane; j < hi; j += 32) {
+        const float f[1] = {pr[j]}, g[1] = {qr[j]};
+        double r[1];
+        rest(r, f, g, j, 1);
+        acc[0] += r[0];
       }
+    } else {
+      for (int j = lo + lane * 4; j < hi; j += 512) {
+        float f[4][4], g[4][4] = {};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        double r[4];
-        rest(r, f[k], g[k], j + 128 * k, 4);
+        for (int k = 0; k < 4; ++k) {
+          load4<VEC>(pr, j + 128 * k, hi, f[k]);
+          if constexpr (HASQ) {
+            if (rej > 0) load4<VEC>(qr, j + 128 * k, hi, g[k]);
+          }
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] += r[i];
+        for (int k = 0; k < 4; ++k) {
+          double r[4];
+          if constexpr (HASQ) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = clear_negative(__fma_rn(-S, (double)g[k][i], (double)f[k][i]));   // S = 0: r = p
+          } else {
+            rest(r, f[k], g[k], j + 128 * k, 4);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] += r[i];
+        }
       }
     }
     double s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
@@ -353,7 +368,8 @@ std::vector<at::Tensor> verify_tree(at::Tensor tokens, at::Tensor parents, at::T
   // fit on a SM; more than that wait their turn, which pays only while a CTA's range is long: turns
   // at most as many as times 16384 entries a CTA.  131072 entries, 24 nodes, with 1 / 2 / 4 / 8 CTAs:
   // 32 sequences 60 / 38 / 25 / 22 us, 64: 65 / 42 / 34 / 40, 128: 92 / 65 / 57 / 70, 256: 113 / 87 / 89 / 125;
-  // 32768 entries: 128 sequences 30 / 27 / 31 / 56, 512: 53 / 64 / 94 / 191.
+  // 32768 entries: 128 sequences 30 / 27 / 31 / 56, 512: 53 / 64 / 94 / 191 (all 5 to 8 % less than now:
+  // before small remainders were taken one by one).
   const int64_t slots = 2 * num_sms(p.device().index());
   int C = 1;
   while (C < kVerCluster && (int64_t)C * 16384 < V && B * (2 * C) * (2 * C) * 16384 <= slots * V) C *= 2;
