@@ -1,0 +1,57 @@
+"""Speculative-decoding operators at the ends of their number formats: NaN codes and scales, infinite
+scores, rows near the least and the greatest numbers."""
+import math
+
+import pytest
+import torch
+
+from tests._specutil import BF16, E4M3, attention64, make_cache, quant_row, raw
+from trainium_frontier_b200 import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+# nodes and query heads a key/value head: 1, 8, 16, 17, 120 and 256 query rows, for every kernel and tile form
+ROWS = [(1, 1), (4, 2), (2, 8), (1, 17), (6, 20), (4, 64)]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def i32(x, device):
+    return torch.tensor(x, dtype=torch.int32, device=device)
+
+
+def attend(q, cache, lens, parents, scale=None):
+    """tree_attention against the formula in 64 bits, infinities and NaN included."""
+    kc, vc, ks, vs = cache
+    device, D = kc.device, q.shape[-1]
+    o = ops.tree_attention(q.to(device), kc, vc, i32(lens, device), None if parents is None else parents.to(device), scale, ks, vs)
+    o = o.double().cpu()
+    want, bound = attention64(q, kc, vc, lens, parents, D ** -0.5 if scale is None else scale, ks, vs)
+    assert torch.equal(torch.isnan(o), torch.isnan(want)), (torch.isnan(o).sum(), torch.isnan(want).sum())
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(o), inf) and torch.equal(o[inf], want[inf])
+    fine = torch.isfinite(want)
+    err = (o - want).abs()
+    assert bool((err <= bound)[fine].all()), float((err / bound)[fine].max())
+    return want
+
+
+def queries(B, N, Hq, D, seed=4):
+    return torch.randn(B, N, Hq, D, generator=gen(seed)).to(BF16)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("N,G", ROWS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_nan_value_row_reaches_all_that_see_it(device, N, G, D):
+    """Quantised value rows with the scale NaN: the newest token's, by itself among its neighbours or
+    not, and a run of 16 context rows."""
+    lens = [0, 16, 37, 128, 192]
+    cache = make_cache(len(lens) + 1, 2, 270, D, E4M3, "head", device, gen(D))
+    for b, ln in enumerate(lens):
+        raw(cache[3])[b, 0, ln + N - 1] = 255
+    raw(cache[3])[-1, 1, 16:32] = 255
+    want = attend(queries(len(lens) + 1, N, 2 * G, D), cache, lens + [200], None)
+    assert bool(want[:-1, N - 1, :G].isnan().all()) and bool(want[-1, :, G:].isnan().all())
+    assert bool(want[:-1, :, G:].isfinite().all()) and bool(want[:-1, :N - 1].isfinite().all())

@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 
     // ---- exponentials: element k of fragment t is (row half k >> 1, key 8 t + 2 j + (k & 1))
     float fk[4], ev[4];
-    bool alive[4];                                        // the key's row holds something that counts
+    bool alive[4], lost[4];                               // the key's row holds something that counts; its scale is NaN
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int at = off + key_of(i) - warp * 16;
@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         const float nan = __int_as_float(0x7fffffff);
         const uint32_t ck = __shfl_sync(0xffffffffu, bytes, key_of(i) - warp * 16), cv = __shfl_sync(0xffffffffu, bytes, 16 + key_of(i) - warp * 16);
         fk[i] = ck == (uint32_t)kScaleNan ? nan : __uint_as_float(max(ck, 1u) << 23);
-        ev[i] = cv == (uint32_t)kScaleNan ? nan : (float)((int)cv - 127);
-        alive[i] = alive[i] && cv != (uint32_t)kScaleNan;   // such a row's weight is NaN already
+        lost[i] = cv == (uint32_t)kScaleNan;              // its values are NaN; the weight is an ordinary one
+        ev[i] = lost[i] ? 0.f : (float)((int)cv - 127);
       }
     }
     uint32_t pa[MT][4];
@@ -429,9 +429,18 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           const uint2 x = *reinterpret_cast<const uint2*>(sV + code_chunk<D>(row, gq >> 1) + (gq & 1) * 8);
           v[i][0] = x.x; v[i][1] = x.y;
         }
-        if (!alive[i]) {
+      }
+      // NaN codes for a context row whose scale is NaN, since all queries see it; zeros for rows that
+      // nothing may see, and for such a drafted row, which is added at the segment's end
+      if (masked || __any_sync(0xffffffffu, lane >= 16 && bytes == (uint32_t)kScaleNan)) {
 #pragma unroll
-          for (int w = 0; w < W; ++w) v[i][w] = 0;
+        for (int i = 0; i < 4; ++i) {
+          const int at = off + key_of(i) - warp * 16;
+          if (!alive[i] || lost[i]) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) v[i][w] = alive[i] && at < 0 ? 0x7f7f7f7fu : 0u;
+          }
+          if (alive[i] && lost[i] && at >= 0) atomicOr(&s_bad[seg & 1], 1ull << at);
         }
       }
 #pragma unroll
@@ -564,12 +573,16 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           const int n = r / a.G, hd = r - n * a.G;
           const unsigned long long ln = s_line[r];
           const int col = h0 + 4 * c4;
-          unsigned long long bad = QUANT ? 0 : s_bad[seg & 1] & ln;
+          unsigned long long bad = s_bad[seg & 1] & ln;
           for (; bad; bad &= bad - 1) {                    // drafted rows with an infinity or a NaN: those entries
+            float* xs = &x.x;
+            if constexpr (QUANT) {                         // the row's scale is NaN
+              for (int k = 0; k < 4; ++k) xs[k] = __int_as_float(0x7fffffff);
+              continue;
+            }
             const int node = __ffsll((long long)bad) - 1;
             const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(c.p[1] + it.b * c.b + it.h * c.h +
                                                                               ((long long)it.len + node) * c.t) + col;
-            float* xs = &x.x;
             for (int k = 0; k < 4; ++k) {
               const float y = __bfloat162float(row[k]);
               if (!(fabsf(y) < INFINITY)) xs[k] += y;
