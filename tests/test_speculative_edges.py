@@ -55,3 +55,27 @@ def test_a_nan_value_row_reaches_all_that_see_it(device, N, G, D):
     want = attend(queries(len(lens) + 1, N, 2 * G, D), cache, lens + [200], None)
     assert bool(want[:-1, N - 1, :G].isnan().all()) and bool(want[-1, :, G:].isnan().all())
     assert bool(want[:-1, :, G:].isfinite().all()) and bool(want[:-1, :N - 1].isfinite().all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("N,G", ROWS)
+def test_a_nan_value_counts_however_small_its_weight(device, dtype, N, G):
+    """64 neighbouring context rows whose weights are below 2^-300 of the others', one of them with a
+    NaN value: a product with NaN is NaN."""
+    D, T = 64, 270
+    cache = make_cache(1, 1, T, D, dtype, "head", device, gen(1))
+    kc, vc, ks, vs = cache
+    if dtype == E4M3:
+        raw(kc)[:, :, 64:128] = 0xd0          # -8
+        raw(ks)[:, :, 64:128] = 127
+        raw(vs)[:, :, 70] = 255
+    else:
+        kc[:, :, 64:128] = -8.0
+        vc[:, :, 70, 3:] = math.nan
+    q = (queries(1, N, G, D).abs() * 0.25 + 4).to(BF16)
+    par = torch.arange(-1, N - 1, dtype=torch.int32)[None]
+    if N > 2:
+        par[0, 1] = -2                        # and the nodes behind it: unused, zero all the same
+    want = attend(q, cache, [130], par)
+    assert bool(want[0, 0, :, 3:].isnan().all())

@@ -702,8 +702,9 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
           tmem_ld_wait();
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            f[k] = f0 != 0.f ? __uint_as_float(o[k]) * f0 : 0.f;
-            if constexpr (NT == 1) f[k] += f1 != 0.f ? __uint_as_float(o1[k]) * f1 : 0.f;
+            f[k] = __uint_as_float(o[k]) * f0;       // the factors may be 0: a NaN stays
+            if constexpr (NT == 1) f[k] += __uint_as_float(o1[k]) * f1;
+            if (line == 0) f[k] = 0.f;
           }
           if (bad) tree_add_bad<QUANT>(f, bad, c, it.b, it.h, it.len, cc * 16);
           if (!live) continue;

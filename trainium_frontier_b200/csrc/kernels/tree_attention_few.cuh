@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
             for (int q = 0; q < MT; ++q)
               if (q == mt) x = o[q][i][k];
-            if (d >= 0 && d < hc && (k >> 1) * 8 + gq < rp) dst[((k >> 1) * 8 + gq) * (hc + 4) + d] = f[k >> 1] == 0.f ? 0.f : x * f[k >> 1];
+            if (d >= 0 && d < hc && (k >> 1) * 8 + gq < rp) dst[((k >> 1) * 8 + gq) * (hc + 4) + d] = x * f[k >> 1];   // f may be 0: a NaN stays
           }
         __syncthreads();
         const int per = hc / 4, rr = threadIdx.x / per, r = mt * 16 + rr, c4 = threadIdx.x - rr * per;
