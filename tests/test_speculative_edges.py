@@ -79,3 +79,28 @@ def test_a_nan_value_counts_however_small_its_weight(device, dtype, N, G):
         par[0, 1] = -2                        # and the nodes behind it: unused, zero all the same
     want = attend(q, cache, [130], par)
     assert bool(want[0, 0, :, 3:].isnan().all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("N,G", ROWS)
+def test_scores_of_minus_infinity_alone(device, N, G):
+    """Where every visible score is -inf the softmax is 0 / 0; beside a finite one they count nothing,
+    and unused nodes stay zero."""
+    D, T = 128, 1300
+    lens = [0, 3, 1000, 1000, 1000]
+    kc, vc, _, _ = cache = make_cache(5, 1, T, D, BF16, "head", device, gen(2))
+    kc[0, 0, 0, 0] = -math.inf                # node 0
+    kc[1, 0, :4, 0] = -math.inf               # the context and node 0
+    kc[2, 0, :, 0] = -math.inf                # everything: a NaN row over many tiles
+    kc[3, 0, :, 0] = -math.inf
+    kc[3, 0, 700, 0] = 1.0                    # all but one
+    kc[4, 0, :, 0] = -math.inf
+    par = torch.arange(-1, N - 1, dtype=torch.int32).expand(5, N).contiguous()
+    if N > 1:
+        par[4, -1] = -2
+    q = queries(5, N, G, D)
+    q[..., 0] = q[..., 0].abs() + 1
+    want = attend(q, cache, lens, par)
+    assert bool(want[[0, 1, 2], 0].isnan().all()) and bool(want[2].isnan().all()) and bool(want[3].isfinite().all())
+    if N > 1:
+        assert bool(want[0, 1:].isfinite().all()) and bool((want[4, -1] == 0).all())

@@ -64,7 +64,8 @@ struct TreeArgs {
   float scale_log2;          // |scale| log2(e), never 0
   int neg;                   // scale < 0
   float4* part;              // [2 * grid][NT][D / 4][128 rows] unnormalised partial outputs
-  float2* part_ml;           // [2 * grid][NT * 128] their maximum (log2 units) and sum
+  float2* part_ml;           // [2 * grid][NT * 128] their maximum (log2 units) and sum: (-inf, 0) where no score
+                             // is above -inf, (inf, 0) for an unused node
   float2* pair_ml;           // [grid][128] group 1's, for group 0 (NT = 1)
   int* err;
 };
@@ -686,8 +687,7 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
       if (warp_live) {
         const bool whole = it.k0 == 0 && it.k1 == it.kt;
         const long long slot = 2LL * blockIdx.x + (it.k0 == 0 ? 1 : 0);
-        const float inv = line != 0 && l != 0.f ? 1.f / l : 0.f;
-        if (line == 0 || l == 0.f) f0 = f1 = 0.f;   // an unused node, or nothing seen
+        const float inv = line != 0 ? 1.f / l : 0.f;   // l = 0: all scores are -inf, and 0 / 0 is NaN
         const unsigned long long bad = s_poison[it.seg & (kSegRing - 1)] & line;
         __nv_bfloat16* dst = a.o + (((long long)it.b * a.N + n) * a.Hq + it.h * a.G + head) * D;
         float4* pd = a.part + (slot * NT + (NT == 1 ? 0 : t)) * (D / 4) * 128 + r;
@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
             for (int k = 0; k < 4; ++k) pd[(cc * 4 + k) * 128] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
           }
         }
-        if (live && !whole) a.part_ml[(slot * NT + (NT == 1 ? 0 : t)) * 128 + r] = line != 0 ? make_float2(m_run, l) : make_float2(-INFINITY, 0.f);
+        if (live && !whole) a.part_ml[(slot * NT + (NT == 1 ? 0 : t)) * 128 + r] = line != 0 ? make_float2(m_run, l) : make_float2(INFINITY, 0.f);
       }
       tc_fence_before();
       if (NT == 1) mbar_arrive(o_free);
@@ -899,7 +899,7 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeArgs a, con
   if (live)
     for (int i = c0 + ps; i <= c1; i += PS) {
       const float2 ml = __ldcg(&a.part_ml[place(i) * 128 + r]);
-      if (ml.y != 0.f) M = fmaxf(M, ml.x);
+      M = fmaxf(M, ml.x);
     }
   for (int o = RP; o < 32; o *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   float4 acc[Q];
@@ -914,8 +914,7 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeArgs a, con
       float4 v[Q];
 #pragma unroll
       for (int q = 0; q < Q; ++q) v[q] = __ldcg(p + q * 128);
-      if (ml.y == 0.f) continue;             // the row saw nothing there
-      const float f = tree_ex2(ml.x - M);
+      const float f = ml.y == 0.f ? 0.f : tree_ex2(ml.x - M);   // 0: the row saw nothing there, or -inf only
       L += f * ml.y;
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
@@ -934,7 +933,12 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeArgs a, con
     }
   }
   if (!live || ps != 0) return;
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const bool used = !(L == 0.f && M == INFINITY);
+  const float inv = used ? 1.f / L : 0.f;    // L = 0: all scores are -inf, and 0 / 0 is NaN
+  if (!used) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   __nv_bfloat16* dst = a.o + (((long long)b * a.N + n) * a.Hq + h * a.G + head) * D + warp * Q * 4;
 #pragma unroll
   for (int q = 0; q < Q; q += 2) {

@@ -589,13 +589,13 @@ __global__ void __launch_bounds__(kFewThreads, 1)
             }
           }
           if (whole) {
-            const float inv = ln == 0 || L == 0.f ? 0.f : 1.f / L;
-            if (inv == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float inv = ln == 0 ? 0.f : 1.f / L;     // L = 0: all scores are -inf, and 0 / 0 is NaN
+            if (ln == 0) x = make_float4(0.f, 0.f, 0.f, 0.f);
             *reinterpret_cast<uint2*>(a.o + (((long long)it.b * a.N + n) * a.Hq + it.h * a.G + hd) * D + col) =
                 make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
           } else {
             a.part[(part * (D / 4) + (col >> 2)) * 128 + r] = x;
-            if (h0 == 0 && c4 == 0) a.part_ml[part * 128 + r] = ln == 0 ? make_float2(-INFINITY, 0.f) : make_float2(M, L);
+            if (h0 == 0 && c4 == 0) a.part_ml[part * 128 + r] = ln == 0 ? make_float2(INFINITY, 0.f) : make_float2(M, L);
           }
         }
         __syncthreads();
