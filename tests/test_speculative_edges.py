@@ -104,3 +104,40 @@ def test_scores_of_minus_infinity_alone(device, N, G):
     assert bool(want[[0, 1, 2], 0].isnan().all()) and bool(want[2].isnan().all()) and bool(want[3].isfinite().all())
     if N > 1:
         assert bool(want[0, 1:].isfinite().all()) and bool((want[4, -1] == 0).all())
+
+
+def nan_codes(device, N, G, D, code):
+    """e4m3's two NaN codes, single ones under ordinary scales, in key and value rows of the context, of
+    drafted nodes and of rows that no node sees."""
+    B, T = 6, 280
+    lens = [130, 130, 125, 125, 60, 0]
+    cache = make_cache(B, 1, T, D, E4M3, "head", device, gen(3))
+    kc, vc = raw(cache[0]), raw(cache[1])
+    vc[0, 0, 7, 5] = code
+    vc[0, 0, 129, D - 1] = code
+    kc[1, 0, 66, D - 2] = code
+    vc[2, 0, 125, 9] = code                   # node 0, seen by all nodes below it
+    vc[2, 0, 125 + N - 1, D - 3] = code       # the last one, seen by itself
+    kc[3, 0, 125 + N - 1, 1] = code
+    vc[4, 0, 60 + N:, ::3] = code             # behind the nodes
+    kc[4, 0, 60 + N:, ::3] = code
+    vc[5, 0, N - 1, 2] = code
+    par = torch.arange(-1, N - 1, dtype=torch.int32).expand(B, N).contiguous()
+    par[:, -1] = -1                           # a root of its own
+    if N > 2:
+        par[4, 1] = -2
+        vc[4, 0, 61, :] = code                # an unused node's
+        kc[4, 0, 61, :] = code
+    want = attend(queries(B, N, G, D), cache, lens, par)
+    assert bool(want[1].isnan().all()) and bool(want[4].isfinite().all())
+    assert bool(want[2, 0, :, 9].isnan().all()) and bool(want[5, N - 1, :, 2].isnan().all())
+    if N > 1:
+        assert bool(want[2, 0, :, D - 3].isfinite().all()) and bool(want[3, 0].isfinite().all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("N,G", ROWS[:3])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("code", [0x7f, 0xff])
+def test_nan_codes_with_few_rows(device, N, G, D, code):
+    nan_codes(device, N, G, D, code)

@@ -68,6 +68,15 @@ __device__ __forceinline__ uint32_t codes2(uint32_t x) {
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(y) : "r"(x));
   return y;
 }
+// Bit 7 of every byte: whether that e4m3 code is one of the two NaNs.
+__device__ __forceinline__ uint32_t code4_nan(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ float e4m3_float(uint8_t x) {
+  const uint32_t h = codes2(x);
+  return __half2float(__ushort_as_half((unsigned short)h));
+}
+__device__ __forceinline__ float scale_float(uint8_t e) {
+  return e == kScaleNan ? __int_as_float(0x7fffffff) : e == 0 ? 0x1p-127f : __uint_as_float((uint32_t)e << 23);
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t y;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
@@ -81,6 +90,21 @@ __device__ __forceinline__ uint32_t code_chunk(int row, int chunk) {
 __device__ __forceinline__ bool bf16_bad(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
 // bits 15 and 31: whether the halves are infinite or NaN
 __device__ __forceinline__ uint32_t bf16x2_bad(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+
+// x plus four columns of an e4m3 value row, times its weight and scale.  Out of line since it is rare, and in
+// line it cost the loop over the tiles registers (16 rows: 114 against 111 us).
+template <int D>
+__device__ __noinline__ float4 tree_add_row(float4 x, const __nv_bfloat16* q, const uint8_t* key, const uint8_t* value, float scale, float M,
+                                          float vscale) {
+  float y = 0.f;
+  for (int d = 0; d < D; ++d) y += __bfloat162float(q[d]) * e4m3_float(key[d]);
+  const float p = tree_ex2(y * scale - M) * vscale;
+  x.x += p * e4m3_float(value[0]);
+  x.y += p * e4m3_float(value[1]);
+  x.z += p * e4m3_float(value[2]);
+  x.w += p * e4m3_float(value[3]);
+  return x;
+}
 
 // EH: halves of the 16-row tile that hold rows
 template <int D, bool QUANT, int EH>
@@ -195,6 +219,18 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   if (nx.next(lens, a.rg)) fetch_scales(nx);
   while (it.next(lens, a.rg)) {
     if (it.first()) {
+      // Drafted value rows (at most 16) that hold a NaN code (0 * NaN is NaN): they are left out of the
+      // product like unused ones, and what the nodes that see them get of them is added at the segment's
+      // end.  (Looked for in every tile, the branch alone cost 2 to 7 %: 118 against 109 us for 16 rows.)
+      uint32_t drafted[2] = {0, 0};
+      if constexpr (QUANT) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int n = warp + i * kFewWarps;
+          if (lane < D / 4 && it.k1 * 128 > it.len && n < a.N && it.len + n < c.tmax)
+            drafted[i] = reinterpret_cast<const uint32_t*>(c.p[1] + it.b * c.b + it.h * c.h + ((long long)it.len + n) * c.t)[lane];
+        }
+      }
       // queries as fragments, a step of 16 dimensions a warp at a time
       if constexpr (QUANT) {
         // f16, each row by a power of two that takes its largest value to 2^14 .. 2^15
@@ -247,6 +283,11 @@ __global__ void __launch_bounds__(kFewThreads, 1)
             cr[mt][e] = a.neg ? -a.scale_log2 : a.scale_log2;
           }
       }
+      if constexpr (QUANT) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (__any_sync(0xffffffffu, code4_nan(drafted[i]) != 0) && lane == 0) atomicOr(&s_bad[seg & 1], 1ull << (warp + i * kFewWarps));
+      }
       unsigned long long m0, m1;
       tree_lines(a.parents ? a.parents + (long long)it.b * a.N : nullptr, a.N, c.tmax - it.len, m0, m1);
       used = used_nodes(m0, m1);
@@ -268,6 +309,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
           for (int k = 0; k < 4; ++k) o[mt][i][k] = 0.f;
       __syncthreads();
+      if constexpr (QUANT) used &= ~s_bad[seg & 1];
     }
     const uint32_t bytes = ahead;
     if (nx.next(lens, a.rg)) fetch_scales(nx);
@@ -326,7 +368,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 
     // ---- exponentials: element k of fragment t is (row half k >> 1, key 8 t + 2 j + (k & 1))
     float fk[4], ev[4];
-    bool alive[4], lost[4];                               // the key's row holds something that counts; its scale is NaN
+    bool alive[4];                                        // the key's row holds something that counts
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int at = off + key_of(i) - warp * 16;
@@ -335,8 +377,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         const float nan = __int_as_float(0x7fffffff);
         const uint32_t ck = __shfl_sync(0xffffffffu, bytes, key_of(i) - warp * 16), cv = __shfl_sync(0xffffffffu, bytes, 16 + key_of(i) - warp * 16);
         fk[i] = ck == (uint32_t)kScaleNan ? nan : __uint_as_float(max(ck, 1u) << 23);
-        lost[i] = cv == (uint32_t)kScaleNan;              // its values are NaN; the weight is an ordinary one
-        ev[i] = lost[i] ? 0.f : (float)((int)cv - 127);
+        ev[i] = cv == (uint32_t)kScaleNan ? nan : (float)((int)cv - 127);
+        alive[i] = alive[i] && cv != (uint32_t)kScaleNan;   // such a row's weight is NaN for the queries that see it
       }
     }
     uint32_t pa[MT][4];
@@ -429,18 +471,9 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           const uint2 x = *reinterpret_cast<const uint2*>(sV + code_chunk<D>(row, gq >> 1) + (gq & 1) * 8);
           v[i][0] = x.x; v[i][1] = x.y;
         }
-      }
-      // NaN codes for a context row whose scale is NaN, since all queries see it; zeros for rows that
-      // nothing may see, and for such a drafted row, which is added at the segment's end
-      if (masked || __any_sync(0xffffffffu, lane >= 16 && bytes == (uint32_t)kScaleNan)) {
+        if (!alive[i]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = off + key_of(i) - warp * 16;
-          if (!alive[i] || lost[i]) {
-#pragma unroll
-            for (int w = 0; w < W; ++w) v[i][w] = alive[i] && at < 0 ? 0x7f7f7f7fu : 0u;
-          }
-          if (alive[i] && lost[i] && at >= 0) atomicOr(&s_bad[seg & 1], 1ull << at);
+          for (int w = 0; w < W; ++w) v[i][w] = 0;
         }
       }
 #pragma unroll
@@ -574,15 +607,18 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           const unsigned long long ln = s_line[r];
           const int col = h0 + 4 * c4;
           unsigned long long bad = s_bad[seg & 1] & ln;
-          for (; bad; bad &= bad - 1) {                    // drafted rows with an infinity or a NaN: those entries
-            float* xs = &x.x;
-            if constexpr (QUANT) {                         // the row's scale is NaN
-              for (int k = 0; k < 4; ++k) xs[k] = __int_as_float(0x7fffffff);
+          for (; bad; bad &= bad - 1) {                    // drafted rows with an infinity or a NaN
+            const long long t = (long long)it.len + __ffsll((long long)bad) - 1;
+            const uint8_t* base = c.p[1] + it.b * c.b + it.h * c.h + t * c.t;
+            if constexpr (QUANT) {                         // the whole row, with its weight once more
+              if ((t >> 7) < it.k0 || (t >> 7) >= it.k1) continue;
+              const long long si = it.b * c.sb + it.h * c.sh + t * c.st;
+              x = tree_add_row<D>(x, Q + it.b * qb + ((long long)it.h * a.G + hd) * qh + n * qn, c.p[0] + (base - c.p[1]), base + col,
+                              (a.neg ? -a.scale_log2 : a.scale_log2) * scale_float(c.s[0][si]), M, scale_float(c.s[1][si]));
               continue;
             }
-            const int node = __ffsll((long long)bad) - 1;
-            const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(c.p[1] + it.b * c.b + it.h * c.h +
-                                                                              ((long long)it.len + node) * c.t) + col;
+            const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(base) + col;   // those entries
+            float* xs = &x.x;
             for (int k = 0; k < 4; ++k) {
               const float y = __bfloat162float(row[k]);
               if (!(fabsf(y) < INFINITY)) xs[k] += y;
