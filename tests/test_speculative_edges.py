@@ -141,3 +141,11 @@ def nan_codes(device, N, G, D, code):
 @pytest.mark.parametrize("code", [0x7f, 0xff])
 def test_nan_codes_with_few_rows(device, N, G, D, code):
     nan_codes(device, N, G, D, code)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("N,G", ROWS[3:])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("code", [0x7f, 0xff])
+def test_nan_codes_with_many_rows(device, N, G, D, code):
+    nan_codes(device, N, G, D, code)

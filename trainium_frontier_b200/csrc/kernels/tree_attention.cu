@@ -40,6 +40,8 @@
 // used but holds an infinity or a NaN is zeroed likewise and added afterwards, entry by entry,
 // to the nodes that see it.
 // The reference has no decode path; the attention is the math of train.py:2564-2567.
+#include <climits>
+
 #include "kv_cache.cuh"
 
 namespace tfb {
@@ -271,14 +273,20 @@ __device__ __forceinline__ void tree_mma_p(uint32_t d, uint32_t a_tmem, uint32_t
       "r"(kDescHi));
 }
 
-// 4 e4m3 codes -> 4 bf16 (two words), times m1 (and m2 unless it is 1).  The code's exponent and
+// Bit 7 of every byte: whether that e4m3 code is one of the two NaNs.
+__device__ __forceinline__ uint32_t code4_nan(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// 4 e4m3 codes -> 4 bf16 (two words), times m1.  The code's exponent and
 // significand bits, moved to a bf16's place, are the value times 2^-120 (subnormals included),
 // so a multiplication by 2^120 times the row's scale is all that is left; scales whose
-// exponent does not fit that factor take a second one.
-__device__ __forceinline__ uint2 codes4(uint32_t x, __nv_bfloat162 m1) {
+// exponent does not fit that factor take a second one.  la, ha: the moved bits, 0x07f0 of a NaN code,
+// which the multiplication would make +-480 times the scale.
+__device__ __forceinline__ uint2 codes4(uint32_t x, __nv_bfloat162 m1, uint32_t& la, uint32_t& ha) {
   const uint32_t lo = __byte_perm(x, 0, 0x1404), hi = __byte_perm(x, 0, 0x3424);
-  uint32_t a = (lo & 0x80008000u) | ((lo >> 4) & 0x07f007f0u);
-  uint32_t b = (hi & 0x80008000u) | ((hi >> 4) & 0x07f007f0u);
+  la = (lo >> 4) & 0x07f007f0u;
+  ha = (hi >> 4) & 0x07f007f0u;
+  uint32_t a = (lo & 0x80008000u) | la;
+  uint32_t b = (hi & 0x80008000u) | ha;
   const __nv_bfloat162 u = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), m1);
   const __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&b), m1);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
@@ -301,16 +309,42 @@ __device__ __forceinline__ void tree_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 template <bool QUANT>
 __device__ __noinline__ void tree_add_bad(float (&f)[16], unsigned long long bad, const KvView& c, int b, int h, int len, int col) {
   for (; bad; bad &= bad - 1) {
-    const int j = __ffsll((long long)bad) - 1;
-    if (QUANT) {                             // the row's scale is NaN
-      for (int k = 0; k < 16; ++k) f[k] = __int_as_float(0x7fffffff);
+    const long long t = (long long)len + __ffsll((long long)bad) - 1;
+    const uint8_t* base = c.p[1] + b * c.b + h * c.h + t * c.t;
+    if (QUANT) {                             // NaN codes, or all of them where the row's scale is NaN
+      const bool all = c.s[1][b * c.sb + h * c.sh + t * c.st] == kScaleNan;
+      for (int k = 0; k < 16; ++k)
+        if (all || (base[col + k] & 0x7f) == 0x7f) f[k] = __int_as_float(0x7fffffff);
     } else {
-      const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(c.p[1] + b * c.b + h * c.h + ((long long)len + j) * c.t) + col;
+      const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(base) + col;
       for (int k = 0; k < 16; ++k) {
         const float v = __bfloat162float(row[k]);
         if (!(fabsf(v) < INFINITY)) f[k] += v;
       }
     }
+  }
+}
+
+// Mends the bf16 forms of NaN codes, which codes4 turns into +-480 times the scale, in a converting lane's part
+// (16 codes from `src` on of every RPI-th row) of a warp's 32 rows, cw * 32 .. of the tile at `dst`.  off: the
+// tile's first row from the first node's.  A NaN where a row is seen by all; in drafted value rows 0 and a bit in
+// `poison`, for the nodes that see them.  Rows whose factor (`mine`, a row a lane) is 0 are nobody's.
+template <int D>
+__device__ __noinline__ void tree_fix_nan(const uint8_t* src, uint8_t* dst, int cw, uint32_t mine, int off, unsigned long long* poison) {
+  constexpr int CH = D / 16, RPI = 32 / CH;
+  const int lane = threadIdx.x & 31, ch = lane % CH;
+#pragma unroll 1
+  for (int i = 0; i < CH; ++i) {
+    const int r32 = i * RPI + lane / CH, at = off + cw * 32 + r32;
+    const bool zeroed = __shfl_sync(0xffffffffu, mine, r32) == 0;
+    bool hit = false;
+#pragma unroll 1
+    for (int q = 0; q < 16; ++q)
+      if ((src[i * RPI * D + q] & 0x7f) == 0x7f && !zeroed) {
+        hit = true;
+        *reinterpret_cast<uint16_t*>(dst + sw128_chunk_offset(cw * 32 + r32, 2 * (ch & 3) + (q >> 3)) + (q & 7) * 2) = at >= 0 ? 0 : 0x7fff;
+      }
+    if (hit && at >= 0) atomicOr(poison, 1ull << at);
   }
 }
 
@@ -820,11 +854,16 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
         const bool swap = ch >= 4;
         const int c0 = 2 * (ch & 3) + (swap ? 1 : 0);
         const bool wide = __any_sync(0xffffffffu, second != 0x3f80u);
+        // the largest codes: looking for NaNs costs 335 against 319 us (8 sequences of 32768 .. 65535 rows, 32 / 8
+        // heads, 24 nodes; 341 with what mends them in line, 349 by a carry trick on the codes)
+        uint32_t top = 0;
 #pragma unroll 2
         for (int i = 0; i < CH; ++i) {
           const uint4 u = *reinterpret_cast<const uint4*>(src + i * RPI * D);
           const __nv_bfloat162 f = bf16x2_bits(__shfl_sync(0xffffffffu, mine, i * RPI + lane / CH));
-          const uint2 p0 = codes4(u.x, f), p1 = codes4(u.y, f), p2 = codes4(u.z, f), p3 = codes4(u.w, f);
+          uint32_t m[8];
+          const uint2 p0 = codes4(u.x, f, m[0], m[1]), p1 = codes4(u.y, f, m[2], m[3]), p2 = codes4(u.z, f, m[4], m[5]), p3 = codes4(u.w, f, m[6], m[7]);
+          top = __vimax3_u16x2(__vimax3_u16x2(m[0], m[1], m[2]), __vimax3_u16x2(m[3], m[4], m[5]), __vimax3_u16x2(top, m[6], m[7]));
           const uint4 o0 = make_uint4(p0.x, p0.y, p1.x, p1.y), o1 = make_uint4(p2.x, p2.y, p3.x, p3.y);
           const int row = cw * 32 + i * RPI + lane / CH;
           *reinterpret_cast<uint4*>(dst + sw128_chunk_offset(row, c0)) = swap ? o1 : o0;
@@ -841,6 +880,9 @@ __global__ void __launch_bounds__(TreeCfg<D, QUANT, NT>::THREADS, 1)
               w[q] = *reinterpret_cast<const uint32_t*>(&y);
             }
           }
+        }
+        if (__any_sync(0xffffffffu, max(top >> 16, top & 0xffffu) == 0x07f0u)) {
+          tree_fix_nan<D>(src, dst, cw, mine, v != 0 ? it.k * 128 - it.len : INT_MIN, &s_poison[it.seg & (kSegRing - 1)]);
         }
         fence_proxy_async_smem();
         mbar_arrive(&out_full[slot]);

@@ -68,11 +68,8 @@ __device__ __forceinline__ uint32_t codes2(uint32_t x) {
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(y) : "r"(x));
   return y;
 }
-// Bit 7 of every byte: whether that e4m3 code is one of the two NaNs.
-__device__ __forceinline__ uint32_t code4_nan(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ float e4m3_float(uint8_t x) {
-  const uint32_t h = codes2(x);
-  return __half2float(__ushort_as_half((unsigned short)h));
+  return __half2float(__ushort_as_half((unsigned short)codes2(x)));
 }
 __device__ __forceinline__ float scale_float(uint8_t e) {
   return e == kScaleNan ? __int_as_float(0x7fffffff) : e == 0 ? 0x1p-127f : __uint_as_float((uint32_t)e << 23);
