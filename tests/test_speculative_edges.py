@@ -149,3 +149,19 @@ def test_nan_codes_with_few_rows(device, N, G, D, code):
 @pytest.mark.parametrize("code", [0x7f, 0xff])
 def test_nan_codes_with_many_rows(device, N, G, D, code):
     nan_codes(device, N, G, D, code)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("N,G", ROWS)
+@pytest.mark.parametrize("qe,ke,scale", [(-120, 100, 2.0 ** 17), (-122, 117, None), (-110, 105, None), (110, -112, None)])
+def test_queries_and_keys_of_opposite_sizes(device, dtype, N, G, qe, ke, scale):
+    """Queries near the least (greatest) numbers over keys whose sizes make up for it, so that the
+    scores are ordinary ones."""
+    B, T, D, lens = 2, 300, 64, [257, 20]
+    kc, vc, ks, vs = ops.kv_cache_alloc(B, 1, T, D, dtype, device=device)
+    k = (torch.randn(B, T, 1, D, generator=gen(1)) * 2.0 ** ke).to(BF16).to(device)
+    v = torch.randn(B, T, 1, D, generator=gen(2)).to(BF16).to(device)
+    ops.kv_cache_write(k, v, kc, vc, i32([0, 0], device), None, ks, vs)
+    q = (torch.randn(B, N, G, D, generator=gen(3)) * 2.0 ** qe).to(BF16)
+    attend(q, (kc, vc, ks, vs), lens, None, scale)

@@ -230,7 +230,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       }
       // queries as fragments, a step of 16 dimensions a warp at a time
       if constexpr (QUANT) {
-        // f16, each row by a power of two that takes its largest value to 2^14 .. 2^15
+        // f16, each row by a power of two that takes its largest value to 2^14 .. 2^15.  Entries below
+        // 2^-31 of that value lose bits, those below 2^-40 are 0.
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -249,9 +250,11 @@ __global__ void __launch_bounds__(kFewThreads, 1)
             uint32_t top = max(mx & 0xffffu, mx >> 16);
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int ex = (int)(top >> 7), fe = min(268 - ex, 254);     // exponent bytes of the maximum and of the factor
+            // exponent bytes of the maximum and of the factor: 2^111 at most, which takes bf16's least step,
+            // 2^-133, to 2^-22 (exact in f16) and leaves its inverse a normal number
+            const int ex = (int)(top >> 7), fe = min(268 - ex, 238);
             const float f = __uint_as_float((uint32_t)fe << 23);
-            cr[mt][e] = a.scale_log2 * __uint_as_float((uint32_t)max(254 - fe, 0) << 23);
+            cr[mt][e] = a.scale_log2 * __uint_as_float((uint32_t)(254 - fe) << 23);
             if (a.neg) cr[mt][e] = -cr[mt][e];
             const uint32_t lo = pack_f16x2(__uint_as_float(mine.x << 16) * f, __uint_as_float(mine.x & 0xffff0000u) * f);
             const uint32_t hi = pack_f16x2(__uint_as_float(mine.y << 16) * f, __uint_as_float(mine.y & 0xffff0000u) * f);
