@@ -165,3 +165,27 @@ def test_queries_and_keys_of_opposite_sizes(device, dtype, N, G, qe, ke, scale):
     ops.kv_cache_write(k, v, kc, vc, i32([0, 0], device), None, ks, vs)
     q = (torch.randn(B, N, G, D, generator=gen(3)) * 2.0 ** qe).to(BF16)
     attend(q, (kc, vc, ks, vs), lens, None, scale)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N", [1, 3, 200])
+def test_rows_near_the_greatest_bf16(device, D, N):
+    """A finite row reads back finite: a value that would round to 2^128 is held as 1.875 * 2^127."""
+    x = torch.randn(1, N, 1, D, generator=gen(N)).to(BF16).float()
+    top = torch.tensor([1.9921875, 1.9375, 1.9296875, 1.75, 1.875, -1.9921875, -1.9375, 1.0]) * 2.0 ** 127
+    x[..., :8] = top
+    x[:, 0, :, 8:] *= 2.0 ** 126
+    x = x.to(BF16)
+    assert bool(x.isfinite().all())
+    kc, vc, ks, vs = ops.kv_cache_alloc(1, 1, N, D, E4M3, device=device)
+    ops.kv_cache_write(x.to(device), x.neg().to(device), kc, vc, i32([0], device), None, ks, vs)
+    got = ops.kv_cache_read(kc, vc, i32([N], device), N, ks, vs)
+    for y, rows in zip(got, (x, x.neg())):
+        for n in range(N):
+            codes, scale = quant_row(rows[0, n, 0])
+            want = torch.tensor(codes, dtype=torch.float64).clamp(-240, 240) * scale
+            assert scale == 2.0 ** 120 and torch.equal(y[0, n, 0].double().cpu(), want)
+    if N == 1:
+        for G in (1, 17):
+            attend(queries(1, 1, G, D) * 2.0 ** -126, (kc, vc, ks, vs), [0], None)

@@ -51,6 +51,9 @@ __device__ __forceinline__ uint2 quant8(const uint4& u, float inv) {
   return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }
 
+// Codes under the largest scale: 256 (0x78), which stands for 2^128, becomes 240.  No other code is above 240 there.
+__device__ __forceinline__ uint32_t hold_top(uint32_t c) { return c - ((((c & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u) >> 7); }
+
 __device__ __forceinline__ uint32_t absmax8(const uint4& u) {
   const uint32_t m = 0x7fff7fffu;
   return __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
@@ -117,6 +120,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_cache_write_kernel(const KvRows
       if (on[i]) {
         uint2 codes = make_uint2(0, 0);        // a row with an inf or NaN: its scale says so
         if (e != kScaleNan) codes = quant8(u[i], __uint_as_float((uint32_t)(254 - e) << 23));   // times 2^-(e - 127)
+        if (e == kScaleMax) codes = make_uint2(hold_top(codes.x), hold_top(codes.y));
         reinterpret_cast<uint2*>(dp + i * c.t)[l] = codes;
       }
       if (l == i) {                            // lane i stores row i's scale

@@ -3,7 +3,10 @@
 //
 // Quantised rows: e4m3 codes and one e8m0 scale byte a row (value = code * 2^(byte - 127),
 // 255 = NaN).  The scale is a power of two, so quantising is one exact multiplication and one
-// rounding, and every cached value is exactly a bf16 number: reading back never rounds.  An
+// rounding, and every cached value is exactly a bf16 number: reading back never rounds.  (Under the
+// largest scale that a bf16 row can need, 2^120, code 256 would stand for 2^128: such a value is held
+// as 240 instead.  Under larger ones, which only a caller's own cache can hold, values past bf16's
+// range may become infinite.)  An
 // fp32 scale would use the top of the e4m3 range up to one binade better, which changes no
 // significand bit of a value above the subnormals, and costs four bytes a row instead of one.
 #pragma once
@@ -18,6 +21,7 @@
 namespace tfb {
 
 constexpr int kScaleMin = 10;    // exponent byte of the least scale, 2^-117: every e4m3 normal times it is a bf16 normal
+constexpr int kScaleMax = 247;   // of the largest one that is written, 2^120
 constexpr int kScaleNan = 255;
 
 struct KvView {

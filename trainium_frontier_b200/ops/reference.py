@@ -118,6 +118,7 @@ def quantise_rows(x: torch.Tensor):
     e = torch.where(amax == 0, -117, e).clamp_min(-117)
     bad = ~torch.isfinite(amax)
     y = torch.ldexp(torch.ldexp(x, -(e // 2)[..., None]), -(e - e // 2)[..., None])
+    y = torch.where(e[..., None] == 120, y.clamp(-240, 240), y)           # 256 would be 2^128, which no bf16 is
     codes = torch.where(bad[..., None], 0.0, y).to(torch.float8_e4m3fn)   # the scale says that such a row is NaN
     return codes, torch.where(bad, 255, e + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
 
