@@ -189,3 +189,26 @@ def test_rows_near_the_greatest_bf16(device, D, N):
     if N == 1:
         for G in (1, 17):
             attend(queries(1, 1, G, D) * 2.0 ** -126, (kc, vc, ks, vs), [0], None)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_broadcast_scales_are_read_and_not_written(device):
+    """One scale for all rows of a cache may be read; a row's own scale cannot be stored in it."""
+    B, H, T, D, N = 2, 2, 40, 64, 3
+    kc, vc, ks, vs = make_cache(B, H, T, D, E4M3, "head", device, gen(1))
+    one = ks[:, :, :1].expand(B, H, T)
+    lens = i32([30, 5], device)
+    attend(queries(B, N, 4, D), (kc, vc, one, one), [30, 5], None)
+    full = one.contiguous()
+    for a, b in zip(ops.kv_cache_read(kc, vc, lens, T, one, one), ops.kv_cache_read(kc, vc, lens, T, full, full)):
+        assert torch.equal(a, b)
+    x = torch.zeros(B, N, H, D, dtype=BF16, device=device)
+    heads = ks[:, :1].expand(B, H, T)
+    path, count = i32([[0, 2, -1]] * B, device), i32([2, 2], device)
+    before = raw(one).clone(), raw(kc).clone()
+    for s in (one, heads):
+        with pytest.raises(RuntimeError, match="scales"):
+            ops.kv_cache_write(x, x, kc, vc, lens, None, s, s)
+        with pytest.raises(RuntimeError, match="scales"):
+            ops.kv_cache_commit(kc, vc, lens, path, count, s, s)
+    assert torch.equal(raw(one), before[0]) and torch.equal(raw(kc), before[1])

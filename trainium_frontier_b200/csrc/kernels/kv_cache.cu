@@ -265,6 +265,7 @@ void kv_cache_write(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor vc, at
                     c10::optional<at::Tensor> count, c10::optional<at::Tensor> ks, c10::optional<at::Tensor> vs) {
   bool quant;
   const KvView c = kv_view(kc, vc, ks, vs, quant);
+  kv_check_scales_written(ks);
   TORCH_CHECK(k.dim() == 4, "k and v: bfloat16 [B, N, H, D]");
   const KvRows r = kv_rows(k, v, kc);
   const int64_t B = kc.size(0), N = k.size(1), H = kc.size(1), D = kc.size(3);
@@ -317,6 +318,7 @@ void kv_cache_commit(at::Tensor kc, at::Tensor vc, at::Tensor lens, at::Tensor p
                      c10::optional<at::Tensor> ks, c10::optional<at::Tensor> vs) {
   bool quant;
   const KvView c = kv_view(kc, vc, ks, vs, quant);
+  kv_check_scales_written(ks);
   const int64_t B = kc.size(0), H = kc.size(1), D = kc.size(3);
   TORCH_CHECK(path.dim() == 2, "path: int32 [B, N]");
   const int64_t N = path.size(1);

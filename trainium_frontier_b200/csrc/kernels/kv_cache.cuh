@@ -71,6 +71,13 @@ inline KvView kv_view(const at::Tensor& kc, const at::Tensor& vc, const c10::opt
   return v;
 }
 
+// Whether every row has a scale byte of its own, as storing one needs.
+inline void kv_check_scales_written(const c10::optional<at::Tensor>& ks) {
+  if (!ks.has_value()) return;
+  for (int i = 0; i < 3; ++i)
+    TORCH_CHECK(ks->size(i) <= 1 || ks->stride(i) > 0, "scales that are written: no broadcast dimension");
+}
+
 // An int32 tensor [B] (or [B, N]) on the caches' device, packed.
 inline const int* kv_ints(const at::Tensor& t, const char* name, c10::Device dev, int64_t B, int64_t N = -1) {
   const bool fits = N < 0 ? t.dim() == 1 && t.size(0) == B : t.dim() == 2 && t.size(0) == B && t.size(1) == N;

@@ -135,6 +135,7 @@ def _raw(t: torch.Tensor) -> torch.Tensor:
 def kv_cache_write(k, v, k_cache, v_cache, pos, count=None, k_scale=None, v_scale=None) -> None:
     from . import speculative as sp
     sp.check_cache(k_cache, v_cache, k_scale, v_scale)
+    sp.check_scales_written(k_scale)
     sp.check_rows(k, v, k_cache)
     B, N = k.shape[:2]
     sp.check_ints(pos, "pos", k_cache.device, B)
@@ -170,6 +171,7 @@ def kv_cache_read(k_cache, v_cache, lens, T: int, k_scale=None, v_scale=None):
 def kv_cache_commit(k_cache, v_cache, lens, path, count, k_scale=None, v_scale=None) -> None:
     from . import speculative as sp
     sp.check_cache(k_cache, v_cache, k_scale, v_scale)
+    sp.check_scales_written(k_scale)
     B, T = k_cache.shape[0], k_cache.shape[2]
     if path.dim() != 2:
         raise RuntimeError("path: int32 [B, N]")

@@ -70,6 +70,11 @@ def check_cache(k_cache, v_cache, k_scale, v_scale) -> None:
                "scales: [B, H, T] of the same strides")
 
 
+def check_scales_written(k_scale) -> None:
+    _check(k_scale is None or all(st > 0 or n <= 1 for st, n in zip(k_scale.stride(), k_scale.shape)),
+           "scales that are written: no broadcast dimension")
+
+
 def check_ints(t, name: str, device, *sizes) -> None:
     _check(t.dtype == torch.int32 and t.device == device and tuple(t.shape) == sizes and t.is_contiguous(),
            f"{name}: contiguous int32 of {'[B]' if len(sizes) == 1 else '[B, N]'} entries on the caches' device")
