@@ -212,3 +212,17 @@ def test_broadcast_scales_are_read_and_not_written(device):
         with pytest.raises(RuntimeError, match="scales"):
             ops.kv_cache_commit(kc, vc, lens, path, count, s, s)
     assert torch.equal(raw(one), before[0]) and torch.equal(raw(kc), before[1])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("N,G", ROWS)
+def test_key_scales_of_the_least_byte(device, N, G):
+    """Scale byte 0 is 2^-127, for keys as for values."""
+    T, D = 200, 64
+    cache = make_cache(1, 1, T, D, E4M3, "head", device, gen(6))
+    kc, _, ks, _ = cache
+    codes = torch.randint(0x28, 0x7f, (T, D), generator=gen(7)) + 128 * torch.randint(0, 2, (T, D), generator=gen(8))
+    raw(kc)[0, 0] = codes.to(torch.uint8).to(device)   # 2^-2 and more: exact in bf16 under this scale
+    raw(ks)[0, 0, ::2] = 0
+    raw(ks)[0, 0, 1::2] = 1
+    attend(queries(1, N, G, D) * 2.0 ** 118, cache, [150], None)

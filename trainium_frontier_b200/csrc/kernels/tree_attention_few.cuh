@@ -311,7 +311,10 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       __syncthreads();
       if constexpr (QUANT) used &= ~s_bad[seg & 1];
     }
-    const uint32_t bytes = ahead;
+    // the lane's scale: a key's as it is, a value's as its log2 (decoded by its lane: once, not by every lane that needs it)
+    const float factor = ahead == (uint32_t)kScaleNan ? __int_as_float(0x7fffffff)
+                         : lane >= 16                 ? (float)((int)ahead - 127)
+                                                      : __uint_as_float(ahead == 0 ? 1u << 22 : ahead << 23);
     if (nx.next(lens, a.rg)) fetch_scales(nx);
     const int slot = g % NS;
     mbar_wait(&full[slot], (g / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
@@ -374,11 +377,9 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       const int at = off + key_of(i) - warp * 16;
       alive[i] = !masked || at < 0 || (at < kTreeNodes && ((used >> at) & 1));
       if constexpr (QUANT) {
-        const float nan = __int_as_float(0x7fffffff);
-        const uint32_t ck = __shfl_sync(0xffffffffu, bytes, key_of(i) - warp * 16), cv = __shfl_sync(0xffffffffu, bytes, 16 + key_of(i) - warp * 16);
-        fk[i] = ck == (uint32_t)kScaleNan ? nan : __uint_as_float(max(ck, 1u) << 23);
-        ev[i] = cv == (uint32_t)kScaleNan ? nan : (float)((int)cv - 127);
-        alive[i] = alive[i] && cv != (uint32_t)kScaleNan;   // such a row's weight is NaN for the queries that see it
+        fk[i] = __shfl_sync(0xffffffffu, factor, key_of(i) - warp * 16);
+        ev[i] = __shfl_sync(0xffffffffu, factor, 16 + key_of(i) - warp * 16);
+        alive[i] = alive[i] && ev[i] == ev[i];            // NaN: the weight is NaN for the queries that see the row
       }
     }
     uint32_t pa[MT][4];

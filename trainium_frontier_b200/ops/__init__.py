@@ -216,8 +216,9 @@ def kv_cache_write(k, v, k_cache, v_cache, pos, count=None, k_scale=None, v_scal
     ``count`` are int32 [B] in device memory.
 
     ``float8_e4m3fn`` caches hold each row's codes ``x * 2^-e`` rounded to nearest even and its
-    scale ``2^e`` (``float8_e8m0fnu`` [B, H, T], a byte of its own for every row), ``e`` being the least integer (-117 at the
-    least) with ``max|x| <= 448 * 2^e``; a row with an infinity or a NaN reads back as NaN.
+    scale ``2^e`` (``float8_e8m0fnu`` [B, H, T], a byte of its own for every row), ``e`` being the
+    least integer (-117 at the least) with ``max|x| <= 448 * 2^e``; a row with an infinity or a NaN
+    reads back as NaN.
     A value that would round to ``2^128``, which is no bfloat16, is held as ``1.875 * 2^127``.
     CUDA: k, v bfloat16 with 16-byte aligned rows, head_dim 64 / 128."""
     if _cuda(k_cache):
