@@ -155,3 +155,33 @@ def test_speculative_decoding_where_attention_decides(cuda_device, head_dim):
     # a logit is a product of n_embd terms of a normed state and weights of 0.05, each state off by
     # some roundings of 2^-8 in either path: sqrt(256) * 0.05 * 2^-8 * 8 roundings * 2 paths, four times over
     assert float(gap.max()) <= 4 * 256 ** 0.5 * 0.05 * 2 ** -8 * 16, gap
+
+
+@pytest.mark.parametrize("T", [1, 100, 130])
+def test_speculative_prompts_of_any_length_use_the_kernels(cuda_device, T, monkeypatch):
+    """Prompts that are no multiple of 128 tokens: no library attention is called, and the new tokens
+    are the largest of the same model's logits by recomputation, or nearer to them than the two
+    paths' bf16 rounding."""
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    from trainium_frontier_b200.ops import reference
+    from trainium_frontier_b200.ops._ext import check_errors
+    m = _model(cuda_device, head_dim=128)
+    with torch.no_grad():
+        for b in m.transformer.h:
+            b.attn.c_proj.weight.normal_(0, 0.2)
+    B, N = 3, 8
+    prompts = torch.randint(1, 8192, (B, T), device=cuda_device, dtype=torch.int32)
+
+    def library(*a, **k):
+        raise AssertionError("library attention")
+    with monkeypatch.context() as mp:
+        mp.setattr(reference.F, "scaled_dot_product_attention", library)
+        out = SpeculativeGenerator(m, B, T + N).generate(prompts, N).long()
+    check_errors()
+    text = torch.cat([prompts.long(), out], 1)
+    with torch.no_grad():
+        z = m(torch.nn.functional.pad(text, (0, 256 - T - N)).to(torch.int32))[:, T - 1:T + N - 1].double()
+    gap = z.amax(-1) - z.gather(-1, out[..., None])[..., 0]
+    # a logit is a product of n_embd terms of a normed state and weights of 0.05, each state off by
+    # some roundings of 2^-8 in either path: sqrt(256) * 0.05 * 2^-8 * 8 roundings * 2 paths, four times over
+    assert float(gap.max()) <= 4 * 256 ** 0.5 * 0.05 * 2 ** -8 * 16, gap

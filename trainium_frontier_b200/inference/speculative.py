@@ -17,6 +17,7 @@ Everything goes through the public ops, so a model on the CPU runs the fp32 orac
 from __future__ import annotations
 
 import torch
+import torch.nn.functional as F
 
 from .. import ops
 from .generate import _is_plain
@@ -85,12 +86,20 @@ class SpeculativeGenerator:
             v = v.unflatten(-1, (self.H, self.D))
             ops.kv_cache_write(k, v, kc, vc, lens, None, ks, vs)
             if prompt:
-                y = ops.attention(q, k, v.contiguous(), True, self.scale)
+                y = self._causal(q, k, v)
             else:
                 y = ops.tree_attention(q, kc, vc, lens, parents, self.scale, ks, vs)
             x = ops.linear(y.reshape(B, N, -1), blk.attn.c_proj.weight, residual=xm)
             x = blk.mlp(ops.norm(x), residual=x)
         return ops.norm(x)
+
+    def _causal(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """Causal attention of a prompt of any length: the kernel takes whole tiles of 128 rows, and no
+        row sees the ones that fill up the last tile."""
+        T = q.shape[1]
+        if q.is_cuda and T % 128:
+            q, k, v = (F.pad(t, (0, 0, 0, 0, 0, -T % 128)) for t in (q, k, v))
+        return ops.attention(q, k, v.contiguous(), True, self.scale)[:, :T]
 
     def _probabilities(self, hidden: torch.Tensor, temperature: float) -> torch.Tensor:
         z = ops.softcap_logits(hidden, self.m.lm_head.weight, self.m.rc.logit_softcap, self.V)
