@@ -172,3 +172,57 @@ def test_ngram_draft():
     assert q is None
     assert tok.tolist() == [[-1] * 3, [7, 1, 2], [-1] * 3, [4, -1, -1]]
     assert par.tolist() == [[-2] * 3, [0, 1, 2], [-2] * 3, [0, -2, -2]]
+
+
+def test_speculative_sampling_follows_the_target_token_by_token(monkeypatch):
+    """Sampled with a draft whose distributions overlap the target's (two siblings and a child, drawn
+    from flattened rows of the same model): the second and third tokens follow the target's law given
+    the most common tokens before them.  Each share of a token is within 5 standard deviations,
+    sqrt(p (1 - p) / n), of p, over the tokens that are expected 10 times or more."""
+    from trainium_frontier_b200 import ops
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    m = _attending_model()
+    M, T, n, temp = 800, 4, 4, 0.12
+    p = torch.randint(1, 8192, (1, T), generator=torch.Generator().manual_seed(4)).expand(M, T).contiguous()
+    g = torch.Generator().manual_seed(3)
+    rows = torch.arange(M)
+
+    def law(text, at, t):
+        with torch.no_grad():
+            return torch.softmax(m(text)[torch.arange(len(text)), at] / t, -1)
+
+    def draft(text, lens):
+        ln = lens.long()
+        q = torch.full((M, 4, 8192), 1 / 8192)    # no token was drawn from the rows of nodes 2 and 3
+        q[:, 0] = law(text, ln - 1, 2 * temp)
+        tok = torch.empty(M, 3, dtype=torch.int32)
+        tok[:, :2] = torch.multinomial(q[:, 0], 2, replacement=True, generator=g)
+        longer = text.clone()
+        longer[rows, ln] = tok[:, 0].long()
+        q[:, 1] = law(longer, ln, 2 * temp)       # node 1's children
+        tok[:, 2] = torch.multinomial(q[:, 1], 1, generator=g)[:, 0]
+        return tok, torch.tensor([[0, 0, 1]] * M, dtype=torch.int32), q
+    taken, verify = [], ops.verify_tree
+
+    def counting(*a):
+        res = verify(*a)
+        if a[0].shape[1] > 1:
+            taken.append(res)
+        return res
+    monkeypatch.setattr(ops, "verify_tree", counting)
+    out = SpeculativeGenerator(m, M, T + n + 2, draft).generate(p, n, temp, g).long()
+    counts = torch.stack([c for _, c, _ in taken])
+    assert int((counts == 1).sum()) > M // 10 and int((counts == 2).sum()) > M // 10 and int((counts == 3).sum()) > M // 10
+    second = torch.cat([path[count > 1][:, 1] for path, count, _ in taken])
+    assert int((second == 2).sum()) > M // 50   # the first sibling rejected, the second one accepted
+    text, some, checked = p[:1], out, []
+    for i in range(3):
+        want = law(text, torch.tensor([T + i - 1]), temp)[0].double()
+        share = torch.bincount(some[:, i], minlength=8192).double() / len(some)
+        seen = want * len(some) >= 10
+        checked.append(int(seen.sum()))
+        assert bool(((share - want).abs() <= 5 * (want * (1 - want) / len(some)).sqrt())[seen].all()), i
+        top = share.argmax()
+        some = some[some[:, i] == top]
+        text = torch.cat([text, top.view(1, 1)], 1)
+    assert min(checked) >= 2
