@@ -140,3 +140,30 @@ def make_tree(B, N, gen, unused=False):
         drop = torch.rand(B, N, generator=gen) < 0.2
         par = torch.where(drop, torch.where(torch.rand(B, N, generator=gen) < 0.5, -2, N + 5), par)
     return par.to(torch.int32)
+
+
+@torch.no_grad()
+def quantised_logits(m, text, T):
+    """Logits [B, L, V] of a plain model on the CPU for text [B, L], by recomputation: the T tokens of the
+    prompt see each other's keys and values as they are, every later token sees all rows, its own
+    among them, as an e4m3 cache holds them."""
+    from trainium_frontier_b200 import ops
+    B, L = text.shape
+    cfg = m.config
+    H, D = cfg.n_head, cfg.head_dim
+    scale = cfg.attn_scale if cfg.attn_scale > 0 else D ** -0.5
+    cos, sin = (t.reshape(-1, t.shape[-1])[:L][None, :, None].float() for t in (m.cos, m.sin))
+    causal = torch.ones(L, L, dtype=torch.bool).tril()
+    x = x0 = ops.embed_norm(text, m.transformer.wte.weight, m.compute_dtype)
+    for blk in m.transformer.h:
+        xm, h = ops.mix_norm(x, x0, blk.resid_lambda, blk.x0_lambda)
+        q, k, v = (t.view(B, L, H, D) for t in ops.linear_multi(h, [blk.attn.c_q.weight, blk.attn.c_k.weight, blk.attn.c_v.weight]).chunk(3, -1))
+        q, k = ops.rope_norm(q, cos, sin), ops.rope_norm(k, cos, sin)
+        rows = []
+        for kk, vv in ((k, v), tuple(ops.ref.cache_values(*ops.ref.quantise_rows(t)) for t in (k, v))):
+            w = torch.einsum("bqhd,bkhd->bhqk", q, kk) * scale
+            rows.append(torch.einsum("bhqk,bkhd->bqhd", torch.softmax(w.masked_fill(~causal, -math.inf), -1), vv))
+        y = torch.cat([rows[0][:, :T], rows[1][:, T:]], 1).reshape(B, L, H * D)
+        x = ops.linear(y, blk.attn.c_proj.weight, residual=xm)
+        x = blk.mlp(ops.norm(x), residual=x)
+    return ops.softcap_logits(ops.norm(x), m.lm_head.weight, m.rc.logit_softcap, cfg.vocab_size)

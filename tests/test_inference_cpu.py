@@ -226,3 +226,37 @@ def test_speculative_sampling_follows_the_target_token_by_token(monkeypatch):
         some = some[some[:, i] == top]
         text = torch.cat([text, top.view(1, 1)], 1)
     assert min(checked) >= 2
+
+
+def test_speculative_quantised_cache_reads_what_it_wrote():
+    """Over an e4m3 cache one token a round gives the tokens of a recomputation with quantised keys and
+    values.  A node reads the same rows in a tree, so trees with the right tokens on scattered nodes,
+    and the draft by rule, give the same, in fewer rounds."""
+    from tests._specutil import quantised_logits
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator, ngram_draft
+    m = _attending_model()
+    g = torch.Generator().manual_seed(5)
+    with torch.no_grad():   # value rows of very unequal sizes, and so of unequal scales
+        for b in m.transformer.h:
+            b.attn.c_v.weight.mul_(torch.exp2(torch.randint(-3, 4, b.attn.c_v.weight.shape[:1], generator=g).float())[:, None])
+        m.transformer.wte.weight.mul_(torch.exp2(torch.randint(-3, 4, (1, m.transformer.wte.weight.shape[1]), generator=g).float()))
+    p = torch.randint(1, 8192, (3, 10), generator=g)
+    n, e4m3 = 14, torch.float8_e4m3fn
+
+    def nothing(text, lens):
+        return torch.empty(3, 0, dtype=torch.int32), torch.empty(3, 0, dtype=torch.int32), None
+    want = SpeculativeGenerator(m, 3, 32, nothing, e4m3).generate(p, n)
+    assert not torch.equal(want.long(), generate_reference(m, p, n))      # the rounding of the cache matters here
+    full = torch.cat([p, want.long()], 1)
+    assert torch.equal(quantised_logits(m, full, 10)[:, 9:-1].argmax(-1), want.long())
+
+    def draft(text, lens):
+        tok = torch.full((3, 9), 3, dtype=torch.int32)
+        for b in range(3):
+            for k, t in enumerate(full[b, int(lens[b]):][:3].tolist()):
+                tok[b, (2, 5, 7)[k]] = t                                  # nodes 3, 6 and 8
+        return tok, torch.tensor([[0, 0, 0, 3, 3, 3, 6, 6, 8]] * 3, dtype=torch.int32), None
+    for d, most in ((draft, 5), (ngram_draft(4), n - 1)):
+        s = SpeculativeGenerator(m, 3, 32, d, e4m3)
+        assert torch.equal(s.generate(p, n), want)
+        assert s.rounds <= most

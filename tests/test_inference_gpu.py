@@ -185,3 +185,50 @@ def test_speculative_prompts_of_any_length_use_the_kernels(cuda_device, T, monke
     # a logit is a product of n_embd terms of a normed state and weights of 0.05, each state off by
     # some roundings of 2^-8 in either path: sqrt(256) * 0.05 * 2^-8 * 8 roundings * 2 paths, four times over
     assert float(gap.max()) <= 4 * 256 ** 0.5 * 0.05 * 2 ** -8 * 16, gap
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_speculative_decoding_over_a_quantised_cache(cuda_device, head_dim):
+    """Over an e4m3 cache, with right tokens on scattered nodes of a small and of a wide tree: the new
+    tokens against logits by recomputation on the CPU with quantised keys and values."""
+    import copy
+
+    from tests._specutil import quantised_logits
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    from trainium_frontier_b200.ops._ext import check_errors
+    m = _model(cuda_device, head_dim=head_dim)
+    with torch.no_grad():
+        for b in m.transformer.h:
+            b.attn.c_proj.weight.normal_(0, 0.2)
+    plain = copy.deepcopy(m).cpu()
+    plain.set_compute_dtype(torch.float32)
+    B, T, N = 3, 128, 10
+    prompts = torch.randint(1, 8192, (B, T), device=cuda_device, dtype=torch.int32)
+    e4m3 = torch.float8_e4m3fn
+
+    def nothing(text, lens):
+        none = torch.empty(B, 0, dtype=torch.int32, device=cuda_device)
+        return none, none, None
+    one = SpeculativeGenerator(m, B, T + N, nothing, e4m3)
+    full = torch.cat([prompts.long(), one.generate(prompts, N).long(), torch.zeros(B, 8, device=cuda_device, dtype=torch.long)], 1)
+
+    def draft_of(n, at, parents):
+        def draft(text, lens):
+            tok = torch.full((B, n), 3, dtype=torch.int32, device=cuda_device)
+            for k, node in enumerate(at):
+                tok[:, node - 1] = full.gather(1, (lens.long() + k).clamp_max(full.shape[1] - 1)[:, None])[:, 0].to(torch.int32)
+            return tok, torch.tensor([parents] * B, dtype=torch.int32, device=cuda_device), None
+        return draft
+    for draft in (nothing, draft_of(9, (3, 6, 8), [0, 0, 0, 3, 3, 3, 6, 6, 8]), draft_of(63, (62, 63), [0] * 62 + [62])):
+        g = SpeculativeGenerator(m, B, T + N, draft, e4m3)
+        out = g.generate(prompts, N).long()
+        check_errors()
+        assert draft is nothing or g.rounds < N - 1
+        text = torch.cat([prompts.long(), out], 1).cpu()
+        z = quantised_logits(plain, text, T)[:, T - 1:-1].double()
+        gap = z.amax(-1) - z.gather(-1, out.cpu()[..., None])[..., 0]
+        # a logit is a product of n_embd terms of a normed state and weights of 0.05, each state off by some
+        # roundings of 2^-8: sqrt(256) * 0.05 * 2^-8 * 8 roundings, four times over.  A rounding that moves a
+        # key or value entry by 2^-9 of it moves its code by a whole step, 2^-3, in 2^-9 / 2^-3 of the cases:
+        # 2^-6 by root mean square, four roundings' worth, twice a block (keys and values), 2 blocks
+        assert float(gap.max()) <= 4 * 256 ** 0.5 * 0.05 * 2 ** -8 * (8 + 4 * 2 * 2), gap

@@ -3,8 +3,9 @@
 ``SpeculativeGenerator(model, max_batch, max_len).generate(prompts, n)`` runs the target once a
 round over a small tree of tokens -- the last token of the text and the tokens that a draft
 proposes behind it -- and keeps the path that the target agrees with (``ops.verify_tree``), at
-least one new token a round.  The text's law is the target's own: greedy decoding gives the
-tokens of plain greedy decoding, sampling draws from the same distribution.
+least one new token a round.  The text's law is that of one token a round over the same cache:
+sampling draws from the same distribution, and greedy decoding over an unquantised cache gives
+the tokens of plain greedy decoding.
 
 Keys and values live in a cache with a length of its own for every sequence, as bfloat16 or
 quantised to ``float8_e4m3fn`` with a power-of-two scale per row (half the memory): each layer
