@@ -24,7 +24,7 @@
 // brought to the largest scale of 32 rows convert in a fifth of the instructions, but a small row
 // beside a large one that the query does not see then loses its bits.)
 //
-// Up to 16 query rows a key/value head take the kernel of tree_attention_few.cuh.
+// Up to 16 query rows a key/value head (8 of bf16 heads of 128) take the kernel of tree_attention_few.cuh.
 //
 // Measured on a B200 (calls replayed from a graph; the floor is the bytes at 6.54 TB/s or the
 // products at 1.68 PFLOP/s): 64-node trees, 32 / 8 heads, 16 sequences of 4096 .. 8191 bf16 rows: 137 us
@@ -1065,11 +1065,15 @@ at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor
   TORCH_CHECK(B * N * Hq < (1LL << 31), "too many query rows");
   const int G = (int)(Hq / H);
   a.B = (int)B; a.N = (int)N; a.Hq = (int)Hq; a.Hkv = (int)H; a.G = G;
-  // up to 16 rows a key/value head: the register kernel.  16 sequences of 8191 rows, 8 heads of 128:
-  // bf16 76 us against 79 for the tensor-core tiles at 1 .. 8 rows, 85 against 81 at 16; e4m3 82 against
-  // 110 and 96 against 112; 32 sequences of 575 bf16 rows 25 against 33.  With 32 rows it spilled: 180
-  // against 83.
-  const int rows = (int)std::min<int64_t>(N * G, 1 << 20), EH = rows <= 8 ? 1 : rows <= 16 ? 2 : 0;
+  // Few rows a key/value head: the register kernel, up to 16 rows of e4m3 caches or heads of 64, up to 8 of bf16
+  // rows of 128, whose 16-row form keeps too much in registers.  Register kernel / tensor-core tiles, us, 16
+  // sequences of 4095 .. 8190 rows, 8 heads; and 64 sequences of 100 .. 200 rows:
+  //   bf16, 128: 8 rows 74 / 76, 38 / 42;  9 rows 83 / 79, 52 / 42;  16 rows 83 / 79, 52 / 44
+  //   bf16, 64:  8 rows 53 / 63, 27 / 34;  9 rows 62 / 64, 35 / 35;  16 rows 63 / 64, 36 / 37
+  //   e4m3, 128: 8 rows 70 / 107, 41 / 47;  9 rows 87 / 111, 54 / 50;  16 rows 88 / 112, 60 / 52
+  //   e4m3, 64:  8 rows 58 / 96, 29 / 40;  9 rows 71 / 98, 39 / 41;  16 rows 72 / 99, 40 / 42
+  // With 32 rows it spilled: 180 against 83.
+  const int rows = (int)std::min<int64_t>(N * G, 1 << 20), EH = rows <= 8 ? 1 : rows <= 16 && (quant || D == 64) ? 2 : 0;
   // rows of a tile: nb nodes of gb heads each
   a.gb = std::min(G, 128);
   a.nb = std::min((int)N, 128 / a.gb);
@@ -1102,7 +1106,7 @@ at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor
   if (EH) {
 #define TFB_FEW(DD, QQ) \
   (EH == 1 ? few_launch<DD, QQ, 1>(tk, tv, q, a, c, grid, s) : few_launch<DD, QQ, 2>(tk, tv, q, a, c, grid, s))
-    if (D == 128) { if (quant) TFB_FEW(128, true); else TFB_FEW(128, false); }
+    if (D == 128) { if (quant) TFB_FEW(128, true); else few_launch<128, false, 1>(tk, tv, q, a, c, grid, s); }
     else { if (quant) TFB_FEW(64, true); else TFB_FEW(64, false); }
 #undef TFB_FEW
     return o;

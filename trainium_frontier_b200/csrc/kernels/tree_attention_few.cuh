@@ -39,7 +39,7 @@ struct FewCfg {
   static constexpr size_t SMEM = 2 * NS * TILE + QF + OUT + kFewWarps * 16 * MT * 8 + 2 * NS * 8 + 16 + 16 * MT * 8 + kLenCache * 4 + 16;
 };
 static_assert(FewCfg<128, true, 2>::NS <= kFewWarps && FewCfg<64, true, 2>::NS <= kFewWarps, "a warp a stage");
-static_assert(FewCfg<128, false, 2>::SMEM <= 232448 && FewCfg<128, true, 2>::SMEM <= 232448 && FewCfg<64, false, 2>::SMEM <= 232448,
+static_assert(FewCfg<128, false, 1>::SMEM <= 232448 && FewCfg<128, true, 2>::SMEM <= 232448 && FewCfg<64, false, 2>::SMEM <= 232448,
               "shared memory");
 
 template <bool F16>
