@@ -260,3 +260,15 @@ def test_speculative_quantised_cache_reads_what_it_wrote():
         s = SpeculativeGenerator(m, 3, 32, d, e4m3)
         assert torch.equal(s.generate(p, n), want)
         assert s.rounds <= most
+
+
+def test_speculative_prompts_outside_the_vocabulary_are_refused():
+    import pytest
+
+    from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
+    g = SpeculativeGenerator(_small_model(), 2, 32)
+    for bad in (8192, -1, 2 ** 31 - 1):
+        p = torch.ones(2, 4, dtype=torch.int32)
+        p[1, 2] = bad
+        with pytest.raises(ValueError, match="prompts"):
+            g.generate(p, 2)

@@ -120,6 +120,8 @@ class SpeculativeGenerator:
             raise ValueError("a generator is built for a fixed batch")
         if T < 1 or max_new_tokens < 1 or T + max_new_tokens > self.max_len:
             raise ValueError(f"prompt and new tokens must fit in max_len {self.max_len}")
+        if int(prompts.min()) < 0 or int(prompts.max()) >= self.V:   # they index the embedding
+            raise ValueError(f"prompts: tokens 0 .. {self.V - 1}")
         dev = self.dev
         uniform = lambda *s: torch.rand(*s, device=dev, generator=generator)  # noqa: E731
         text = torch.zeros(B, self.max_len, dtype=torch.long, device=dev)
