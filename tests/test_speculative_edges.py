@@ -226,3 +226,20 @@ def test_key_scales_of_the_least_byte(device, N, G):
     raw(ks)[0, 0, ::2] = 0
     raw(ks)[0, 0, 1::2] = 1
     attend(queries(1, N, G, D) * 2.0 ** 118, cache, [150], None)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("N,G", ROWS)
+def test_a_scale_of_zero(device, N, G):
+    """Every visible row weighs the same, and 0 times an infinite score is NaN."""
+    D, T = 64, 300
+    kc, _, _, _ = cache = make_cache(3, 1, T, D, BF16, "head", device, gen(2))
+    kc[1, 0, 70, 0] = math.inf
+    kc[2, 0, 200 + N - 1, 0] = -math.inf
+    q = queries(3, N, G, D)
+    q[..., 0] = q[..., 0].abs() + 1
+    par = torch.arange(-1, N - 1, dtype=torch.int32).expand(3, N).contiguous()
+    par[:, -1] = -1
+    want = attend(q, cache, [200, 200, 200], par, 0.0)
+    assert bool(want[0].isfinite().all()) and bool(want[1].isnan().all()) and bool(want[2, -1].isnan().all())
+    assert bool(want[2, :-1].isfinite().all())

@@ -38,6 +38,8 @@ def kv_cache_commit(k_cache, v_cache, lens, path, count, k_scale, v_scale) -> No
 
 
 def tree_attention(q, k_cache, v_cache, lens, parents, scale, k_scale, v_scale):
+    if scale == 0:   # 0 * (q . k): NaN where q . k is infinite, and the masks' -inf stays what it is
+        q, scale = q * 0, 1.0
     return C().tree_attention(q, k_cache, v_cache, lens, parents, scale, k_scale, v_scale, err_word(q.device))
 
 
