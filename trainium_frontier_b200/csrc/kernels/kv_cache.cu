@@ -7,10 +7,11 @@
 // leave as one 8-byte store.  A block has one head's neighbouring rows, so that it writes (or
 // reads) one contiguous piece of a head-major cache and of its scales.
 //
-// Measured on a B200 (calls replayed from a graph; floors at 6.54 TB/s): one e4m3 row for 32 sequences
-// of 10 heads 1.9 us; 16 x 4096 rows of 8 heads 70 us of 62; read of 8 x 16384 rows 119 us of 118;
-// commit of 256 trees of 64 nodes, 8 bf16 heads, 21.6 us of 10 (rows of 256 bytes, two dependent
-// loads and a barrier apart).
+// Measured on a B200 (calls replayed from a graph; floors at 6.54 TB/s): one row for 32 sequences of 10 heads
+// 2.1 us, e4m3 or bf16; 16 x 4096 rows of 8 heads e4m3 71 us of 62, bf16 83 of 82; read of 8 x 16384 rows e4m3
+// 119 us of 118, bf16 150 of 154; commit of 256 trees of 64 nodes, 8 heads, bf16 22.5 us of 10, e4m3 13.7 of 5
+// (4096 blocks of a unit each, some five waves of them, and in every one the loads wait for each other: length,
+// count, path, row).
 // The reference has no decode path; these serve the cache of inference/generate.py.
 #include <cuda_fp8.h>
 

@@ -27,18 +27,22 @@
 // Up to 16 query rows a key/value head (8 of bf16 heads of 128) take the kernel of tree_attention_few.cuh.
 //
 // Measured on a B200 (calls replayed from a graph; the floor is the bytes at 6.54 TB/s or the
-// products at 1.68 PFLOP/s): 64-node trees, 32 / 8 heads, 16 sequences of 4096 .. 8191 bf16 rows: 137 us
-// of 65; 24-node trees, 32 / 8 heads, 8 sequences of 32768 .. 65535 e4m3 rows: 352 us of 125.  What is
-// left there is mostly the softmax and conversion warps' latency.  Parts left out in a copy: the first
-// case, 138 us whole, took 126 without exponentials and 113 with an eighth of the products besides;
-// the second, 527 us before the conversion loop was shortened, 392 without conversion, 454 without
-// exponentials and 318 without either (376 after it, 350 without polynomial exponentials
-// as well).  Tiles of 64 keys with deeper rings were slower (145 and 705 us).
+// products at 1.68 PFLOP/s).  64-node trees, 32 / 8 heads, 16 sequences of 4096 .. 8191 bf16 rows: 136 us
+// of 65 (160 in a long loop, where the power cap holds the SMs at 1.6 GHz).  By clock stamps a CTA takes
+// 193 to 234 thousand cycles, 211 in the mean, at 1.80 GHz: 84 half tiles of 2130 cycles, 1350 of them
+// exponentials, and segment starts and ends; the slowest ends at 129 us, then comes the second kernel.
+// Parts left out in a copy: 132 us without exponentials, 134 with an eighth of the products, 105 with
+// neither, so the two hide each other, and the rest is loads, reads of TMEM and hand-overs.
+// 24-node trees, 32 / 8 heads, 8 sequences of 32768 .. 65535 e4m3 rows: 375 us of 125 (391 in a long
+// loop).  318 without conversion, 386 without exponentials, 340 without either, 317 without either and an
+// eighth of the products: of these only the conversion counts.  By stamps a group is busy for 2100 of a
+// tile's 3790 cycles, and some 1200 lie between one tile's P and its first step of the next.
+// Tiles of 64 keys with deeper rings were slower (145 and 705 us).
 //
 // A row behind the context that no node uses may hold anything: its scores are masked, and its
 // values are zeroed in shared memory before the product (0 * NaN is NaN).  A drafted row that is
-// used but holds an infinity or a NaN is zeroed likewise and added afterwards, entry by entry,
-// to the nodes that see it.
+// used but holds an infinity or a NaN (in e4m3: a NaN code, or the scale NaN) is zeroed likewise and
+// added afterwards, entry by entry, to the nodes that see it.
 // The reference has no decode path; the attention is the math of train.py:2564-2567.
 #include <climits>
 

@@ -12,14 +12,16 @@
 // two codes.  The rows' scales never touch the codes: a key's is a factor of its score, and a
 // value's joins the exponent: w = 2^(score + log2 scale - m') against plain codes is p times the
 // value, with a reference m' of its own, so that w fits f16 (11 bits of significand) whatever the
-// scales are.  The sum of p = 2^(score - m) is kept apart in 32 bits.
+// scales are.  Weights below 2^-14 of the reference lose bits, and those below 2^-25 count nothing,
+// also in columns where the rows of large weight hold zeros.  The sum of p = 2^(score - m) is kept
+// apart in 32 bits.
 //
-// Measured on a B200 (calls replayed from a graph): a decode step of 32 sequences x 10 heads over
-// 288 .. 575 bf16 rows 30 us, floor 11 (each CTA has
-// two or three short segments; in the first version half of its cycles lay outside the tiles); one sequence of
-// 1023 e4m3 rows, 6 nodes x 10 heads of 64, 10.3 us; 16 sequences of 8191 bf16 rows, 8 heads, 76 us of
-// 62.  e4m3 tiles take as long as bf16 ones (82 us of 31): with two warps a sub-core the chain of
-// instructions is the limit.  Two CTAs of 128 registers a SM spilled (101 us).
+// Measured on a B200 (calls replayed from a graph).  A decode step of 32 sequences x 10 heads over
+// 288 .. 575 rows: bf16 30 us of 11, e4m3 32 of 5.5 (each CTA has two or three short segments, whose starts and
+// ends cost more than the tiles, and the second kernel takes 7 us by itself).  16 sequences of 4095 .. 8190
+// rows, 8 heads, 8 rows: bf16 74 us of 62, e4m3 70 of 31 (with two warps a sub-core the chain of
+// instructions of a tile is the limit).  One sequence of 1023 e4m3 rows, 6 nodes x 10 heads of 64: 11 to 12 us, two
+// dependent launches.  Two CTAs of 128 registers a SM spilled (101 us).
 #pragma once
 
 namespace tfb {

@@ -24,10 +24,11 @@
 // decisions from the same sums, read from each other's shared memory.  The last pass leaves the
 // warps' sums behind, so the draw re-reads only the range in which its token lies.
 //
-// Measured on a B200 (calls replayed from a graph): 8 sequences x 6 nodes, vocabulary 8192: 6.7 us;
-// 64 x 24 nodes, 131072: 38 us (47 with one subtraction a rejection and eight CTAs a row), where the
-// last rows alone are 10 us at the memory's rate.  The bound is the slowest sequence's chain of
-// passes, up to four there, each of which waits for the one before.
+// Measured on a B200 (calls replayed from a graph).  8 chains of 6 nodes, vocabulary 8192: 7.5 us with q, 6.2
+// without.  64 x 24 nodes, 131072: 39 us with q (47 with one subtraction a rejection and eight CTAs a row), where
+// the last rows alone are 10 us at the memory's rate, and 50 without, of 5: every rejection is a pass over the
+// row, though without q it changes one entry.  The bound is the slowest sequence's chain of passes, with q up to
+// four there, each of which waits for the one before and takes 8 to 10 us.
 // The reference has no decode path.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -362,14 +363,13 @@ std::vector<at::Tensor> verify_tree(at::Tensor tokens, at::Tensor parents, at::T
   a.path = path.data_ptr<int>(); a.count = count.data_ptr<int>(); a.out = out.data_ptr<int>();
   a.N = (int)N; a.V = (int)V;
   TORCH_CHECK(B <= (1LL << 31) / kVerCluster - 1, "too many sequences");
-  // CTAs of a cluster: at most one for each 16384 entries, since exchanging sums costs a pass about
-  // 1 us (8 sequences x 6 nodes, 8192 entries: 6.7 us with one, 7.9 with two, 8.4 with eight,
-  // when a pass still took one subtraction a rejection).  Two CTAs
-  // fit on a SM; more than that wait their turn, which pays only while a CTA's range is long: turns
-  // at most as many as times 16384 entries a CTA.  131072 entries, 24 nodes, with 1 / 2 / 4 / 8 CTAs:
-  // 32 sequences 60 / 38 / 25 / 22 us, 64: 65 / 42 / 34 / 40, 128: 92 / 65 / 57 / 70, 256: 113 / 87 / 89 / 125;
-  // 32768 entries: 128 sequences 30 / 27 / 31 / 56, 512: 53 / 64 / 94 / 191 (all 5 to 8 % less than now:
-  // before small remainders were taken one by one).
+  // CTAs of a cluster: at most one for each 16384 entries, since exchanging sums costs every pass about 1 us.
+  // Two CTAs fit on a SM; more than that wait their turn, which pays only while a CTA's range is long: turns
+  // at most as many as times 16384 entries a CTA.  Trees with q, us with 1 / 2 / 4 / 8 CTAs (the rule's choice):
+  //   131072 entries, 24 nodes: 8 sequences 56 / 35 / 25 / 19 (8), 32: 65 / 41 / 28 / 26 (8), 64: 72 / 46 / 37 / 41 (4),
+  //                             128: 88 / 64 / 58 / 76 (4), 256: 115 / 94 / 99 / 141 (2)
+  //   32768, 24:                32: 24 / 21 / 18 / 22 (2), 128: 30 / 29 / 37 / 64 (2), 512: 58 / 74 / 111 / 222 (1)
+  //   8192, 6:                  8: 11 / 14 / 15 / 15 (1), 64: 12 / 17 / 21 / 29 (1), 512: 24 / 44 / 81 / 162 (1)
   const int64_t slots = 2 * num_sms(p.device().index());
   int C = 1;
   while (C < kVerCluster && (int64_t)C * 16384 < V && B * (2 * C) * (2 * C) * 16384 <= slots * V) C *= 2;

@@ -260,7 +260,11 @@ def tree_attention(q, k_cache, v_cache, lens, parents=None, scale: float | None 
     n's parent), so N = 1 is a plain decode step.  A node whose line of parents meets any other
     value is unused (the padding of a smaller tree: -2), as is one whose own row lies past the
     cache; its output is zero, and what its row holds reaches no other node.  ``scale`` defaults
-    to D^-0.5.  No gradient."""
+    to D^-0.5.  An infinity or a NaN in a row (in e4m3: a NaN code, or the scale NaN) reaches every
+    node that sees it; where all scores that a node sees are -inf its output is NaN.  Weights are
+    rounded to bfloat16 for the product with the values, or, for few rows over a quantised cache, to
+    float16 relative to the largest weight times scale, below 2^-25 of which a row may count nothing.
+    No gradient."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if _cuda(k_cache):
