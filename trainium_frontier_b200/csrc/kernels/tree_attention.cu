@@ -235,7 +235,7 @@ __device__ __forceinline__ float tree_ex2(float x) {
 // lands in the low bits of v + 1.5 * 2^23), 2^f on [-1/2, 1/2] by a polynomial of degree 4 fitted
 // here for the least relative error (2.7e-6), n added to its exponent.  A quarter of the
 // exponentials goes this way, since the two groups' 128 a row pair are all that the MUFU unit
-// of a sub-core does in 1024 cycles (bf16 caches: 126 instead of 138 us without any exponentials at
+// of a sub-core does in 1024 cycles (bf16 caches: 132 instead of 135 us without any exponentials at
 // all, so little is left; beside the conversion of quantised tiles the extra instructions cost
 // more than they save, 376 against 350 us).  NaN stays NaN.
 __device__ __forceinline__ float2 tree_exp2_pair(float2 v) {
