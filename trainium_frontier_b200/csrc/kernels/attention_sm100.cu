@@ -27,7 +27,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
-#include "sm100_common.cuh"
+#include "attention_tiles.cuh"
 
 namespace tfb {
 
@@ -60,10 +60,6 @@ __device__ __forceinline__ void fa_stamp(long long* tr, int role, int i, int e) 
   if (tr != nullptr && blockIdx.x == 0 && i < 64) tr[(role * 64 + i) * 8 + e] = clock64();
 }
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr uint32_t kPanel = 128u * 128u;  // one 64-column panel of 128 rows (bytes)
-
 template <int D>
 struct FaCfg {
   static constexpr int PANELS = D / 64;
@@ -89,15 +85,6 @@ __device__ __forceinline__ void grouped_item(int idx, int BH, int tiles, bool he
   tile = heavy_high ? tiles - 1 - t : t;
 }
 
-// K-major operand tile with K = 128 elements (two 64-element panels): k-step kk of 16.
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t base, int kk) {
-  return umma_desc_sw128(base + (uint32_t)(kk >> 2) * kPanel + (uint32_t)(kk & 3) * 32u, 16, 1024);
-}
-// MN-major operand tile (MN in 64-element panels, K along the 128 rows): k-step kk of 16.
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t base, int kk) {
-  return umma_desc_sw128(base + (uint32_t)kk * 2048u, kPanel, 1024);
-}
-
 // Write 128 fp32 values (one row) as bf16 into a 128-row x 128-col swizzled tile.
 __device__ __forceinline__ void store_row_bf16_sw128(uint8_t* tile, int row, const float* v) {
 #pragma unroll
@@ -108,17 +95,6 @@ __device__ __forceinline__ void store_row_bf16_sw128(uint8_t* tile, int row, con
     u.z = pack_bf16x2(v[8 * c + 4], v[8 * c + 5]);
     u.w = pack_bf16x2(v[8 * c + 6], v[8 * c + 7]);
     *reinterpret_cast<uint4*>(tile + (c >> 3) * kPanel + sw128_chunk_offset(row, c & 7)) = u;
-  }
-}
-
-__device__ __forceinline__ void store_row_bf16_global(__nv_bfloat16* dst, const float* v, int n) {
-  for (int c = 0; c < n / 8; ++c) {
-    uint4 u;
-    u.x = pack_bf16x2(v[8 * c + 0], v[8 * c + 1]);
-    u.y = pack_bf16x2(v[8 * c + 2], v[8 * c + 3]);
-    u.z = pack_bf16x2(v[8 * c + 4], v[8 * c + 5]);
-    u.w = pack_bf16x2(v[8 * c + 6], v[8 * c + 7]);
-    reinterpret_cast<uint4*>(dst)[c] = u;
   }
 }
 
@@ -365,38 +341,6 @@ __global__ void __launch_bounds__(192, 1)
 // three-input max; a quarter of the exponentials is computed on the FMA pipe
 // (exp2_poly) so the MUFU unit, whose 16 results per clock per SM match the tensor core's
 // 16 score elements per clock at head_dim 128, is not the limit.
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-// 2^v on the FMA pipe for v <= 8 (0 below -126): v = n + f with n the nearest integer
-// (added and subtracted 1.5 * 2^23, whose low mantissa bits then hold n) and f in
-// [-1/2, 1/2]; 2^f from a degree-3 polynomial fitted here for relative error on that
-// interval (max relative error 7.5e-5, far below the bf16 rounding of P); 2^n added
-// into the exponent field as n << 23, which is the magic sum's bits shifted by 23.
-// Clamping v at -126 keeps that exponent field from underflowing.
-__device__ __forceinline__ float2 exp2_poly2(float2 v) {
-  const float2 vc = make_float2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
-  const float2 t = __fadd2_rn(vc, make_float2(12582912.f, 12582912.f));
-  const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
-  const float2 f = __fadd2_rn(vc, make_float2(-n.x, -n.y));
-  float2 p = __ffma2_rn(make_float2(0.055170949548482895f, 0.055170949548482895f), f,
-                        make_float2(0.2426096349954605f, 0.2426096349954605f));
-  p = __ffma2_rn(p, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
-  p = __ffma2_rn(p, f, make_float2(0.9999281764030457f, 0.9999281764030457f));
-  const float rx = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
-  const float ry = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
-  return make_float2(v.x < -126.f ? 0.f : rx, v.y < -126.f ? 0.f : ry);
-}
-
 constexpr int kFwd2Slots = 5;  // K / V ring depth
 constexpr size_t kFwd2Smem = 1024 + 2 * 32768 + kFwd2Slots * 32768 + 24 * 8 + 16;
 

@@ -16,6 +16,8 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 
+#include <cuda_fp8.h>
+
 #include "sm100_common.cuh"
 
 namespace tfb {
@@ -84,6 +86,40 @@ inline const int* kv_ints(const at::Tensor& t, const char* name, c10::Device dev
   TORCH_CHECK(t.scalar_type() == at::kInt && t.device() == dev && fits && t.is_contiguous(), name, ": contiguous int32 of ",
               N < 0 ? "[B]" : "[B, N]", " entries on the caches' device");
   return t.data_ptr<int>();
+}
+
+// Keys' or values' entry of a parameter array.  Indexed, the array is copied to local memory by every
+// thread: 109 instead of 70 us for 16 x 4096 written rows of 8 heads, 159 instead of 119 for 8 x 16384 read.
+template <typename T>
+__device__ __forceinline__ T pick(const T (&a)[2], int kv) { return kv ? a[1] : a[0]; }
+
+// Exponent byte of the least power-of-two scale (2^-117 at the least) under which a row whose
+// largest magnitude has the bf16 bits `amax` fits +-448 = 1.75 * 2^8; 255 if it is not finite.
+__device__ __forceinline__ int scale_byte(uint32_t amax) {
+  const int ex = (int)(amax >> 7);
+  if (ex == 255) return kScaleNan;
+  const int e = ex - 8 + ((amax & 127u) > 96u ? 1 : 0);
+  return e < kScaleMin ? kScaleMin : e;
+}
+
+// 8 bf16 (one 16-byte load) times `inv` as 8 e4m3 codes, rounded to nearest even.
+__device__ __forceinline__ uint2 quant8(const uint4& u, float inv) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = make_float2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
+    c[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+  }
+  return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+}
+
+// Codes under the largest scale: 256 (0x78), which stands for 2^128, becomes 240.  No other code is above 240 there.
+__device__ __forceinline__ uint32_t hold_top(uint32_t c) { return c - ((((c & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u) >> 7); }
+
+__device__ __forceinline__ uint32_t absmax8(const uint4& u) {
+  const uint32_t m = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
 }
 
 }  // namespace tfb

@@ -24,6 +24,8 @@
 // dependent launches.  Two CTAs of 128 registers a SM spilled (101 us).
 #pragma once
 
+#include "warp_mma.cuh"
+
 namespace tfb {
 
 constexpr int kFewWarps = 8;
@@ -44,17 +46,6 @@ static_assert(FewCfg<128, true, 2>::NS <= kFewWarps && FewCfg<64, true, 2>::NS <
 static_assert(FewCfg<128, false, 1>::SMEM <= 232448 && FewCfg<128, true, 2>::SMEM <= 232448 && FewCfg<64, false, 2>::SMEM <= 232448,
               "shared memory");
 
-template <bool F16>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (F16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 template <bool TRANS>
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
   if constexpr (TRANS)
@@ -63,23 +54,6 @@ __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
   else
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-// Two e4m3 codes (low byte first) as two f16.
-__device__ __forceinline__ uint32_t codes2(uint32_t x) {
-  uint32_t y;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(y) : "r"(x));
-  return y;
-}
-__device__ __forceinline__ float e4m3_float(uint8_t x) {
-  return __half2float(__ushort_as_half((unsigned short)codes2(x)));
-}
-__device__ __forceinline__ float scale_float(uint8_t e) {
-  return e == kScaleNan ? __int_as_float(0x7fffffff) : e == 0 ? 0x1p-127f : __uint_as_float((uint32_t)e << 23);
-}
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t y;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-  return y;
 }
 // 16-byte chunk of a row of an e4m3 tile as TMA lays it out (128- or 64-byte swizzle).
 template <int D>
