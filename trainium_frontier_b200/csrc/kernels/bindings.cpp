@@ -90,6 +90,17 @@ torch::Tensor tree_attention(torch::Tensor q, torch::Tensor kc, torch::Tensor vc
                              c10::optional<torch::Tensor> vs, torch::Tensor err);
 std::vector<torch::Tensor> verify_tree(torch::Tensor tokens, torch::Tensor parents, torch::Tensor p, c10::optional<torch::Tensor> q,
                                        torch::Tensor u);
+std::vector<torch::Tensor> packed_attention_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu, double scale,
+                                                bool want_lse, torch::Tensor err);
+std::vector<torch::Tensor> packed_attention_bwd(torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                                torch::Tensor out, torch::Tensor lse, torch::Tensor cu, double scale, torch::Tensor err);
+void paged_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor kp, torch::Tensor vp, torch::Tensor table, torch::Tensor pos,
+                       c10::optional<torch::Tensor> cu, c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs);
+torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor vp, torch::Tensor table, torch::Tensor lens, double scale,
+                              c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs);
+std::vector<torch::Tensor> token_logprobs(torch::Tensor z, torch::Tensor tok, int64_t top, bool stats);
+torch::Tensor token_logprobs_grad(torch::Tensor z, torch::Tensor tok, torch::Tensor stat, c10::optional<torch::Tensor> g,
+                                  c10::optional<torch::Tensor> h);
 }  // namespace tfb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -123,6 +134,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_cache_commit", &tfb::kv_cache_commit, "accepted rows of a drafted tree moved behind the context");
   m.def("tree_attention", &tfb::tree_attention, "attention of a drafted tree over a KV cache");
   m.def("verify_tree", &tfb::verify_tree, "drafted tokens verified against the target's probabilities");
+  m.def("packed_attention_fwd", &tfb::packed_attention_fwd, "causal attention of packed sequences with shared key/value heads");
+  m.def("packed_attention_bwd", &tfb::packed_attention_bwd, "gradients of packed_attention_fwd");
+  m.def("paged_cache_write", &tfb::paged_cache_write, "packed rows into the pages of their sequences (bf16, or e4m3 quantised)");
+  m.def("paged_attention", &tfb::paged_attention, "attention of one new token a sequence over a cache of pages");
+  m.def("token_logprobs", &tfb::token_logprobs, "log probabilities of given tokens, entropies, likeliest alternatives");
+  m.def("token_logprobs_grad", &tfb::token_logprobs_grad, "gradient of the log probabilities and entropies");
   m.def("step_advance", &tfb::step_advance);
   m.def("argmax_rows", &tfb::argmax_rows);
   m.def("rope_norm_bwd", &tfb::rope_norm_bwd);

@@ -1,0 +1,1149 @@
+// Causal attention of sequences that lie behind one another in one buffer, with shared key/value
+// heads, forward and backward, on the 5th-generation tensor cores.
+//
+//   o_i = sum_{j <= i} p_ij v_j,   p_ij = exp(scale q_i . k_j - lse_i),   i, j rows of one sequence;
+//   D_i = dO_i . o_i,  ds_ij = p_ij (dO_i . v_j - D_i),
+//   dQ_i = scale sum_j ds_ij k_j,  dK_j = scale sum_i ds_ij q_i,  dV_j = sum_i p_ij dO_i.
+//
+// q [M, Hq, D], k and v [M, Hkv, D] are read where they lie (TMA tiles of 128 rows from any row on); a
+// tile that reaches past its sequence holds rows of the next one.  Those keys lie behind every
+// query of the sequence, so the causal mask hides them, and what they hold never enters a product: score
+// and weight are chosen, not multiplied by 0, and rows of an operand that the tensor core would multiply by
+// a weight of 0 are cleared in shared memory first.
+//
+// Which rows a CTA has follows from cu_seqlens alone (packed.cuh): no plan, no launch before the kernel, nothing
+// kept between calls, and rows outside all sequences get zeros.
+//
+// Forward: two 128-row tiles a CTA, which share every K / V tile and alternate on the tensor core: while one
+// tile's softmax runs, the other's products do.  The tiles are two query heads of one key/value head
+// where there are an even number of them (both see the same keys: no tile waits for the other's end, and
+// short sequences fill both), else neighbouring rows of one head.
+//   warp 0      TMA: Q tiles, then K_0, V_0, K_1, .. through a ring
+//   warp 1      MMA: per step P0 V, S0(next), P1 V, S1(next); P from TMEM, over its own scores
+//   warps 2-9   softmax of tile 0 / 1, a row a thread; a quarter of the exponentials on the FMA pipe
+// The running maximum moves only when it grows by more than 8 (in log2), so outputs are rarely rescaled.
+//
+// Backward: two kernels and no sum through memory.  One has 128 queries and goes over the keys (dQ, three
+// products a tile); one has 128 keys of a key/value head and goes over all queries of its query heads (dK and
+// dV, four).  Scores are formed twice, seven products instead of the five of a single pass, but that
+// pass would add every dQ tile into 32-bit memory (an accumulator written, added to, read and rounded, in an
+// order that changes from run to run).  Here each gradient is a sum in TMEM, in order, and rounded once.
+#include <ATen/core/Tensor.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "attention_tiles.cuh"
+#include "packed.cuh"
+
+namespace tfb {
+
+CUtensorMap make_tmap_bf16(const void* ptr, uint64_t inner, uint64_t outer, uint64_t row_stride_elems,
+                           uint32_t box_inner, uint32_t box_outer, uint64_t batch, uint64_t batch_stride_elems);
+
+constexpr float kPkLowest = -3.4028234663852886e38f;
+
+struct PkArgs {
+  Pieces pc;
+  int Hq, Hkv, G;
+  int by_heads;                  // the forward's two tiles are two heads (else neighbouring rows)
+  float scale, scale_log2;
+  const __nv_bfloat16 *q, *k, *v, *o, *dout;           // rows and heads, strides in elements
+  long long qr, qh, kr, kh, vr, vh, gr, gh;
+  __nv_bfloat16 *out, *dq, *dk, *dv;                   // [M, H, D]
+  float *lse, *dvec;             // [Hq, M]
+  int* err;
+};
+
+// max that keeps a NaN
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// Row `row` of a tile of D columns (swizzled panels of 64): whether it holds an infinity or a NaN.
+template <int D>
+__device__ __forceinline__ bool tile_row_bad(const uint8_t* tile, int row) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) {
+    const uint4 u = *reinterpret_cast<const uint4*>(tile + (c >> 3) * kPanel + sw128_chunk_offset(row, c & 7));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+      bad |= ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    }
+  }
+  return bad != 0;
+}
+template <int D>
+__device__ __forceinline__ void tile_row_clear(uint8_t* tile, int row) {
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c)
+    *reinterpret_cast<uint4*>(tile + (c >> 3) * kPanel + sw128_chunk_offset(row, c & 7)) = make_uint4(0, 0, 0, 0);
+}
+
+// Zeros into rows [row0, row0 + n) x heads of out [M, H, D] (rows outside all sequences).
+template <int D>
+__device__ __forceinline__ void clear_rows(__nv_bfloat16* out, int H, int h0, int heads, long long row0, int n) {
+  for (int i = threadIdx.x; i < n * heads * (D / 8); i += blockDim.x) {
+    const int c = i % (D / 8), h = i / (D / 8) % heads, r = i / (D / 8) / heads;
+    reinterpret_cast<uint4*>(out + ((row0 + r) * H + h0 + h) * D)[c] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// A row's output by itself, keys one after another in 32 bits: for the rows of a diagonal tile whose masked
+// values hold an infinity or a NaN, which the tensor core would multiply by 0.
+template <int D>
+__device__ __noinline__ void packed_row(const PkArgs& a, int begin, int i, int h, float lse2, __nv_bfloat16* dst) {
+  const __nv_bfloat16* q = a.q + (long long)(begin + i) * a.qr + h * a.qh;
+  const int hk = h / a.G;
+#pragma unroll 1
+  for (int d0 = 0; d0 < D; d0 += 32) {
+    float o[32];
+#pragma unroll
+    for (int d = 0; d < 32; ++d) o[d] = 0.f;
+#pragma unroll 1
+    for (int j = 0; j <= i; ++j) {
+      const __nv_bfloat16* k = a.k + (long long)(begin + j) * a.kr + hk * a.kh;
+      const __nv_bfloat16* v = a.v + (long long)(begin + j) * a.vr + hk * a.vh + d0;
+      float s = 0.f;
+#pragma unroll 1
+      for (int d = 0; d < D; ++d) s += __bfloat162float(q[d]) * __bfloat162float(k[d]);
+      const float p = ex2_approx(s * a.scale_log2 - lse2);
+#pragma unroll
+      for (int d = 0; d < 32; ++d) o[d] += p * __bfloat162float(v[d]);
+    }
+    store_row_bf16_global(dst + d0, o, 32);
+  }
+}
+
+template <int D>
+struct PkFwd {
+  static constexpr uint32_t TILE = 128u * D * 2u;
+  static constexpr int NS = D == 128 ? 5 : 8;          // K / V ring
+  static constexpr size_t SMEM = 1024 + (2 + NS) * TILE + 32 * 8 + 64;
+};
+
+template <int D>
+__global__ void __launch_bounds__(320, 1)
+    packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                      const __grid_constant__ CUtensorMap tmV, const PkArgs a) {
+  constexpr uint32_t TILE = PkFwd<D>::TILE;
+  constexpr int NS = PkFwd<D>::NS, PANELS = D / 64;
+  constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, false, false);
+  constexpr uint32_t IDESC_O = umma_idesc_bf16(128, D, false, true);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                 // [2] tiles
+  uint8_t* sKV = sQ + 2 * TILE;       // [NS] slots
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + NS * TILE);
+  uint64_t* bar_q = bars + 0;
+  uint64_t* kv_full = bars + 1;          // [NS]
+  uint64_t* kv_empty = bars + 1 + NS;    // [NS]
+  uint64_t* s_full = bars + 1 + 2 * NS;  // [2]
+  uint64_t* p_full = s_full + 2;         // [2]
+  uint64_t* o_done = p_full + 2;         // [2]
+  uint64_t* drain = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* by_row = abort_flag + 1;               // [2] the tile's rows are computed one by one
+  PieceUnit* s_unit = reinterpret_cast<PieceUnit*>(tmem_slot + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nh = a.by_heads ? a.Hq / 2 : a.Hq;
+  const int hx = (int)(blockIdx.x % nh);
+  const int slot_id = (int)(gridDim.x / nh - 1 - blockIdx.x / nh);   // a sequence's last rows have the most keys: first
+  if (warp == 0) {
+    const PieceUnit u = a.by_heads ? piece_unit<128>(a.pc, slot_id) : piece_unit<256>(a.pc, slot_id);
+    if (lane == 0) *s_unit = u;
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  } else if (threadIdx.x == 64) {
+    mbar_init(bar_q, 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 128);
+      mbar_init(&o_done[t], 1);
+      by_row[t] = 0;
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const PieceUnit un = *s_unit;
+  const int U = a.by_heads ? 128 : 256;
+  const bool live = un.unit >= 0 && a.pc.real(un.piece);
+  // tile t: its head, first row in the sequence, and number of K / V tiles (0: there is none)
+  const int h0 = a.by_heads ? 2 * hx : hx, h1 = a.by_heads ? h0 + 1 : hx;
+  const int r0 = un.unit * U, r1 = a.by_heads ? r0 : r0 + 128;
+  const int n0 = live ? r0 / 128 + 1 : 0, n1 = live && r1 < un.len ? r1 / 128 + 1 : 0;
+  const int nk = max(n0, n1);
+  const int hk = h0 / a.G;
+
+  if (!live) {
+    if (un.unit >= 0) clear_rows<D>(a.out, a.Hq, h0, a.by_heads ? 2 : 1, un.begin + r0, min(U, un.len - r0));
+  } else if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t out_valid = 0, out_parity = 0;
+      mbar_arrive_expect_tx(bar_q, (n1 ? 2 : 1) * TILE);
+#pragma unroll
+      for (int p = 0; p < PANELS; ++p) {
+        tma_load_3d(sQ + p * kPanel, &tmQ, bar_q, p * 64, un.begin + r0, h0);
+        if (n1) tma_load_3d(sQ + TILE + p * kPanel, &tmQ, bar_q, p * 64, un.begin + r1, h1);
+      }
+      const int items = 2 * nk;
+      for (int i = 0; i < items && ok; ++i) {
+        const int slot = i % NS;
+        if (i >= NS && !mbar_wait(&kv_empty[slot], ((i / NS) + 1) & 1, abort_flag, a.err, ERR_TIMEOUT_PRODUCER)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(&kv_full[slot], TILE);
+        out_valid |= 1u << slot;
+        out_parity = (out_parity & ~(1u << slot)) | ((uint32_t)((i / NS) & 1) << slot);
+        const int krow = un.begin + (i >> 1) * 128;
+        const CUtensorMap* map = (i & 1) ? &tmV : &tmK;
+#pragma unroll
+        for (int p = 0; p < PANELS; ++p) tma_load_3d(sKV + slot * TILE + p * kPanel, map, &kv_full[slot], p * 64, krow, hk);
+      }
+      if (!ok) {
+        for (int s = 0; s < NS; ++s) {
+          if (!((out_valid >> s) & 1u)) continue;
+          const unsigned long long t0 = globaltimer_ns();
+          while (!mbar_try_wait(&kv_full[s], (out_parity >> s) & 1u))
+            if (globaltimer_ns() - t0 > 100000000ull) break;
+        }
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(bar_q, 0))
+          if (globaltimer_ns() - t0 > 100000000ull) break;
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      bool ok = mbar_wait(bar_q, 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
+      const uint32_t q_addr[2] = {smem_u32(sQ), smem_u32(sQ + TILE)};
+      auto kv_wait = [&](int item) -> bool {
+        return mbar_wait(&kv_full[item % NS], (item / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA);
+      };
+      auto issue_s = [&](int t, int j) -> bool {
+        if (!kv_wait(2 * j)) return false;
+        tc_fence_after();
+        const uint32_t k_addr = smem_u32(sKV + ((2 * j) % NS) * TILE);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16(tmem + t * 128, desc_kmajor(q_addr[t], kk), desc_kmajor(k_addr, kk), IDESC_S, kk > 0 ? 1u : 0u);
+        umma_commit(&s_full[t]);
+        return true;
+      };
+      auto issue_pv = [&](int t, int j) -> bool {
+        if (!kv_wait(2 * j + 1)) return false;
+        if (!mbar_wait(&p_full[t], j & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+        tc_fence_after();
+        const uint32_t v_addr = smem_u32(sKV + ((2 * j + 1) % NS) * TILE);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)  // P_t(j): 16 keys = 8 packed columns per MMA
+          umma_bf16_tmem_a(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, desc_mnmajor(v_addr, kk), IDESC_O,
+                           (j > 0 || kk > 0) ? 1u : 0u);
+        return true;
+      };
+      if (ok) ok = issue_s(0, 0) && (n1 == 0 || issue_s(1, 0));
+      if (ok) umma_commit(&kv_empty[0]);  // K_0 read by both tiles
+      for (int j = 0; j < nk && ok; ++j) {
+        // one thread's tcgen05 MMAs run in issue order: S_t(j + 1) may overwrite P_t(j)
+        if (j < n0) {
+          if (!issue_pv(0, j)) { ok = false; break; }
+          if (j + 1 < n0) {
+            if (!issue_s(0, j + 1)) { ok = false; break; }
+          } else {
+            umma_commit(&o_done[0]);
+          }
+        }
+        if (j < n1) {
+          if (!issue_pv(1, j)) { ok = false; break; }
+          if (j + 1 < n1) {
+            if (!issue_s(1, j + 1)) { ok = false; break; }
+          } else {
+            umma_commit(&o_done[1]);
+          }
+        }
+        if (j + 1 < nk) umma_commit(&kv_empty[(2 * (j + 1)) % NS]);  // K_{j+1} read by both tiles
+        umma_commit(&kv_empty[(2 * j + 1) % NS]);                    // V_j done
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        umma_commit(drain);
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0))
+          if (globaltimer_ns() - t0 > 100000000ull) break;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax (tile t)
+    const int t = (warp - 2) >> 2;
+    const int q4 = warp & 3;
+    const int r = q4 * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+    const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
+    const int n_t = t == 0 ? n0 : n1;
+    const int row = (t == 0 ? r0 : r1) + r, head = t == 0 ? h0 : h1;   // row of the sequence
+    const float c = a.scale_log2;
+    float m_run = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n_t; ++j) {
+      if (!mbar_wait_warp(&s_full[t], j & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      tc_fence_after();
+      float x[128];
+      {
+        uint32_t* xr = reinterpret_cast<uint32_t*>(x);
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          __syncwarp();
+          tmem_ld_32x32b_x32(tS + lane_off + cc * 32, *reinterpret_cast<uint32_t(*)[32]>(xr + 32 * cc));
+        }
+        tmem_ld_wait();
+      }
+      if (j == n_t - 1) {  // diagonal tile: keys after this query row are masked, those past the sequence among them
+#pragma unroll
+        for (int i = 0; i < 128; ++i)
+          if (i > r) x[i] = -INFINITY;
+        // masked rows of V: past the sequence (another's) cleared, the sequence's own looked over
+        if (!mbar_wait_warp(&kv_full[(2 * j + 1) % NS], ((2 * j + 1) / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+        uint8_t* v = sKV + ((2 * j + 1) % NS) * TILE;
+        if (j * 128 + r >= un.len) {
+          tile_row_clear<D>(v, r);
+          fence_proxy_async_smem();
+        } else if (tile_row_bad<D>(v, r)) {
+          by_row[t] = 1;
+        }
+      }
+      // four independent max chains, two new elements per three-input max
+      float mx4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+      for (int i = 4; i < 128; i += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx4[k] = max3_nan(mx4[k], x[i + k], x[i + 4 + k]);
+      // visible scores of -inf count as the lowest number, so that their weights are 0
+      float mxs = max_nan(max_nan(max_nan(mx4[0], mx4[1]), max_nan(mx4[2], mx4[3])) * c, kPkLowest);
+      if (mxs == INFINITY) mxs = NAN;            // inf - inf
+      float alpha = 1.f;
+      const bool grow = !(mxs <= m_run + 8.f);   // true for a NaN, which then stays
+      if (grow) {
+        alpha = ex2_approx(m_run - mxs);
+        m_run = mxs;
+      }
+      // p = 2^(x c - m): packed pairs; columns 96..127 of every row on the FMA pipe
+      const float2 c2 = make_float2(c, c), nm2 = make_float2(-m_run, -m_run);
+      float2 sm4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      uint32_t pk[64];  // the row of P as packed bf16 pairs
+#pragma unroll
+      for (int i = 0; i < 128; i += 2) {
+        const float2 v = __ffma2_rn(make_float2(x[i], x[i + 1]), c2, nm2);
+        float2 p2;
+        if (i >= 96) p2 = exp2_poly2(v);
+        else p2 = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+        pk[i >> 1] = pack_bf16x2(p2.x, p2.y);
+        sm4[(i >> 1) & 3] = __fadd2_rn(sm4[(i >> 1) & 3], p2);
+      }
+      const float2 s01 = __fadd2_rn(__fadd2_rn(sm4[0], sm4[1]), __fadd2_rn(sm4[2], sm4[3]));
+      l = l * alpha + (s01.x + s01.y);
+      // O_t is stable: the commit that signalled S_t(j) covered P_t(j-1) V_{j-1}
+      if (j >= 1 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+        for (int cc = 0; cc < D / 32; ++cc) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(tO + lane_off + cc * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st_32x32b_x32(tO + lane_off + cc * 32, o);
+        }
+      }
+      // P_t(j) over the first 64 columns of S_t(j) (already in registers)
+      __syncwarp();
+      tmem_st_32x32b_x32(tS + lane_off, *reinterpret_cast<const uint32_t(*)[32]>(pk));
+      tmem_st_32x32b_x32(tS + lane_off + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[t]);
+    }
+    if (n_t > 0 && ok && mbar_wait_warp(&o_done[t], 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
+      tc_fence_after();
+      const float inv_l = 1.f / l, lse2 = m_run + log2f(l);
+      __nv_bfloat16* dst = a.out + ((long long)(un.begin + row) * a.Hq + head) * D;
+      const bool mine = row < un.len, alone = by_row[t] != 0;
+#pragma unroll 1
+      for (int cc = 0; cc < D / 32; ++cc) {
+        uint32_t o[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tO + lane_off + cc * 32, o);
+        tmem_ld_wait();
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * inv_l;
+        if (mine && !alone) store_row_bf16_global(dst + cc * 32, f, 32);
+      }
+      if (mine && alone) packed_row<D>(a, un.begin, row, head, lse2, dst);
+      if (mine && a.lse) a.lse[(long long)head * a.pc.M + un.begin + row] = lse2 * kLn2;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ================================================================================ backward: dQ
+// One CTA per 128 queries of a head, over the keys.  TMEM: S | dP | dQ | two dS (bf16).
+//   warp 0      TMA: Q and dO, then K_0, V_0, K_1, .. through a ring
+//   warp 1      MMA: per step S(next) = Q K^T, dP(next) = dO V^T, dQ += dS K with dS from TMEM
+//   warps 2-9   p = 2^(S c - lse), dS = p (dP - D): two warps a lane quarter, 64 columns each
+// S and dP are given back as soon as they are in registers, so the next ones are formed meanwhile.
+template <int D>
+struct PkDq {
+  static constexpr uint32_t TILE = 128u * D * 2u;
+  static constexpr int NS = D == 128 ? 5 : 8;
+  static constexpr size_t SMEM = 1024 + (2 + NS) * TILE + 1024 + 32 * 8 + 64;
+};
+
+template <int D>
+__global__ void __launch_bounds__(320, 1)
+    packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const PkArgs a) {
+  constexpr uint32_t TILE = PkDq<D>::TILE;
+  constexpr int NS = PkDq<D>::NS, PANELS = D / 64;
+  constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, false, false);
+  constexpr uint32_t IDESC_Q = umma_idesc_bf16(128, D, false, true);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sG = sQ + TILE;
+  uint8_t* sKV = sG + TILE;
+  float* sD = reinterpret_cast<float*>(sKV + NS * TILE);   // [256]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sD + 256);
+  uint64_t* bar_q = bars + 0;
+  uint64_t* kv_full = bars + 1;          // [NS]
+  uint64_t* kv_empty = bars + 1 + NS;    // [NS]
+  uint64_t* s_full = bars + 1 + 2 * NS;
+  uint64_t* s_free = s_full + 1;
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* dp_free = s_full + 3;
+  uint64_t* ds_full = s_full + 4;
+  uint64_t* done = s_full + 5;
+  uint64_t* drain = s_full + 6;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  PieceUnit* s_unit = reinterpret_cast<PieceUnit*>(tmem_slot + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = (int)(blockIdx.x % a.Hq), hk = h / a.G;
+  if (warp == 0) {
+    const PieceUnit u = piece_unit<128>(a.pc, (int)(gridDim.x / a.Hq - 1 - blockIdx.x / a.Hq));
+    if (lane == 0) *s_unit = u;
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  } else if (threadIdx.x == 64) {
+    mbar_init(bar_q, 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(s_free, 256);
+    mbar_init(dp_full, 1);
+    mbar_init(dp_free, 256);
+    mbar_init(ds_full, 256);
+    mbar_init(done, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmG);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tS = tmem, tP = tmem + 128, tQ = tmem + 256, tD = tmem + 384;
+  const PieceUnit un = *s_unit;
+  const int row0 = un.unit * 128, n = un.unit + 1;
+
+  if (un.unit < 0 || !a.pc.real(un.piece)) {
+    if (un.unit >= 0) clear_rows<D>(a.dq, a.Hq, h, 1, un.begin + row0, min(128, un.len - row0));
+  } else if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t out_valid = 0, out_parity = 0;
+      mbar_arrive_expect_tx(bar_q, 2 * TILE);
+#pragma unroll
+      for (int p = 0; p < PANELS; ++p) {
+        tma_load_3d(sQ + p * kPanel, &tmQ, bar_q, p * 64, un.begin + row0, h);
+        tma_load_3d(sG + p * kPanel, &tmG, bar_q, p * 64, un.begin + row0, h);
+      }
+      for (int i = 0; i < 2 * n && ok; ++i) {
+        const int slot = i % NS;
+        if (i >= NS && !mbar_wait(&kv_empty[slot], ((i / NS) + 1) & 1, abort_flag, a.err, ERR_TIMEOUT_PRODUCER)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(&kv_full[slot], TILE);
+        out_valid |= 1u << slot;
+        out_parity = (out_parity & ~(1u << slot)) | ((uint32_t)((i / NS) & 1) << slot);
+        const CUtensorMap* map = (i & 1) ? &tmV : &tmK;
+#pragma unroll
+        for (int p = 0; p < PANELS; ++p)
+          tma_load_3d(sKV + slot * TILE + p * kPanel, map, &kv_full[slot], p * 64, un.begin + (i >> 1) * 128, hk);
+      }
+      if (!ok) {
+        for (int s = 0; s < NS; ++s) {
+          if (!((out_valid >> s) & 1u)) continue;
+          const unsigned long long t0 = globaltimer_ns();
+          while (!mbar_try_wait(&kv_full[s], (out_parity >> s) & 1u))
+            if (globaltimer_ns() - t0 > 100000000ull) break;
+        }
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(bar_q, 0))
+          if (globaltimer_ns() - t0 > 100000000ull) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = mbar_wait(bar_q, 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
+      const uint32_t q_addr = smem_u32(sQ), g_addr = smem_u32(sG);
+      auto kv_addr = [&](int item) { return smem_u32(sKV + (item % NS) * TILE); };
+      auto kv_wait = [&](int item) { return mbar_wait(&kv_full[item % NS], (item / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA); };
+      // S(j) = Q K_j^T, dP(j) = dO V_j^T, once the compute warps have the tiles before in registers
+      auto issue = [&](int j) -> bool {
+        if (!kv_wait(2 * j)) return false;
+        if (j >= 1 && !mbar_wait(s_free, (j - 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16(tS, desc_kmajor(q_addr, kk), desc_kmajor(kv_addr(2 * j), kk), IDESC_S, kk > 0 ? 1u : 0u);
+        umma_commit(s_full);
+        if (!kv_wait(2 * j + 1)) return false;
+        if (j >= 1 && !mbar_wait(dp_free, (j - 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16(tP, desc_kmajor(g_addr, kk), desc_kmajor(kv_addr(2 * j + 1), kk), IDESC_S, kk > 0 ? 1u : 0u);
+        umma_commit(dp_full);
+        umma_commit(&kv_empty[(2 * j + 1) % NS]);
+        return true;
+      };
+      if (ok) ok = issue(0);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n && !issue(j + 1)) { ok = false; break; }
+        if (!mbar_wait(ds_full, j & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)  // dQ += dS(j) K_j
+          umma_bf16_tmem_a(tQ, tD + (j & 1) * 64 + kk * 8, desc_mnmajor(kv_addr(2 * j), kk), IDESC_Q, (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&kv_empty[(2 * j) % NS]);
+      }
+      if (ok) {
+        umma_commit(done);
+      } else {
+        *abort_flag = 1;
+        umma_commit(drain);
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0))
+          if (globaltimer_ns() - t0 > 100000000ull) break;
+      }
+    }
+  } else {
+    const int q4 = warp & 3, half = (warp - 2) >> 2, cb = half * 64;
+    const int r = q4 * 32 + lane, row = row0 + r;
+    const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+    const bool mine = row < un.len;
+    const long long at = (long long)h * a.pc.M + un.begin + row;
+    // D_i = dO_i . o_i, half of the columns a thread; kept for the other kernel
+    float dsum = 0.f;
+    if (mine) {
+      const uint4* g = reinterpret_cast<const uint4*>(a.dout + (long long)(un.begin + row) * a.gr + h * a.gh + half * (D / 2));
+      const uint4* o = reinterpret_cast<const uint4*>(a.o + ((long long)(un.begin + row) * a.Hq + h) * D + half * (D / 2));
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint4 x = g[i], y = o[i];
+        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          dsum += __uint_as_float(xw[w] << 16) * __uint_as_float(yw[w] << 16);
+          dsum += __uint_as_float(xw[w] & 0xffff0000u) * __uint_as_float(yw[w] & 0xffff0000u);
+        }
+      }
+    }
+    sD[half * 128 + r] = dsum;
+    named_bar_sync(1, 256);              // no wait comes before it: all 256 threads arrive
+    dsum = sD[r] + sD[128 + r];
+    if (mine && half == 0) a.dvec[at] = dsum;
+    const float nlse = mine ? -a.lse[at] * kLog2e : -INFINITY;
+    const float2 c2 = make_float2(a.scale_log2, a.scale_log2), nl2 = make_float2(nlse, nlse), nd2 = make_float2(-dsum, -dsum);
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const bool diag = j == n - 1;
+      if (!mbar_wait_warp(s_full, j & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      tc_fence_after();
+      float p[64];
+      uint32_t* pr = reinterpret_cast<uint32_t*>(p);
+      __syncwarp();
+      tmem_ld_32x32b_x32(tS + lane_off + cb, *reinterpret_cast<uint32_t(*)[32]>(pr));
+      tmem_ld_32x32b_x32(tS + lane_off + cb + 32, *reinterpret_cast<uint32_t(*)[32]>(pr + 32));
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(s_free);
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) {
+        const float2 v = __ffma2_rn(make_float2(p[e], p[e + 1]), c2, nl2);
+        float2 y;
+        if (e >= 48) y = exp2_poly2(v);
+        else y = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+        p[e] = y.x;
+        p[e + 1] = y.y;
+      }
+      if (diag) {
+        // rows of K past the sequence, which weights of 0 would meet
+        if (half == 0 && j * 128 + r >= un.len) {
+          const int item = 2 * j;
+          mbar_wait(&kv_full[item % NS], (item / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
+          tile_row_clear<D>(sKV + (item % NS) * TILE, r);
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+      }
+      if (!mbar_wait_warp(dp_full, j & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t pk[32];
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        uint32_t dp[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tP + lane_off + cb + h2 * 32, dp);
+        tmem_ld_wait();
+        if (h2 == 1) {
+          tc_fence_before();
+          mbar_arrive(dp_free);
+        }
+#pragma unroll
+        for (int e0 = 0; e0 < 32; e0 += 2) {
+          const int e = h2 * 32 + e0;
+          float2 d = __fmul2_rn(make_float2(p[e], p[e + 1]), __fadd2_rn(make_float2(__uint_as_float(dp[e0]), __uint_as_float(dp[e0 + 1])), nd2));
+          if (diag) {
+            if (cb + e > r) d.x = 0.f;
+            if (cb + e + 1 > r) d.y = 0.f;
+          }
+          pk[e >> 1] = pack_bf16x2(d.x, d.y);
+        }
+      }
+      // dS(j - 2) has been read: the commit that signalled S(j) covered dQ(j - 2)
+      __syncwarp();
+      tmem_st_32x32b_x32(tD + (j & 1) * 64 + lane_off + half * 32, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(ds_full);
+    }
+    if (ok && mbar_wait_warp(done, 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
+      tc_fence_after();
+      __nv_bfloat16* dst = a.dq + ((long long)(un.begin + row) * a.Hq + h) * D + half * (D / 2);
+#pragma unroll 1
+      for (int cc = 0; cc < D / 64; ++cc) {
+        uint32_t o[32];
+        float f[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tQ + lane_off + half * (D / 2) + cc * 32, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * a.scale;
+        if (mine) store_row_bf16_global(dst + cc * 32, f, 32);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ================================================================================ backward: dK, dV
+// One CTA per 128 keys of a key/value head, over the queries from there on of all its query heads, in the
+// transposed frame (a key a TMEM lane).  TMEM: S^T | dP^T | dV | dK; P^T and dS^T lie over the scores they came
+// from, each warp's over columns that it alone has read.  MMA order dV(i), S(i+1), dK(i), dP(i+1): while the
+// compute warps turn dP into dS the tensor core runs dV and the next S, and while they take the next exponentials dK
+// and the next dP.
+template <int D>
+struct PkDkv {
+  static constexpr uint32_t TILE = 128u * D * 2u;
+  static constexpr size_t SMEM = 1024 + 6 * TILE + 4 * 512 + 32 * 8 + 64;
+};
+
+template <int D>
+__global__ void __launch_bounds__(320, 1)
+    packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const PkArgs a) {
+  constexpr uint32_t TILE = PkDkv<D>::TILE;
+  constexpr int PANELS = D / 64;
+  constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, false, false);
+  constexpr uint32_t IDESC_KV = umma_idesc_bf16(128, D, false, true);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = sK + TILE;
+  uint8_t* sQ = sV + TILE;             // [2]
+  uint8_t* sG = sQ + 2 * TILE;         // [2]
+  float* sL = reinterpret_cast<float*>(sG + 2 * TILE);   // [2][128] -lse in log2
+  float* sD = sL + 256;                                  // [2][128] -D
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sD + 256);
+  uint64_t* bar_kv = bars + 0;
+  uint64_t* q_full = bars + 1;         // [2]
+  uint64_t* q_empty = bars + 3;        // [2]
+  uint64_t* g_full = bars + 5;         // [2]
+  uint64_t* g_empty = bars + 7;        // [2]
+  uint64_t* l_full = bars + 9;         // [2]
+  uint64_t* s_full = bars + 11;
+  uint64_t* p_full = bars + 12;
+  uint64_t* dp_full = bars + 13;
+  uint64_t* ds_full = bars + 14;
+  uint64_t* done = bars + 15;
+  uint64_t* drain = bars + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  PieceUnit* s_unit = reinterpret_cast<PieceUnit*>(tmem_slot + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = (int)(blockIdx.x % a.Hkv);
+  if (warp == 0) {
+    const PieceUnit u = piece_unit<128>(a.pc, (int)(blockIdx.x / a.Hkv));   // a sequence's first keys have the most queries
+    if (lane == 0) *s_unit = u;
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  } else if (threadIdx.x == 64) {
+    mbar_init(bar_kv, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&g_full[i], 1);
+      mbar_init(&g_empty[i], 1);
+      mbar_init(&l_full[i], 256);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 256);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, 256);
+    mbar_init(done, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmG);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tS = tmem, tP = tmem + 128, tDV = tmem + 256, tDK = tmem + 384;
+  const PieceUnit un = *s_unit;
+  const int kt = un.unit, row0 = kt * 128;
+  const int tiles = (un.len + 127) / 128, nq = tiles - kt, n = nq * a.G;   // steps: query tiles kt .. of every query head
+
+  if (un.unit < 0 || !a.pc.real(un.piece)) {
+    if (un.unit >= 0) {
+      clear_rows<D>(a.dk, a.Hkv, hk, 1, un.begin + row0, min(128, un.len - row0));
+      clear_rows<D>(a.dv, a.Hkv, hk, 1, un.begin + row0, min(128, un.len - row0));
+    }
+  } else if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t valid = 0, parity = 0;    // bits 0, 1: Q; 2, 3: dO
+      mbar_arrive_expect_tx(bar_kv, 2 * TILE);
+#pragma unroll
+      for (int p = 0; p < PANELS; ++p) {
+        tma_load_3d(sK + p * kPanel, &tmK, bar_kv, p * 64, un.begin + row0, hk);
+        tma_load_3d(sV + p * kPanel, &tmV, bar_kv, p * 64, un.begin + row0, hk);
+      }
+      int qi = kt, h = hk * a.G;
+      for (int it = 0; it < n && ok; ++it) {
+        const int b = it & 1;
+#pragma unroll
+        for (int w = 0; w < 2 && ok; ++w) {
+          if (it >= 2 && !mbar_wait(w ? &g_empty[b] : &q_empty[b], ((it - 2) >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          uint64_t* bar = w ? &g_full[b] : &q_full[b];
+          mbar_arrive_expect_tx(bar, TILE);
+          valid |= 1u << (2 * w + b);
+          parity = (parity & ~(1u << (2 * w + b))) | ((uint32_t)((it >> 1) & 1) << (2 * w + b));
+#pragma unroll
+          for (int p = 0; p < PANELS; ++p)
+            tma_load_3d((w ? sG : sQ) + b * TILE + p * kPanel, w ? &tmG : &tmQ, bar, p * 64, un.begin + qi * 128, h);
+        }
+        if (++qi == tiles) { qi = kt; ++h; }
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        const unsigned long long t0 = globaltimer_ns();
+        for (int s = 0; s < 4; ++s) {
+          if (!((valid >> s) & 1u)) continue;
+          while (!mbar_try_wait(s < 2 ? &q_full[s] : &g_full[s - 2], (parity >> s) & 1u))
+            if (globaltimer_ns() - t0 > 200000000ull) break;
+        }
+        while (!mbar_try_wait(bar_kv, 0))
+          if (globaltimer_ns() - t0 > 300000000ull) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = mbar_wait(bar_kv, 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
+      const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV);
+      auto issue_s = [&](int it) -> bool {   // S^T = K Q^T
+        const int b = it & 1;
+        if (!mbar_wait(&q_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+        tc_fence_after();
+        const uint32_t q_addr = smem_u32(sQ + b * TILE);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16(tS, desc_kmajor(k_addr, kk), desc_kmajor(q_addr, kk), IDESC_S, kk > 0 ? 1u : 0u);
+        umma_commit(s_full);
+        return true;
+      };
+      auto issue_dp = [&](int it) -> bool {  // dP^T = V dO^T
+        const int b = it & 1;
+        if (!mbar_wait(&g_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+        tc_fence_after();
+        const uint32_t g_addr = smem_u32(sG + b * TILE);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16(tP, desc_kmajor(v_addr, kk), desc_kmajor(g_addr, kk), IDESC_S, kk > 0 ? 1u : 0u);
+        umma_commit(dp_full);
+        return true;
+      };
+      if (ok) ok = issue_s(0) && issue_dp(0);
+      for (int it = 0; it < n && ok; ++it) {
+        const int b = it & 1;
+        const uint32_t q_addr = smem_u32(sQ + b * TILE), g_addr = smem_u32(sG + b * TILE);
+        if (!mbar_wait(p_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)  // dV += P^T dO: the weights of queries 0-63 in columns 0-31, of 64-127 in 64-95
+          umma_bf16_tmem_a(tDV, tS + (kk >> 2) * 64 + (kk & 3) * 8, desc_mnmajor(g_addr, kk), IDESC_KV, (it > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&g_empty[b]);
+        if (it + 1 < n && !issue_s(it + 1)) { ok = false; break; }
+        if (!mbar_wait(ds_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)  // dK += dS^T Q
+          umma_bf16_tmem_a(tDK, tP + (kk >> 2) * 64 + (kk & 3) * 8, desc_mnmajor(q_addr, kk), IDESC_KV, (it > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&q_empty[b]);
+        if (it + 1 < n && !issue_dp(it + 1)) { ok = false; break; }
+      }
+      if (ok) {
+        umma_commit(done);
+      } else {
+        *abort_flag = 1;
+        umma_commit(drain);
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0))
+          if (globaltimer_ns() - t0 > 100000000ull) break;
+      }
+    }
+  } else {
+    const int q4 = warp & 3, half = (warp - 2) >> 2, cb = half * 64;
+    const int r = q4 * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+    const float2 c2 = make_float2(a.scale_log2, a.scale_log2);
+    const float* stats = half == 0 ? a.lse : a.dvec;
+    int qi = kt, h = hk * a.G;
+    // this thread's query's lse (half 0) or D (half 1), a step ahead; a query past the sequence weighs nothing
+    auto stat = [&](int i, int hh) -> float {
+      const int qrow = i * 128 + r;
+      if (qrow >= un.len) return half == 0 ? -INFINITY : 0.f;
+      const float v = stats[(long long)hh * a.pc.M + un.begin + qrow];
+      return half == 0 ? -v * kLog2e : -v;
+    };
+    float next = stat(qi, h);
+    bool ok = true;
+    for (int it = 0; it < n; ++it) {
+      const int b = it & 1;
+      float *nl = sL + b * 128, *nd = sD + b * 128;
+      (half == 0 ? nl : nd)[r] = next;
+      mbar_arrive(&l_full[b]);
+      const bool diag = qi == kt;
+      const int lim = un.len - qi * 128;     // queries of this tile
+      if (++qi == tiles) { qi = kt; ++h; }
+      if (it + 1 < n) next = stat(qi, h);
+      if (!mbar_wait_warp(&l_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      if (!mbar_wait_warp(s_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      tc_fence_after();
+      const bool part = diag || lim < 128;   // some of its weights are chosen to be 0
+      if (lim < 128) {
+        // rows of dO and Q past the sequence, which weights of 0 would meet
+        if (r >= lim) {
+          mbar_wait(half == 0 ? &g_full[b] : &q_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
+          tile_row_clear<D>((half == 0 ? sG : sQ) + b * TILE, r);
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+      }
+      uint32_t pk[32];  // this thread's 64 columns of the P^T row, packed bf16 pairs (kept for dS)
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        uint32_t sv[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tS + lane_off + cb + h2 * 32, sv);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e0 = 0; e0 < 32; e0 += 4) {
+          const int e = h2 * 32 + e0, cc = cb + e;
+          const float4 n4 = *reinterpret_cast<const float4*>(nl + cc);
+          const float2 v0 = __ffma2_rn(make_float2(__uint_as_float(sv[e0]), __uint_as_float(sv[e0 + 1])), c2, make_float2(n4.x, n4.y));
+          const float2 v1 = __ffma2_rn(make_float2(__uint_as_float(sv[e0 + 2]), __uint_as_float(sv[e0 + 3])), c2, make_float2(n4.z, n4.w));
+          float2 p0, p1;
+          if (e >= 48) {
+            p0 = exp2_poly2(v0);
+            p1 = exp2_poly2(v1);
+          } else {
+            p0 = make_float2(ex2_approx(v0.x), ex2_approx(v0.y));
+            p1 = make_float2(ex2_approx(v1.x), ex2_approx(v1.y));
+          }
+          if (part) {
+            const int lo = diag ? r : 0;     // queries lo .. lim - 1 see this key
+            if (cc < lo || cc >= lim) p0.x = 0.f;
+            if (cc + 1 < lo || cc + 1 >= lim) p0.y = 0.f;
+            if (cc + 2 < lo || cc + 2 >= lim) p1.x = 0.f;
+            if (cc + 3 < lo || cc + 3 >= lim) p1.y = 0.f;
+          }
+          pk[e >> 1] = pack_bf16x2(p0.x, p0.y);
+          pk[(e >> 1) + 1] = pack_bf16x2(p1.x, p1.y);
+        }
+      }
+      __syncwarp();
+      tmem_st_32x32b_x32(tS + lane_off + cb, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_full);
+      if (!mbar_wait_warp(dp_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        uint32_t dp[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tP + lane_off + cb + h2 * 32, dp);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e0 = 0; e0 < 32; e0 += 4) {
+          const int e = h2 * 32 + e0, cc = cb + e;
+          const float4 d4 = *reinterpret_cast<const float4*>(nd + cc);
+          const float2 pa = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&pk[e >> 1]));
+          const float2 pb = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&pk[(e >> 1) + 1]));
+          float2 da = __fmul2_rn(pa, __fadd2_rn(make_float2(__uint_as_float(dp[e0]), __uint_as_float(dp[e0 + 1])), make_float2(d4.x, d4.y)));
+          float2 db = __fmul2_rn(pb, __fadd2_rn(make_float2(__uint_as_float(dp[e0 + 2]), __uint_as_float(dp[e0 + 3])), make_float2(d4.z, d4.w)));
+          if (part) {
+            const int lo = diag ? r : 0;
+            if (cc < lo || cc >= lim) da.x = 0.f;
+            if (cc + 1 < lo || cc + 1 >= lim) da.y = 0.f;
+            if (cc + 2 < lo || cc + 2 >= lim) db.x = 0.f;
+            if (cc + 3 < lo || cc + 3 >= lim) db.y = 0.f;
+          }
+          pk[e >> 1] = pack_bf16x2(da.x, da.y);   // dS^T over P^T
+          pk[(e >> 1) + 1] = pack_bf16x2(db.x, db.y);
+        }
+      }
+      __syncwarp();
+      tmem_st_32x32b_x32(tP + lane_off + cb, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(ds_full);
+    }
+    if (ok && mbar_wait_warp(done, 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
+      tc_fence_after();
+      const bool mine = row0 + r < un.len;
+      const long long at = ((long long)(un.begin + row0 + r) * a.Hkv + hk) * D + half * (D / 2);
+#pragma unroll 1
+      for (int cc = 0; cc < D / 64; ++cc) {
+        uint32_t o[32];
+        float f[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tDV + lane_off + half * (D / 2) + cc * 32, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]);
+        if (mine) store_row_bf16_global(a.dv + at + cc * 32, f, 32);
+        __syncwarp();
+        tmem_ld_32x32b_x32(tDK + lane_off + half * (D / 2) + cc * 32, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * a.scale;
+        if (mine) store_row_bf16_global(a.dk + at + cc * 32, f, 32);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------ host
+template <typename K>
+static void pk_smem(K kern, size_t bytes) {
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+struct PkView {
+  const __nv_bfloat16* p;
+  long long r, h;
+  CUtensorMap map;
+};
+
+static PkView pk_view(const at::Tensor& t, const char* name, const at::Tensor& q, int64_t H) {
+  TORCH_CHECK(t.is_cuda() && t.device() == q.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(0) == q.size(0) &&
+                  t.size(1) == H && t.size(2) == q.size(2), name, ": bfloat16 [M, H, D] of q's M and D on its device");
+  const int64_t M = t.size(0), D = t.size(2);
+  PkView v{};
+  v.p = reinterpret_cast<const __nv_bfloat16*>(t.data_ptr());
+  v.h = H > 1 ? t.stride(1) : D;
+  v.r = M > 1 ? t.stride(0) : H * D;
+  TORCH_CHECK(t.stride(2) == 1 && v.r > 0 && v.h > 0 && v.r % 8 == 0 && v.h % 8 == 0 && (reinterpret_cast<uintptr_t>(v.p) & 15) == 0, name,
+              ": unit inner stride, 16-byte aligned rows, no broadcast dimension");
+  if (M > 0) v.map = make_tmap_bf16(v.p, D, M, v.r, 64, 128, H, v.h);
+  return v;
+}
+
+struct PkCall {
+  PkArgs a;
+  PkView q, k, v;
+  int64_t M, D;
+};
+
+static PkCall pk_check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, double scale, const at::Tensor& err) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.scalar_type() == at::kBFloat16, "q: bfloat16 [M, Hq, D]");
+  TORCH_CHECK(k.dim() == 3 && v.dim() == 3, "k and v: bfloat16 [M, Hkv, D]");
+  PkCall c{};
+  const int64_t Hq = q.size(1), Hkv = k.size(1);
+  c.M = q.size(0); c.D = q.size(2);
+  TORCH_CHECK(c.D == 64 || c.D == 128, "head_dim 64 or 128");
+  TORCH_CHECK(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0, "the query heads: a multiple of the key/value heads");
+  TORCH_CHECK(c.M <= (1 << 30), "at most 2^30 rows");
+  TORCH_CHECK(cu.scalar_type() == at::kInt && cu.device() == q.device() && cu.dim() == 1 && cu.size(0) >= 1 && cu.size(0) <= (1 << 30) && cu.is_contiguous(),
+              "cu_seqlens: contiguous int32 [S + 1] on q's device");
+  TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale: a positive finite number");
+  c.q = pk_view(q, "q", q, Hq);
+  c.k = pk_view(k, "k", q, Hkv);
+  c.v = pk_view(v, "v", q, Hkv);
+  PkArgs& a = c.a;
+  a.pc.cu = cu.data_ptr<int>(); a.pc.S = (int)cu.size(0) - 1; a.pc.M = (int)c.M;
+  a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.G = (int)(Hq / Hkv);
+  a.scale = (float)scale; a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.q = c.q.p; a.qr = c.q.r; a.qh = c.q.h;
+  a.k = c.k.p; a.kr = c.k.r; a.kh = c.k.h;
+  a.v = c.v.p; a.vr = c.v.r; a.vh = c.v.h;
+  a.err = err.data_ptr<int>();
+  return c;
+}
+
+static unsigned pk_grid(long long slots, long long heads) {
+  TORCH_CHECK(slots * heads < (1LL << 31), "too many rows and heads");
+  return (unsigned)(slots * heads);
+}
+
+// {out [M, Hq, D], lse [Hq, M] (empty unless asked for)}
+std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu, double scale, bool want_lse,
+                                             at::Tensor err) {
+  PkCall c = pk_check(q, k, v, cu, scale, err);
+  c10::cuda::CUDAGuard guard(q.device());
+  PkArgs& a = c.a;
+  auto out = at::empty({c.M, a.Hq, c.D}, q.options());
+  auto lse = at::empty({want_lse ? a.Hq : 0, c.M}, q.options().dtype(at::kFloat));
+  if (c.M == 0) return {out, lse};
+  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  a.by_heads = a.G % 2 == 0;
+  const unsigned grid = pk_grid(piece_slots(c.M, a.pc.S, a.by_heads ? 128 : 256), a.by_heads ? a.Hq / 2 : a.Hq);
+  auto s = at::cuda::getCurrentCUDAStream();
+  if (c.D == 128) {
+    pk_smem(packed_fwd_kernel<128>, PkFwd<128>::SMEM);
+    packed_fwd_kernel<128><<<grid, 320, PkFwd<128>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, a);
+  } else {
+    pk_smem(packed_fwd_kernel<64>, PkFwd<64>::SMEM);
+    packed_fwd_kernel<64><<<grid, 320, PkFwd<64>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, a);
+  }
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {out, lse};
+}
+
+// {dq, dk, dv}, packed [M, H, D]; out and lse are the forward's.
+std::vector<at::Tensor> packed_attention_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor lse,
+                                             at::Tensor cu, double scale, at::Tensor err) {
+  PkCall c = pk_check(q, k, v, cu, scale, err);
+  PkArgs& a = c.a;
+  const PkView g = pk_view(dout, "the output's gradient", q, a.Hq);
+  TORCH_CHECK(out.device() == q.device() && out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes() && out.is_contiguous(), "out: the forward's");
+  TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.numel() == a.Hq * c.M && lse.is_contiguous(), "lse: the forward's");
+  c10::cuda::CUDAGuard guard(q.device());
+  auto dq = at::empty({c.M, a.Hq, c.D}, q.options()), dk = at::empty({c.M, a.Hkv, c.D}, q.options()), dv = at::empty({c.M, a.Hkv, c.D}, q.options());
+  if (c.M == 0) return {dq, dk, dv};
+  auto dvec = at::empty({a.Hq, c.M}, lse.options());
+  a.o = reinterpret_cast<const __nv_bfloat16*>(out.data_ptr());
+  a.dout = g.p; a.gr = g.r; a.gh = g.h;
+  a.dq = reinterpret_cast<__nv_bfloat16*>(dq.data_ptr());
+  a.dk = reinterpret_cast<__nv_bfloat16*>(dk.data_ptr());
+  a.dv = reinterpret_cast<__nv_bfloat16*>(dv.data_ptr());
+  a.lse = lse.data_ptr<float>(); a.dvec = dvec.data_ptr<float>();
+  const long long slots = piece_slots(c.M, a.pc.S, 128);
+  const unsigned gq = pk_grid(slots, a.Hq), gk = pk_grid(slots, a.Hkv);
+  auto s = at::cuda::getCurrentCUDAStream();
+  if (c.D == 128) {
+    pk_smem(packed_dq_kernel<128>, PkDq<128>::SMEM);
+    pk_smem(packed_dkv_kernel<128>, PkDkv<128>::SMEM);
+    packed_dq_kernel<128><<<gq, 320, PkDq<128>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    packed_dkv_kernel<128><<<gk, 320, PkDkv<128>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
+  } else {
+    pk_smem(packed_dq_kernel<64>, PkDq<64>::SMEM);
+    pk_smem(packed_dkv_kernel<64>, PkDkv<64>::SMEM);
+    packed_dq_kernel<64><<<gq, 320, PkDq<64>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    packed_dkv_kernel<64><<<gk, 320, PkDkv<64>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
+  }
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dq, dk, dv};
+}
+
+}  // namespace tfb

@@ -294,3 +294,67 @@ def verify_tree(tokens, parents, p, q, u):
         from .speculative import verify_tree as f
         return f(tokens, parents, p, q, u)
     return ref.verify_tree(tokens, parents, p, q, u)
+
+
+def packed_attention(q, k, v, cu_seqlens, scale: float | None = None):
+    """Causal attention of sequences that lie behind one another: q [M, Hq, D], k and v [M, Hkv, D]
+    with Hkv dividing Hq (query head h reads head ``h // (Hq // Hkv)``), sequence s in rows
+    ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` (int32 [S + 1] in device memory, ascending; a sequence may
+    be empty).  Returns [M, Hq, D]; rows outside all sequences are zero.  ``scale`` defaults to D^-0.5.
+
+    Differentiable in q, k and v; rows outside all sequences get zero gradients, and what they hold
+    reaches nothing.  An infinity or a NaN of a token reaches the outputs of the tokens that see it, and no
+    other; in the backward pass it may also reach gradients of tokens of its own sequence that lie in
+    the same 128 rows of it.  CUDA: bfloat16, head_dim 64 / 128; inputs are read in place (slices of
+    a projection's rows, say) where rows are 16-byte aligned, else copied."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if _cuda(q):
+        from .packed import packed_attention as f
+        return f(q, k, v, cu_seqlens, scale)
+    return ref.packed_attention(q, k, v, cu_seqlens, scale)
+
+
+def paged_cache_write(k, v, k_pages, v_pages, page_table, pos, cu_seqlens=None, k_scale=None, v_scale=None) -> None:
+    """Rows k, v [M, H, D] into pages [P, H, page, D] (``kv_cache_alloc(P, H, page, D, ...)``, page a
+    power of two from 16 on): the n-th new row of sequence b goes to row ``t % page`` of page
+    ``page_table[b, t // page]`` with ``t = pos[b] + n``.  ``cu_seqlens`` int32 [B + 1] cuts the rows into
+    sequences as in ``packed_attention``; None: one row a sequence.  ``page_table`` int32 [B, W] and ``pos``
+    int32 [B] in device memory.  Rows outside all sequences, rows that the table has no page for and those
+    whose table entry is no page are left out; every other row of the pages stays as it is.  Quantised
+    pages as in ``kv_cache_write``.  CUDA: k, v bfloat16 with 16-byte aligned rows, head_dim 64 / 128."""
+    if _cuda(k_pages):
+        from .packed import paged_cache_write as f
+        return f(k, v, k_pages, v_pages, page_table, pos, cu_seqlens, k_scale, v_scale)
+    return ref.paged_cache_write(k, v, k_pages, v_pages, page_table, pos, cu_seqlens, k_scale, v_scale)
+
+
+def paged_attention(q, k_pages, v_pages, page_table, lens, scale: float | None = None, k_scale=None, v_scale=None):
+    """Attention of one new token a sequence, q [B, Hq, D], over the first ``lens[b]`` rows (int32 [B] in device
+    memory) of its pages, its own row among them (``paged_cache_write``, ``page_table`` as there).  Query
+    head h reads head ``h // (Hq // H)``; returns [B, Hq, D].  ``scale`` defaults to D^-0.5.
+
+    Rows of table entries that are no page are not seen; a sequence that sees no row gets zeros.  An
+    infinity or a NaN in a seen row (in e4m3: a NaN code, or the scale NaN) reaches its sequence's output
+    and what other rows hold reaches nothing; where all scores are -inf the output is NaN.  Weights are
+    rounded as in ``tree_attention``.  No gradient."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if _cuda(k_pages):
+        from .packed import paged_attention as f
+        return f(q, k_pages, v_pages, page_table, lens, scale, k_scale, v_scale)
+    return ref.paged_attention(q, k_pages, v_pages, page_table, lens, scale, k_scale, v_scale)
+
+
+def token_logprobs(logits, tokens, top: int = 0):
+    """``(logprob [...], entropy [...], top_tokens [..., top], top_logprobs [..., top])`` of logits [..., V]
+    (float32 or bfloat16) and given tokens [...] (int64 or int32): log softmax at the token (0 where it is
+    outside the vocabulary: padding), entropy in nats, and the ``top`` <= 32 likeliest tokens (int32) with
+    their log probabilities, equal logits by the lowest token, NaN first.  float32.
+
+    A logit of -inf has probability 0; a row with a NaN, a +inf, or nothing but -inf gives NaN.
+    Differentiable in the logits through logprob and entropy."""
+    if _cuda(logits):
+        from .scoring import token_logprobs as f
+        return f(logits, tokens, top)
+    return ref.token_logprobs(logits, tokens, top)

@@ -8,6 +8,8 @@ reference's CPU numerics: ``norm`` = parameter-free ``F.rms_norm`` (train.py:143
 """
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -273,3 +275,109 @@ def verify_tree(tokens, parents, p, q, u):
     out[:, :-1] = torch.where(path[:, 1:] >= 0, tokens.gather(1, path[:, 1:].clamp_min(0)), -1)
     out[at, count - 1] = last
     return path.to(torch.int32), count.to(torch.int32), out.to(torch.int32)
+
+
+# ------------------------------------------------------------------------- packed prompts, paged cache, scores
+def _weighted(w, see, v):
+    """w @ v for w [H, N, T] and v [H, T, D]: an infinity or a NaN of v reaches the rows that see it, and no other."""
+    bad = ~torch.isfinite(v)
+    if not bool(bad.any()):
+        return w @ v
+    o = w @ torch.where(bad, 0.0, v)
+    s = see.to(w.dtype).expand(w.shape)
+    hit = [(s @ f.to(w.dtype)) > 0 for f in (v == float("inf"), v == float("-inf"), torch.isnan(v))]
+    o = o + torch.where(hit[0], float("inf"), 0.0) - torch.where(hit[1], float("inf"), 0.0)
+    return torch.where(hit[2], float("nan"), o)
+
+
+def packed_attention(q, k, v, cu_seqlens, scale: float):
+    from . import packed as pk
+    pk.check_packed(q, k, v, cu_seqlens)
+    if not math.isfinite(scale):
+        raise RuntimeError("scale: a finite number")
+    M, Hq, _ = q.shape
+    g = Hq // k.shape[1]
+    cu = [min(max(int(c), 0), M) for c in cu_seqlens.tolist()]
+    out, at = [], 0
+    for a, b in zip(cu[:-1], cu[1:]):
+        if b <= a:
+            continue
+        if a > at:
+            out.append(q.new_zeros(a - at, Hq, q.shape[2], dtype=torch.float32))
+        see = torch.ones(b - a, b - a, dtype=torch.bool, device=q.device).tril()
+        qs, ks, vs = q[a:b].float().transpose(0, 1), *(t[a:b].float().transpose(0, 1).repeat_interleave(g, 0) for t in (k, v))
+        w = torch.softmax((qs @ ks.transpose(1, 2) * scale).masked_fill(~see, float("-inf")), -1)
+        out.append(_weighted(w, see, vs).transpose(0, 1))
+        at = b
+    out.append(q.new_zeros(M - at, Hq, q.shape[2], dtype=torch.float32))
+    return torch.cat(out).to(q.dtype)
+
+
+def paged_cache_write(k, v, k_pages, v_pages, page_table, pos, cu_seqlens=None, k_scale=None, v_scale=None) -> None:
+    from . import packed as pk
+    pk.check_paged_write(k, v, k_pages, v_pages, page_table, pos, cu_seqlens, k_scale, v_scale)
+    P, _, page, _ = k_pages.shape
+    M, W = k.shape[0], page_table.shape[1]
+    n = torch.arange(M, device=k.device)
+    if cu_seqlens is None:
+        seq, t = n, pos.long()
+    else:
+        cu = cu_seqlens.long().clamp(0, M)
+        seq = torch.searchsorted(cu, n, right=True) - 1
+        live = (seq >= 0) & (seq < pos.shape[0])
+        n, seq = n[live], seq[live]
+        t = pos.long()[seq] + n - cu[seq]
+    live = (t >= 0) & (t < W * page)
+    n, seq, t = n[live], seq[live], t[live]
+    to = page_table.long()[seq, t // page]
+    live = (to >= 0) & (to < P)
+    n, to, t = n[live], to[live], t[live] % page
+    for x, pages, scale in ((k, k_pages, k_scale), (v, v_pages, v_scale)):
+        rows = x[n]
+        if scale is not None:
+            rows, codes = quantise_rows(rows)
+            _raw(scale)[to, :, t] = _raw(codes)
+        _raw(pages)[to, :, t] = _raw(rows.to(pages.dtype))
+
+
+def paged_attention(q, k_pages, v_pages, page_table, lens, scale: float, k_scale=None, v_scale=None):
+    from . import packed as pk
+    pk.check_paged_attention(q, k_pages, v_pages, page_table, lens, scale, k_scale, v_scale)
+    B, Hq, D = q.shape
+    P, H, page, _ = k_pages.shape
+    out = []
+    for b in range(B):
+        n = min(max(int(lens[b]), 0), page_table.shape[1] * page)
+        row = page_table[b, :-(-n // page)].long()
+        there = (row >= 0) & (row < P)
+        see = (there[:, None].expand(-1, page).reshape(-1) & (torch.arange(row.numel() * page, device=q.device) < n))
+        if not bool(see.any()):
+            out.append(q.new_zeros(Hq, D, dtype=torch.float32))
+            continue
+        kk, vv = (cache_values(_raw(c)[row[there]].view(c.dtype), None if s is None else _raw(s)[row[there]].view(s.dtype))
+                  .transpose(0, 1).reshape(H, -1, D)[:, see[there[:, None].expand(-1, page).reshape(-1)]]
+                  for c, s in ((k_pages, k_scale), (v_pages, v_scale)))
+        w = torch.softmax(q[b].float().view(H, Hq // H, D) @ kk.transpose(1, 2) * scale, -1)
+        out.append(_weighted(w, torch.ones((), dtype=torch.bool, device=q.device), vv).reshape(Hq, D))
+    return (torch.stack(out) if out else q.new_zeros(0, Hq, D)).to(q.dtype)
+
+
+def token_logprobs(logits, tokens, top: int = 0):
+    from . import scoring
+    shape, V = scoring.check_logprobs(logits, tokens, top)
+    z = logits.float()
+    m = z.detach().amax(-1, keepdim=True)
+    lp = z - m   # -inf - -inf and inf - inf are NaN: rows that sum to no number have no logarithms
+    lp = lp - torch.log(lp.exp().sum(-1, keepdim=True))
+    t = tokens.long()
+    there = (t >= 0) & (t < V)
+    own = torch.where(there, lp.gather(-1, t.clamp(0, V - 1)[..., None])[..., 0], 0.0)
+    p = lp.exp()
+    ent = -torch.where(p == 0, 0.0, p * lp.clamp_min(-1e4)).sum(-1)
+    with torch.no_grad():
+        # ordered by value, NaN first; stable: equal logits by the lowest token (-0 equals 0)
+        order = torch.where(torch.isnan(z), float("inf"), z)
+        at = torch.sort(torch.isnan(z).int(), dim=-1, descending=True, stable=True).indices
+        best = torch.sort(order.gather(-1, at), dim=-1, descending=True, stable=True).indices
+        tok = at.gather(-1, best)[..., :top]
+    return own, ent, tok.to(torch.int32), lp.detach().gather(-1, tok)
