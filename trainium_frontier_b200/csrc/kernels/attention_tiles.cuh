@@ -42,6 +42,18 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
   return d;
 }
 
+// max that keeps a NaN
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // 2^v on the FMA pipe for v <= 8 (0 below -126): v = n + f with n the nearest integer
 // (added and subtracted 1.5 * 2^23, whose low mantissa bits then hold n) and f in
 // [-1/2, 1/2]; 2^f from a degree-3 polynomial fitted here for relative error on that

@@ -55,18 +55,6 @@ struct PkArgs {
   int* err;
 };
 
-// max that keeps a NaN
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 // Row `row` of a tile of D columns (swizzled panels of 64): whether it holds an infinity or a NaN.
 template <int D>
 __device__ __forceinline__ bool tile_row_bad(const uint8_t* tile, int row) {
