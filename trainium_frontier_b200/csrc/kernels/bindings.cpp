@@ -97,7 +97,7 @@ std::vector<torch::Tensor> packed_attention_bwd(torch::Tensor dout, torch::Tenso
 void paged_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor kp, torch::Tensor vp, torch::Tensor table, torch::Tensor pos,
                        c10::optional<torch::Tensor> cu, c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs);
 torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor vp, torch::Tensor table, torch::Tensor lens, double scale,
-                              c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs);
+                              c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs, torch::Tensor err);
 std::vector<torch::Tensor> token_logprobs(torch::Tensor z, torch::Tensor tok, int64_t top, bool stats);
 torch::Tensor token_logprobs_grad(torch::Tensor z, torch::Tensor tok, torch::Tensor stat, c10::optional<torch::Tensor> g,
                                   c10::optional<torch::Tensor> h);

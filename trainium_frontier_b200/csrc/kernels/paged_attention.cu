@@ -3,7 +3,7 @@
 //   o = sum_t softmax_t(scale q . k_t) v_t,   t < lens[b], row t being row t % page of page table[b, t / page].
 //
 // The cache's bytes bound the time: 2 D products a byte at most with 8 query heads a key/value head.  So
-// nothing is staged: a warp takes 32 keys a step, reads their rows as 16-byte pieces straight into the
+// nothing is staged: a warp takes 16 keys a step, reads their rows as 16-byte pieces straight into the
 // registers of warp-level matrix instructions (16 keys or dimensions x 8 heads x 16), and the rows of its next
 // step are on their way while it computes.  The order of the dimensions is free in q . k, and that of the
 // output's rows in p v, so both operands' fragments are what a lane's own pieces hold:
@@ -15,9 +15,9 @@
 // sequence is cut evenly into as many pieces as the batch needs to fill the GPU, whatever its length, and
 // the pieces are joined in order by a second kernel that is launched under the first.
 //
-// Quantised rows: codes become f16 in registers.  A key's scale multiplies its score; a value's joins the
-// exponent of its weight, 2^(score + log2 scale - m') with a maximum m' of its own, so that weights fit f16
-// whatever the scales are.
+// Quantised rows: codes become f16 in registers.  A key's scale multiplies its score; a value's multiplies its
+// weight, which is taken relative to a maximum m' of score + log2 scale, so that weights fit f16 whatever the
+// scales are.
 #include <ATen/ops/empty.h>
 
 #include "attention_tiles.cuh"
@@ -44,6 +44,7 @@ struct PaArgs {
   float scale_log2;
   float* part;                   // [B, Hq, splits, D + 4]: output, then m, m', sum
   __nv_bfloat16* out;            // [B, Hq, D]
+  int* err;
 };
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -51,30 +52,48 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// A 16-byte piece of a cached row; rows are read once.
-__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
+__device__ __forceinline__ float min_nan(float a, float b) {   // min that keeps a NaN
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
   uint4 u;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at) : "memory");
   return u;
 }
-__device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
+__device__ __forceinline__ uint2 ld_shared8(uint32_t at) {
   uint2 u;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(p));
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(u.x), "=r"(u.y) : "r"(at) : "memory");
   return u;
 }
 
-// KT: tiles of 16 keys a step of a warp; NT: groups of 8 query heads.
-template <int D, bool QUANT, int KT, int NT>
-__global__ void __launch_bounds__(32 * kPaWarps, NT == 1 && (QUANT || D == 64) ? 3 : 2)
+template <int D, bool QUANT, int NT>
+struct PaCfg {
+  static constexpr int R = 8 * NT;                 // rows for query heads
+  static constexpr int KP = QUANT ? D / 64 : D / 32;      // pieces of a key row a lane
+  static constexpr int VP = QUANT ? 1 : D / 64;           // of a value row (e4m3 heads of 64: half a piece)
+  static constexpr int VB = QUANT && D == 64 ? 8 : 16;    // bytes of one
+  static constexpr int NS = QUANT || D == 64 ? 3 : 2;     // steps of a warp in flight and in use
+  static constexpr uint32_t ROW = D * (QUANT ? 1u : 2u);
+  static constexpr uint32_t STEP = 2 * 16 * ROW;          // 16 key rows, 16 value rows
+  static constexpr uint32_t RING = kPaWarps * NS * STEP;
+  static constexpr uint32_t OUT = kPaWarps * R * (D + 4) * 4u;
+  static constexpr uint32_t REST = (RING > OUT ? RING : OUT);
+  static constexpr uint32_t SMEM = REST + kPaWarps * R * 3 * 4u + kPaWarps * NS * 8u + 16;
+};
+
+template <int D, bool QUANT, int NT>
+__global__ void __launch_bounds__(32 * kPaWarps, NT == 2 ? 2 : D == 64 || QUANT ? 4 : 3)
     paged_attention_kernel(const PaArgs a, const __grid_constant__ KvView c) {
-  constexpr int KEYS = 16 * KT;
-  constexpr int KP = QUANT ? D / 64 : D / 32;      // pieces of a key row a lane
-  constexpr int VP = QUANT ? 1 : D / 64;           // of a value row (e4m3 heads of 64: half a piece)
+  using Cfg = PaCfg<D, QUANT, NT>;
+  constexpr int KP = Cfg::KP, VP = Cfg::VP, VB = Cfg::VB, R = Cfg::R, NS = Cfg::NS;
   constexpr int KS = D / 16, MT = D / 16;          // steps of 16 dimensions; tiles of them in the output
-  constexpr int R = 8 * NT;                        // rows for query heads
-  constexpr int TABLE = 32 / KT;                   // steps whose pages a warp holds, an entry a lane
-  __shared__ float sO[kPaWarps][R][D + 4];
-  __shared__ float sML[kPaWarps][R][3];
+  extern __shared__ __align__(128) uint8_t smem[];
+  float (*sO)[R][D + 4] = reinterpret_cast<float (*)[R][D + 4]>(smem);   // over the ring, once all is read
+  float (*sML)[R][3] = reinterpret_cast<float (*)[R][3]>(smem + Cfg::REST);
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + Cfg::REST + kPaWarps * R * 3 * 4);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(bars + kPaWarps * NS);
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, j = lane & 3;
   const int units = a.Hkv * a.rg;
@@ -83,10 +102,9 @@ __global__ void __launch_bounds__(32 * kPaWarps, NT == 1 && (QUANT || D == 64) ?
   const int h = hr / a.rg, g0 = (hr % a.rg) * R;   // key/value head, first query head of it
   const int rows = min(R, a.G - g0);
   const int len = (int)max(0LL, min((long long)a.lens[b], (long long)a.width << a.lg));
-  const long long steps = ((long long)len + KEYS - 1) / KEYS;
+  const long long steps = ((long long)len + 15) / 16;
   const int u0 = (int)(steps * split / a.splits), u1 = (int)(steps * (split + 1) / a.splits);
   const int* table = a.table + b * a.tb;
-
   // ------------------------------------------------------------------ queries: fragments of all dimensions
   uint32_t q[NT][2 * KS];
   float cr[NT][2];                                 // what a product is times, of heads 2j and 2j + 1
@@ -132,245 +150,290 @@ __global__ void __launch_bounds__(32 * kPaWarps, NT == 1 && (QUANT || D == 64) ?
   }
 
   // ------------------------------------------------------------------ loads of a step
-  uint4 kr[KT][2][KP], vr[KT][4][VP];
-  bool see[KT][2];                                 // keys gq and gq + 8 of a tile
-  uint32_t sc = 0;                                 // scale bytes of key and value row `lane`
-  int page[KT];                                    // of the step's tiles, -1: not there
-  // the pages of the warp's next TABLE steps from step u on, one a lane
+  // A warp has a ring of its own, filled by bulk copies: one for a tile whose rows are one behind another, else one a
+  // lane for a row.
+  uint64_t* const full = bars + warp * NS;
+  if (lane == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1);
+    if (warp == 0) *abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  uint8_t* const ring = smem + warp * (NS * Cfg::STEP);
+  constexpr uint32_t VAT = 16 * Cfg::ROW;          // values behind the keys
+  const bool dense = c.t == Cfg::ROW;
+  // lanes 0-15 copy key rows, the others value rows (dense: lanes 0 and 16 all of them)
+  const uint8_t* const r0 = (lane < 16 ? c.p[0] : c.p[1]) + h * c.h + (lane & 15) * c.t;
+  const uint8_t* const s0 = QUANT ? (lane < 16 ? c.s[0] : c.s[1]) + h * c.sh + (lane & 15) * c.st : nullptr;
+  const int inside = (1 << a.lg) - 1;
+  // the pages of the warp's next 32 steps from step u on, one a lane
   auto fetch = [&](int u) {
-    u += (lane / KT) * kPaWarps;
-    const long long key = (long long)u * KEYS + 16 * (lane % KT);
+    u += lane * kPaWarps;
     int pg = -1;
-    if (u < u1 && key < len) pg = table[key >> a.lg];
+    if (u < u1) pg = table[(u * 16) >> a.lg];
     return pg >= 0 && pg < a.pages ? pg : -1;
   };
-  auto load_k = [&](int u, int pages, int slot) {
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      page[t] = __shfl_sync(0xffffffffu, pages, slot * KT + t);
-      const int key = u * KEYS + 16 * t + gq, in = key & ((1 << a.lg) - 1);
-      const uint8_t* src = c.p[0] + page[t] * c.b + h * c.h + in * c.t + 16 * j;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        see[t][i] = page[t] >= 0 && key + 8 * i < len;
-#pragma unroll
-        for (int p = 0; p < KP; ++p) {
-          kr[t][i][p] = make_uint4(0, 0, 0, 0);
-          if (see[t][i]) kr[t][i][p] = ld_stream(src + 8 * i * c.t + 64 * p);
-        }
-      }
+  int ul = u0 + warp, slot = 0, stage = 0;         // next step to load, where its page and its rows are
+  int here = fetch(ul), next = fetch(ul + 32 * kPaWarps);
+  int pages[NS];                                   // of the steps in flight, oldest first (-1: not there)
+  uint32_t scale = 127u;                           // scale byte of key row `lane` or of value row lane - 16, of the oldest
+  // starts the loads of step ul, into the stage that all lanes have left; returns its page
+  auto load = [&]() -> int {
+    if (ul >= u1) return -1;
+    const int page = __shfl_sync(0xffffffffu, here, slot);
+    uint8_t* const to = ring + stage * Cfg::STEP + (lane < 16 ? 0 : VAT);
+    const uint8_t* const src = r0 + page * c.b + (ul * 16 & inside) * c.t;
+    if (page < 0) {
+      if (lane == 0) mbar_arrive(&full[stage]);
+    } else if (dense) {
+      if (lane == 0) mbar_arrive_expect_tx(&full[stage], Cfg::STEP);
+      __syncwarp();
+      if ((lane & 15) == 0) bulk_load(to, src, VAT, &full[stage]);
+    } else {
+      if (lane == 0) mbar_arrive_expect_tx(&full[stage], Cfg::STEP);
+      __syncwarp();
+      bulk_load(to + (lane & 15) * Cfg::ROW, src, Cfg::ROW, &full[stage]);
     }
-    if constexpr (QUANT) {
-      int pg = page[0];
-#pragma unroll
-      for (int t = 1; t < KT; ++t) pg = lane / 16 == t ? page[t] : pg;
-      const int key = u * KEYS + lane;
-      sc = 127u | (127u << 8);
-      if (lane < KEYS && pg >= 0 && key < len) {
-        const long long at = pg * c.sb + h * c.sh + (key & ((1 << a.lg) - 1)) * c.st;
-        sc = c.s[0][at] | ((uint32_t)c.s[1][at] << 8);
-      }
+    if (++stage == NS) stage = 0;
+    ul += kPaWarps;
+    if (++slot == 32) {
+      slot = 0;
+      here = next;
+      next = fetch(ul + 32 * kPaWarps);
     }
+    return page;
   };
-  auto load_v = [&](int u) {                       // rows that are not seen: zeros
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      const int key = u * KEYS + 16 * t + 2 * j, in = key & ((1 << a.lg) - 1);
-      const uint8_t* src = c.p[1] + page[t] * c.b + h * c.h + in * c.t + (QUANT && D == 64 ? 8 : 16) * gq;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {                // keys 2j, 2j + 1, 2j + 8, 2j + 9
-        const int off = (i >> 1) * 8 + (i & 1);
-#pragma unroll
-        for (int p = 0; p < VP; ++p) {
-          vr[t][i][p] = make_uint4(0, 0, 0, 0);
-          if (page[t] >= 0 && key + off < len) {
-            if constexpr (QUANT && D == 64) {
-              const uint2 w = ld_stream8(src + off * c.t);
-              vr[t][i][p].x = w.x; vr[t][i][p].y = w.y;
-            } else {
-              vr[t][i][p] = ld_stream(src + off * c.t + 128 * p);
-            }
-          }
-        }
-      }
-    }
+  // the scale byte of step u in page `page`
+  auto load_scale = [&](int u, int page) -> uint32_t {
+    const int key = u * 16, in = key & inside;
+    if (!QUANT || page < 0 || key + (lane & 15) >= len) return 127u;
+    return s0[page * c.sb + in * c.st];
   };
 
-  float o[NT][MT][4], m[NT][2], mw[NT][2], l[NT][2];   // mw: the weights' reference (QUANT; else m)
+  // References of the weights: m of the sum's, mw of those that the values are multiplied by (QUANT; else m).  They move
+  // when a score is above them by more than 8 (in log2), so weights are at most 2^8 and outputs rarely rescaled.
+  float o[NT][MT][4];
+  float2 m[NT], mw[NT], nref[NT], back[NT], l[NT];  // of heads 2j, 2j + 1; -m (0 for none), 2^(m - mw)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int e = 0; e < MT; ++e) o[nt][e][0] = o[nt][e][1] = o[nt][e][2] = o[nt][e][3] = 0.f;
-    m[nt][0] = m[nt][1] = mw[nt][0] = mw[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
+    m[nt] = mw[nt] = make_float2(-INFINITY, -INFINITY);
+    nref[nt] = l[nt] = make_float2(0.f, 0.f);
+    back[nt] = make_float2(1.f, 1.f);
   }
 
   // ------------------------------------------------------------------ the warp's steps
-  int u = u0 + warp, slot = 0;
-  int here = fetch(u), next = fetch(u + TABLE * kPaWarps);
-  if (u < u1) {
-    load_k(u, here, 0);
-    load_v(u);
-  }
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) pages[i] = load();
+  uint32_t at = smem_u32(ring), phase = 0;
+  int cur = 0;
+  scale = load_scale(u0 + warp, pages[0]);
 #pragma unroll 1
-  for (; u < u1; u += kPaWarps) {
-    float x[KT][NT][4];
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) x[t][nt][0] = x[t][nt][1] = x[t][nt][2] = x[t][nt][3] = 0.f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        uint32_t f[4];
-        if constexpr (QUANT) {
-          const uint4 r0 = kr[t][0][s >> 2], r1 = kr[t][1][s >> 2];
-          const uint32_t w0 = (s & 3) == 0 ? r0.x : (s & 3) == 1 ? r0.y : (s & 3) == 2 ? r0.z : r0.w;
-          const uint32_t w1 = (s & 3) == 0 ? r1.x : (s & 3) == 1 ? r1.y : (s & 3) == 2 ? r1.z : r1.w;
-          f[0] = codes2(w0); f[1] = codes2(w1); f[2] = codes2(w0 >> 16); f[3] = codes2(w1 >> 16);
-        } else {
-          const uint4 r0 = kr[t][0][s >> 1], r1 = kr[t][1][s >> 1];
-          f[0] = s & 1 ? r0.z : r0.x; f[1] = s & 1 ? r1.z : r1.x; f[2] = s & 1 ? r0.w : r0.y; f[3] = s & 1 ? r1.w : r1.y;
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<QUANT>(x[t][nt], f, q[nt][2 * s], q[nt][2 * s + 1]);
+  for (int u = u0 + warp; u < u1; u += kPaWarps) {
+    if (!mbar_wait_warp(&full[cur], phase, abort_flag, a.err, ERR_TIMEOUT_PRODUCER)) {
+      // give up, once what was started has come or had its time
+      const unsigned long long t0 = globaltimer_ns();
+      for (int v = u; v < ul; v += kPaWarps) {
+        while (!mbar_try_wait(&full[cur], phase))
+          if (globaltimer_ns() - t0 > 100000000ull) break;
+        if (++cur == NS) { cur = 0; phase ^= 1; }
       }
+      break;
     }
-    float lv[KT][2];                               // log2 of the values' scales
+    uint4 kr[2][KP];
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int p = 0; p < KP; ++p) kr[i][p] = ld_shared(at + (gq + 8 * i) * Cfg::ROW + 64 * p + 16 * j);
+    const uint32_t sc = scale;
+    const int left = pages[0] >= 0 ? len - u * 16 : 0;   // rows that are seen (16 or more: all)
+    const bool seen[2] = {gq < left, gq + 8 < left};
+    if (QUANT) scale = load_scale(u + kPaWarps, u + kPaWarps < u1 ? pages[1] : -1);
+    // into the stage of the step before
+    __syncwarp();
+    pages[NS - 1] = load();
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) pages[i] = pages[i + 1];
+    float x[NT][4], x1[NT][4];                     // of even and odd steps: two chains of products
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = x1[nt][0] = x1[nt][1] = x1[nt][2] = x1[nt][3] = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      uint32_t f[4];
+      if constexpr (QUANT) {
+        const uint4 r0 = kr[0][s >> 2], r1 = kr[1][s >> 2];
+        const uint32_t w0 = (s & 3) == 0 ? r0.x : (s & 3) == 1 ? r0.y : (s & 3) == 2 ? r0.z : r0.w;
+        const uint32_t w1 = (s & 3) == 0 ? r1.x : (s & 3) == 1 ? r1.y : (s & 3) == 2 ? r1.z : r1.w;
+        f[0] = codes2(w0); f[1] = codes2(w1); f[2] = codes2_high(w0); f[3] = codes2_high(w1);
+      } else {
+        const uint4 r0 = kr[0][s >> 1], r1 = kr[1][s >> 1];
+        f[0] = s & 1 ? r0.z : r0.x; f[1] = s & 1 ? r1.z : r1.x; f[2] = s & 1 ? r0.w : r0.y; f[3] = s & 1 ? r1.w : r1.y;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma16816<QUANT>(s & 1 ? x1[nt] : x[nt], f, q[nt][2 * s], q[nt][2 * s + 1]);
+    }
+    float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};   // scales of keys gq (0) and gq + 8, log2 of the values'
+    if constexpr (QUANT) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float ks = 1.f;
-        lv[t][i] = 0.f;
-        if constexpr (QUANT) {
-          const uint32_t s2 = __shfl_sync(0xffffffffu, sc, 16 * t + 8 * i + gq);
-          ks = scale_float((uint8_t)s2);
-          lv[t][i] = (s2 >> 8) == kScaleNan ? __int_as_float(0x7fffffff) : (float)((int)(s2 >> 8) - 127);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float& y = x[t][nt][2 * i + k];
-            y = see[t][i] ? y * cr[nt][k] * ks : -INFINITY;
-          }
+        ks[i] = scale_float((uint8_t)__shfl_sync(0xffffffffu, sc, 8 * i + gq));
+        const uint32_t e = __shfl_sync(0xffffffffu, sc, 16 + 8 * i + gq);
+        vs[i] = scale_float((uint8_t)e);
+        lv[i] = __uint_as_float(0x4b000000u | e) - 8388735.f;   // 2^23 + e less 2^23 + 127 (a NaN's is not used)
       }
-    // maxima of the heads 2j, 2j + 1; a visible score of -inf counts as the lowest number
-    bool grow = false;
-    float nm[NT][2], nw[NT][2];
+    }
+    float2 y[NT][2];                               // scores, heads 2j and 2j + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float v = -INFINITY, w = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float y = x[t][nt][2 * i + k];
-            v = fmaxf(v, see[t][i] ? fmaxf(y, kLowest) : -INFINITY);
-            if constexpr (QUANT) w = fmaxf(w, see[t][i] ? fmaxf(y + lv[t][i], kLowest) : -INFINITY);
-          }
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-          if constexpr (QUANT) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, d));
-        }
-        nm[nt][k] = fmaxf(m[nt][k], v);
-        nw[nt][k] = QUANT ? fmaxf(mw[nt][k], w) : nm[nt][k];
-        grow |= nm[nt][k] > m[nt][k] || (QUANT && nw[nt][k] > mw[nt][k]);
+      for (int i = 0; i < 2; ++i) {
+        const float2 f = QUANT ? __fmul2_rn(make_float2(cr[nt][0], cr[nt][1]), make_float2(ks[i], ks[i])) : make_float2(cr[nt][0], cr[nt][1]);
+        y[nt][i] = __fmul2_rn(__fadd2_rn(make_float2(x[nt][2 * i], x[nt][2 * i + 1]), make_float2(x1[nt][2 * i], x1[nt][2 * i + 1])), f);
+        if (!seen[i]) y[nt][i] = make_float2(-INFINITY, -INFINITY);
       }
+    // the lane's maxima; a visible score of -inf counts as the lowest number, so that something is seen
+    const float low = seen[0] || seen[1] ? kLowest : -INFINITY;
+    float2 v[NT], w[NT];
+    bool grow = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      v[nt] = make_float2(max3f(y[nt][0].x, y[nt][1].x, low), max3f(y[nt][0].y, y[nt][1].y, low));
+      grow |= v[nt].x > m[nt].x + 8.f || v[nt].y > m[nt].y + 8.f;
+      if constexpr (QUANT) {
+        const float2 w0 = __fadd2_rn(y[nt][0], make_float2(lv[0], lv[0])), w1 = __fadd2_rn(y[nt][1], make_float2(lv[1], lv[1]));
+        w[nt] = make_float2(max3f(w0.x, w1.x, low), max3f(w0.y, w1.y, low));
+        grow |= w[nt].x > mw[nt].x + 8.f || w[nt].y > mw[nt].y + 8.f;
+      }
+    }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        if constexpr (!QUANT) w[nt] = v[nt];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float al = m[nt][k] == nm[nt][k] ? 1.f : ex2_approx(m[nt][k] - nm[nt][k]);
-          const float aw = QUANT ? (mw[nt][k] == nw[nt][k] ? 1.f : ex2_approx(mw[nt][k] - nw[nt][k])) : al;
-          l[nt][k] *= al;
-#pragma unroll
-          for (int e = 0; e < MT; ++e) {
-            o[nt][e][k] *= aw;
-            o[nt][e][2 + k] *= aw;
+        for (int d = 4; d < 32; d <<= 1) {
+          v[nt].x = fmaxf(v[nt].x, __shfl_xor_sync(0xffffffffu, v[nt].x, d));
+          v[nt].y = fmaxf(v[nt].y, __shfl_xor_sync(0xffffffffu, v[nt].y, d));
+          if constexpr (QUANT) {
+            w[nt].x = fmaxf(w[nt].x, __shfl_xor_sync(0xffffffffu, w[nt].x, d));
+            w[nt].y = fmaxf(w[nt].y, __shfl_xor_sync(0xffffffffu, w[nt].y, d));
           }
-          m[nt][k] = nm[nt][k];
-          mw[nt][k] = nw[nt][k];
         }
-    }
-    uint32_t p[KT][NT][2];                         // weights: 16 keys x 8 heads a fragment
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float w[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float y = x[t][nt][2 * i + k];
-            const float e = ex2_approx(y - (m[nt][k] == -INFINITY ? 0.f : m[nt][k]));
-            l[nt][k] += e;
-            w[k] = QUANT ? ex2_approx(y + lv[t][i] - (mw[nt][k] == -INFINITY ? 0.f : mw[nt][k])) : e;
-          }
-          p[t][nt][i] = transpose8x8(QUANT ? pack_f16x2(w[0], w[1]) : pack_bf16x2(w[0], w[1]));
-        }
-    // the next step's keys, before this one's values are used
-    const int un = u + kPaWarps;
-    if (un < u1) {
-      if (++slot == TABLE) {
-        slot = 0;
-        here = next;
-        next = fetch(un + TABLE * kPaWarps);
-      }
-      load_k(un, here, slot);
-    }
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-#pragma unroll
-      for (int e = 0; e < MT; ++e) {
-        uint32_t f[4];
+        if constexpr (!QUANT) w[nt] = v[nt];
+        auto step = [](float& ref, float to, float& factor) {   // ref moves up to `to`: what it scales, times factor
+          factor = to > ref ? ex2_approx(ref - to) : 1.f;
+          ref = fmaxf(ref, to);
+        };
+        float2 al, aw;
+        step(m[nt].x, v[nt].x, al.x);
+        step(m[nt].y, v[nt].y, al.y);
         if constexpr (QUANT) {
-          // rows: code e of the lane's first 8 (4) codes, and of its last ones; two codes of two keys a word
-          constexpr int HALF = D / 16;             // codes of a half
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {            // f[0], f[1]: keys 2j, 2j + 1; f[2], f[3]: 2j + 8, 2j + 9
-            const int code = e + (i & 1) * HALF, w = code >> 2;
-            const uint4 ra = vr[t][i & 2][0], rb = vr[t][(i & 2) + 1][0];
-            const uint32_t x0 = w == 0 ? ra.x : w == 1 ? ra.y : w == 2 ? ra.z : ra.w;
-            const uint32_t x1 = w == 0 ? rb.x : w == 1 ? rb.y : w == 2 ? rb.z : rb.w;
-            const uint32_t pair = __byte_perm(x0, x1, code & 2 ? 0x7362 : 0x5140);
-            f[i] = codes2(code & 1 ? pair >> 16 : pair);
-          }
+          step(mw[nt].x, w[nt].x, aw.x);
+          step(mw[nt].y, w[nt].y, aw.y);
         } else {
-          // rows: entry e of the lane's first piece and of its second (heads of 64: e and e + 4 of its only one)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int entry = VP == 2 ? e : e + 4 * (i & 1), pc = VP == 2 ? (i & 1) : 0, w = entry >> 1;
-            const uint4 ra = vr[t][i & 2][pc], rb = vr[t][(i & 2) + 1][pc];
-            const uint32_t x0 = w == 0 ? ra.x : w == 1 ? ra.y : w == 2 ? ra.z : ra.w;
-            const uint32_t x1 = w == 0 ? rb.x : w == 1 ? rb.y : w == 2 ? rb.z : rb.w;
-            f[i] = __byte_perm(x0, x1, entry & 1 ? 0x7632 : 0x5410);
-          }
+          mw[nt] = m[nt];
+          aw = al;
         }
+        l[nt] = __fmul2_rn(l[nt], al);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<QUANT>(o[nt][e], f, p[t][nt][0], p[t][nt][1]);
+        for (int e = 0; e < MT; ++e) {
+          o[nt][e][0] *= aw.x; o[nt][e][1] *= aw.y;
+          o[nt][e][2] *= aw.x; o[nt][e][3] *= aw.y;
+        }
+        nref[nt] = make_float2(m[nt].x == -INFINITY ? 0.f : -m[nt].x, m[nt].y == -INFINITY ? 0.f : -m[nt].y);
+        if constexpr (QUANT)
+          back[nt] = make_float2(m[nt].x == -INFINITY ? 1.f : ex2_approx(m[nt].x - mw[nt].x), m[nt].y == -INFINITY ? 1.f : ex2_approx(m[nt].y - mw[nt].y));
       }
     }
-    if (un < u1) load_v(un);
+    uint32_t p[NT][2];                             // weights: 16 keys x 8 heads a fragment
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float2 e = __fadd2_rn(y[nt][i], nref[nt]);
+        e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+        l[nt] = __fadd2_rn(l[nt], e);
+        if constexpr (QUANT) {
+          // 2^(score - mw) times the value's scale.  The factor is 2^126 at most, so that 0 times it is 0 (a weight of 0 with a
+          // factor beyond that counts less than 2^-100 of the others unless scales are that far apart); a NaN stays.
+          const float2 f = __fmul2_rn(back[nt], make_float2(vs[i], vs[i]));
+          e = __fmul2_rn(e, make_float2(min_nan(f.x, 0x1p126f), min_nan(f.y, 0x1p126f)));
+        }
+        p[nt][i] = transpose8x8(QUANT ? pack_f16x2(e.x, e.y) : pack_bf16x2(e.x, e.y));
+      }
+    uint4 vr[4][VP];                               // keys 2j, 2j + 1, 2j + 8, 2j + 9; rows that are not seen: zeros
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = 2 * j + (i >> 1) * 8 + (i & 1);
+#pragma unroll
+      for (int p = 0; p < VP; ++p) {
+        const uint32_t from = at + VAT + key * Cfg::ROW + VB * gq + 128 * p;
+        if constexpr (VB == 8) {
+          const uint2 w2 = ld_shared8(from);
+          vr[i][p] = make_uint4(w2.x, w2.y, 0, 0);
+        } else {
+          vr[i][p] = ld_shared(from);
+        }
+      }
+    }
+    if (left < 16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (2 * j + (i >> 1) * 8 + (i & 1) >= left)
+#pragma unroll
+          for (int p = 0; p < VP; ++p) vr[i][p] = make_uint4(0, 0, 0, 0);
+    }
+    at += Cfg::STEP;
+    if (++cur == NS) {
+      cur = 0;
+      at = smem_u32(ring);
+      phase ^= 1;
+    }
+#pragma unroll
+    for (int e = 0; e < MT; ++e) {
+      uint32_t f[4];
+      if constexpr (QUANT) {
+        // rows: code e of the lane's first 8 (4) codes, and of its last ones; two codes of two keys a word
+        constexpr int HALF = D / 16;               // codes of a half
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {              // f[0], f[1]: keys 2j, 2j + 1; f[2], f[3]: 2j + 8, 2j + 9
+          const int code = e + (i & 1) * HALF, wd = code >> 2;
+          const uint4 ra = vr[i & 2][0], rb = vr[(i & 2) + 1][0];
+          const uint32_t x0 = wd == 0 ? ra.x : wd == 1 ? ra.y : wd == 2 ? ra.z : ra.w;
+          const uint32_t x1 = wd == 0 ? rb.x : wd == 1 ? rb.y : wd == 2 ? rb.z : rb.w;
+          const uint32_t pair = __byte_perm(x0, x1, code & 2 ? 0x7362 : 0x5140);
+          f[i] = code & 1 ? codes2_high(pair) : codes2(pair);
+        }
+      } else {
+        // rows: entry e of the lane's first piece and of its second (heads of 64: e and e + 4 of its only one)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int entry = VP == 2 ? e : e + 4 * (i & 1), pc = VP == 2 ? (i & 1) : 0, wd = entry >> 1;
+          const uint4 ra = vr[i & 2][pc], rb = vr[(i & 2) + 1][pc];
+          const uint32_t x0 = wd == 0 ? ra.x : wd == 1 ? ra.y : wd == 2 ? ra.z : ra.w;
+          const uint32_t x1 = wd == 0 ? rb.x : wd == 1 ? rb.y : wd == 2 ? rb.z : rb.w;
+          f[i] = __byte_perm(x0, x1, entry & 1 ? 0x7632 : 0x5410);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma16816<QUANT>(o[nt][e], f, p[nt][0], p[nt][1]);
+    }
   }
+
+  __syncthreads();                                 // no warp is in its ring any more
 
   // ------------------------------------------------------------------ the four warps' outputs
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      float s = l[nt][k];
+      float s = k ? l[nt].y : l[nt].x;
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
       const int r = nt * 8 + 2 * j + k;
       if (gq == 0) {
-        sML[warp][r][0] = m[nt][k];
-        sML[warp][r][1] = QUANT ? mw[nt][k] : m[nt][k];
+        sML[warp][r][0] = k ? m[nt].y : m[nt].x;
+        sML[warp][r][1] = k ? mw[nt].y : mw[nt].x;
         sML[warp][r][2] = s;
       }
 #pragma unroll
@@ -405,44 +468,77 @@ __global__ void __launch_bounds__(32 * kPaWarps, NT == 1 && (QUANT || D == 64) ?
     } else {
       float* dst = a.part + (at * a.splits + split) * (D + 4);
       dst[d] = O;
-      if (d == 0) { dst[D] = M; dst[D + 1] = W; dst[D + 2] = L; }
+      if (d == 0) *reinterpret_cast<float4*>(dst + D) = make_float4(M, W, L, 0.f);
     }
   }
 }
 
-// The pieces of a (sequence, head) joined in order, a dimension a thread.
+// The pieces of a (sequence, head) joined: eight warps take every eighth piece, in order, and their sums are added in order.
+constexpr int kJoinWarps = 8;
 template <int D, bool QUANT>
-__global__ void __launch_bounds__(D) paged_join_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ out, int splits) {
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ out, int splits) {
+  constexpr int E = D / 32;
+  __shared__ float sO[kJoinWarps][D], sL[kJoinWarps];
   griddep_wait();
   const float* src = part + (long long)blockIdx.x * splits * (D + 4);
-  const int d = threadIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float M = -INFINITY, W = -INFINITY;
-  for (int i = 0; i < splits; ++i) {
-    M = fmaxf(M, src[i * (D + 4) + D]);
-    W = fmaxf(W, src[i * (D + 4) + D + 1]);
+  for (int i = lane; i < splits; i += 32) {
+    M = fmaxf(M, src[(long long)i * (D + 4) + D]);
+    W = fmaxf(W, src[(long long)i * (D + 4) + D + 1]);
   }
-  float L = 0.f, O = 0.f;
-  for (int i = 0; i < splits; ++i) {
-    const float* s = src + i * (D + 4);
-    if (s[D] == -INFINITY) continue;
-    L += ex2_approx(s[D] - M) * s[D + 2];
-    O += ex2_approx(s[D + 1] - W) * s[d];
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    W = fmaxf(W, __shfl_xor_sync(0xffffffffu, W, d));
   }
-  const float y = M == -INFINITY ? 0.f : O / L * (QUANT ? ex2_approx(W - M) : 1.f);
-  out[(long long)blockIdx.x * D + d] = __float2bfloat16_rn(y);
+  float L = 0.f, O[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) O[e] = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < splits; i += kJoinWarps) {
+    const float* s = src + (long long)i * (D + 4);
+    const float4 ml = *reinterpret_cast<const float4*>(s + D);
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = s[e * 32 + lane];
+    const bool any = ml.x != -INFINITY;            // a piece that saw nothing
+    L += any ? ex2_approx(ml.x - M) * ml.z : 0.f;
+    const float f = any ? ex2_approx(ml.y - W) : 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) O[e] += any ? f * o[e] : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sO[warp][e * 32 + lane] = O[e];
+  if (lane == 0) sL[warp] = L;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  L = 0.f;
+  float y = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    L += sL[w];
+    y += sO[w][threadIdx.x];
+  }
+  y = M == -INFINITY ? 0.f : y / L * (QUANT ? ex2_approx(W - M) : 1.f);
+  out[(long long)blockIdx.x * D + threadIdx.x] = __float2bfloat16_rn(y);
 }
 
 template <int D, bool QUANT>
 static void pa_launch(PaArgs& a, const KvView& c, int64_t B, cudaStream_t s) {
   const unsigned grid = (unsigned)(B * a.splits * a.Hkv * a.rg);
-  if (a.G <= 8) paged_attention_kernel<D, QUANT, 2, 1><<<grid, 32 * kPaWarps, 0, s>>>(a, c);
-  else paged_attention_kernel<D, QUANT, 1, 2><<<grid, 32 * kPaWarps, 0, s>>>(a, c);
+  auto launch = [&](auto kern, uint32_t smem) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kern<<<grid, 32 * kPaWarps, smem, s>>>(a, c);
+  };
+  if (a.G <= 8) launch(paged_attention_kernel<D, QUANT, 1>, PaCfg<D, QUANT, 1>::SMEM);
+  else launch(paged_attention_kernel<D, QUANT, 2>, PaCfg<D, QUANT, 2>::SMEM);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (a.splits == 1) return;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3((unsigned)(B * a.Hq));
-  cfg.blockDim = dim3(D);
+  cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = s;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -452,7 +548,7 @@ static void pa_launch(PaArgs& a, const KvView& c, int64_t B, cudaStream_t s) {
 }
 
 at::Tensor paged_attention(at::Tensor q, at::Tensor kp, at::Tensor vp, at::Tensor table, at::Tensor lens, double scale,
-                           c10::optional<at::Tensor> ks, c10::optional<at::Tensor> vs) {
+                           c10::optional<at::Tensor> ks, c10::optional<at::Tensor> vs, at::Tensor err) {
   TORCH_CHECK(kp.is_cuda(), "pages: CUDA tensors");
   bool quant;
   const KvView c = kv_view(kp, vp, ks, vs, quant);
@@ -480,10 +576,14 @@ at::Tensor paged_attention(at::Tensor q, at::Tensor kp, at::Tensor vp, at::Tenso
   a.rg = a.G <= 8 ? 1 : (a.G + 15) / 16;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
-  // pieces: as many as give every SM some eight CTAs, of 128 keys at the least
-  const int64_t base = B * Hkv * a.rg, room = ((int64_t)a.width << a.lg) / 128;
-  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(8LL * num_sms(kp.get_device()) + base - 1) / base, room, 256}));
-  TORCH_CHECK(base * a.splits < (1LL << 31), "too many sequences and heads");
+  a.err = err.data_ptr<int>();
+  // Pieces.  One sequence: as many as fill the GPU once, since they are alike, of 128 rows at the least.  More
+  // sequences, whose lengths the host does not know: six times as many as fit, so that long ones do not stand out, of
+  // 512 rows at the least.
+  const int64_t base = Hkv * a.rg, slots = (int64_t)num_sms(kp.get_device()) * (quant ? 3 : 2), rows = (int64_t)a.width << a.lg;
+  const int64_t want = B == 1 ? std::min(slots / base, rows / 128) : std::min((6 * slots + B * base - 1) / (B * base), rows / 512);
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, 256));
+  TORCH_CHECK(B * base * a.splits < (1LL << 31), "too many sequences and heads");
   at::Tensor part;
   if (a.splits > 1) {
     part = at::empty({B * Hq * a.splits * (D + 4)}, q.options().dtype(at::kFloat));

@@ -94,7 +94,7 @@ __device__ __forceinline__ void lp_rebase(float m, float M, float& S, float& T) 
 template <bool BF, bool VEC>
 struct LpStep {
   static constexpr int EPL = VEC ? (BF ? 8 : 4) : 1;           // elements of a load
-  static constexpr int LOADS = VEC ? kLpLoads : 4 * kLpLoads;
+  static constexpr int LOADS = VEC ? (BF ? kLpLoads / 2 : kLpLoads) : 4 * kLpLoads;   // 16 elements a lane
   static constexpr int EL = EPL * LOADS;                       // elements of a lane
   static constexpr int SIZE = 32 * EL;                         // of a step
   static constexpr int WORDS = VEC ? 4 * LOADS : LOADS;
@@ -241,7 +241,7 @@ __device__ __forceinline__ u64 best_of_share(const char* z, int V, int top, int 
 }
 
 template <bool BF, bool VEC>
-__global__ void __launch_bounds__(32 * kLpWarps, BF && VEC ? 3 : 4) token_logprobs_kernel(const LpArgs a) {
+__global__ void __launch_bounds__(32 * kLpWarps, 4) token_logprobs_kernel(const LpArgs a) {
   typedef LpStep<BF, VEC> Step;
   __shared__ LpShare sShare[kLpWarps];
   __shared__ float sStat[kLpWarps][3];
@@ -512,7 +512,7 @@ std::vector<at::Tensor> token_logprobs(at::Tensor z, at::Tensor tok, int64_t top
   a.V = (int)s.V; a.top = (int)top; a.N = s.N;
   // warps a row: one where the rows alone give every SM's 24 warps several rows each, else more while each has 16
   // steps of it, or, to have a warp for every scheduler four times over, two
-  const int64_t step = 32 * (s.vec ? kLpLoads * (s.bf ? 8 : 4) : 4 * kLpLoads), sms = num_sms(z.get_device());
+  const int64_t step = 512, sms = num_sms(z.get_device());
   int W = 1, C = 1;
   while (W < kLpWarps && ((s.N * W < 192 * sms && 32 * W * step <= s.V) || (s.N * W < 16 * sms && 2 * W * step < s.V))) W *= 2;
   while (W == kLpWarps && C < 8 && s.N * W * C < 16 * sms && 2 * W * C * step < s.V) C *= 2;

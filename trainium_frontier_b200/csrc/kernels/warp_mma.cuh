@@ -24,6 +24,12 @@ __device__ __forceinline__ uint32_t codes2(uint32_t x) {
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(y) : "r"(x));
   return y;
 }
+// The two codes of the upper half.
+__device__ __forceinline__ uint32_t codes2_high(uint32_t x) {
+  uint32_t y;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ float e4m3_float(uint8_t x) {
   return __half2float(__ushort_as_half((unsigned short)codes2(x)));
 }

@@ -65,7 +65,7 @@ def paged_cache_write(k, v, k_pages, v_pages, page_table, pos, cu_seqlens, k_sca
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lens, scale, k_scale, v_scale):
-    return C().paged_attention(q, k_pages, v_pages, page_table, lens, scale, k_scale, v_scale)
+    return C().paged_attention(q, k_pages, v_pages, page_table, lens, scale, k_scale, v_scale, err_word(q.device))
 
 
 # ------------------------------------------------------------------------------- checks of the CPU oracle
