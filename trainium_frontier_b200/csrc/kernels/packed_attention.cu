@@ -55,6 +55,28 @@ struct PkArgs {
   int* err;
 };
 
+// Operand descriptors of a tile, whose address is `d`'s first field (in 16 bytes), at k-step kk: as desc_kmajor and
+// desc_mnmajor, but a base that is computed once and constants.  (Computed anew for each product, the
+// descriptors took the issuing thread 97 cycles a product; the product takes 64.)
+__device__ __forceinline__ uint64_t kmajor_base(const void* tile) { return umma_desc_sw128(smem_u32(tile), 16, 1024); }
+__device__ __forceinline__ uint64_t mnmajor_base(const void* tile) { return umma_desc_sw128(smem_u32(tile), kPanel, 1024); }
+__device__ __forceinline__ uint64_t kmajor_at(uint64_t d, int kk) { return d + (((uint32_t)(kk >> 2) * kPanel + (uint32_t)(kk & 3) * 32u) >> 4); }
+__device__ __forceinline__ uint64_t mnmajor_at(uint64_t d, int kk) { return d + ((uint32_t)kk * 2048u >> 4); }
+
+// D += A B over a tile, A and B by descriptors: 16 dimensions a step
+template <int STEPS>
+__device__ __forceinline__ void mma_kk(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < STEPS; ++kk) umma_bf16(d, kmajor_at(a, kk), kmajor_at(b, kk), idesc, kk > 0 ? 1u : 0u);
+}
+// D (+)= A B, A the weights of 128 columns in TMEM: 16 of them a step, the upper 64 `gap` columns behind the lower
+template <int GAP>
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    umma_bf16_tmem_a(d, a + (kk >> 2) * GAP + (kk & 3) * 8, mnmajor_at(b, kk), idesc, kk > 0 ? 1u : add ? 1u : 0u);
+}
+
 // Row `row` of a tile of D columns (swizzled panels of 64): whether it holds an infinity or a NaN.
 template <int D>
 __device__ __forceinline__ bool tile_row_bad(const uint8_t* tile, int row) {
@@ -177,7 +199,8 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;           // all 512 columns are this CTA's: they start at 0
+  if (threadIdx.x == 0 && *tmem_slot != tmem) atomicOr(a.err, ERR_BAD_ARG);
   const PieceUnit un = *s_unit;
   const int U = a.by_heads ? 128 : 256;
   const bool live = un.unit >= 0 && a.pc.real(un.piece);
@@ -230,63 +253,77 @@ __global__ void __launch_bounds__(320, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      bool ok = mbar_wait(bar_q, 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
-      const uint32_t q_addr[2] = {smem_u32(sQ), smem_u32(sQ + TILE)};
-      auto kv_wait = [&](int item) -> bool {
-        return mbar_wait(&kv_full[item % NS], (item / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA);
-      };
-      auto issue_s = [&](int t, int j) -> bool {
-        if (!kv_wait(2 * j)) return false;
-        tc_fence_after();
-        const uint32_t k_addr = smem_u32(sKV + ((2 * j) % NS) * TILE);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tmem + t * 128, desc_kmajor(q_addr[t], kk), desc_kmajor(k_addr, kk), IDESC_S, kk > 0 ? 1u : 0u);
+    // The warp runs as one, so that operands stay in uniform registers; one lane issues.
+    bool ok = mbar_wait_warp(bar_q, 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
+    const bool leader = elect_one();
+    const uint64_t qd[2] = {kmajor_base(sQ), kmajor_base(sQ + TILE)};
+    const uint64_t kd = kmajor_base(sKV), vd = mnmajor_base(sKV);
+    constexpr uint64_t STEP = TILE >> 4;
+    // slots and parities of the K / V tiles: S takes K_j, the products after it V_j
+    int ks = 0, vs = 1;
+    uint32_t kp = 0, vp = 0;
+    auto issue_s = [&](int t) {
+      tc_fence_after();
+      if (leader) {
+        mma_kk<D / 16>(tmem + t * 128, qd[t], kd + ks * STEP, IDESC_S);
         umma_commit(&s_full[t]);
-        return true;
-      };
-      auto issue_pv = [&](int t, int j) -> bool {
-        if (!kv_wait(2 * j + 1)) return false;
-        if (!mbar_wait(&p_full[t], j & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
-        tc_fence_after();
-        const uint32_t v_addr = smem_u32(sKV + ((2 * j + 1) % NS) * TILE);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)  // P_t(j): 16 keys = 8 packed columns per MMA
-          umma_bf16_tmem_a(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, desc_mnmajor(v_addr, kk), IDESC_O,
-                           (j > 0 || kk > 0) ? 1u : 0u);
-        return true;
-      };
-      if (ok) ok = issue_s(0, 0) && (n1 == 0 || issue_s(1, 0));
-      if (ok) umma_commit(&kv_empty[0]);  // K_0 read by both tiles
-      for (int j = 0; j < nk && ok; ++j) {
-        // one thread's tcgen05 MMAs run in issue order: S_t(j + 1) may overwrite P_t(j)
-        if (j < n0) {
-          if (!issue_pv(0, j)) { ok = false; break; }
-          if (j + 1 < n0) {
-            if (!issue_s(0, j + 1)) { ok = false; break; }
-          } else {
-            umma_commit(&o_done[0]);
-          }
-        }
-        if (j < n1) {
-          if (!issue_pv(1, j)) { ok = false; break; }
-          if (j + 1 < n1) {
-            if (!issue_s(1, j + 1)) { ok = false; break; }
-          } else {
-            umma_commit(&o_done[1]);
-          }
-        }
-        if (j + 1 < nk) umma_commit(&kv_empty[(2 * (j + 1)) % NS]);  // K_{j+1} read by both tiles
-        umma_commit(&kv_empty[(2 * j + 1) % NS]);                    // V_j done
       }
-      if (!ok) {
-        *abort_flag = 1;
-        umma_commit(drain);
-        const unsigned long long t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain, 0))
-          if (globaltimer_ns() - t0 > 100000000ull) break;
+      __syncwarp();
+    };
+    auto issue_pv = [&](int t, int j) -> bool {
+      if (!mbar_wait_warp(&p_full[t], j & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+      tc_fence_after();
+      if (leader) mma_tmem<32>(tmem + 256 + t * 128, tmem + t * 128, vd + vs * STEP, IDESC_O, j > 0);
+      __syncwarp();
+      return true;
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (leader) umma_commit(bar);
+      __syncwarp();
+    };
+    if (ok) ok = mbar_wait_warp(&kv_full[0], 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
+    if (ok) {
+      issue_s(0);
+      if (n1) issue_s(1);
+      commit(&kv_empty[0]);              // K_0 read by both tiles
+    }
+    for (int j = 0; j < nk && ok; ++j) {
+      // one thread's tcgen05 MMAs run in issue order: S_t(j + 1) may overwrite P_t(j)
+      const bool more = j + 1 < nk;
+      if (more) {
+        ks += 2;
+        if (ks >= NS) { ks -= NS; kp ^= 1; }
       }
+      if (!mbar_wait_warp(&kv_full[vs], vp, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
+      if (j < n0) {
+        if (!issue_pv(0, j)) { ok = false; break; }
+        if (j + 1 < n0) {
+          if (!mbar_wait_warp(&kv_full[ks], kp, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
+          issue_s(0);
+        } else {
+          commit(&o_done[0]);
+        }
+      }
+      if (j < n1) {
+        if (!issue_pv(1, j)) { ok = false; break; }
+        if (j + 1 < n1) {
+          if (!mbar_wait_warp(&kv_full[ks], kp, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
+          issue_s(1);
+        } else {
+          commit(&o_done[1]);
+        }
+      }
+      if (more) commit(&kv_empty[ks]);   // K_{j+1} read by both tiles
+      commit(&kv_empty[vs]);             // V_j done
+      vs += 2;
+      if (vs >= NS) { vs -= NS; vp ^= 1; }
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      commit(drain);
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain, 0))
+        if (globaltimer_ns() - t0 > 100000000ull) break;
     }
   } else {
     // ------------------------------------------------------------------ softmax (tile t)
@@ -408,14 +445,14 @@ __global__ void __launch_bounds__(320, 1)
 
 // ================================================================================ backward: dQ
 // One CTA per 128 queries of a head, over the keys.  TMEM: S | dP | dQ | two dS (bf16).
-//   warp 0      TMA: Q and dO, then K_0, V_0, K_1, .. through a ring
+//   warp 0      TMA: Q and dO, then K_0, V_0, K_1, .. through a ring each
 //   warp 1      MMA: per step S(next) = Q K^T, dP(next) = dO V^T, dQ += dS K with dS from TMEM
 //   warps 2-9   p = 2^(S c - lse), dS = p (dP - D): two warps a lane quarter, 64 columns each
 // S and dP are given back as soon as they are in registers, so the next ones are formed meanwhile.
 template <int D>
 struct PkDq {
   static constexpr uint32_t TILE = 128u * D * 2u;
-  static constexpr int NS = D == 128 ? 5 : 8;
+  static constexpr int NK = D == 128 ? 3 : 5, NV = D == 128 ? 2 : 4, NS = NK + NV;   // rings of K (held until dQ has read it) and V
   static constexpr size_t SMEM = 1024 + (2 + NS) * TILE + 1024 + 32 * 8 + 64;
 };
 
@@ -424,7 +461,7 @@ __global__ void __launch_bounds__(320, 1)
     packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const PkArgs a) {
   constexpr uint32_t TILE = PkDq<D>::TILE;
-  constexpr int NS = PkDq<D>::NS, PANELS = D / 64;
+  constexpr int NK = PkDq<D>::NK, NS = PkDq<D>::NS, PANELS = D / 64;
   constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, false, false);
   constexpr uint32_t IDESC_Q = umma_idesc_bf16(128, D, false, true);
 
@@ -436,8 +473,8 @@ __global__ void __launch_bounds__(320, 1)
   float* sD = reinterpret_cast<float*>(sKV + NS * TILE);   // [256]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sD + 256);
   uint64_t* bar_q = bars + 0;
-  uint64_t* kv_full = bars + 1;          // [NS]
-  uint64_t* kv_empty = bars + 1 + NS;    // [NS]
+  uint64_t* kv_full = bars + 1;          // [NK + NV]
+  uint64_t* kv_empty = bars + 1 + NS;    // [NK + NV]
   uint64_t* s_full = bars + 1 + 2 * NS;
   uint64_t* s_free = s_full + 1;
   uint64_t* dp_full = s_full + 2;
@@ -480,7 +517,8 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;           // all 512 columns are this CTA's: they start at 0
+  if (threadIdx.x == 0 && *tmem_slot != tmem) atomicOr(a.err, ERR_BAD_ARG);
   const uint32_t tS = tmem, tP = tmem + 128, tQ = tmem + 256, tD = tmem + 384;
   const PieceUnit un = *s_unit;
   const int row0 = un.unit * 128, n = un.unit + 1;
@@ -497,19 +535,24 @@ __global__ void __launch_bounds__(320, 1)
         tma_load_3d(sQ + p * kPanel, &tmQ, bar_q, p * 64, un.begin + row0, h);
         tma_load_3d(sG + p * kPanel, &tmG, bar_q, p * 64, un.begin + row0, h);
       }
+      int slot[2] = {0, NK};             // K's and V's next
+      uint32_t lap[2] = {0, 0};          // times round
       for (int i = 0; i < 2 * n && ok; ++i) {
-        const int slot = i % NS;
-        if (i >= NS && !mbar_wait(&kv_empty[slot], ((i / NS) + 1) & 1, abort_flag, a.err, ERR_TIMEOUT_PRODUCER)) {
+        const int w = i & 1, sl = w ? slot[1] : slot[0];
+        const uint32_t r = w ? lap[1] : lap[0];
+        if (r > 0 && !mbar_wait(&kv_empty[sl], (r - 1) & 1, abort_flag, a.err, ERR_TIMEOUT_PRODUCER)) {
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(&kv_full[slot], TILE);
-        out_valid |= 1u << slot;
-        out_parity = (out_parity & ~(1u << slot)) | ((uint32_t)((i / NS) & 1) << slot);
-        const CUtensorMap* map = (i & 1) ? &tmV : &tmK;
+        mbar_arrive_expect_tx(&kv_full[sl], TILE);
+        out_valid |= 1u << sl;
+        out_parity = (out_parity & ~(1u << sl)) | ((r & 1) << sl);
+        const CUtensorMap* map = w ? &tmV : &tmK;
 #pragma unroll
         for (int p = 0; p < PANELS; ++p)
-          tma_load_3d(sKV + slot * TILE + p * kPanel, map, &kv_full[slot], p * 64, un.begin + (i >> 1) * 128, hk);
+          tma_load_3d(sKV + sl * TILE + p * kPanel, map, &kv_full[sl], p * 64, un.begin + (i >> 1) * 128, hk);
+        if (w) { if (++slot[1] == NS) { slot[1] = NK; ++lap[1]; } }
+        else if (++slot[0] == NK) { slot[0] = 0; ++lap[0]; }
       }
       if (!ok) {
         for (int s = 0; s < NS; ++s) {
@@ -524,49 +567,62 @@ __global__ void __launch_bounds__(320, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = mbar_wait(bar_q, 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
-      const uint32_t q_addr = smem_u32(sQ), g_addr = smem_u32(sG);
-      auto kv_addr = [&](int item) { return smem_u32(sKV + (item % NS) * TILE); };
-      auto kv_wait = [&](int item) { return mbar_wait(&kv_full[item % NS], (item / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA); };
-      // S(j) = Q K_j^T, dP(j) = dO V_j^T, once the compute warps have the tiles before in registers
-      auto issue = [&](int j) -> bool {
-        if (!kv_wait(2 * j)) return false;
-        if (j >= 1 && !mbar_wait(s_free, (j - 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tS, desc_kmajor(q_addr, kk), desc_kmajor(kv_addr(2 * j), kk), IDESC_S, kk > 0 ? 1u : 0u);
+    bool ok = mbar_wait_warp(bar_q, 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
+    const bool leader = elect_one();
+    const uint64_t qd = kmajor_base(sQ), gd = kmajor_base(sG), kd = kmajor_base(sKV), kn = mnmajor_base(sKV);
+    constexpr uint64_t STEP = TILE >> 4;
+    int ks = 0, vs = NK, kq = 0;         // slots of the next K and V, and of the K that dQ takes next
+    uint32_t kp = 0, vp = 0;
+    auto commit = [&](uint64_t* bar) {
+      if (leader) umma_commit(bar);
+      __syncwarp();
+    };
+    // S(j) = Q K_j^T, dP(j) = dO V_j^T, once the compute warps have the tiles before in registers
+    auto issue_s = [&](int j) -> bool {
+      if (!mbar_wait_warp(&kv_full[ks], kp, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+      if (j >= 1 && !mbar_wait_warp(s_free, (j - 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+      tc_fence_after();
+      if (leader) {
+        mma_kk<D / 16>(tS, qd, kd + ks * STEP, IDESC_S);
         umma_commit(s_full);
-        if (!kv_wait(2 * j + 1)) return false;
-        if (j >= 1 && !mbar_wait(dp_free, (j - 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tP, desc_kmajor(g_addr, kk), desc_kmajor(kv_addr(2 * j + 1), kk), IDESC_S, kk > 0 ? 1u : 0u);
+      }
+      __syncwarp();
+      if (++ks == NK) { ks = 0; kp ^= 1; }
+      return true;
+    };
+    auto issue_dp = [&](int j) -> bool {
+      if (!mbar_wait_warp(&kv_full[vs], vp, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+      if (j >= 1 && !mbar_wait_warp(dp_free, (j - 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+      tc_fence_after();
+      if (leader) {
+        mma_kk<D / 16>(tP, gd, kd + vs * STEP, IDESC_S);
         umma_commit(dp_full);
-        umma_commit(&kv_empty[(2 * j + 1) % NS]);
-        return true;
-      };
-      if (ok) ok = issue(0);
-      for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n && !issue(j + 1)) { ok = false; break; }
-        if (!mbar_wait(ds_full, j & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)  // dQ += dS(j) K_j
-          umma_bf16_tmem_a(tQ, tD + (j & 1) * 64 + kk * 8, desc_mnmajor(kv_addr(2 * j), kk), IDESC_Q, (j > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&kv_empty[(2 * j) % NS]);
+        umma_commit(&kv_empty[vs]);
       }
-      if (ok) {
-        umma_commit(done);
-      } else {
-        *abort_flag = 1;
-        umma_commit(drain);
-        const unsigned long long t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain, 0))
-          if (globaltimer_ns() - t0 > 100000000ull) break;
+      __syncwarp();
+      if (++vs == NS) { vs = NK; vp ^= 1; }
+      return true;
+    };
+    if (ok) ok = issue_s(0) && issue_dp(0);
+    for (int j = 0; j < n && ok; ++j) {
+      if (j + 1 < n && !(issue_s(j + 1) && issue_dp(j + 1))) { ok = false; break; }
+      if (!mbar_wait_warp(ds_full, j & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
+      tc_fence_after();
+      if (leader) {
+        mma_tmem<32>(tQ, tD + (j & 1) * 64, kn + kq * STEP, IDESC_Q, j > 0);   // dQ += dS(j) K_j
+        umma_commit(&kv_empty[kq]);
       }
+      __syncwarp();
+      if (++kq == NK) kq = 0;
+    }
+    if (ok) {
+      commit(done);
+    } else {
+      *abort_flag = 1;
+      commit(drain);
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain, 0))
+        if (globaltimer_ns() - t0 > 100000000ull) break;
     }
   } else {
     const int q4 = warp & 3, half = (warp - 2) >> 2, cb = half * 64;
@@ -621,9 +677,8 @@ __global__ void __launch_bounds__(320, 1)
       if (diag) {
         // rows of K past the sequence, which weights of 0 would meet
         if (half == 0 && j * 128 + r >= un.len) {
-          const int item = 2 * j;
-          mbar_wait(&kv_full[item % NS], (item / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
-          tile_row_clear<D>(sKV + (item % NS) * TILE, r);
+          mbar_wait(&kv_full[j % NK], (j / NK) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
+          tile_row_clear<D>(sKV + (j % NK) * TILE, r);
           fence_proxy_async_smem();
         }
         __syncwarp();
@@ -762,7 +817,8 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;           // all 512 columns are this CTA's: they start at 0
+  if (threadIdx.x == 0 && *tmem_slot != tmem) atomicOr(a.err, ERR_BAD_ARG);
   const uint32_t tS = tmem, tP = tmem + 128, tDV = tmem + 256, tDK = tmem + 384;
   const PieceUnit un = *s_unit;
   const int kt = un.unit, row0 = kt * 128;
@@ -815,59 +871,65 @@ __global__ void __launch_bounds__(320, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = mbar_wait(bar_kv, 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
-      const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV);
-      auto issue_s = [&](int it) -> bool {   // S^T = K Q^T
-        const int b = it & 1;
-        if (!mbar_wait(&q_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
-        tc_fence_after();
-        const uint32_t q_addr = smem_u32(sQ + b * TILE);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tS, desc_kmajor(k_addr, kk), desc_kmajor(q_addr, kk), IDESC_S, kk > 0 ? 1u : 0u);
+    bool ok = mbar_wait_warp(bar_kv, 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
+    const bool leader = elect_one();
+    const uint64_t kd = kmajor_base(sK), vd = kmajor_base(sV), qk = kmajor_base(sQ), gk = kmajor_base(sG), qm = mnmajor_base(sQ), gm = mnmajor_base(sG);
+    constexpr uint64_t STEP = TILE >> 4;
+    auto commit = [&](uint64_t* bar) {
+      if (leader) umma_commit(bar);
+      __syncwarp();
+    };
+    auto issue_s = [&](int it) -> bool {   // S^T = K Q^T
+      const int b = it & 1;
+      if (!mbar_wait_warp(&q_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+      tc_fence_after();
+      if (leader) {
+        mma_kk<D / 16>(tS, kd, qk + b * STEP, IDESC_S);
         umma_commit(s_full);
-        return true;
-      };
-      auto issue_dp = [&](int it) -> bool {  // dP^T = V dO^T
-        const int b = it & 1;
-        if (!mbar_wait(&g_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
-        tc_fence_after();
-        const uint32_t g_addr = smem_u32(sG + b * TILE);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tP, desc_kmajor(v_addr, kk), desc_kmajor(g_addr, kk), IDESC_S, kk > 0 ? 1u : 0u);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto issue_dp = [&](int it) -> bool {  // dP^T = V dO^T
+      const int b = it & 1;
+      if (!mbar_wait_warp(&g_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
+      tc_fence_after();
+      if (leader) {
+        mma_kk<D / 16>(tP, vd, gk + b * STEP, IDESC_S);
         umma_commit(dp_full);
-        return true;
-      };
-      if (ok) ok = issue_s(0) && issue_dp(0);
-      for (int it = 0; it < n && ok; ++it) {
-        const int b = it & 1;
-        const uint32_t q_addr = smem_u32(sQ + b * TILE), g_addr = smem_u32(sG + b * TILE);
-        if (!mbar_wait(p_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)  // dV += P^T dO: the weights of queries 0-63 in columns 0-31, of 64-127 in 64-95
-          umma_bf16_tmem_a(tDV, tS + (kk >> 2) * 64 + (kk & 3) * 8, desc_mnmajor(g_addr, kk), IDESC_KV, (it > 0 || kk > 0) ? 1u : 0u);
+      }
+      __syncwarp();
+      return true;
+    };
+    if (ok) ok = issue_s(0) && issue_dp(0);
+    for (int it = 0; it < n && ok; ++it) {
+      const int b = it & 1;
+      if (!mbar_wait_warp(p_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
+      tc_fence_after();
+      if (leader) {
+        // dV += P^T dO: the weights of queries 0-63 in columns 0-31, of 64-127 in 64-95
+        mma_tmem<64>(tDV, tS, gm + b * STEP, IDESC_KV, it > 0);
         umma_commit(&g_empty[b]);
-        if (it + 1 < n && !issue_s(it + 1)) { ok = false; break; }
-        if (!mbar_wait(ds_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)  // dK += dS^T Q
-          umma_bf16_tmem_a(tDK, tP + (kk >> 2) * 64 + (kk & 3) * 8, desc_mnmajor(q_addr, kk), IDESC_KV, (it > 0 || kk > 0) ? 1u : 0u);
+      }
+      __syncwarp();
+      if (it + 1 < n && !issue_s(it + 1)) { ok = false; break; }
+      if (!mbar_wait_warp(ds_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
+      tc_fence_after();
+      if (leader) {
+        mma_tmem<64>(tDK, tP, qm + b * STEP, IDESC_KV, it > 0);   // dK += dS^T Q
         umma_commit(&q_empty[b]);
-        if (it + 1 < n && !issue_dp(it + 1)) { ok = false; break; }
       }
-      if (ok) {
-        umma_commit(done);
-      } else {
-        *abort_flag = 1;
-        umma_commit(drain);
-        const unsigned long long t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain, 0))
-          if (globaltimer_ns() - t0 > 100000000ull) break;
-      }
+      __syncwarp();
+      if (it + 1 < n && !issue_dp(it + 1)) { ok = false; break; }
+    }
+    if (ok) {
+      commit(done);
+    } else {
+      *abort_flag = 1;
+      commit(drain);
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain, 0))
+        if (globaltimer_ns() - t0 > 100000000ull) break;
     }
   } else {
     const int q4 = warp & 3, half = (warp - 2) >> 2, cb = half * 64;
@@ -876,19 +938,19 @@ __global__ void __launch_bounds__(320, 1)
     const float2 c2 = make_float2(a.scale_log2, a.scale_log2);
     const float* stats = half == 0 ? a.lse : a.dvec;
     int qi = kt, h = hk * a.G;
-    // this thread's query's lse (half 0) or D (half 1), a step ahead; a query past the sequence weighs nothing
+    // this thread's query's lse (half 0) or D (half 1), a step ahead and as it is (what is computed from it waits for
+    // it); a query past the sequence weighs nothing
     auto stat = [&](int i, int hh) -> float {
       const int qrow = i * 128 + r;
-      if (qrow >= un.len) return half == 0 ? -INFINITY : 0.f;
-      const float v = stats[(long long)hh * a.pc.M + un.begin + qrow];
-      return half == 0 ? -v * kLog2e : -v;
+      return qrow < un.len ? stats[(long long)hh * a.pc.M + un.begin + qrow] : half == 0 ? INFINITY : 0.f;
     };
+    const float turn = half == 0 ? -kLog2e : -1.f;
     float next = stat(qi, h);
     bool ok = true;
     for (int it = 0; it < n; ++it) {
       const int b = it & 1;
       float *nl = sL + b * 128, *nd = sD + b * 128;
-      (half == 0 ? nl : nd)[r] = next;
+      (half == 0 ? nl : nd)[r] = next * turn;
       mbar_arrive(&l_full[b]);
       const bool diag = qi == kt;
       const int lim = un.len - qi * 128;     // queries of this tile
@@ -907,37 +969,39 @@ __global__ void __launch_bounds__(320, 1)
         }
         __syncwarp();
       }
-      uint32_t pk[32];  // this thread's 64 columns of the P^T row, packed bf16 pairs (kept for dS)
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        uint32_t sv[32];
+      float p[64];      // this thread's 64 columns of the P^T row
+      uint32_t pk[32];  // packed bf16 pairs of it, then of dS^T
+      {
+        uint32_t* pr = reinterpret_cast<uint32_t*>(p);
         __syncwarp();
-        tmem_ld_32x32b_x32(tS + lane_off + cb + h2 * 32, sv);
+        tmem_ld_32x32b_x32(tS + lane_off + cb, *reinterpret_cast<uint32_t(*)[32]>(pr));
+        tmem_ld_32x32b_x32(tS + lane_off + cb + 32, *reinterpret_cast<uint32_t(*)[32]>(pr + 32));
         tmem_ld_wait();
+      }
 #pragma unroll
-        for (int e0 = 0; e0 < 32; e0 += 4) {
-          const int e = h2 * 32 + e0, cc = cb + e;
-          const float4 n4 = *reinterpret_cast<const float4*>(nl + cc);
-          const float2 v0 = __ffma2_rn(make_float2(__uint_as_float(sv[e0]), __uint_as_float(sv[e0 + 1])), c2, make_float2(n4.x, n4.y));
-          const float2 v1 = __ffma2_rn(make_float2(__uint_as_float(sv[e0 + 2]), __uint_as_float(sv[e0 + 3])), c2, make_float2(n4.z, n4.w));
-          float2 p0, p1;
-          if (e >= 48) {
-            p0 = exp2_poly2(v0);
-            p1 = exp2_poly2(v1);
-          } else {
-            p0 = make_float2(ex2_approx(v0.x), ex2_approx(v0.y));
-            p1 = make_float2(ex2_approx(v1.x), ex2_approx(v1.y));
-          }
-          if (part) {
-            const int lo = diag ? r : 0;     // queries lo .. lim - 1 see this key
-            if (cc < lo || cc >= lim) p0.x = 0.f;
-            if (cc + 1 < lo || cc + 1 >= lim) p0.y = 0.f;
-            if (cc + 2 < lo || cc + 2 >= lim) p1.x = 0.f;
-            if (cc + 3 < lo || cc + 3 >= lim) p1.y = 0.f;
-          }
-          pk[e >> 1] = pack_bf16x2(p0.x, p0.y);
-          pk[(e >> 1) + 1] = pack_bf16x2(p1.x, p1.y);
+      for (int e = 0; e < 64; e += 4) {
+        const int cc = cb + e;
+        const float4 n4 = *reinterpret_cast<const float4*>(nl + cc);
+        const float2 v0 = __ffma2_rn(make_float2(p[e], p[e + 1]), c2, make_float2(n4.x, n4.y));
+        const float2 v1 = __ffma2_rn(make_float2(p[e + 2], p[e + 3]), c2, make_float2(n4.z, n4.w));
+        float2 p0, p1;
+        if (e >= 48) {
+          p0 = exp2_poly2(v0);
+          p1 = exp2_poly2(v1);
+        } else {
+          p0 = make_float2(ex2_approx(v0.x), ex2_approx(v0.y));
+          p1 = make_float2(ex2_approx(v1.x), ex2_approx(v1.y));
         }
+        if (part) {
+          const int lo = diag ? r : 0;       // queries lo .. lim - 1 see this key
+          if (cc < lo || cc >= lim) p0.x = 0.f;
+          if (cc + 1 < lo || cc + 1 >= lim) p0.y = 0.f;
+          if (cc + 2 < lo || cc + 2 >= lim) p1.x = 0.f;
+          if (cc + 3 < lo || cc + 3 >= lim) p1.y = 0.f;
+        }
+        p[e] = p0.x; p[e + 1] = p0.y; p[e + 2] = p1.x; p[e + 3] = p1.y;
+        pk[e >> 1] = pack_bf16x2(p0.x, p0.y);
+        pk[(e >> 1) + 1] = pack_bf16x2(p1.x, p1.y);
       }
       __syncwarp();
       tmem_st_32x32b_x32(tS + lane_off + cb, pk);
@@ -956,8 +1020,7 @@ __global__ void __launch_bounds__(320, 1)
         for (int e0 = 0; e0 < 32; e0 += 4) {
           const int e = h2 * 32 + e0, cc = cb + e;
           const float4 d4 = *reinterpret_cast<const float4*>(nd + cc);
-          const float2 pa = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&pk[e >> 1]));
-          const float2 pb = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&pk[(e >> 1) + 1]));
+          const float2 pa = make_float2(p[e], p[e + 1]), pb = make_float2(p[e + 2], p[e + 3]);
           float2 da = __fmul2_rn(pa, __fadd2_rn(make_float2(__uint_as_float(dp[e0]), __uint_as_float(dp[e0 + 1])), make_float2(d4.x, d4.y)));
           float2 db = __fmul2_rn(pb, __fadd2_rn(make_float2(__uint_as_float(dp[e0 + 2]), __uint_as_float(dp[e0 + 3])), make_float2(d4.z, d4.w)));
           if (part) {
@@ -967,7 +1030,7 @@ __global__ void __launch_bounds__(320, 1)
             if (cc + 2 < lo || cc + 2 >= lim) db.x = 0.f;
             if (cc + 3 < lo || cc + 3 >= lim) db.y = 0.f;
           }
-          pk[e >> 1] = pack_bf16x2(da.x, da.y);   // dS^T over P^T
+          pk[e >> 1] = pack_bf16x2(da.x, da.y);
           pk[(e >> 1) + 1] = pack_bf16x2(db.x, db.y);
         }
       }
