@@ -20,7 +20,7 @@
 // short sequences fill both), else neighbouring rows of one head.
 //   warp 0      TMA: Q tiles, then K_0, V_0, K_1, .. through a ring
 //   warp 1      MMA: per step P0 V, S0(next), P1 V, S1(next); P from TMEM, over its own scores
-//   warps 2-9   softmax of tile 0 / 1, a row a thread; a quarter of the exponentials on the FMA pipe
+//   warps 2-9   softmax of tile 0 / 1, a row a thread
 // The running maximum moves only when it grows by more than 8 (in log2), so outputs are rarely rescaled.
 //
 // Backward: two kernels and no sum through memory.  One has 128 queries and goes over the keys (dQ, three
@@ -69,12 +69,13 @@ __device__ __forceinline__ void mma_kk(uint32_t d, uint64_t a, uint64_t b, uint3
 #pragma unroll
   for (int kk = 0; kk < STEPS; ++kk) umma_bf16(d, kmajor_at(a, kk), kmajor_at(b, kk), idesc, kk > 0 ? 1u : 0u);
 }
-// D (+)= A B, A the weights of 128 columns in TMEM: 16 of them a step, the upper 64 `gap` columns behind the lower
+// D (+)= A B, A the weights of 128 columns in TMEM, packed: 16 of them a step, those of every 32 columns GAP behind the
+// ones before
 template <int GAP>
 __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
-    umma_bf16_tmem_a(d, a + (kk >> 2) * GAP + (kk & 3) * 8, mnmajor_at(b, kk), idesc, kk > 0 ? 1u : add ? 1u : 0u);
+    umma_bf16_tmem_a(d, a + (kk >> 1) * GAP + (kk & 1) * 8, mnmajor_at(b, kk), idesc, kk > 0 ? 1u : add ? 1u : 0u);
 }
 
 // Row `row` of a tile of D columns (swizzled panels of 64): whether it holds an infinity or a NaN.
@@ -97,6 +98,13 @@ __device__ __forceinline__ void tile_row_clear(uint8_t* tile, int row) {
 #pragma unroll
   for (int c = 0; c < D / 8; ++c)
     *reinterpret_cast<uint4*>(tile + (c >> 3) * kPanel + sw128_chunk_offset(row, c & 7)) = make_uint4(0, 0, 0, 0);
+}
+
+// One arrival for a warp, once all its lanes have come here: an mbarrier takes the arrivals of 32 lanes one after
+// another (dQ of 4 x 8192 rows took 2.3 instead of 1.8 ms with 512 of them a barrier).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // Zeros into rows [row0, row0 + n) x heads of out [M, H, D] (rows outside all sequences).
@@ -134,26 +142,30 @@ __device__ __noinline__ void packed_row(const PkArgs& a, int begin, int i, int h
   }
 }
 
-template <int D>
+template <int D, int TILES>
 struct PkFwd {
   static constexpr uint32_t TILE = 128u * D * 2u;
-  static constexpr int NS = D == 128 ? 5 : 8;          // K / V ring
-  static constexpr size_t SMEM = 1024 + (2 + NS) * TILE + 32 * 8 + 64;
+  static constexpr int NS = TILES == 1 ? (D == 128 ? 2 : 4) : D == 128 ? 5 : 8;   // K / V ring
+  static constexpr size_t SMEM = 1024 + (TILES + NS) * TILE + 32 * 8 + 64;
+  static constexpr int THREADS = 64 + 128 * TILES;
+  static constexpr uint32_t COLUMNS = 256 * TILES;     // of TMEM: S and O of each tile
 };
+static_assert(2 * PkFwd<128, 1>::SMEM <= 227 * 1024 && PkFwd<128, 2>::SMEM <= 227 * 1024, "shared memory");
 
-template <int D>
-__global__ void __launch_bounds__(320, 1)
+template <int D, int TILES>
+__global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
     packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const PkArgs a) {
-  constexpr uint32_t TILE = PkFwd<D>::TILE;
-  constexpr int NS = PkFwd<D>::NS, PANELS = D / 64;
+  using Cfg = PkFwd<D, TILES>;
+  constexpr uint32_t TILE = Cfg::TILE;
+  constexpr int NS = Cfg::NS, PANELS = D / 64;
   constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, false, false);
   constexpr uint32_t IDESC_O = umma_idesc_bf16(128, D, false, true);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                 // [2] tiles
-  uint8_t* sKV = sQ + 2 * TILE;       // [NS] slots
+  uint8_t* sQ = smem;                 // [TILES]
+  uint8_t* sKV = sQ + TILES * TILE;       // [NS] slots
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + NS * TILE);
   uint64_t* bar_q = bars + 0;
   uint64_t* kv_full = bars + 1;          // [NS]
@@ -168,14 +180,14 @@ __global__ void __launch_bounds__(320, 1)
   PieceUnit* s_unit = reinterpret_cast<PieceUnit*>(tmem_slot + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int nh = a.by_heads ? a.Hq / 2 : a.Hq;
+  const int nh = TILES == 2 && a.by_heads ? a.Hq / 2 : a.Hq;
   const int hx = (int)(blockIdx.x % nh);
   const int slot_id = (int)(gridDim.x / nh - 1 - blockIdx.x / nh);   // a sequence's last rows have the most keys: first
   if (warp == 0) {
-    const PieceUnit u = a.by_heads ? piece_unit<128>(a.pc, slot_id) : piece_unit<256>(a.pc, slot_id);
+    const PieceUnit u = TILES == 1 || a.by_heads ? piece_unit<128>(a.pc, slot_id) : piece_unit<256>(a.pc, slot_id);
     if (lane == 0) *s_unit = u;
   } else if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(tmem_slot, Cfg::COLUMNS);
     tmem_relinquish();
   } else if (threadIdx.x == 64) {
     mbar_init(bar_q, 1);
@@ -185,7 +197,7 @@ __global__ void __launch_bounds__(320, 1)
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 128);
+      mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
       by_row[t] = 0;
     }
@@ -199,20 +211,22 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  constexpr uint32_t tmem = 0;           // all 512 columns are this CTA's: they start at 0
-  if (threadIdx.x == 0 && *tmem_slot != tmem) atomicOr(a.err, ERR_BAD_ARG);
+  const uint32_t tmem = TILES == 2 ? 0 : *tmem_slot;   // all 512 columns start at 0
+  if (TILES == 2 && threadIdx.x == 0 && *tmem_slot != tmem) atomicOr(a.err, ERR_BAD_ARG);
+  constexpr uint32_t OAT = 128 * TILES;                // outputs behind the scores
   const PieceUnit un = *s_unit;
-  const int U = a.by_heads ? 128 : 256;
+  const bool pair = TILES == 2 && a.by_heads;
+  const int U = TILES == 1 || pair ? 128 : 256;
   const bool live = un.unit >= 0 && a.pc.real(un.piece);
   // tile t: its head, first row in the sequence, and number of K / V tiles (0: there is none)
-  const int h0 = a.by_heads ? 2 * hx : hx, h1 = a.by_heads ? h0 + 1 : hx;
-  const int r0 = un.unit * U, r1 = a.by_heads ? r0 : r0 + 128;
-  const int n0 = live ? r0 / 128 + 1 : 0, n1 = live && r1 < un.len ? r1 / 128 + 1 : 0;
+  const int h0 = pair ? 2 * hx : hx, h1 = pair ? h0 + 1 : hx;
+  const int r0 = un.unit * U, r1 = pair ? r0 : r0 + 128;
+  const int n0 = live ? r0 / 128 + 1 : 0, n1 = TILES == 2 && live && r1 < un.len ? r1 / 128 + 1 : 0;
   const int nk = max(n0, n1);
   const int hk = h0 / a.G;
 
   if (!live) {
-    if (un.unit >= 0) clear_rows<D>(a.out, a.Hq, h0, a.by_heads ? 2 : 1, un.begin + r0, min(U, un.len - r0));
+    if (un.unit >= 0) clear_rows<D>(a.out, a.Hq, h0, pair ? 2 : 1, un.begin + r0, min(U, un.len - r0));
   } else if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
@@ -273,7 +287,7 @@ __global__ void __launch_bounds__(320, 1)
     auto issue_pv = [&](int t, int j) -> bool {
       if (!mbar_wait_warp(&p_full[t], j & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
       tc_fence_after();
-      if (leader) mma_tmem<32>(tmem + 256 + t * 128, tmem + t * 128, vd + vs * STEP, IDESC_O, j > 0);
+      if (leader) mma_tmem<16>(tmem + OAT + t * 128, tmem + t * 128, vd + vs * STEP, IDESC_O, j > 0);
       __syncwarp();
       return true;
     };
@@ -331,7 +345,7 @@ __global__ void __launch_bounds__(320, 1)
     const int q4 = warp & 3;
     const int r = q4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
-    const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
+    const uint32_t tS = tmem + t * 128, tO = tmem + OAT + t * 128;
     const int n_t = t == 0 ? n0 : n1;
     const int row = (t == 0 ? r0 : r1) + r, head = t == 0 ? h0 : h1;   // row of the sequence
     const float c = a.scale_log2;
@@ -379,13 +393,15 @@ __global__ void __launch_bounds__(320, 1)
         alpha = ex2_approx(m_run - mxs);
         m_run = mxs;
       }
-      // p = 2^(x c - m): packed pairs; columns 96..127 of every row on the FMA pipe
+      // p = 2^(x c - m): packed pairs
       const float2 c2 = make_float2(c, c), nm2 = make_float2(-m_run, -m_run);
       float2 sm4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       uint32_t pk[64];  // the row of P as packed bf16 pairs
 #pragma unroll
       for (int i = 0; i < 128; i += 2) {
         const float2 v = __ffma2_rn(make_float2(x[i], x[i + 1]), c2, nm2);
+        // a quarter on the FMA pipe, which the MUFU unit's 16 a cycle of an SM leave idle (5.6 ms without, for 16 x 8191 rows).  A
+        // NaN is lost there, but then the row's maximum is NaN and with it all of its other weights.
         float2 p2;
         if (i >= 96) p2 = exp2_poly2(v);
         else p2 = make_float2(ex2_approx(v.x), ex2_approx(v.y));
@@ -413,7 +429,7 @@ __global__ void __launch_bounds__(320, 1)
       tmem_st_32x32b_x32(tS + lane_off + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[t]);
+      warp_arrive(&p_full[t]);
     }
     if (n_t > 0 && ok && mbar_wait_warp(&o_done[t], 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
       tc_fence_after();
@@ -439,15 +455,16 @@ __global__ void __launch_bounds__(320, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, Cfg::COLUMNS);
   }
 }
 
 // ================================================================================ backward: dQ
 // One CTA per 128 queries of a head, over the keys.  TMEM: S | dP | dQ | two dS (bf16).
 //   warp 0      TMA: Q and dO, then K_0, V_0, K_1, .. through a ring each
-//   warp 1      MMA: per step S(next) = Q K^T, dP(next) = dO V^T, dQ += dS K with dS from TMEM
-//   warps 2-9   p = 2^(S c - lse), dS = p (dP - D): two warps a lane quarter, 64 columns each
+//   warp 1      MMA: S(next) = Q K^T, dP(next) = dO V^T
+//   warp 18     MMA: dQ += dS K with dS from TMEM (by itself, so that it waits for nothing but dS)
+//   warps 2-17  p = 2^(S c - lse), dS = p (dP - D): four warps a lane quarter, 32 columns each
 // S and dP are given back as soon as they are in registers, so the next ones are formed meanwhile.
 template <int D>
 struct PkDq {
@@ -457,7 +474,7 @@ struct PkDq {
 };
 
 template <int D>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(608, 1)
     packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const PkArgs a) {
   constexpr uint32_t TILE = PkDq<D>::TILE;
@@ -470,7 +487,7 @@ __global__ void __launch_bounds__(320, 1)
   uint8_t* sQ = smem;
   uint8_t* sG = sQ + TILE;
   uint8_t* sKV = sG + TILE;
-  float* sD = reinterpret_cast<float*>(sKV + NS * TILE);   // [256]
+  float* sD = reinterpret_cast<float*>(sKV + NS * TILE);   // [2][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sD + 256);
   uint64_t* bar_q = bars + 0;
   uint64_t* kv_full = bars + 1;          // [NK + NV]
@@ -480,9 +497,10 @@ __global__ void __launch_bounds__(320, 1)
   uint64_t* dp_full = s_full + 2;
   uint64_t* dp_free = s_full + 3;
   uint64_t* ds_full = s_full + 4;
-  uint64_t* done = s_full + 5;
-  uint64_t* drain = s_full + 6;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* ds_free = s_full + 5;      // [2]
+  uint64_t* done = s_full + 7;
+  uint64_t* drain = s_full + 8;        // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PieceUnit* s_unit = reinterpret_cast<PieceUnit*>(tmem_slot + 4);
 
@@ -501,12 +519,15 @@ __global__ void __launch_bounds__(320, 1)
       mbar_init(&kv_empty[i], 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(s_free, 256);
+    mbar_init(s_free, 16);
     mbar_init(dp_full, 1);
-    mbar_init(dp_free, 256);
-    mbar_init(ds_full, 256);
+    mbar_init(dp_free, 16);
+    mbar_init(ds_full, 16);
+    mbar_init(&ds_free[0], 1);
+    mbar_init(&ds_free[1], 1);
     mbar_init(done, 1);
-    mbar_init(drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmQ);
@@ -569,9 +590,9 @@ __global__ void __launch_bounds__(320, 1)
   } else if (warp == 1) {
     bool ok = mbar_wait_warp(bar_q, 0, abort_flag, a.err, ERR_TIMEOUT_MMA);
     const bool leader = elect_one();
-    const uint64_t qd = kmajor_base(sQ), gd = kmajor_base(sG), kd = kmajor_base(sKV), kn = mnmajor_base(sKV);
+    const uint64_t qd = kmajor_base(sQ), gd = kmajor_base(sG), kd = kmajor_base(sKV);
     constexpr uint64_t STEP = TILE >> 4;
-    int ks = 0, vs = NK, kq = 0;         // slots of the next K and V, and of the K that dQ takes next
+    int ks = 0, vs = NK;                 // slots of the next K and V
     uint32_t kp = 0, vp = 0;
     auto commit = [&](uint64_t* bar) {
       if (leader) umma_commit(bar);
@@ -603,38 +624,51 @@ __global__ void __launch_bounds__(320, 1)
       if (++vs == NS) { vs = NK; vp ^= 1; }
       return true;
     };
-    if (ok) ok = issue_s(0) && issue_dp(0);
-    for (int j = 0; j < n && ok; ++j) {
-      if (j + 1 < n && !(issue_s(j + 1) && issue_dp(j + 1))) { ok = false; break; }
+    for (int j = 0; j < n && ok; ++j) ok = issue_s(j) && issue_dp(j);
+    if (!ok) {
+      *abort_flag = 1;
+      commit(&drain[0]);
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(&drain[0], 0))
+        if (globaltimer_ns() - t0 > 100000000ull) break;
+    }
+  } else if (warp == 18) {
+    const bool leader = elect_one();
+    const uint64_t kn = mnmajor_base(sKV);
+    constexpr uint64_t STEP = TILE >> 4;
+    int kq = 0;                          // slot of K_j
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
       if (!mbar_wait_warp(ds_full, j & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
       tc_fence_after();
       if (leader) {
-        mma_tmem<32>(tQ, tD + (j & 1) * 64, kn + kq * STEP, IDESC_Q, j > 0);   // dQ += dS(j) K_j
+        mma_tmem<16>(tQ, tD + (j & 1) * 64, kn + kq * STEP, IDESC_Q, j > 0);
         umma_commit(&kv_empty[kq]);
+        umma_commit(&ds_free[j & 1]);
+        if (j == n - 1) umma_commit(done);
       }
       __syncwarp();
       if (++kq == NK) kq = 0;
     }
-    if (ok) {
-      commit(done);
-    } else {
+    if (!ok) {
       *abort_flag = 1;
-      commit(drain);
+      if (leader) umma_commit(&drain[1]);
+      __syncwarp();
       const unsigned long long t0 = globaltimer_ns();
-      while (!mbar_try_wait(drain, 0))
+      while (!mbar_try_wait(&drain[1], 0))
         if (globaltimer_ns() - t0 > 100000000ull) break;
     }
   } else {
-    const int q4 = warp & 3, half = (warp - 2) >> 2, cb = half * 64;
+    const int q4 = warp & 3, quarter = (warp - 2) >> 2, cb = quarter * 32;
     const int r = q4 * 32 + lane, row = row0 + r;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
     const bool mine = row < un.len;
     const long long at = (long long)h * a.pc.M + un.begin + row;
-    // D_i = dO_i . o_i, half of the columns a thread; kept for the other kernel
+    // D_i = dO_i . o_i, half of the columns a thread of the first two quarters; kept for the other kernel
     float dsum = 0.f;
-    if (mine) {
-      const uint4* g = reinterpret_cast<const uint4*>(a.dout + (long long)(un.begin + row) * a.gr + h * a.gh + half * (D / 2));
-      const uint4* o = reinterpret_cast<const uint4*>(a.o + ((long long)(un.begin + row) * a.Hq + h) * D + half * (D / 2));
+    if (mine && quarter < 2) {
+      const uint4* g = reinterpret_cast<const uint4*>(a.dout + (long long)(un.begin + row) * a.gr + h * a.gh + quarter * (D / 2));
+      const uint4* o = reinterpret_cast<const uint4*>(a.o + ((long long)(un.begin + row) * a.Hq + h) * D + quarter * (D / 2));
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         const uint4 x = g[i], y = o[i];
@@ -646,10 +680,10 @@ __global__ void __launch_bounds__(320, 1)
         }
       }
     }
-    sD[half * 128 + r] = dsum;
-    named_bar_sync(1, 256);              // no wait comes before it: all 256 threads arrive
+    if (quarter < 2) sD[quarter * 128 + r] = dsum;
+    named_bar_sync(1, 512);              // no wait comes before it: all 512 threads arrive
     dsum = sD[r] + sD[128 + r];
-    if (mine && half == 0) a.dvec[at] = dsum;
+    if (mine && quarter == 0) a.dvec[at] = dsum;
     const float nlse = mine ? -a.lse[at] * kLog2e : -INFINITY;
     const float2 c2 = make_float2(a.scale_log2, a.scale_log2), nl2 = make_float2(nlse, nlse), nd2 = make_float2(-dsum, -dsum);
     bool ok = true;
@@ -657,26 +691,21 @@ __global__ void __launch_bounds__(320, 1)
       const bool diag = j == n - 1;
       if (!mbar_wait_warp(s_full, j & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
       tc_fence_after();
-      float p[64];
-      uint32_t* pr = reinterpret_cast<uint32_t*>(p);
+      float p[32];
       __syncwarp();
-      tmem_ld_32x32b_x32(tS + lane_off + cb, *reinterpret_cast<uint32_t(*)[32]>(pr));
-      tmem_ld_32x32b_x32(tS + lane_off + cb + 32, *reinterpret_cast<uint32_t(*)[32]>(pr + 32));
+      tmem_ld_32x32b_x32(tS + lane_off + cb, *reinterpret_cast<uint32_t(*)[32]>(p));
       tmem_ld_wait();
       tc_fence_before();
-      mbar_arrive(s_free);
+      warp_arrive(s_free);
 #pragma unroll
-      for (int e = 0; e < 64; e += 2) {
+      for (int e = 0; e < 32; e += 2) {
         const float2 v = __ffma2_rn(make_float2(p[e], p[e + 1]), c2, nl2);
-        float2 y;
-        if (e >= 48) y = exp2_poly2(v);
-        else y = make_float2(ex2_approx(v.x), ex2_approx(v.y));
-        p[e] = y.x;
-        p[e + 1] = y.y;
+        p[e] = ex2_approx(v.x);
+        p[e + 1] = ex2_approx(v.y);
       }
       if (diag) {
         // rows of K past the sequence, which weights of 0 would meet
-        if (half == 0 && j * 128 + r >= un.len) {
+        if (quarter == 0 && j * 128 + r >= un.len) {
           mbar_wait(&kv_full[j % NK], (j / NK) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
           tile_row_clear<D>(sKV + (j % NK) * TILE, r);
           fence_proxy_async_smem();
@@ -685,48 +714,41 @@ __global__ void __launch_bounds__(320, 1)
       }
       if (!mbar_wait_warp(dp_full, j & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
       tc_fence_after();
-      uint32_t pk[32];
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        uint32_t dp[32];
-        __syncwarp();
-        tmem_ld_32x32b_x32(tP + lane_off + cb + h2 * 32, dp);
-        tmem_ld_wait();
-        if (h2 == 1) {
-          tc_fence_before();
-          mbar_arrive(dp_free);
-        }
-#pragma unroll
-        for (int e0 = 0; e0 < 32; e0 += 2) {
-          const int e = h2 * 32 + e0;
-          float2 d = __fmul2_rn(make_float2(p[e], p[e + 1]), __fadd2_rn(make_float2(__uint_as_float(dp[e0]), __uint_as_float(dp[e0 + 1])), nd2));
-          if (diag) {
-            if (cb + e > r) d.x = 0.f;
-            if (cb + e + 1 > r) d.y = 0.f;
-          }
-          pk[e >> 1] = pack_bf16x2(d.x, d.y);
-        }
-      }
-      // dS(j - 2) has been read: the commit that signalled S(j) covered dQ(j - 2)
+      uint32_t dp[32], pk[16];
       __syncwarp();
-      tmem_st_32x32b_x32(tD + (j & 1) * 64 + lane_off + half * 32, pk);
+      tmem_ld_32x32b_x32(tP + lane_off + cb, dp);
+      tmem_ld_wait();
+      tc_fence_before();
+      warp_arrive(dp_free);
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        float2 y = __fmul2_rn(make_float2(p[e], p[e + 1]), __fadd2_rn(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), nd2));
+        if (diag) {
+          if (cb + e > r) y.x = 0.f;
+          if (cb + e + 1 > r) y.y = 0.f;
+        }
+        pk[e >> 1] = pack_bf16x2(y.x, y.y);
+      }
+      if (j >= 2 && !mbar_wait_warp(&ds_free[j & 1], ((j - 2) >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      __syncwarp();
+      tmem_st_32x32b_x16(tD + (j & 1) * 64 + lane_off + quarter * 16, pk);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(ds_full);
+      warp_arrive(ds_full);
     }
     if (ok && mbar_wait_warp(done, 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
       tc_fence_after();
-      __nv_bfloat16* dst = a.dq + ((long long)(un.begin + row) * a.Hq + h) * D + half * (D / 2);
-#pragma unroll 1
+      __nv_bfloat16* dst = a.dq + ((long long)(un.begin + row) * a.Hq + h) * D + quarter * (D / 4);
+#pragma unroll
       for (int cc = 0; cc < D / 64; ++cc) {
-        uint32_t o[32];
-        float f[32];
+        uint32_t o[16];
+        float f[16];
         __syncwarp();
-        tmem_ld_32x32b_x32(tQ + lane_off + half * (D / 2) + cc * 32, o);
+        tmem_ld_32x32b_x16(tQ + lane_off + quarter * (D / 4) + cc * 16, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * a.scale;
-        if (mine) store_row_bf16_global(dst + cc * 32, f, 32);
+        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]) * a.scale;
+        if (mine) store_row_bf16_global(dst + cc * 16, f, 16);
       }
     }
   }
@@ -741,7 +763,7 @@ __global__ void __launch_bounds__(320, 1)
 // ================================================================================ backward: dK, dV
 // One CTA per 128 keys of a key/value head, over the queries from there on of all its query heads, in the
 // transposed frame (a key a TMEM lane).  TMEM: S^T | dP^T | dV | dK; P^T and dS^T lie over the scores they came
-// from, each warp's over columns that it alone has read.  MMA order dV(i), S(i+1), dK(i), dP(i+1): while the
+// from, each warp's over columns that it alone has read (four warps a lane quarter, 32 columns each).  MMA order dV(i), S(i+1), dK(i), dP(i+1): while the
 // compute warps turn dP into dS the tensor core runs dV and the next S, and while they take the next exponentials dK
 // and the next dP.
 template <int D>
@@ -751,7 +773,7 @@ struct PkDkv {
 };
 
 template <int D>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(576, 1)
     packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const PkArgs a) {
   constexpr uint32_t TILE = PkDkv<D>::TILE;
@@ -799,12 +821,12 @@ __global__ void __launch_bounds__(320, 1)
       mbar_init(&q_empty[i], 1);
       mbar_init(&g_full[i], 1);
       mbar_init(&g_empty[i], 1);
-      mbar_init(&l_full[i], 256);
+      mbar_init(&l_full[i], 8);
     }
     mbar_init(s_full, 1);
-    mbar_init(p_full, 256);
+    mbar_init(p_full, 16);
     mbar_init(dp_full, 1);
-    mbar_init(ds_full, 256);
+    mbar_init(ds_full, 16);
     mbar_init(done, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -907,8 +929,8 @@ __global__ void __launch_bounds__(320, 1)
       if (!mbar_wait_warp(p_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
       tc_fence_after();
       if (leader) {
-        // dV += P^T dO: the weights of queries 0-63 in columns 0-31, of 64-127 in 64-95
-        mma_tmem<64>(tDV, tS, gm + b * STEP, IDESC_KV, it > 0);
+        // dV += P^T dO: the weights of 32 queries in the first 16 of their scores' columns
+        mma_tmem<32>(tDV, tS, gm + b * STEP, IDESC_KV, it > 0);
         umma_commit(&g_empty[b]);
       }
       __syncwarp();
@@ -916,7 +938,7 @@ __global__ void __launch_bounds__(320, 1)
       if (!mbar_wait_warp(ds_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
       tc_fence_after();
       if (leader) {
-        mma_tmem<64>(tDK, tP, qm + b * STEP, IDESC_KV, it > 0);   // dK += dS^T Q
+        mma_tmem<32>(tDK, tP, qm + b * STEP, IDESC_KV, it > 0);   // dK += dS^T Q
         umma_commit(&q_empty[b]);
       }
       __syncwarp();
@@ -932,66 +954,57 @@ __global__ void __launch_bounds__(320, 1)
         if (globaltimer_ns() - t0 > 100000000ull) break;
     }
   } else {
-    const int q4 = warp & 3, half = (warp - 2) >> 2, cb = half * 64;
+    const int q4 = warp & 3, quarter = (warp - 2) >> 2, cb = quarter * 32;
     const int r = q4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
     const float2 c2 = make_float2(a.scale_log2, a.scale_log2);
-    const float* stats = half == 0 ? a.lse : a.dvec;
+    const bool reads = quarter < 2;      // the first 256 threads: a query's lse (quarter 0) or D
+    const float* stats = quarter == 0 ? a.lse : a.dvec;
     int qi = kt, h = hk * a.G;
-    // this thread's query's lse (half 0) or D (half 1), a step ahead and as it is (what is computed from it waits for
-    // it); a query past the sequence weighs nothing
+    // a step ahead and as it is (what is computed from it waits for it); a query past the sequence weighs nothing
     auto stat = [&](int i, int hh) -> float {
       const int qrow = i * 128 + r;
-      return qrow < un.len ? stats[(long long)hh * a.pc.M + un.begin + qrow] : half == 0 ? INFINITY : 0.f;
+      return reads && qrow < un.len ? stats[(long long)hh * a.pc.M + un.begin + qrow] : quarter == 0 ? INFINITY : 0.f;
     };
-    const float turn = half == 0 ? -kLog2e : -1.f;
+    const float turn = quarter == 0 ? -kLog2e : -1.f;
     float next = stat(qi, h);
     bool ok = true;
     for (int it = 0; it < n; ++it) {
       const int b = it & 1;
       float *nl = sL + b * 128, *nd = sD + b * 128;
-      (half == 0 ? nl : nd)[r] = next * turn;
-      mbar_arrive(&l_full[b]);
+      if (reads) {
+        (quarter == 0 ? nl : nd)[r] = next * turn;
+        warp_arrive(&l_full[b]);
+      }
       const bool diag = qi == kt;
       const int lim = un.len - qi * 128;     // queries of this tile
       if (++qi == tiles) { qi = kt; ++h; }
       if (it + 1 < n) next = stat(qi, h);
-      if (!mbar_wait_warp(&l_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
       if (!mbar_wait_warp(s_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
       tc_fence_after();
       const bool part = diag || lim < 128;   // some of its weights are chosen to be 0
       if (lim < 128) {
         // rows of dO and Q past the sequence, which weights of 0 would meet
-        if (r >= lim) {
-          mbar_wait(half == 0 ? &g_full[b] : &q_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
-          tile_row_clear<D>((half == 0 ? sG : sQ) + b * TILE, r);
+        if (reads && r >= lim) {
+          mbar_wait(quarter == 0 ? &g_full[b] : &q_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
+          tile_row_clear<D>((quarter == 0 ? sG : sQ) + b * TILE, r);
           fence_proxy_async_smem();
         }
         __syncwarp();
       }
-      float p[64];      // this thread's 64 columns of the P^T row
-      uint32_t pk[32];  // packed bf16 pairs of it, then of dS^T
-      {
-        uint32_t* pr = reinterpret_cast<uint32_t*>(p);
-        __syncwarp();
-        tmem_ld_32x32b_x32(tS + lane_off + cb, *reinterpret_cast<uint32_t(*)[32]>(pr));
-        tmem_ld_32x32b_x32(tS + lane_off + cb + 32, *reinterpret_cast<uint32_t(*)[32]>(pr + 32));
-        tmem_ld_wait();
-      }
+      float p[32];      // this thread's 32 columns of the P^T row
+      uint32_t pk[16];  // packed bf16 pairs of it, then of dS^T
+      __syncwarp();
+      tmem_ld_32x32b_x32(tS + lane_off + cb, *reinterpret_cast<uint32_t(*)[32]>(p));
+      if (!mbar_wait_warp(&l_full[b], (it >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      tmem_ld_wait();
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
+      for (int e = 0; e < 32; e += 4) {
         const int cc = cb + e;
         const float4 n4 = *reinterpret_cast<const float4*>(nl + cc);
         const float2 v0 = __ffma2_rn(make_float2(p[e], p[e + 1]), c2, make_float2(n4.x, n4.y));
         const float2 v1 = __ffma2_rn(make_float2(p[e + 2], p[e + 3]), c2, make_float2(n4.z, n4.w));
-        float2 p0, p1;
-        if (e >= 48) {
-          p0 = exp2_poly2(v0);
-          p1 = exp2_poly2(v1);
-        } else {
-          p0 = make_float2(ex2_approx(v0.x), ex2_approx(v0.y));
-          p1 = make_float2(ex2_approx(v1.x), ex2_approx(v1.y));
-        }
+        float2 p0 = make_float2(ex2_approx(v0.x), ex2_approx(v0.y)), p1 = make_float2(ex2_approx(v1.x), ex2_approx(v1.y));
         if (part) {
           const int lo = diag ? r : 0;       // queries lo .. lim - 1 see this key
           if (cc < lo || cc >= lim) p0.x = 0.f;
@@ -1004,62 +1017,58 @@ __global__ void __launch_bounds__(320, 1)
         pk[(e >> 1) + 1] = pack_bf16x2(p1.x, p1.y);
       }
       __syncwarp();
-      tmem_st_32x32b_x32(tS + lane_off + cb, pk);
+      tmem_st_32x32b_x16(tS + lane_off + cb, pk);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(p_full);
+      warp_arrive(p_full);
       if (!mbar_wait_warp(dp_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
       tc_fence_after();
+      uint32_t dp[32];
+      __syncwarp();
+      tmem_ld_32x32b_x32(tP + lane_off + cb, dp);
+      tmem_ld_wait();
 #pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        uint32_t dp[32];
-        __syncwarp();
-        tmem_ld_32x32b_x32(tP + lane_off + cb + h2 * 32, dp);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e0 = 0; e0 < 32; e0 += 4) {
-          const int e = h2 * 32 + e0, cc = cb + e;
-          const float4 d4 = *reinterpret_cast<const float4*>(nd + cc);
-          const float2 pa = make_float2(p[e], p[e + 1]), pb = make_float2(p[e + 2], p[e + 3]);
-          float2 da = __fmul2_rn(pa, __fadd2_rn(make_float2(__uint_as_float(dp[e0]), __uint_as_float(dp[e0 + 1])), make_float2(d4.x, d4.y)));
-          float2 db = __fmul2_rn(pb, __fadd2_rn(make_float2(__uint_as_float(dp[e0 + 2]), __uint_as_float(dp[e0 + 3])), make_float2(d4.z, d4.w)));
-          if (part) {
-            const int lo = diag ? r : 0;
-            if (cc < lo || cc >= lim) da.x = 0.f;
-            if (cc + 1 < lo || cc + 1 >= lim) da.y = 0.f;
-            if (cc + 2 < lo || cc + 2 >= lim) db.x = 0.f;
-            if (cc + 3 < lo || cc + 3 >= lim) db.y = 0.f;
-          }
-          pk[e >> 1] = pack_bf16x2(da.x, da.y);
-          pk[(e >> 1) + 1] = pack_bf16x2(db.x, db.y);
+      for (int e = 0; e < 32; e += 4) {
+        const int cc = cb + e;
+        const float4 d4 = *reinterpret_cast<const float4*>(nd + cc);
+        float2 da = __fmul2_rn(make_float2(p[e], p[e + 1]), __fadd2_rn(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), make_float2(d4.x, d4.y)));
+        float2 db = __fmul2_rn(make_float2(p[e + 2], p[e + 3]), __fadd2_rn(make_float2(__uint_as_float(dp[e + 2]), __uint_as_float(dp[e + 3])), make_float2(d4.z, d4.w)));
+        if (part) {
+          const int lo = diag ? r : 0;
+          if (cc < lo || cc >= lim) da.x = 0.f;
+          if (cc + 1 < lo || cc + 1 >= lim) da.y = 0.f;
+          if (cc + 2 < lo || cc + 2 >= lim) db.x = 0.f;
+          if (cc + 3 < lo || cc + 3 >= lim) db.y = 0.f;
         }
+        pk[e >> 1] = pack_bf16x2(da.x, da.y);
+        pk[(e >> 1) + 1] = pack_bf16x2(db.x, db.y);
       }
       __syncwarp();
-      tmem_st_32x32b_x32(tP + lane_off + cb, pk);
+      tmem_st_32x32b_x16(tP + lane_off + cb, pk);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(ds_full);
+      warp_arrive(ds_full);
     }
     if (ok && mbar_wait_warp(done, 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
       tc_fence_after();
       const bool mine = row0 + r < un.len;
-      const long long at = ((long long)(un.begin + row0 + r) * a.Hkv + hk) * D + half * (D / 2);
-#pragma unroll 1
+      const long long at = ((long long)(un.begin + row0 + r) * a.Hkv + hk) * D + quarter * (D / 4);
+#pragma unroll
       for (int cc = 0; cc < D / 64; ++cc) {
-        uint32_t o[32];
-        float f[32];
+        uint32_t o[16];
+        float f[16];
         __syncwarp();
-        tmem_ld_32x32b_x32(tDV + lane_off + half * (D / 2) + cc * 32, o);
+        tmem_ld_32x32b_x16(tDV + lane_off + quarter * (D / 4) + cc * 16, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]);
-        if (mine) store_row_bf16_global(a.dv + at + cc * 32, f, 32);
+        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]);
+        if (mine) store_row_bf16_global(a.dv + at + cc * 16, f, 16);
         __syncwarp();
-        tmem_ld_32x32b_x32(tDK + lane_off + half * (D / 2) + cc * 32, o);
+        tmem_ld_32x32b_x16(tDK + lane_off + quarter * (D / 4) + cc * 16, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * a.scale;
-        if (mine) store_row_bf16_global(a.dk + at + cc * 32, f, 32);
+        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]) * a.scale;
+        if (mine) store_row_bf16_global(a.dk + at + cc * 16, f, 16);
       }
     }
   }
@@ -1146,14 +1155,24 @@ std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Ten
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
   a.by_heads = a.G % 2 == 0;
-  const unsigned grid = pk_grid(piece_slots(c.M, a.pc.S, a.by_heads ? 128 : 256), a.by_heads ? a.Hq / 2 : a.Hq);
   auto s = at::cuda::getCurrentCUDAStream();
-  if (c.D == 128) {
-    pk_smem(packed_fwd_kernel<128>, PkFwd<128>::SMEM);
-    packed_fwd_kernel<128><<<grid, 320, PkFwd<128>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, a);
+  auto launch = [&](auto cfg, auto kern, int64_t slots, int64_t heads) {
+    typedef decltype(cfg) Cfg;
+    pk_smem(kern, Cfg::SMEM);
+    kern<<<pk_grid(slots, heads), Cfg::THREADS, Cfg::SMEM, s>>>(c.q.map, c.k.map, c.v.map, a);
+  };
+  // One tile a CTA, two CTAs an SM, where a tile has few keys and no second head shares them: one's start and end lie under the
+  // other's products (10 heads, 65536 rows: 236 instead of 256 us for sequences of 512, 379 instead of 588 for 64; from 1024 on
+  // two tiles that share their keys are as fast or faster).
+  const bool one = !a.by_heads && c.M < 1024 * (int64_t)a.pc.S;
+  if (one) {
+    const int64_t slots = piece_slots(c.M, a.pc.S, 128);
+    if (c.D == 128) launch(PkFwd<128, 1>{}, packed_fwd_kernel<128, 1>, slots, a.Hq);
+    else launch(PkFwd<64, 1>{}, packed_fwd_kernel<64, 1>, slots, a.Hq);
   } else {
-    pk_smem(packed_fwd_kernel<64>, PkFwd<64>::SMEM);
-    packed_fwd_kernel<64><<<grid, 320, PkFwd<64>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, a);
+    const int64_t slots = piece_slots(c.M, a.pc.S, a.by_heads ? 128 : 256), heads = a.by_heads ? a.Hq / 2 : a.Hq;
+    if (c.D == 128) launch(PkFwd<128, 2>{}, packed_fwd_kernel<128, 2>, slots, heads);
+    else launch(PkFwd<64, 2>{}, packed_fwd_kernel<64, 2>, slots, heads);
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {out, lse};
@@ -1183,15 +1202,15 @@ std::vector<at::Tensor> packed_attention_bwd(at::Tensor dout, at::Tensor q, at::
   if (c.D == 128) {
     pk_smem(packed_dq_kernel<128>, PkDq<128>::SMEM);
     pk_smem(packed_dkv_kernel<128>, PkDkv<128>::SMEM);
-    packed_dq_kernel<128><<<gq, 320, PkDq<128>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
+    packed_dq_kernel<128><<<gq, 608, PkDq<128>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
-    packed_dkv_kernel<128><<<gk, 320, PkDkv<128>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
+    packed_dkv_kernel<128><<<gk, 576, PkDkv<128>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
   } else {
     pk_smem(packed_dq_kernel<64>, PkDq<64>::SMEM);
     pk_smem(packed_dkv_kernel<64>, PkDkv<64>::SMEM);
-    packed_dq_kernel<64><<<gq, 320, PkDq<64>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
+    packed_dq_kernel<64><<<gq, 608, PkDq<64>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
-    packed_dkv_kernel<64><<<gk, 320, PkDkv<64>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
+    packed_dkv_kernel<64><<<gk, 576, PkDkv<64>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {dq, dk, dv};
