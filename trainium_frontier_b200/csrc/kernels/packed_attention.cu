@@ -116,6 +116,37 @@ __device__ __forceinline__ void clear_rows(__nv_bfloat16* out, int H, int h0, in
   }
 }
 
+// A warp's 32 rows of 16-byte CHUNKS, from TMEM columns at `from` on, each row times its lane's `by`, rounded and stored
+// through `stage` (shared memory of the warp's own, 16-byte aligned, 32 x 16 x CHUNKS bytes), so
+// that a store covers whole rows.  dst: the first row's, `stride` elements between rows; n: rows that are there.
+// (Rows stored by their own lanes took 4500 of a one-tile CTA's 15000 cycles.)
+template <int CHUNKS>
+__device__ __forceinline__ void store_rows(uint32_t from, float by, uint8_t* stage, __nv_bfloat16* dst, long long stride, int n) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; c += 2) {
+    uint32_t o[16];
+    __syncwarp();
+    tmem_ld_32x32b_x16(from + c * 8, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(o[8 * k + 2 * i]) * by, __uint_as_float(o[8 * k + 2 * i + 1]) * by);
+      *reinterpret_cast<uint4*>(stage + lane * (16 * CHUNKS) + (((c + k) ^ (lane & (CHUNKS - 1) & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int row = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
+    if (row < n)
+      reinterpret_cast<uint4*>(dst + row * stride)[c] = *reinterpret_cast<const uint4*>(stage + row * (16 * CHUNKS) + ((c ^ (row & (CHUNKS - 1) & 7)) << 4));
+  }
+  __syncwarp();
+}
+
 // A row's output by itself, keys one after another in 32 bits: for the rows of a diagonal tile whose masked
 // values hold an infinity or a NaN, which the tensor core would multiply by 0.
 template <int D>
@@ -434,19 +465,11 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
     if (n_t > 0 && ok && mbar_wait_warp(&o_done[t], 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
       tc_fence_after();
       const float inv_l = 1.f / l, lse2 = m_run + log2f(l);
-      __nv_bfloat16* dst = a.out + ((long long)(un.begin + row) * a.Hq + head) * D;
       const bool mine = row < un.len, alone = by_row[t] != 0;
-#pragma unroll 1
-      for (int cc = 0; cc < D / 32; ++cc) {
-        uint32_t o[32];
-        __syncwarp();
-        tmem_ld_32x32b_x32(tO + lane_off + cc * 32, o);
-        tmem_ld_wait();
-        float f[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * inv_l;
-        if (mine && !alone) store_row_bf16_global(dst + cc * 32, f, 32);
-      }
+      const int first = row - lane;      // the warp's first row; Q's tile is free: all products of it are done
+      __nv_bfloat16* dst = a.out + ((long long)(un.begin + first) * a.Hq + head) * D;
+      if (!alone) store_rows<D / 8>(tO + lane_off, inv_l, sQ + t * TILE + q4 * (32 * D * 2), dst, (long long)a.Hq * D, un.len - first);
+      dst += (long long)lane * a.Hq * D;
       if (mine && alone) packed_row<D>(a, un.begin, row, head, lse2, dst);
       if (mine && a.lse) a.lse[(long long)head * a.pc.M + un.begin + row] = lse2 * kLn2;
     }
@@ -738,18 +761,9 @@ __global__ void __launch_bounds__(608, 1)
     }
     if (ok && mbar_wait_warp(done, 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
       tc_fence_after();
-      __nv_bfloat16* dst = a.dq + ((long long)(un.begin + row) * a.Hq + h) * D + quarter * (D / 4);
-#pragma unroll
-      for (int cc = 0; cc < D / 64; ++cc) {
-        uint32_t o[16];
-        float f[16];
-        __syncwarp();
-        tmem_ld_32x32b_x16(tQ + lane_off + quarter * (D / 4) + cc * 16, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]) * a.scale;
-        if (mine) store_row_bf16_global(dst + cc * 16, f, 16);
-      }
+      // Q's tile is free: all products of it are done
+      __nv_bfloat16* dst = a.dq + ((long long)(un.begin + row0 + q4 * 32) * a.Hq + h) * D + quarter * (D / 4);
+      store_rows<D / 32>(tQ + lane_off + quarter * (D / 4), a.scale, sQ + (warp - 2) * (32 * (D / 4) * 2), dst, (long long)a.Hq * D, un.len - row0 - q4 * 32);
     }
   }
   tc_fence_before();
@@ -1051,25 +1065,12 @@ __global__ void __launch_bounds__(576, 1)
     }
     if (ok && mbar_wait_warp(done, 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
       tc_fence_after();
-      const bool mine = row0 + r < un.len;
-      const long long at = ((long long)(un.begin + row0 + r) * a.Hkv + hk) * D + quarter * (D / 4);
-#pragma unroll
-      for (int cc = 0; cc < D / 64; ++cc) {
-        uint32_t o[16];
-        float f[16];
-        __syncwarp();
-        tmem_ld_32x32b_x16(tDV + lane_off + quarter * (D / 4) + cc * 16, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]);
-        if (mine) store_row_bf16_global(a.dv + at + cc * 16, f, 16);
-        __syncwarp();
-        tmem_ld_32x32b_x16(tDK + lane_off + quarter * (D / 4) + cc * 16, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]) * a.scale;
-        if (mine) store_row_bf16_global(a.dk + at + cc * 16, f, 16);
-      }
+      // K's and V's tiles are free: all products of them are done
+      const int first = row0 + q4 * 32, n_rows = un.len - first;
+      const long long at = ((long long)(un.begin + first) * a.Hkv + hk) * D + quarter * (D / 4), stride = (long long)a.Hkv * D;
+      const uint32_t stage = (warp - 2) * (32 * (D / 4) * 2);
+      store_rows<D / 32>(tDV + lane_off + quarter * (D / 4), 1.f, sV + stage, a.dv + at, stride, n_rows);
+      store_rows<D / 32>(tDK + lane_off + quarter * (D / 4), a.scale, sK + stage, a.dk + at, stride, n_rows);
     }
   }
   tc_fence_before();
