@@ -185,6 +185,9 @@ class RunConfig:
     coalesced_swiglu_hidden: int = 0   # forced coalesced-SwiGLU hidden width (multiple of 128); 0 = parameter-matched
     parallel_block: bool = False
     doc_mask: bool = False
+    # doc_mask's full-window layers through packed attention: no [T, T] masks, and causal inside each document (the
+    # dense document mask by itself hides no later token)
+    doc_mask_packed: bool = False
     window_pattern: str = "L"
     short_window_frac: float = 0.5
     out_bigram: bool = False

@@ -17,8 +17,8 @@ value embeddings (``ngram_ve``), depthwise causal conv (``local_conv``), causal 
 token shift (``qk_shift``), per-head output gate (``head_gate``), output pooling of the
 last layers (``out_pool``), input-dependent x0 gate (``x0_gate``), MLP sandwich norm,
 shifted relu^2 (``relu2_tau``), gated / SwiGLU MLP, GQA (``n_kv_heads``), explicit
-attention scale, document masking and sliding-window layers, the output bigram table
-(``out_bigram``).
+attention scale, document masking (``doc_mask``; with ``doc_mask_packed`` causal inside each document, through
+packed attention instead of dense masks) and sliding-window layers, the output bigram table (``out_bigram``).
 
 Hot path: on CUDA with the plain configuration each block is five fused kernels plus
 attention: [mix + norm] -> [QKV GEMM] -> [RoPE + QK-norm + attention] -> [proj GEMM +
@@ -156,7 +156,9 @@ class CausalSelfAttention(nn.Module):
         q = ops.linear(x_q, self.c_q.weight).view(b, t, self.n_head, self.head_dim)
         k = ops.linear(x_k, self.c_k.weight).view(b, t, self.n_kv_heads, self.head_dim)
         v = ops.linear(x_v, self.c_v.weight).view(b, t, self.n_kv_heads, self.head_dim)
-        if self.kv_repeat > 1:
+        packed = isinstance(attn_mask, PackedDocs)
+        # packed attention shares heads by itself; value embeddings have a row for every query head
+        if self.kv_repeat > 1 and not (packed and ve is None and ve_bi is None and ve_tri is None):
             k = k.repeat_interleave(self.kv_repeat, dim=2).contiguous()
             v = v.repeat_interleave(self.kv_repeat, dim=2).contiguous()
         gc = self.gate_channels
@@ -171,8 +173,11 @@ class CausalSelfAttention(nn.Module):
             v = v + g_tri.unsqueeze(-1) * ve_tri.view(b, t, self.n_head, self.head_dim)
         q = ops.rope_norm(q, cos, sin)
         k = ops.rope_norm(k, cos, sin)
-        y = ops.attention(q, k, v, causal=attn_mask is None, scale=self.attn_scale,
-                          attn_mask=None if attn_mask is None else attn_mask[..., :t, :t].to(q.dtype))
+        if packed:
+            y = ops.packed_attention(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), attn_mask.cu_seqlens, self.attn_scale)
+        else:
+            y = ops.attention(q, k, v, causal=attn_mask is None, scale=self.attn_scale,
+                              attn_mask=None if attn_mask is None else attn_mask[..., :t, :t].to(q.dtype))
         y = y.reshape(b, t, c)
         if self.head_gate is not None:
             yh = y.view(b, t, self.n_head, self.head_dim)
@@ -382,6 +387,17 @@ def doc_boundary_mask(idx: torch.Tensor, bos: int = 0) -> torch.Tensor:
     m = torch.zeros(same.shape, dtype=torch.float32, device=idx.device)
     m.masked_fill_(~same, float("-inf"))
     return m[:, None]
+
+
+class PackedDocs:
+    """In the place of an additive mask: the documents of idx [B, T] as sequences that lie behind one another
+    (``ops.packed_attention``), each starting at its BOS or its row's first token.  Their number is read back."""
+
+    def __init__(self, idx: torch.Tensor, bos: int = 0):
+        first = (idx == bos).clone()
+        first[:, 0] = True
+        starts = first.reshape(-1).nonzero()[:, 0]
+        self.cu_seqlens = torch.cat([starts, starts.new_tensor([idx.numel()])]).to(torch.int32)
 
 
 class GPT(nn.Module):
@@ -619,7 +635,8 @@ class GPT(nn.Module):
         cos, sin = self.cos[:, :t], self.sin[:, :t]
         x = ops.embed_norm(idx, self.transformer.wte.weight, dt)
         x0 = x
-        doc_mask = doc_boundary_mask(idx) if self.rc.doc_mask else None
+        docs = PackedDocs(idx) if self.rc.doc_mask and self.rc.doc_mask_packed else None
+        doc_mask = doc_boundary_mask(idx) if self.rc.doc_mask and (docs is None or any(self.layer_is_short)) else None
         ngram_idx = self._ngram_hash_indices(idx) if (len(self.ngram_embeds) or self.engram is not None) else None
         engram_raw = {} if (self.engram is not None and self.engram.share) else None
         pool_from = self.config.n_layer - self.out_pool_lambdas.numel() if self.out_pool_lambdas is not None else 1 << 30
@@ -632,7 +649,9 @@ class GPT(nn.Module):
                     ve_bi = self._ngram_lookup(f"b{i}", ngram_idx[f"b{i}"], dt, engram_raw, idx)
                 if f"t{i}" in self.ngram_embeds:
                     ve_tri = self._ngram_lookup(f"t{i}", ngram_idx[f"t{i}"], dt, engram_raw, idx)
-            if doc_mask is None and not self.layer_is_short[i]:
+            if docs is not None and not self.layer_is_short[i]:
+                attn_mask = docs
+            elif doc_mask is None and not self.layer_is_short[i]:
                 attn_mask = None
             else:
                 static = self.mask_short[:t, :t] if self.layer_is_short[i] else torch.zeros(t, t, device=idx.device)
