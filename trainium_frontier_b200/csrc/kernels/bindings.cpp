@@ -90,7 +90,7 @@ torch::Tensor tree_attention(torch::Tensor q, torch::Tensor kc, torch::Tensor vc
                              c10::optional<torch::Tensor> vs, torch::Tensor err);
 std::vector<torch::Tensor> verify_tree(torch::Tensor tokens, torch::Tensor parents, torch::Tensor p, c10::optional<torch::Tensor> q,
                                        torch::Tensor u);
-std::vector<torch::Tensor> packed_attention_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu, double scale,
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> packed_attention_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu, double scale,
                                                 bool want_lse, torch::Tensor err);
 std::vector<torch::Tensor> packed_attention_bwd(torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v,
                                                 torch::Tensor out, torch::Tensor lse, torch::Tensor cu, double scale, torch::Tensor err);
@@ -98,8 +98,9 @@ void paged_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor kp, torch
                        c10::optional<torch::Tensor> cu, c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs);
 torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor vp, torch::Tensor table, torch::Tensor lens, double scale,
                               c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs, torch::Tensor err);
-std::vector<torch::Tensor> token_logprobs(torch::Tensor z, torch::Tensor tok, int64_t top, bool stats);
-torch::Tensor token_logprobs_grad(torch::Tensor z, torch::Tensor tok, torch::Tensor stat, c10::optional<torch::Tensor> g,
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> token_logprobs(
+    torch::Tensor logits, torch::Tensor tokens, int64_t top, bool stats);
+torch::Tensor token_logprobs_grad(torch::Tensor logits, torch::Tensor tokens, torch::Tensor stat, c10::optional<torch::Tensor> g,
                                   c10::optional<torch::Tensor> h);
 }  // namespace tfb
 

@@ -30,8 +30,13 @@
 // order that changes from run to run).  Here each gradient is a sum in TMEM, in order, and rounded once.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/ops/clone.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
+
+#include <atomic>
+#include <tuple>
+#include <vector>
 
 #include "attention_tiles.cuh"
 #include "packed.cuh"
@@ -1082,27 +1087,42 @@ __global__ void __launch_bounds__(576, 1)
 }
 
 // ------------------------------------------------------------------------------ host
-template <typename K>
-static void pk_smem(K kern, size_t bytes) {
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+// A kernel's shared memory, said once a device: the call takes longer than the launch.
+template <auto KERN>
+static void pk_smem(size_t bytes, int dev) {
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
 }
 
+template <auto KERN>
+struct PkKern {
+  static constexpr auto value = KERN;
+};
+
 struct PkView {
+  at::Tensor t;                  // a copy where the rows cannot be read in place
   const __nv_bfloat16* p;
   long long r, h;
   CUtensorMap map;
 };
 
-static PkView pk_view(const at::Tensor& t, const char* name, const at::Tensor& q, int64_t H) {
-  TORCH_CHECK(t.is_cuda() && t.device() == q.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(0) == q.size(0) &&
-                  t.size(1) == H && t.size(2) == q.size(2), name, ": bfloat16 [M, H, D] of q's M and D on its device");
-  const int64_t M = t.size(0), D = t.size(2);
+static PkView pk_view(const at::Tensor& given, const char* name, const at::Tensor& q, int64_t H) {
+  TORCH_CHECK(given.is_cuda() && given.device() == q.device() && given.scalar_type() == at::kBFloat16 && given.dim() == 3 &&
+                  given.size(0) == q.size(0) && given.size(1) == H && given.size(2) == q.size(2),
+              name, ": bfloat16 [M, H, D] of q's M and D on its device");
+  const int64_t M = given.size(0), D = given.size(2);
   PkView v{};
-  v.p = reinterpret_cast<const __nv_bfloat16*>(t.data_ptr());
-  v.h = H > 1 ? t.stride(1) : D;
-  v.r = M > 1 ? t.stride(0) : H * D;
-  TORCH_CHECK(t.stride(2) == 1 && v.r > 0 && v.h > 0 && v.r % 8 == 0 && v.h % 8 == 0 && (reinterpret_cast<uintptr_t>(v.p) & 15) == 0, name,
-              ": unit inner stride, 16-byte aligned rows, no broadcast dimension");
+  auto take = [&](const at::Tensor& t) {
+    v.t = t;
+    v.p = reinterpret_cast<const __nv_bfloat16*>(t.data_ptr());
+    v.h = H > 1 ? t.stride(1) : D;
+    v.r = M > 1 ? t.stride(0) : H * D;
+    return t.stride(2) == 1 && v.r > 0 && v.h > 0 && v.r % 8 == 0 && v.h % 8 == 0 && (reinterpret_cast<uintptr_t>(v.p) & 15) == 0;
+  };
+  if (!take(given)) take(given.clone(at::MemoryFormat::Contiguous));   // broadcast, misaligned or strided inside
   if (M > 0) v.map = make_tmap_bf16(v.p, D, M, v.r, 64, 128, H, v.h);
   return v;
 }
@@ -1144,23 +1164,25 @@ static unsigned pk_grid(long long slots, long long heads) {
   return (unsigned)(slots * heads);
 }
 
-// {out [M, Hq, D], lse [Hq, M] (empty unless asked for)}
-std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu, double scale, bool want_lse,
+// (out [M, Hq, D], lse [Hq, M] if asked for)
+std::tuple<at::Tensor, c10::optional<at::Tensor>> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu, double scale, bool want_lse,
                                              at::Tensor err) {
   PkCall c = pk_check(q, k, v, cu, scale, err);
   c10::cuda::CUDAGuard guard(q.device());
   PkArgs& a = c.a;
   auto out = at::empty({c.M, a.Hq, c.D}, q.options());
-  auto lse = at::empty({want_lse ? a.Hq : 0, c.M}, q.options().dtype(at::kFloat));
+  c10::optional<at::Tensor> lse;
+  if (want_lse) lse = at::empty({a.Hq, c.M}, q.options().dtype(at::kFloat));
   if (c.M == 0) return {out, lse};
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
-  a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  a.lse = want_lse ? lse->data_ptr<float>() : nullptr;
   a.by_heads = a.G % 2 == 0;
   auto s = at::cuda::getCurrentCUDAStream();
   auto launch = [&](auto cfg, auto kern, int64_t slots, int64_t heads) {
     typedef decltype(cfg) Cfg;
-    pk_smem(kern, Cfg::SMEM);
-    kern<<<pk_grid(slots, heads), Cfg::THREADS, Cfg::SMEM, s>>>(c.q.map, c.k.map, c.v.map, a);
+    constexpr auto KERN = decltype(kern)::value;
+    pk_smem<KERN>(Cfg::SMEM, q.get_device());
+    KERN<<<pk_grid(slots, heads), Cfg::THREADS, Cfg::SMEM, s>>>(c.q.map, c.k.map, c.v.map, a);
   };
   // One tile a CTA, two CTAs an SM, where a tile has few keys and no second head shares them: one's start and end lie under the
   // other's products (10 heads, 65536 rows: 236 instead of 256 us for sequences of 512, 379 instead of 588 for 64; from 1024 on
@@ -1168,12 +1190,12 @@ std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Ten
   const bool one = !a.by_heads && c.M < 1024 * (int64_t)a.pc.S;
   if (one) {
     const int64_t slots = piece_slots(c.M, a.pc.S, 128);
-    if (c.D == 128) launch(PkFwd<128, 1>{}, packed_fwd_kernel<128, 1>, slots, a.Hq);
-    else launch(PkFwd<64, 1>{}, packed_fwd_kernel<64, 1>, slots, a.Hq);
+    if (c.D == 128) launch(PkFwd<128, 1>{}, PkKern<packed_fwd_kernel<128, 1>>{}, slots, a.Hq);
+    else launch(PkFwd<64, 1>{}, PkKern<packed_fwd_kernel<64, 1>>{}, slots, a.Hq);
   } else {
     const int64_t slots = piece_slots(c.M, a.pc.S, a.by_heads ? 128 : 256), heads = a.by_heads ? a.Hq / 2 : a.Hq;
-    if (c.D == 128) launch(PkFwd<128, 2>{}, packed_fwd_kernel<128, 2>, slots, heads);
-    else launch(PkFwd<64, 2>{}, packed_fwd_kernel<64, 2>, slots, heads);
+    if (c.D == 128) launch(PkFwd<128, 2>{}, PkKern<packed_fwd_kernel<128, 2>>{}, slots, heads);
+    else launch(PkFwd<64, 2>{}, PkKern<packed_fwd_kernel<64, 2>>{}, slots, heads);
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {out, lse};
@@ -1201,14 +1223,14 @@ std::vector<at::Tensor> packed_attention_bwd(at::Tensor dout, at::Tensor q, at::
   const unsigned gq = pk_grid(slots, a.Hq), gk = pk_grid(slots, a.Hkv);
   auto s = at::cuda::getCurrentCUDAStream();
   if (c.D == 128) {
-    pk_smem(packed_dq_kernel<128>, PkDq<128>::SMEM);
-    pk_smem(packed_dkv_kernel<128>, PkDkv<128>::SMEM);
+    pk_smem<packed_dq_kernel<128>>(PkDq<128>::SMEM, q.get_device());
+    pk_smem<packed_dkv_kernel<128>>(PkDkv<128>::SMEM, q.get_device());
     packed_dq_kernel<128><<<gq, 608, PkDq<128>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     packed_dkv_kernel<128><<<gk, 576, PkDkv<128>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
   } else {
-    pk_smem(packed_dq_kernel<64>, PkDq<64>::SMEM);
-    pk_smem(packed_dkv_kernel<64>, PkDkv<64>::SMEM);
+    pk_smem<packed_dq_kernel<64>>(PkDq<64>::SMEM, q.get_device());
+    pk_smem<packed_dkv_kernel<64>>(PkDkv<64>::SMEM, q.get_device());
     packed_dq_kernel<64><<<gq, 608, PkDq<64>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     packed_dkv_kernel<64><<<gk, 576, PkDkv<64>::SMEM, s>>>(c.q.map, c.k.map, c.v.map, g.map, a);

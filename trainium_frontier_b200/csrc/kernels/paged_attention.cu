@@ -20,6 +20,8 @@
 // scales are.
 #include <ATen/ops/empty.h>
 
+#include <atomic>
+
 #include "attention_tiles.cuh"
 #include "warp_mma.cuh"
 
@@ -524,15 +526,27 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const float
   out[(long long)blockIdx.x * D + threadIdx.x] = __float2bfloat16_rn(y);
 }
 
+template <int D, bool QUANT, int NT>
+static void pa_run(const PaArgs& a, const KvView& c, unsigned grid, cudaStream_t s, bool on) {
+  if (!on) return;
+  constexpr uint32_t smem = PaCfg<D, QUANT, NT>::SMEM;
+  // said once a device: the call takes longer than the launch
+  static std::atomic<uint64_t> done{0};
+  int dev;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(done.load(std::memory_order_relaxed) & bit)) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(paged_attention_kernel<D, QUANT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  paged_attention_kernel<D, QUANT, NT><<<grid, 32 * kPaWarps, smem, s>>>(a, c);
+}
+
 template <int D, bool QUANT>
 static void pa_launch(PaArgs& a, const KvView& c, int64_t B, cudaStream_t s) {
   const unsigned grid = (unsigned)(B * a.splits * a.Hkv * a.rg);
-  auto launch = [&](auto kern, uint32_t smem) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kern<<<grid, 32 * kPaWarps, smem, s>>>(a, c);
-  };
-  if (a.G <= 8) launch(paged_attention_kernel<D, QUANT, 1>, PaCfg<D, QUANT, 1>::SMEM);
-  else launch(paged_attention_kernel<D, QUANT, 2>, PaCfg<D, QUANT, 2>::SMEM);
+  pa_run<D, QUANT, 1>(a, c, grid, s, a.G <= 8);
+  pa_run<D, QUANT, 2>(a, c, grid, s, a.G > 8);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (a.splits == 1) return;
   cudaLaunchConfig_t cfg = {};

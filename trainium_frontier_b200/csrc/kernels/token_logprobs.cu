@@ -21,6 +21,9 @@
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <tuple>
+#include <vector>
+
 #include "attention_tiles.cuh"
 
 namespace tfb {
@@ -478,34 +481,45 @@ __global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const LpGradAr
 }
 
 struct LpShape {
+  at::Tensor z, tok;             // [N, V] and packed [N]
   bool bf, vec;
   int64_t N, V, ld;
 };
 
-static LpShape lp_check(const at::Tensor& z, const at::Tensor& tok) {
-  TORCH_CHECK(z.is_cuda() && z.dim() == 2 && (z.scalar_type() == at::kFloat || z.scalar_type() == at::kBFloat16),
+static LpShape lp_check(const at::Tensor& logits, const at::Tensor& tokens, int64_t top) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() >= 1 && (logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16),
               "logits: float32 or bfloat16 [..., V]");
   LpShape s{};
-  s.bf = z.scalar_type() == at::kBFloat16;
-  s.N = z.size(0); s.V = z.size(1);
+  s.bf = logits.scalar_type() == at::kBFloat16;
+  s.V = logits.size(-1);
   TORCH_CHECK(s.V >= 1 && s.V <= (1 << 30), "vocabulary of 1 .. 2^30 tokens");
-  TORCH_CHECK(s.V == 1 || z.stride(1) == 1, "logits: unit inner stride");
-  s.ld = z.stride(0);
+  TORCH_CHECK(s.V == 1 || logits.stride(-1) == 1, "logits: unit inner stride");
+  TORCH_CHECK((tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt) && tokens.device() == logits.device() &&
+                  tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+              "tokens: int64 or int32, one for each row of the logits, on their device");
+  TORCH_CHECK(top >= 0 && top <= kLpMaxTop && top <= s.V, "top: 0 .. 32 alternatives, at most the vocabulary");
+  s.N = tokens.numel();
   TORCH_CHECK(s.N <= (1 << 27), "at most 2^27 rows");
-  TORCH_CHECK((tok.scalar_type() == at::kLong || tok.scalar_type() == at::kInt) && tok.device() == z.device() && tok.dim() == 1 &&
-                  tok.size(0) == s.N && tok.is_contiguous(), "tokens: int64 or int32, one for each row of the logits, on their device");
-  s.vec = (reinterpret_cast<uintptr_t>(z.data_ptr()) & 15) == 0 && (s.N == 1 || s.ld * z.element_size() % 16 == 0);
+  s.z = logits.dim() == 2 ? logits : logits.reshape({s.N, s.V});
+  s.tok = tokens.contiguous();
+  s.ld = s.z.stride(0);
+  s.vec = (reinterpret_cast<uintptr_t>(s.z.data_ptr()) & 15) == 0 && (s.N <= 1 || s.ld * s.z.element_size() % 16 == 0);
   return s;
 }
 
-std::vector<at::Tensor> token_logprobs(at::Tensor z, at::Tensor tok, int64_t top, bool stats) {
-  const LpShape s = lp_check(z, tok);
-  TORCH_CHECK(top >= 0 && top <= kLpMaxTop && top <= s.V, "top: 0 .. 32 alternatives, at most the vocabulary");
+// (log probabilities, entropies, alternatives and their log probabilities, what the gradient needs or nothing)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, c10::optional<at::Tensor>> token_logprobs(at::Tensor logits, at::Tensor tokens,
+                                                                                                     int64_t top, bool stats) {
+  const LpShape s = lp_check(logits, tokens, top);
+  const at::Tensor &z = s.z, &tok = s.tok;
   c10::cuda::CUDAGuard guard(z.device());
   const auto f32 = z.options().dtype(at::kFloat);
-  auto lp = at::empty({s.N}, f32), ent = at::empty({s.N}, f32), top_lp = at::empty({s.N, top}, f32);
-  auto top_tok = at::empty({s.N, top}, z.options().dtype(at::kInt));
-  auto stat = at::empty({stats ? s.N : 0, 3}, f32);
+  auto lp = at::empty(tokens.sizes(), f32), ent = at::empty(tokens.sizes(), f32);
+  std::vector<int64_t> wide(tokens.sizes().begin(), tokens.sizes().end());
+  wide.push_back(top);
+  auto top_lp = at::empty(wide, f32), top_tok = at::empty(wide, z.options().dtype(at::kInt));
+  c10::optional<at::Tensor> stat;
+  if (stats) stat = at::empty({s.N, 3}, f32);
   if (s.N == 0) return {lp, ent, top_tok, top_lp, stat};
   LpArgs a{};
   a.z = z.data_ptr(); a.ld = s.ld; a.tok = tok.data_ptr(); a.tok64 = tok.scalar_type() == at::kLong;
@@ -517,7 +531,7 @@ std::vector<at::Tensor> token_logprobs(at::Tensor z, at::Tensor tok, int64_t top
   while (W < kLpWarps && ((s.N * W < 192 * sms && 32 * W * step <= s.V) || (s.N * W < 16 * sms && 2 * W * step < s.V))) W *= 2;
   while (W == kLpWarps && C < 8 && s.N * W * C < 16 * sms && 2 * W * C * step < s.V) C *= 2;
   a.W = W; a.C = C;
-  a.lp = lp.data_ptr<float>(); a.ent = ent.data_ptr<float>(); a.stat = stats ? stat.data_ptr<float>() : nullptr;
+  a.lp = lp.data_ptr<float>(); a.ent = ent.data_ptr<float>(); a.stat = stats ? stat->data_ptr<float>() : nullptr;
   a.top_tok = top_tok.data_ptr<int>(); a.top_lp = top_lp.data_ptr<float>();
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -535,17 +549,20 @@ std::vector<at::Tensor> token_logprobs(at::Tensor z, at::Tensor tok, int64_t top
   return {lp, ent, top_tok, top_lp, stat};
 }
 
-// dz [N, V], a view of rows padded to 16 bytes.
-at::Tensor token_logprobs_grad(at::Tensor z, at::Tensor tok, at::Tensor stat, c10::optional<at::Tensor> g, c10::optional<at::Tensor> h) {
-  const LpShape s = lp_check(z, tok);
+// dz [..., V], a view of rows padded to 16 bytes.
+at::Tensor token_logprobs_grad(at::Tensor logits, at::Tensor tokens, at::Tensor stat, c10::optional<at::Tensor> g, c10::optional<at::Tensor> h) {
+  const LpShape s = lp_check(logits, tokens, 0);
+  const at::Tensor &z = s.z, &tok = s.tok;
   TORCH_CHECK(stat.scalar_type() == at::kFloat && stat.device() == z.device() && stat.is_contiguous() && stat.numel() == 3 * s.N, "stat: float32 [N, 3]");
   for (const auto* t : {&g, &h})
     TORCH_CHECK(!t->has_value() || ((*t)->scalar_type() == at::kFloat && (*t)->device() == z.device() && (*t)->is_contiguous() &&
-                                    (*t)->numel() == s.N), "gradients: contiguous float32 [N]");
+                                    (*t)->numel() == s.N), "gradients: contiguous float32, one for each row");
   c10::cuda::CUDAGuard guard(z.device());
   const int64_t pad = s.bf ? 8 : 4, ldo = (s.V + pad - 1) / pad * pad;
-  auto dz = at::empty({s.N, ldo}, z.options());
-  if (s.N == 0) return dz.narrow(1, 0, s.V);
+  std::vector<int64_t> wide(tokens.sizes().begin(), tokens.sizes().end());
+  wide.push_back(ldo);
+  auto dz = at::empty(wide, z.options());
+  if (s.N == 0) return dz.narrow(-1, 0, s.V);
   LpGradArgs a{};
   a.z = z.data_ptr(); a.ld = s.ld; a.ldo = ldo; a.dz = dz.data_ptr(); a.tok = tok.data_ptr(); a.tok64 = tok.scalar_type() == at::kLong;
   a.V = (int)s.V;
@@ -559,7 +576,7 @@ at::Tensor token_logprobs_grad(at::Tensor z, at::Tensor tok, at::Tensor stat, c1
                     : (s.vec ? token_logprobs_grad_kernel<false, true> : token_logprobs_grad_kernel<false, false>);
   kern<<<(unsigned)(s.N * a.chunks), 256, 0, at::cuda::getCurrentCUDAStream()>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return dz.narrow(1, 0, s.V);
+  return dz.narrow(-1, 0, s.V);
 }
 
 }  // namespace tfb

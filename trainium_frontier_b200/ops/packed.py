@@ -22,19 +22,9 @@ from ._ext import C, err_word
 from .speculative import _check, check_cache, check_ints, check_scales_written
 
 
-def _readable(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy where its rows cannot be read in place (broadcast, misaligned, strided inside)."""
-    if t.dim() != 3 or t.dtype != torch.bfloat16:
-        return t   # refused at the launch
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
-        n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:2], t.stride()[:2]))
-    return t if ok else t.contiguous()
-
-
 class PackedAttnFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, scale):
-        q, k, v = _readable(q), _readable(k), _readable(v)
         out, lse = C().packed_attention_fwd(q, k, v, cu_seqlens, scale, True, err_word(q.device))
         ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
         ctx.scale = scale
@@ -44,7 +34,7 @@ class PackedAttnFn(Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
-        dq, dk, dv = C().packed_attention_bwd(_readable(dout), q, k, v, out, lse, cu_seqlens, ctx.scale, err_word(q.device))
+        dq, dk, dv = C().packed_attention_bwd(dout, q, k, v, out, lse, cu_seqlens, ctx.scale, err_word(q.device))
         return dq, dk, dv, None, None
 
 
@@ -56,7 +46,6 @@ def packed_attention(q, k, v, cu_seqlens, scale: float):
         q, scale = q * 0, 1.0
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return PackedAttnFn.apply(q, k, v, cu_seqlens, scale)
-    q, k, v = _readable(q), _readable(k), _readable(v)
     return C().packed_attention_fwd(q, k, v, cu_seqlens, scale, False, err_word(q.device))[0]
 
 

@@ -32,17 +32,14 @@ class TokenLogprobsFn(Function):
 
 
 def token_logprobs(logits, tokens, top: int):
-    shape, V = check_logprobs(logits, tokens, top)
-    z, t = logits.reshape(-1, V), tokens.reshape(-1).contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        lp, ent, tok, top_lp = TokenLogprobsFn.apply(z, t, top)
-    else:
-        lp, ent, tok, top_lp, _ = C().token_logprobs(z, t, top, False)
-    return lp.view(shape), ent.view(shape), tok.view(*shape, top), top_lp.view(*shape, top)
+        return TokenLogprobsFn.apply(logits, tokens, top)
+    return C().token_logprobs(logits, tokens, top, False)[:4]
 
 
 def check_logprobs(logits, tokens, top: int):
-    """(shape of the tokens, vocabulary), or the reason why the arguments do not fit."""
+    """(shape of the tokens, vocabulary), or the reason why the arguments do not fit (the CPU oracle's; the kernel's call
+    makes the same checks)."""
     _check(logits.dim() >= 1 and logits.dtype in (torch.float32, torch.bfloat16), "logits: float32 or bfloat16 [..., V]")
     shape, V = logits.shape[:-1], logits.shape[-1]
     _check(1 <= V <= 1 << 30, "vocabulary of 1 .. 2^30 tokens")
