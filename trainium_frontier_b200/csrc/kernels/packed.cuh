@@ -42,11 +42,26 @@ struct PieceUnit {
 // What slot `slot` of the units of U rows is (warp-collective).
 template <int U>
 __device__ __forceinline__ PieceUnit piece_unit(const Pieces& p, int slot) {
-  const int k = last_piece(p.S + 2, slot, [&](int i) { return (long long)p.begin(i) / U + i; });
+  // as last_piece; the last step's probes hold the piece's begin and the next one's, which is its end
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = p.S + 1, begin = -1, end = -1;
+  while (lo < hi) {
+    const int step = (hi - lo + 32) / 32, i = lo + lane * step;
+    const int at = i <= hi ? p.begin(i) : 0;
+    const unsigned hit = __ballot_sync(0xffffffffu, i <= hi && (lane == 0 || (long long)at / U + i <= slot));
+    const int top = 31 - __clz(hit);
+    begin = __shfl_sync(0xffffffffu, at, top);
+    end = __shfl_sync(0xffffffffu, at, (top + 1) & 31);
+    if (step > 1 || top == 31 || lo + top + 1 > hi) end = -1;   // not probed
+    lo += top * step;
+    hi = min(hi, lo + step - 1);
+  }
+  const int k = lo;
   PieceUnit u;
   u.piece = k;
-  u.begin = p.begin(k);
-  u.len = p.end(k) - u.begin;
+  u.begin = begin;
+  if (end < 0) end = p.end(k);
+  u.len = max(end, begin) - begin;
   u.unit = slot - (u.begin / U + k);
   if (u.unit < 0 || (long long)u.unit * U >= u.len) u.unit = -1;
   return u;

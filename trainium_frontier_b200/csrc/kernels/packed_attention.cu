@@ -209,7 +209,8 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
   uint64_t* s_full = bars + 1 + 2 * NS;  // [2]
   uint64_t* p_full = s_full + 2;         // [2]
   uint64_t* o_done = p_full + 2;         // [2]
-  uint64_t* drain = o_done + 2;
+  uint64_t* looked = o_done + 2;         // [2] by_row is what it will be
+  uint64_t* drain = looked + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* by_row = abort_flag + 1;               // [2] the tile's rows are computed one by one
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
+      mbar_init(&looked[t], 4);
       by_row[t] = 0;
     }
     mbar_init(drain, 1);
@@ -400,19 +402,21 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
         }
         tmem_ld_wait();
       }
-      if (j == n_t - 1) {  // diagonal tile: keys after this query row are masked, those past the sequence among them
+      const bool diag = j == n_t - 1;
+      if (diag) {  // keys after this query row are masked, those past the sequence among them
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i > r) x[i] = -INFINITY;
-        // masked rows of V: past the sequence (another's) cleared, the sequence's own looked over
-        if (!mbar_wait_warp(&kv_full[(2 * j + 1) % NS], ((2 * j + 1) / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
-        uint8_t* v = sKV + ((2 * j + 1) % NS) * TILE;
+        for (int cc = 0; cc < 4; ++cc)
+          if (cc >= q4)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (cc * 32 + i > r) x[cc * 32 + i] = -INFINITY;
+        // rows of V past the sequence (another's) are cleared
         if (j * 128 + r >= un.len) {
-          tile_row_clear<D>(v, r);
+          mbar_wait(&kv_full[(2 * j + 1) % NS], ((2 * j + 1) / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
+          tile_row_clear<D>(sKV + ((2 * j + 1) % NS) * TILE, r);
           fence_proxy_async_smem();
-        } else if (tile_row_bad<D>(v, r)) {
-          by_row[t] = 1;
         }
+        __syncwarp();
       }
       // four independent max chains, two new elements per three-input max
       float mx4[4] = {x[0], x[1], x[2], x[3]};
@@ -466,8 +470,16 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&p_full[t]);
+      // its own rows of V that some queries do not see are looked over, while the product runs (nothing is loaded over a
+      // tile's last V)
+      if (diag && j * 128 + r < un.len) {
+        mbar_wait(&kv_full[(2 * j + 1) % NS], ((2 * j + 1) / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
+        if (tile_row_bad<D>(sKV + ((2 * j + 1) % NS) * TILE, r)) by_row[t] = 1;
+      }
+      if (diag) warp_arrive(&looked[t]);
     }
-    if (n_t > 0 && ok && mbar_wait_warp(&o_done[t], 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
+    if (n_t > 0 && ok && mbar_wait_warp(&o_done[t], 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE) &&
+        mbar_wait_warp(&looked[t], 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
       tc_fence_after();
       const float inv_l = 1.f / l, lse2 = m_run + log2f(l);
       const bool mine = row < un.len, alone = by_row[t] != 0;
