@@ -510,7 +510,7 @@ template <int D>
 struct PkDq {
   static constexpr uint32_t TILE = 128u * D * 2u;
   static constexpr int NK = D == 128 ? 3 : 5, NV = D == 128 ? 2 : 4, NS = NK + NV;   // rings of K (held until dQ has read it) and V
-  static constexpr size_t SMEM = 1024 + (2 + NS) * TILE + 1024 + 32 * 8 + 64;
+  static constexpr size_t SMEM = 1024 + (2 + NS) * TILE + 512 + 32 * 8 + 64;
 };
 
 template <int D>
@@ -527,8 +527,8 @@ __global__ void __launch_bounds__(608, 1)
   uint8_t* sQ = smem;
   uint8_t* sG = sQ + TILE;
   uint8_t* sKV = sG + TILE;
-  float* sD = reinterpret_cast<float*>(sKV + NS * TILE);   // [2][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sD + 256);
+  float* sD = reinterpret_cast<float*>(sKV + NS * TILE);   // [128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sD + 128);
   uint64_t* bar_q = bars + 0;
   uint64_t* kv_full = bars + 1;          // [NK + NV]
   uint64_t* kv_empty = bars + 1 + NS;    // [NK + NV]
@@ -704,25 +704,37 @@ __global__ void __launch_bounds__(608, 1)
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
     const bool mine = row < un.len;
     const long long at = (long long)h * a.pc.M + un.begin + row;
-    // D_i = dO_i . o_i, half of the columns a thread of the first two quarters; kept for the other kernel
-    float dsum = 0.f;
-    if (mine && quarter < 2) {
-      const uint4* g = reinterpret_cast<const uint4*>(a.dout + (long long)(un.begin + row) * a.gr + h * a.gh + quarter * (D / 2));
-      const uint4* o = reinterpret_cast<const uint4*>(a.o + ((long long)(un.begin + row) * a.Hq + h) * D + quarter * (D / 2));
+    // D_i = dO_i . o_i, kept for the other kernel: eight rows a warp, 16-byte loads of whole rows.  (A row a thread took 9000
+    // cycles, longer than three tiles of keys.)
+    {
+      constexpr int L = D / 8;           // lanes a row
+      const int w8 = (warp - 2) * 8;
+      uint4 x[8 * L / 32], y[8 * L / 32];
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint4 x = g[i], y = o[i];
-        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          dsum += __uint_as_float(xw[w] << 16) * __uint_as_float(yw[w] << 16);
-          dsum += __uint_as_float(xw[w] & 0xffff0000u) * __uint_as_float(yw[w] & 0xffff0000u);
+      for (int i = 0; i < 8 * L / 32; ++i) {
+        const int rr = row0 + w8 + i * (32 / L) + lane / L;
+        x[i] = y[i] = make_uint4(0, 0, 0, 0);
+        if (rr < un.len) {
+          x[i] = reinterpret_cast<const uint4*>(a.dout + (long long)(un.begin + rr) * a.gr + h * a.gh)[lane % L];
+          y[i] = reinterpret_cast<const uint4*>(a.o + ((long long)(un.begin + rr) * a.Hq + h) * D)[lane % L];
         }
       }
+#pragma unroll
+      for (int i = 0; i < 8 * L / 32; ++i) {
+        const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, yw[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+        float d = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          d += __uint_as_float(xw[w] << 16) * __uint_as_float(yw[w] << 16);
+          d += __uint_as_float(xw[w] & 0xffff0000u) * __uint_as_float(yw[w] & 0xffff0000u);
+        }
+#pragma unroll
+        for (int k = L / 2; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
+        if (lane % L == 0) sD[w8 + i * (32 / L) + lane / L] = d;
+      }
     }
-    if (quarter < 2) sD[quarter * 128 + r] = dsum;
     named_bar_sync(1, 512);              // no wait comes before it: all 512 threads arrive
-    dsum = sD[r] + sD[128 + r];
+    const float dsum = sD[r];
     if (mine && quarter == 0) a.dvec[at] = dsum;
     const float nlse = mine ? -a.lse[at] * kLog2e : -INFINITY;
     const float2 c2 = make_float2(a.scale_log2, a.scale_log2), nl2 = make_float2(nlse, nlse), nd2 = make_float2(-dsum, -dsum);
@@ -1054,25 +1066,28 @@ __global__ void __launch_bounds__(576, 1)
       warp_arrive(p_full);
       if (!mbar_wait_warp(dp_full, it & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
       tc_fence_after();
-      uint32_t dp[32];
-      __syncwarp();
-      tmem_ld_32x32b_x32(tP + lane_off + cb, dp);
-      tmem_ld_wait();
 #pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        const int cc = cb + e;
-        const float4 d4 = *reinterpret_cast<const float4*>(nd + cc);
-        float2 da = __fmul2_rn(make_float2(p[e], p[e + 1]), __fadd2_rn(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), make_float2(d4.x, d4.y)));
-        float2 db = __fmul2_rn(make_float2(p[e + 2], p[e + 3]), __fadd2_rn(make_float2(__uint_as_float(dp[e + 2]), __uint_as_float(dp[e + 3])), make_float2(d4.z, d4.w)));
-        if (part) {
-          const int lo = diag ? r : 0;
-          if (cc < lo || cc >= lim) da.x = 0.f;
-          if (cc + 1 < lo || cc + 1 >= lim) da.y = 0.f;
-          if (cc + 2 < lo || cc + 2 >= lim) db.x = 0.f;
-          if (cc + 3 < lo || cc + 3 >= lim) db.y = 0.f;
+      for (int h2 = 0; h2 < 2; ++h2) {       // (all 32 at once: registers ran out)
+        uint32_t dp[16];
+        __syncwarp();
+        tmem_ld_32x32b_x16(tP + lane_off + cb + h2 * 16, dp);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e0 = 0; e0 < 16; e0 += 4) {
+          const int e = h2 * 16 + e0, cc = cb + e;
+          const float4 d4 = *reinterpret_cast<const float4*>(nd + cc);
+          float2 da = __fmul2_rn(make_float2(p[e], p[e + 1]), __fadd2_rn(make_float2(__uint_as_float(dp[e0]), __uint_as_float(dp[e0 + 1])), make_float2(d4.x, d4.y)));
+          float2 db = __fmul2_rn(make_float2(p[e + 2], p[e + 3]), __fadd2_rn(make_float2(__uint_as_float(dp[e0 + 2]), __uint_as_float(dp[e0 + 3])), make_float2(d4.z, d4.w)));
+          if (part) {
+            const int lo = diag ? r : 0;
+            if (cc < lo || cc >= lim) da.x = 0.f;
+            if (cc + 1 < lo || cc + 1 >= lim) da.y = 0.f;
+            if (cc + 2 < lo || cc + 2 >= lim) db.x = 0.f;
+            if (cc + 3 < lo || cc + 3 >= lim) db.y = 0.f;
+          }
+          pk[e >> 1] = pack_bf16x2(da.x, da.y);
+          pk[(e >> 1) + 1] = pack_bf16x2(db.x, db.y);
         }
-        pk[e >> 1] = pack_bf16x2(da.x, da.y);
-        pk[(e >> 1) + 1] = pack_bf16x2(db.x, db.y);
       }
       __syncwarp();
       tmem_st_32x32b_x16(tP + lane_off + cb, pk);
