@@ -171,9 +171,39 @@ def test_packed_attention_refuses(device):
     for args in bad:
         with pytest.raises(RuntimeError):
             ops.packed_attention(*args)
-    for scale in (math.nan, math.inf):
+    for scale in (math.nan, math.inf, -math.inf, 1e39, -1e39, 1e-60):
         with pytest.raises(RuntimeError):
             ops.packed_attention(q, k, v, cu, scale)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_packed_attention_any_strides(device):
+    """Inputs whose rows are not 16-byte aligned or lie in another order."""
+    M, H, D = 150, 2, 64
+    g = torch.Generator().manual_seed(13)
+    cu = torch.tensor([0, 100, 150], dtype=torch.int32, device=device)
+    odd = torch.randn(M, H * D + 3, generator=g).to(BF16).to(device)[:, 3:].unflatten(-1, (H, D))
+    turned = torch.randn(D, H, M, generator=g).to(BF16).to(device).permute(2, 1, 0)
+    heads = torch.randn(H, M, D, generator=g).to(BF16).to(device).transpose(0, 1)
+    do = torch.randn(H, M, D, generator=g).to(BF16).to(device).transpose(0, 1)
+    leaves = [t.detach().requires_grad_() for t in (odd, turned, heads)]
+    o = ops.packed_attention(*leaves, cu)
+    grads = torch.autograd.grad(o, leaves, do)
+    want = packed64(odd, turned, heads, cu, 0.125, do)
+    for name, got in zip(("o", "dq", "dk", "dv"), (o.detach(), *grads)):
+        close(got, *want[name], name)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_packed_attention_many_empty_sequences(device):
+    lens = [0] * 700 + [3] + [0] * 900 + [130, 0, 0, 1] + [0] * 40
+    q, k, v, cu, do = pack(lens, 2, 1, 64, device, seed=14)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = ops.packed_attention(*leaves, cu)
+    grads = torch.autograd.grad(o, leaves, do)
+    want = packed64(q, k, v, cu, 0.125, do)
+    for name, got in zip(("o", "dq", "dk", "dv"), (o.detach(), *grads)):
+        close(got, *want[name], name)
 
 
 @pytest.mark.gpu
@@ -376,6 +406,28 @@ def test_paged_refuses(device):
                  (k, k[:1], kp, vp, table, lens, None, ks, vs), (k, k, *odd[:2], table, lens)]:
         with pytest.raises(RuntimeError):
             ops.paged_cache_write(*args)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_paged_nothing(device):
+    """No pages, no table entries, no sequences, no rows."""
+    kp, vp, _, _ = make_pages(3, 2, 16, 64, BF16, "head", device)
+    before = kp.clone()
+    q = torch.ones(2, 4, 64, dtype=BF16, device=device)
+    ln = torch.tensor([5, 40], dtype=torch.int32, device=device)
+    empty = torch.zeros(2, 0, dtype=torch.int32, device=device)
+    assert (ops.paged_attention(q, kp, vp, empty, ln) == 0).all()
+    table = torch.tensor([[0], [2]], dtype=torch.int32, device=device)
+    assert (ops.paged_attention(q, kp[:0], vp[:0], table, ln) == 0).all()
+    assert ops.paged_attention(q[:0], kp, vp, table[:0], ln[:0]).shape == (0, 4, 64)
+    assert torch.equal(ops.paged_attention(q, kp, vp, table, ln * 0 - 3), torch.zeros_like(q))
+    long, full = (ops.paged_attention(q, kp, vp, table, ln * 0 + n) for n in (1000, 16))   # past the table: as much as it has
+    assert torch.equal(long, full)
+    k = torch.ones(2, 2, 64, dtype=BF16, device=device)
+    ops.paged_cache_write(k, k, kp, vp, empty, ln)
+    ops.paged_cache_write(k[:0], k[:0], kp, vp, table, ln, torch.zeros(3, dtype=torch.int32, device=device))
+    ops.paged_cache_write(k, k, kp, vp, table[:0], ln[:0], torch.zeros(1, dtype=torch.int32, device=device))
+    assert torch.equal(kp, before)
 
 
 @pytest.mark.gpu

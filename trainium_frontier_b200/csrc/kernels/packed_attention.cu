@@ -1171,14 +1171,15 @@ static PkCall pk_check(const at::Tensor& q, const at::Tensor& k, const at::Tenso
   TORCH_CHECK(c.M <= (1 << 30), "at most 2^30 rows");
   TORCH_CHECK(cu.scalar_type() == at::kInt && cu.device() == q.device() && cu.dim() == 1 && cu.size(0) >= 1 && cu.size(0) <= (1 << 30) && cu.is_contiguous(),
               "cu_seqlens: contiguous int32 [S + 1] on q's device");
-  TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale: a positive finite number");
+  const float scale_log2 = (float)(scale * 1.4426950408889634);
+  TORCH_CHECK(scale > 0 && scale_log2 > 0 && std::isfinite(scale_log2), "scale: a number within float32's range");
   c.q = pk_view(q, "q", q, Hq);
   c.k = pk_view(k, "k", q, Hkv);
   c.v = pk_view(v, "v", q, Hkv);
   PkArgs& a = c.a;
   a.pc.cu = cu.data_ptr<int>(); a.pc.S = (int)cu.size(0) - 1; a.pc.M = (int)c.M;
   a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.G = (int)(Hq / Hkv);
-  a.scale = (float)scale; a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.scale = (float)scale; a.scale_log2 = scale_log2;
   a.q = c.q.p; a.qr = c.q.r; a.qh = c.q.h;
   a.k = c.k.p; a.kr = c.k.r; a.kh = c.k.h;
   a.v = c.v.p; a.vr = c.v.r; a.vh = c.v.h;
@@ -1194,8 +1195,9 @@ static unsigned pk_grid(long long slots, long long heads) {
 // (out [M, Hq, D], lse [Hq, M] if asked for)
 std::tuple<at::Tensor, c10::optional<at::Tensor>> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu, double scale, bool want_lse,
                                              at::Tensor err) {
-  PkCall c = pk_check(q, k, v, cu, scale, err);
+  TORCH_CHECK(q.is_cuda(), "q: a CUDA tensor");
   c10::cuda::CUDAGuard guard(q.device());
+  PkCall c = pk_check(q, k, v, cu, scale, err);
   PkArgs& a = c.a;
   auto out = at::empty({c.M, a.Hq, c.D}, q.options());
   c10::optional<at::Tensor> lse;
@@ -1231,12 +1233,13 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> packed_attention_fwd(at::Tenso
 // {dq, dk, dv}, packed [M, H, D]; out and lse are the forward's.
 std::vector<at::Tensor> packed_attention_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor lse,
                                              at::Tensor cu, double scale, at::Tensor err) {
+  TORCH_CHECK(q.is_cuda(), "q: a CUDA tensor");
+  c10::cuda::CUDAGuard guard(q.device());
   PkCall c = pk_check(q, k, v, cu, scale, err);
   PkArgs& a = c.a;
   const PkView g = pk_view(dout, "the output's gradient", q, a.Hq);
   TORCH_CHECK(out.device() == q.device() && out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes() && out.is_contiguous(), "out: the forward's");
   TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.numel() == a.Hq * c.M && lse.is_contiguous(), "lse: the forward's");
-  c10::cuda::CUDAGuard guard(q.device());
   auto dq = at::empty({c.M, a.Hq, c.D}, q.options()), dk = at::empty({c.M, a.Hkv, c.D}, q.options()), dv = at::empty({c.M, a.Hkv, c.D}, q.options());
   if (c.M == 0) return {dq, dk, dv};
   auto dvec = at::empty({a.Hq, c.M}, lse.options());

@@ -334,7 +334,8 @@ def paged_attention(q, k_pages, v_pages, page_table, lens, scale: float | None =
     memory) of its pages, its own row among them (``paged_cache_write``, ``page_table`` as there).  Query
     head h reads head ``h // (Hq // H)``; returns [B, Hq, D].  ``scale`` defaults to D^-0.5.
 
-    Rows of table entries that are no page are not seen; a sequence that sees no row gets zeros.  An
+    Rows of table entries that are no page, and those behind the table's last page, are not seen; a sequence
+    that sees no row gets zeros.  An
     infinity or a NaN in a seen row (in e4m3: a NaN code, or the scale NaN) reaches its sequence's output
     and what other rows hold reaches nothing; where all scores are -inf the output is NaN.  Weights are
     rounded as in ``tree_attention``.  No gradient."""

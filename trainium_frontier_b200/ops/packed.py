@@ -39,8 +39,7 @@ class PackedAttnFn(Function):
 
 
 def packed_attention(q, k, v, cu_seqlens, scale: float):
-    _check(math.isfinite(scale), "scale: a finite number")
-    if scale < 0:
+    if scale < 0:   # (what is no number, or beyond float32's range, is refused at the launch)
         q, scale = -q, -scale
     elif scale == 0:   # 0 * (q . k): NaN where q . k is infinite, and the mask stays what it is
         q, scale = q * 0, 1.0

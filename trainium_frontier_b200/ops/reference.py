@@ -293,8 +293,9 @@ def _weighted(w, see, v):
 def packed_attention(q, k, v, cu_seqlens, scale: float):
     from . import packed as pk
     pk.check_packed(q, k, v, cu_seqlens)
-    if not math.isfinite(scale):
-        raise RuntimeError("scale: a finite number")
+    c = abs(scale) * 1.4426950408889634
+    if scale != 0 and not 2.0 ** -149 <= c < 2.0 ** 128:
+        raise RuntimeError("scale: a number within float32's range")
     M, Hq, _ = q.shape
     g = Hq // k.shape[1]
     cu = [min(max(int(c), 0), M) for c in cu_seqlens.tolist()]
