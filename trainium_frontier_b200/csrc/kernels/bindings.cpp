@@ -90,10 +90,11 @@ torch::Tensor tree_attention(torch::Tensor q, torch::Tensor kc, torch::Tensor vc
                              c10::optional<torch::Tensor> vs, torch::Tensor err);
 std::vector<torch::Tensor> verify_tree(torch::Tensor tokens, torch::Tensor parents, torch::Tensor p, c10::optional<torch::Tensor> q,
                                        torch::Tensor u);
-std::tuple<torch::Tensor, c10::optional<torch::Tensor>> packed_attention_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu, double scale,
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> packed_attention_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu, double scale,
                                                 bool want_lse, torch::Tensor err);
 std::vector<torch::Tensor> packed_attention_bwd(torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v,
-                                                torch::Tensor out, torch::Tensor lse, torch::Tensor cu, double scale, torch::Tensor err);
+                                                torch::Tensor out, torch::Tensor low, torch::Tensor lse, torch::Tensor cu, double scale,
+                                                torch::Tensor err);
 void paged_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor kp, torch::Tensor vp, torch::Tensor table, torch::Tensor pos,
                        c10::optional<torch::Tensor> cu, c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs);
 torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor vp, torch::Tensor table, torch::Tensor lens, double scale,

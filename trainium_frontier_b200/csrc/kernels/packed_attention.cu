@@ -2,7 +2,8 @@
 // heads, forward and backward, on the 5th-generation tensor cores.
 //
 //   o_i = sum_{j <= i} p_ij v_j,   p_ij = exp(scale q_i . k_j - lse_i),   i, j rows of one sequence;
-//   D_i = dO_i . o_i,  ds_ij = p_ij (dO_i . v_j - D_i),
+//   D_i = dO_i . o_i,  ds_ij = p_ij (dO_i . v_j - D_i),   (o_i to 16 bits of significand: the forward keeps what the
+//                                                         rounding to bf16 took off; see below)
 //   dQ_i = scale sum_j ds_ij k_j,  dK_j = scale sum_i ds_ij q_i,  dV_j = sum_i p_ij dO_i.
 //
 // q [M, Hq, D], k and v [M, Hkv, D] are read where they lie (TMA tiles of 128 rows from any row on); a
@@ -28,6 +29,9 @@
 // dV, four).  Scores are formed twice, seven products instead of the five of a single pass, but that
 // pass would add every dQ tile into 32-bit memory (an accumulator written, added to, read and rounded, in an
 // order that changes from run to run).  Here each gradient is a sum in TMEM, in order, and rounded once.
+// D of the rounded output would be the largest error of short sequences' gradients (a first row's ds, which is 0, would be D's
+// error: 3.4e-3 instead of 2.4e-3 of the gradients' size), so a forward that a backward follows writes the rest of the
+// output too, 2 bytes an entry (4 % of the time for documents of 340 tokens, 1 % for long ones).
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/ops/clone.h>
@@ -55,7 +59,7 @@ struct PkArgs {
   float scale, scale_log2;
   const __nv_bfloat16 *q, *k, *v, *o, *dout;           // rows and heads, strides in elements
   long long qr, qh, kr, kh, vr, vh, gr, gh;
-  __nv_bfloat16 *out, *dq, *dk, *dv;                   // [M, H, D]
+  __nv_bfloat16 *out, *low, *dq, *dk, *dv;             // [M, H, D]; low: what out's rounding took off, for the gradients
   float *lse, *dvec;             // [Hq, M]
   int* err;
 };
@@ -121,11 +125,12 @@ __device__ __forceinline__ void clear_rows(__nv_bfloat16* out, int H, int h0, in
   }
 }
 
+// LOW: not the rounded results but what the rounding took off them, rounded.
 // A warp's 32 rows of 16-byte CHUNKS, from TMEM columns at `from` on, each row times its lane's `by`, rounded and stored
 // through `stage` (shared memory of the warp's own, 16-byte aligned, 32 x 16 x CHUNKS bytes), so
 // that a store covers whole rows.  dst: the first row's, `stride` elements between rows; n: rows that are there.
 // (Rows stored by their own lanes took 4500 of a one-tile CTA's 15000 cycles.)
-template <int CHUNKS>
+template <int CHUNKS, bool LOW = false>
 __device__ __forceinline__ void store_rows(uint32_t from, float by, uint8_t* stage, __nv_bfloat16* dst, long long stride, int n) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -138,7 +143,11 @@ __device__ __forceinline__ void store_rows(uint32_t from, float by, uint8_t* sta
     for (int k = 0; k < 2; ++k) {
       uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(o[8 * k + 2 * i]) * by, __uint_as_float(o[8 * k + 2 * i + 1]) * by);
+      for (int i = 0; i < 4; ++i) {
+        const float lo = __uint_as_float(o[8 * k + 2 * i]) * by, hi = __uint_as_float(o[8 * k + 2 * i + 1]) * by;
+        w[i] = pack_bf16x2(lo, hi);
+        if constexpr (LOW) w[i] = pack_bf16x2(lo - __uint_as_float(w[i] << 16), hi - __uint_as_float(w[i] & 0xffff0000u));
+      }
       *reinterpret_cast<uint4*>(stage + lane * (16 * CHUNKS) + (((c + k) ^ (lane & (CHUNKS - 1) & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
@@ -485,9 +494,15 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
       const bool mine = row < un.len, alone = by_row[t] != 0;
       const int first = row - lane;      // the warp's first row; Q's tile is free: all products of it are done
       __nv_bfloat16* dst = a.out + ((long long)(un.begin + first) * a.Hq + head) * D;
-      if (!alone) store_rows<D / 8>(tO + lane_off, inv_l, sQ + t * TILE + q4 * (32 * D * 2), dst, (long long)a.Hq * D, un.len - first);
+      uint8_t* const stage = sQ + t * TILE + q4 * (32 * D * 2);
+      if (!alone) store_rows<D / 8>(tO + lane_off, inv_l, stage, dst, (long long)a.Hq * D, un.len - first);
+      if (a.low && !alone) store_rows<D / 8, true>(tO + lane_off, inv_l, stage, a.low + (dst - a.out), (long long)a.Hq * D, un.len - first);
       dst += (long long)lane * a.Hq * D;
-      if (mine && alone) packed_row<D>(a, un.begin, row, head, lse2, dst);
+      if (mine && alone) {
+        packed_row<D>(a, un.begin, row, head, lse2, dst);
+        if (a.low)
+          for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(a.low + (dst - a.out))[i] = make_uint4(0, 0, 0, 0);
+      }
       if (mine && a.lse) a.lse[(long long)head * a.pc.M + un.begin + row] = lse2 * kLn2;
     }
   }
@@ -709,24 +724,26 @@ __global__ void __launch_bounds__(608, 1)
     {
       constexpr int L = D / 8;           // lanes a row
       const int w8 = (warp - 2) * 8;
-      uint4 x[8 * L / 32], y[8 * L / 32];
+      uint4 x[8 * L / 32], y[8 * L / 32], z[8 * L / 32];
 #pragma unroll
       for (int i = 0; i < 8 * L / 32; ++i) {
         const int rr = row0 + w8 + i * (32 / L) + lane / L;
-        x[i] = y[i] = make_uint4(0, 0, 0, 0);
+        x[i] = y[i] = z[i] = make_uint4(0, 0, 0, 0);
         if (rr < un.len) {
           x[i] = reinterpret_cast<const uint4*>(a.dout + (long long)(un.begin + rr) * a.gr + h * a.gh)[lane % L];
-          y[i] = reinterpret_cast<const uint4*>(a.o + ((long long)(un.begin + rr) * a.Hq + h) * D)[lane % L];
+          const long long at = ((long long)(un.begin + rr) * a.Hq + h) * D;
+          y[i] = reinterpret_cast<const uint4*>(a.o + at)[lane % L];
+          z[i] = reinterpret_cast<const uint4*>(a.low + at)[lane % L];
         }
       }
 #pragma unroll
       for (int i = 0; i < 8 * L / 32; ++i) {
-        const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, yw[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+        const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, yw[4] = {y[i].x, y[i].y, y[i].z, y[i].w}, zw[4] = {z[i].x, z[i].y, z[i].z, z[i].w};
         float d = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          d += __uint_as_float(xw[w] << 16) * __uint_as_float(yw[w] << 16);
-          d += __uint_as_float(xw[w] & 0xffff0000u) * __uint_as_float(yw[w] & 0xffff0000u);
+          d += __uint_as_float(xw[w] << 16) * (__uint_as_float(yw[w] << 16) + __uint_as_float(zw[w] << 16));
+          d += __uint_as_float(xw[w] & 0xffff0000u) * (__uint_as_float(yw[w] & 0xffff0000u) + __uint_as_float(zw[w] & 0xffff0000u));
         }
 #pragma unroll
         for (int k = L / 2; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
@@ -1192,19 +1209,23 @@ static unsigned pk_grid(long long slots, long long heads) {
   return (unsigned)(slots * heads);
 }
 
-// (out [M, Hq, D], lse [Hq, M] if asked for)
-std::tuple<at::Tensor, c10::optional<at::Tensor>> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu, double scale, bool want_lse,
+// (out [M, Hq, D]; for a backward also lse [Hq, M] and the rest of the output [M, Hq, D])
+std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu, double scale, bool want_lse,
                                              at::Tensor err) {
   TORCH_CHECK(q.is_cuda(), "q: a CUDA tensor");
   c10::cuda::CUDAGuard guard(q.device());
   PkCall c = pk_check(q, k, v, cu, scale, err);
   PkArgs& a = c.a;
   auto out = at::empty({c.M, a.Hq, c.D}, q.options());
-  c10::optional<at::Tensor> lse;
-  if (want_lse) lse = at::empty({a.Hq, c.M}, q.options().dtype(at::kFloat));
-  if (c.M == 0) return {out, lse};
+  c10::optional<at::Tensor> lse, low;
+  if (want_lse) {
+    lse = at::empty({a.Hq, c.M}, q.options().dtype(at::kFloat));
+    low = at::empty({c.M, a.Hq, c.D}, q.options());
+  }
+  if (c.M == 0) return {out, lse, low};
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.lse = want_lse ? lse->data_ptr<float>() : nullptr;
+  a.low = want_lse ? reinterpret_cast<__nv_bfloat16*>(low->data_ptr()) : nullptr;
   a.by_heads = a.G % 2 == 0;
   auto s = at::cuda::getCurrentCUDAStream();
   auto launch = [&](auto cfg, auto kern, int64_t slots, int64_t heads) {
@@ -1227,23 +1248,26 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> packed_attention_fwd(at::Tenso
     else launch(PkFwd<64, 2>{}, PkKern<packed_fwd_kernel<64, 2>>{}, slots, heads);
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {out, lse};
+  return {out, lse, low};
 }
 
 // {dq, dk, dv}, packed [M, H, D]; out and lse are the forward's.
-std::vector<at::Tensor> packed_attention_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor lse,
-                                             at::Tensor cu, double scale, at::Tensor err) {
+std::vector<at::Tensor> packed_attention_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor low,
+                                             at::Tensor lse, at::Tensor cu, double scale, at::Tensor err) {
   TORCH_CHECK(q.is_cuda(), "q: a CUDA tensor");
   c10::cuda::CUDAGuard guard(q.device());
   PkCall c = pk_check(q, k, v, cu, scale, err);
   PkArgs& a = c.a;
   const PkView g = pk_view(dout, "the output's gradient", q, a.Hq);
-  TORCH_CHECK(out.device() == q.device() && out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes() && out.is_contiguous(), "out: the forward's");
+  for (const auto* t : {&out, &low})
+    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kBFloat16 && t->sizes() == q.sizes() && t->is_contiguous(),
+                "out and its rest: the forward's");
   TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.numel() == a.Hq * c.M && lse.is_contiguous(), "lse: the forward's");
   auto dq = at::empty({c.M, a.Hq, c.D}, q.options()), dk = at::empty({c.M, a.Hkv, c.D}, q.options()), dv = at::empty({c.M, a.Hkv, c.D}, q.options());
   if (c.M == 0) return {dq, dk, dv};
   auto dvec = at::empty({a.Hq, c.M}, lse.options());
   a.o = reinterpret_cast<const __nv_bfloat16*>(out.data_ptr());
+  a.low = reinterpret_cast<__nv_bfloat16*>(low.data_ptr());
   a.dout = g.p; a.gr = g.r; a.gh = g.h;
   a.dq = reinterpret_cast<__nv_bfloat16*>(dq.data_ptr());
   a.dk = reinterpret_cast<__nv_bfloat16*>(dk.data_ptr());

@@ -25,16 +25,16 @@ from .speculative import _check, check_cache, check_ints, check_scales_written
 class PackedAttnFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, scale):
-        out, lse = C().packed_attention_fwd(q, k, v, cu_seqlens, scale, True, err_word(q.device))
-        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
+        out, lse, low = C().packed_attention_fwd(q, k, v, cu_seqlens, scale, True, err_word(q.device))
+        ctx.save_for_backward(q, k, v, out, low, lse, cu_seqlens)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
-        dq, dk, dv = C().packed_attention_bwd(dout, q, k, v, out, lse, cu_seqlens, ctx.scale, err_word(q.device))
+        q, k, v, out, low, lse, cu_seqlens = ctx.saved_tensors
+        dq, dk, dv = C().packed_attention_bwd(dout, q, k, v, out, low, lse, cu_seqlens, ctx.scale, err_word(q.device))
         return dq, dk, dv, None, None
 
 
