@@ -125,40 +125,48 @@ __device__ __forceinline__ void clear_rows(__nv_bfloat16* out, int H, int h0, in
   }
 }
 
-// LOW: not the rounded results but what the rounding took off them, rounded.
 // A warp's 32 rows of 16-byte CHUNKS, from TMEM columns at `from` on, each row times its lane's `by`, rounded and stored
-// through `stage` (shared memory of the warp's own, 16-byte aligned, 32 x 16 x CHUNKS bytes), so
-// that a store covers whole rows.  dst: the first row's, `stride` elements between rows; n: rows that are there.
+// through `stage`, PASS chunks of all rows at a time, so that a store covers whole pieces of rows (shared memory of the
+// warp's own, 16-byte aligned, 512 x PASS bytes, and as many again with `low`).  dst: the first row's, `stride` elements between
+// rows; low (or null): what the rounding took off them, rounded, likewise; n: rows that are there.
 // (Rows stored by their own lanes took 4500 of a one-tile CTA's 15000 cycles.)
-template <int CHUNKS, bool LOW = false>
-__device__ __forceinline__ void store_rows(uint32_t from, float by, uint8_t* stage, __nv_bfloat16* dst, long long stride, int n) {
+template <int CHUNKS, int PASS>
+__device__ __forceinline__ void store_rows(uint32_t from, float by, uint8_t* stage, __nv_bfloat16* dst, __nv_bfloat16* low, long long stride, int n) {
+  static_assert(CHUNKS % PASS == 0 && PASS % 2 == 0, "chunks");
   const int lane = threadIdx.x & 31;
+  auto place = [](int row, int c) { return row * (16 * PASS) + ((c ^ (row & (PASS - 1) & 7)) << 4); };
 #pragma unroll
-  for (int c = 0; c < CHUNKS; c += 2) {
-    uint32_t o[16];
-    __syncwarp();
-    tmem_ld_32x32b_x16(from + c * 8, o);
-    tmem_ld_wait();
+  for (int c0 = 0; c0 < CHUNKS; c0 += PASS) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      uint32_t w[4];
+    for (int c = 0; c < PASS; c += 2) {
+      uint32_t o[16];
+      __syncwarp();
+      tmem_ld_32x32b_x16(from + (c0 + c) * 8, o);
+      tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float lo = __uint_as_float(o[8 * k + 2 * i]) * by, hi = __uint_as_float(o[8 * k + 2 * i + 1]) * by;
-        w[i] = pack_bf16x2(lo, hi);
-        if constexpr (LOW) w[i] = pack_bf16x2(lo - __uint_as_float(w[i] << 16), hi - __uint_as_float(w[i] & 0xffff0000u));
+      for (int k = 0; k < 2; ++k) {
+        uint32_t w[4], v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = __uint_as_float(o[8 * k + 2 * i]) * by, y = __uint_as_float(o[8 * k + 2 * i + 1]) * by;
+          w[i] = pack_bf16x2(x, y);
+          v[i] = pack_bf16x2(x - __uint_as_float(w[i] << 16), y - __uint_as_float(w[i] & 0xffff0000u));
+        }
+        *reinterpret_cast<uint4*>(stage + place(lane, c + k)) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (low) *reinterpret_cast<uint4*>(stage + 512 * PASS + place(lane, c + k)) = make_uint4(v[0], v[1], v[2], v[3]);
       }
-      *reinterpret_cast<uint4*>(stage + lane * (16 * CHUNKS) + (((c + k) ^ (lane & (CHUNKS - 1) & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-  }
-  __syncwarp();
+    __syncwarp();
 #pragma unroll
-  for (int i = 0; i < CHUNKS; ++i) {
-    const int row = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
-    if (row < n)
-      reinterpret_cast<uint4*>(dst + row * stride)[c] = *reinterpret_cast<const uint4*>(stage + row * (16 * CHUNKS) + ((c ^ (row & (CHUNKS - 1) & 7)) << 4));
+    for (int i = 0; i < PASS; ++i) {
+      const int row = (i * 32 + lane) / PASS, c = (i * 32 + lane) % PASS;
+      if (row < n) {
+        reinterpret_cast<uint4*>(dst + row * stride)[c0 + c] = *reinterpret_cast<const uint4*>(stage + place(row, c));
+        if (low) reinterpret_cast<uint4*>(low + row * stride)[c0 + c] = *reinterpret_cast<const uint4*>(stage + 512 * PASS + place(row, c));
+      }
+    }
+    __syncwarp();
   }
-  __syncwarp();
 }
 
 // A row's output by itself, keys one after another in 32 bits: for the rows of a diagonal tile whose masked
@@ -494,9 +502,9 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
       const bool mine = row < un.len, alone = by_row[t] != 0;
       const int first = row - lane;      // the warp's first row; Q's tile is free: all products of it are done
       __nv_bfloat16* dst = a.out + ((long long)(un.begin + first) * a.Hq + head) * D;
-      uint8_t* const stage = sQ + t * TILE + q4 * (32 * D * 2);
-      if (!alone) store_rows<D / 8>(tO + lane_off, inv_l, stage, dst, (long long)a.Hq * D, un.len - first);
-      if (a.low && !alone) store_rows<D / 8, true>(tO + lane_off, inv_l, stage, a.low + (dst - a.out), (long long)a.Hq * D, un.len - first);
+      if (!alone)
+        store_rows<D / 8, D / 16>(tO + lane_off, inv_l, sQ + t * TILE + q4 * (32 * D * 2), dst, a.low ? a.low + (dst - a.out) : nullptr,
+                                  (long long)a.Hq * D, un.len - first);
       dst += (long long)lane * a.Hq * D;
       if (mine && alone) {
         packed_row<D>(a, un.begin, row, head, lse2, dst);
@@ -809,7 +817,7 @@ __global__ void __launch_bounds__(608, 1)
       tc_fence_after();
       // Q's tile is free: all products of it are done
       __nv_bfloat16* dst = a.dq + ((long long)(un.begin + row0 + q4 * 32) * a.Hq + h) * D + quarter * (D / 4);
-      store_rows<D / 32>(tQ + lane_off + quarter * (D / 4), a.scale, sQ + (warp - 2) * (32 * (D / 4) * 2), dst, (long long)a.Hq * D, un.len - row0 - q4 * 32);
+      store_rows<D / 32, D / 32>(tQ + lane_off + quarter * (D / 4), a.scale, sQ + (warp - 2) * (32 * (D / 4) * 2), dst, nullptr, (long long)a.Hq * D, un.len - row0 - q4 * 32);
     }
   }
   tc_fence_before();
@@ -1118,8 +1126,8 @@ __global__ void __launch_bounds__(576, 1)
       const int first = row0 + q4 * 32, n_rows = un.len - first;
       const long long at = ((long long)(un.begin + first) * a.Hkv + hk) * D + quarter * (D / 4), stride = (long long)a.Hkv * D;
       const uint32_t stage = (warp - 2) * (32 * (D / 4) * 2);
-      store_rows<D / 32>(tDV + lane_off + quarter * (D / 4), 1.f, sV + stage, a.dv + at, stride, n_rows);
-      store_rows<D / 32>(tDK + lane_off + quarter * (D / 4), a.scale, sK + stage, a.dk + at, stride, n_rows);
+      store_rows<D / 32, D / 32>(tDV + lane_off + quarter * (D / 4), 1.f, sV + stage, a.dv + at, nullptr, stride, n_rows);
+      store_rows<D / 32, D / 32>(tDK + lane_off + quarter * (D / 4), a.scale, sK + stage, a.dk + at, nullptr, stride, n_rows);
     }
   }
   tc_fence_before();
