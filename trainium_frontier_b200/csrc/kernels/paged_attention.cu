@@ -18,6 +18,14 @@
 // Quantised rows: codes become f16 in registers.  A key's scale multiplies its score; a value's multiplies its
 // weight, which is taken relative to a maximum m' of score + log2 scale, so that weights fit f16 whatever the
 // scales are.
+//
+// Measured on a B200 (calls replayed from a graph; floors at 6.56 TB/s).  One sequence of 131071 bf16 rows, 32 / 8 heads:
+// 84 us of 82.  64 sequences of 8192 .. 16384 e4m3 rows, 32 / 8 heads, pages of 16: 288 us of 248; 360
+// instructions a step, half of the issue slots, 80 of them conversions and interleaving of codes.  A decode step of 32
+// sequences of 288 .. 576 bf16 rows, 10 heads, pages of 16: 16 us of 11; every CTA has one short sequence, whose
+// start (lengths, pages, first rows one after another) costs as much as its rows.  Rows loaded into registers instead of
+// bulk copies into a ring: 350 (e4m3 batch) and 111 us (one sequence), since a wait for one load waits for the ones
+// issued after it; copies by each lane for itself: 320 and 127.
 #include <ATen/ops/empty.h>
 
 #include <atomic>

@@ -15,6 +15,10 @@
 // of 7: 134 us for 16384 rows.)  Nothing waits for another warp until the row's end.
 // With many rows a warp has a whole one; with fewer a CTA's eight warps, or those of a cluster of up to 8
 // CTAs, share it and are joined through (distributed) shared memory.
+// Measured on a B200 (calls replayed from a graph).  16384 rows of 8192 fp32 logits with five alternatives: 107 us of 82 (HBM,
+// 76 % of the copy rate; 3800 instructions a row).  4096 rows of 131072 bf16 logits: 234 us of 164 forward (the
+// exponentials alone, 16 a cycle of an SM, take 120), gradient 358 of 327.  8 rows of 131072 fp32 logits with eight
+// alternatives: 10.8 us; a chain of loads, sums, candidates and a cluster's joins.
 // The reference has no counterpart; its losses are those of fused_ops.cu.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
