@@ -30,8 +30,8 @@
 // pass would add every dQ tile into 32-bit memory (an accumulator written, added to, read and rounded, in an
 // order that changes from run to run).  Here each gradient is a sum in TMEM, in order, and rounded once.
 // D of the rounded output would be the largest error of short sequences' gradients (a first row's ds, which is 0, would be D's
-// error: 3.4e-3 instead of 2.4e-3 of the gradients' size), so a forward that a backward follows writes the rest of the
-// output too, 2 bytes an entry (4 % of the time for documents of 340 tokens, 1 % for long ones).
+// error: 3.4e-3 instead of 2.6e-3 of the gradients' size), so a forward that a backward follows writes the rest of the
+// output too, 2 bytes an entry (4 to 7 % of the time for documents of 340 tokens, 2 % for long ones).
 //
 // Measured on a B200, head_dim 128 (counters: profiles/packed_attention.md).  Forward: 16 sequences of 4096 .. 8191 rows, 32 / 8
 // heads, 5.2 ms = 0.98 PFLOP/s, power capped (floor 3.1 at the burst rate of a library product, 3.7 at the sustained one);
