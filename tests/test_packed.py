@@ -206,6 +206,20 @@ def test_packed_attention_many_empty_sequences(device):
         close(got, *want[name], name)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("M,cut", [(0, [0]), (0, [0, 0, 0]), (9, [0]), (9, [9]), (9, [4, 4])], ids=str)
+def test_packed_attention_nothing(M, cut, device):
+    """No rows, no sequences, or rows of no sequence: zeros, and zero gradients."""
+    g = torch.Generator().manual_seed(14)
+    leaves = [torch.randn(M, h, 64, generator=g).to(BF16).to(device).requires_grad_() for h in (4, 2, 2)]
+    cu = torch.tensor(cut, dtype=torch.int32, device=device)
+    o = ops.packed_attention(*leaves, cu)
+    assert o.shape == (M, 4, 64) and (o == 0).all()
+    for d, x in zip(torch.autograd.grad(o, leaves, torch.ones_like(o)), leaves):
+        assert d.shape == x.shape and (d == 0).all()
+    check_errors(device)
+
+
 @pytest.mark.gpu
 def test_packed_attention_captured():
     """A captured call reads the lengths of the time of its replay; the backward pass is captured with it."""
@@ -430,6 +444,29 @@ def test_paged_nothing(device):
     assert torch.equal(kp, before)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_paged_integers_at_their_ends(dtype, device):
+    """Lengths, positions and table entries at the ends of their type reach no row but their own."""
+    top, least = 2 ** 31 - 1, -2 ** 31
+    pages = make_pages(3, 2, 16, 64, dtype, "head", device)
+    before = [None if t is None else raw(t).clone() for t in pages]
+    _, k, v, cu, _ = pack([4, 4, 2, 3], 1, 2, 64, device, seed=15)
+    table = torch.tensor([[0, 1], [1, 2], [top, 0], [2, least]], dtype=torch.int32, device=device)
+    pos = torch.tensor([top, least, 0, 16], dtype=torch.int32, device=device)
+    ops.paged_cache_write(k, v, *pages[:2], table, pos, cu, *pages[2:])   # past every row, in front of row 0, no pages
+    ops.paged_cache_write(k[:4], v[:4], *pages[:2], table, pos, None, *pages[2:])
+    assert all(t is None or torch.equal(raw(t), b) for t, b in zip(pages, before))
+    q = torch.randn(4, 4, 64, generator=torch.Generator().manual_seed(16)).to(BF16).to(device)
+    lens = torch.tensor([top, least, top, top], dtype=torch.int32, device=device)
+    got = ops.paged_attention(q, *pages[:2], table, lens, None, *pages[2:])
+    assert (got[1] == 0).all()
+    seen = torch.tensor([[0, 1], [1, 2], [0, 0], [2, 0]], dtype=torch.int32, device=device)
+    few = torch.tensor([32, 0, 16, 16], dtype=torch.int32, device=device)
+    close(got, *paged64(q, *pages[:2], seen, few, 0.125, *pages[2:]), "o")
+    check_errors(device)
+
+
 @pytest.mark.gpu
 def test_paged_step_captured():
     """A decode step, rows written and attended, captured once and replayed as the sequences grow."""
@@ -589,6 +626,28 @@ def test_token_logprobs_shapes(device):
     for x, gh in ((a, (one, zero)), (b, (zero, one))):
         value, bound = scores64(z.detach(), tokens, 0, *gh)["dlogits"]
         close(x, value, bound + 2.0 ** -23 * value.abs(), "dlogits")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_token_logprobs_edges(device):
+    """Tokens at the ends of their type, which are outside the vocabulary; rows and tokens shared or cut out of others."""
+    z, g = make_logits(4, 40, torch.float32, device)
+    for t in (torch.tensor([2 ** 63 - 1, -2 ** 63, 2 ** 32 + 1, 3], device=device), torch.tensor([2 ** 31 - 1, -2 ** 31, 40, 3], dtype=torch.int32, device=device)):
+        lp = ops.token_logprobs(z, t)[0]
+        assert (lp[:3] == 0).all() and lp[3] == ops.token_logprobs(z[3], t[3])[0] and lp[3] < 0
+    tokens = torch.randint(0, 40, (3, 5), generator=g).to(device)
+    whole = z[0].expand(3, 4, 40).contiguous()
+    for a, b in zip(ops.token_logprobs(z[0].expand(3, 4, 40), tokens[:, 1:], 3), ops.token_logprobs(whole, tokens[:, 1:].contiguous(), 3)):
+        assert torch.equal(a, b)
+    one = z[:1].clone().requires_grad_()       # a row that four tokens share: the sum of their gradients
+    da, = torch.autograd.grad(ops.token_logprobs(one.expand(4, 40), tokens[0, 1:])[0].sum(), (one,))
+    each = z[:1].expand(4, 40).contiguous().requires_grad_()
+    db, = torch.autograd.grad(ops.token_logprobs(each, tokens[0, 1:])[0].sum(), (each,))
+    value = db.double().sum(0, keepdim=True)
+    close(da, value, 4 * 2.0 ** -24 * db.double().abs().sum(0, keepdim=True), "dlogits")   # a sum of four in any order
+    none = z[:0].clone().requires_grad_()
+    dn, = torch.autograd.grad(ops.token_logprobs(none, tokens[0, :0])[0].sum(), (none,))
+    assert dn.shape == (0, 40)
 
 
 def test_token_logprobs_differences():

@@ -302,7 +302,8 @@ def packed_attention(q, k, v, cu_seqlens, scale: float | None = None):
     ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` (int32 [S + 1] in device memory, ascending; a sequence may
     be empty).  Returns [M, Hq, D]; rows outside all sequences are zero.  ``scale`` defaults to D^-0.5.
 
-    Differentiable in q, k and v; rows outside all sequences get zero gradients, and what they hold
+    Differentiable in q, k and v (a backward pass can be captured in a CUDA graph while no graph recorded before
+    the capture still holds its leaves); rows outside all sequences get zero gradients, and what they hold
     reaches nothing.  An infinity or a NaN of a token reaches the outputs of the tokens that see it, and no
     other; in the backward pass it may also reach gradients of tokens of its own sequence that lie in
     the same 128 rows of it.  CUDA: bfloat16, head_dim 64 / 128; inputs are read in place (slices of
@@ -321,7 +322,8 @@ def paged_cache_write(k, v, k_pages, v_pages, page_table, pos, cu_seqlens=None, 
     ``page_table[b, t // page]`` with ``t = pos[b] + n``.  ``cu_seqlens`` int32 [B + 1] cuts the rows into
     sequences as in ``packed_attention``; None: one row a sequence.  ``page_table`` int32 [B, W] and ``pos``
     int32 [B] in device memory.  Rows outside all sequences, rows that the table has no page for and those
-    whose table entry is no page are left out; every other row of the pages stays as it is.  Quantised
+    whose table entry is no page are left out; every other row of the pages stays as it is.  Where one call
+    sends several rows to one place (a page that padded sequences share, say), what that place holds is open.  Quantised
     pages as in ``kv_cache_write``.  CUDA: k, v bfloat16 with 16-byte aligned rows, head_dim 64 / 128."""
     if _cuda(k_pages):
         from .packed import paged_cache_write as f

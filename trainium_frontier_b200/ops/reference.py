@@ -310,7 +310,8 @@ def packed_attention(q, k, v, cu_seqlens, scale: float):
         w = torch.softmax((qs @ ks.transpose(1, 2) * scale).masked_fill(~see, float("-inf")), -1)
         out.append(_weighted(w, see, vs).transpose(0, 1))
         at = b
-    out.append(q.new_zeros(M - at, Hq, q.shape[2], dtype=torch.float32))
+    nothing = sum(t[:0].float().sum() for t in (q, k, v))   # 0, with a gradient of zeros where no row is in a sequence
+    out.append(q.new_zeros(M - at, Hq, q.shape[2], dtype=torch.float32) + nothing)
     return torch.cat(out).to(q.dtype)
 
 
