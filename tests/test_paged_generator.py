@@ -3,7 +3,7 @@ packed attention."""
 import pytest
 import torch
 
-from trainium_frontier_b200.config import GPTConfig, RunConfig
+from trainium_frontier_b200.config import GPTConfig, RunConfig, validate
 from trainium_frontier_b200.inference.generate import generate_reference
 from trainium_frontier_b200.inference.paged import PagedGenerator
 from trainium_frontier_b200.models import gpt
@@ -111,6 +111,18 @@ def test_refusals():
         PagedGenerator(m, 1, 257)
     with pytest.raises(NotImplementedError):
         PagedGenerator(make_model("cpu", gated_mlp=True), 1, 64)
+
+
+@pytest.mark.parametrize("temperature", [-1.0, float("nan")])
+def test_refuses_temperatures(temperature):
+    with pytest.raises(ValueError):
+        PagedGenerator(make_model("cpu"), 2, 64).generate(make_prompts([3]), 2, temperature=temperature)
+
+
+def test_refuses_packed_documents_without_document_masking():
+    with pytest.raises(ValueError):
+        validate(RunConfig(doc_mask_packed=True))
+    validate(RunConfig(doc_mask_packed=True, doc_mask=True))
 
 
 # ------------------------------------------------------------------------------- document masking

@@ -361,6 +361,8 @@ def validate(cfg: RunConfig) -> None:
         raise ValueError("--synthetic-epoch-tokens must be >= 0")
     if cfg.coalesced_swiglu and cfg.gated_mlp:
         raise ValueError("--coalesced-swiglu and --gated-mlp are mutually exclusive")
+    if cfg.doc_mask_packed and not cfg.doc_mask:
+        raise ValueError("--doc-mask-packed: a form of --doc-mask, which is off")
     if cfg.adam_every_n < 1:
         raise ValueError("--adam-every-n must be >= 1")
     if cfg.tp < 1 or cfg.pp < 1:

@@ -97,6 +97,8 @@ class PagedGenerator:
             raise ValueError(f"prompts: 1-D, not empty, and with the new tokens at most {self.max_len} tokens")
         if not 0 <= top <= min(32, self.V):
             raise ValueError("top: 0 .. 32 alternatives, at most the vocabulary")
+        if not temperature >= 0:
+            raise ValueError("temperature: 0 (greedy) or above")
         text = torch.cat([p.to(self.dev) for p in prompts])
         if int(text.min()) < 0 or int(text.max()) >= self.V:   # they index the embedding
             raise ValueError(f"prompts: tokens 0 .. {self.V - 1}")
