@@ -567,10 +567,10 @@ __global__ void __launch_bounds__(608, 1)
   uint64_t* s_free = s_full + 1;
   uint64_t* dp_full = s_full + 2;
   uint64_t* dp_free = s_full + 3;
-  uint64_t* ds_full = s_full + 4;
-  uint64_t* ds_free = s_full + 5;      // [2]
-  uint64_t* done = s_full + 7;
-  uint64_t* drain = s_full + 8;        // [2]
+  uint64_t* ds_full = s_full + 4;      // [2]: the compute warps may be a tile ahead of dQ
+  uint64_t* ds_free = s_full + 6;      // [2]
+  uint64_t* done = s_full + 8;
+  uint64_t* drain = s_full + 9;        // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PieceUnit* s_unit = reinterpret_cast<PieceUnit*>(tmem_slot + 4);
@@ -593,7 +593,8 @@ __global__ void __launch_bounds__(608, 1)
     mbar_init(s_free, 16);
     mbar_init(dp_full, 1);
     mbar_init(dp_free, 16);
-    mbar_init(ds_full, 16);
+    mbar_init(&ds_full[0], 16);
+    mbar_init(&ds_full[1], 16);
     mbar_init(&ds_free[0], 1);
     mbar_init(&ds_free[1], 1);
     mbar_init(done, 1);
@@ -710,7 +711,7 @@ __global__ void __launch_bounds__(608, 1)
     int kq = 0;                          // slot of K_j
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      if (!mbar_wait_warp(ds_full, j & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
+      if (!mbar_wait_warp(&ds_full[j & 1], (j >> 1) & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) { ok = false; break; }
       tc_fence_after();
       if (leader) {
         mma_tmem<16>(tQ, tD + (j & 1) * 64, kn + kq * STEP, IDESC_Q, j > 0);
@@ -819,7 +820,7 @@ __global__ void __launch_bounds__(608, 1)
       tmem_st_32x32b_x16(tD + (j & 1) * 64 + lane_off + quarter * 16, pk);
       tmem_st_wait();
       tc_fence_before();
-      warp_arrive(ds_full);
+      warp_arrive(&ds_full[j & 1]);
     }
     if (ok && mbar_wait_warp(done, 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
       tc_fence_after();
