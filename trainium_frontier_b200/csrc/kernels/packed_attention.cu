@@ -29,9 +29,10 @@
 // dV, four).  Scores are formed twice, seven products instead of the five of a single pass, but that
 // pass would add every dQ tile into 32-bit memory (an accumulator written, added to, read and rounded, in an
 // order that changes from run to run).  Here each gradient is a sum in TMEM, in order, and rounded once.
-// D of the rounded output would be the largest error of short sequences' gradients (a first row's ds, which is 0, would be D's
-// error: 3.4e-3 instead of 2.6e-3 of the gradients' size), so a forward that a backward follows writes the rest of the
-// output too, 2 bytes an entry (4 to 7 % of the time for documents of 340 tokens, 2 % for long ones).
+// D of the rounded output would be the largest error of short sequences' gradients (a first row's ds, which is 0, would be
+// D's error): 3.4e-3 of their size.  So a forward that a backward follows writes the rest of the output too, 2 bytes an entry
+// (4 to 7 % of the time for documents of 340 tokens, 2 % for long ones): 2.6e-3.  A sequence's first 128 rows, whose weights
+// are all in one tile, take D from those in 32 bits: 2.4e-3, of which 1.7e-3 is the rounding of the result.
 //
 // Measured on a B200, head_dim 128 (counters: profiles/packed_attention.md).  Forward: 16 sequences of 4096 .. 8191 rows, 32 / 8
 // heads, 5.2 ms = 0.98 PFLOP/s, power capped (floor 3.1 at the burst rate of a library product, 3.7 at the sustained one);
@@ -571,7 +572,8 @@ __global__ void __launch_bounds__(608, 1)
   uint64_t* ds_free = s_full + 6;      // [2]
   uint64_t* done = s_full + 8;
   uint64_t* drain = s_full + 9;        // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+  uint64_t* part_full = s_full + 11;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PieceUnit* s_unit = reinterpret_cast<PieceUnit*>(tmem_slot + 4);
 
@@ -598,6 +600,7 @@ __global__ void __launch_bounds__(608, 1)
     mbar_init(&ds_free[0], 1);
     mbar_init(&ds_free[1], 1);
     mbar_init(done, 1);
+    mbar_init(part_full, 16);
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
     *abort_flag = 0;
@@ -737,8 +740,8 @@ __global__ void __launch_bounds__(608, 1)
     const bool mine = row < un.len;
     const long long at = (long long)h * a.pc.M + un.begin + row;
     // D_i = dO_i . o_i, kept for the other kernel: eight rows a warp, 16-byte loads of whole rows.  (A row a thread took 9000
-    // cycles, longer than three tiles of keys.)
-    {
+    // cycles, longer than three tiles of keys.)  A sequence's first 128 rows take it from their one tile of weights, below.
+    if (n > 1) {
       constexpr int L = D / 8;           // lanes a row
       const int w8 = (warp - 2) * 8;
       uint4 x[8 * L / 32], y[8 * L / 32], z[8 * L / 32];
@@ -766,14 +769,44 @@ __global__ void __launch_bounds__(608, 1)
         for (int k = L / 2; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
         if (lane % L == 0) sD[w8 + i * (32 / L) + lane / L] = d;
       }
+      named_bar_sync(1, 512);            // no wait comes before it: all 512 threads arrive
     }
-    named_bar_sync(1, 512);              // no wait comes before it: all 512 threads arrive
-    const float dsum = sD[r];
-    if (mine && quarter == 0) a.dvec[at] = dsum;
     const float nlse = mine ? -a.lse[at] * kLog2e : -INFINITY;
-    const float2 c2 = make_float2(a.scale_log2, a.scale_log2), nl2 = make_float2(nlse, nlse), nd2 = make_float2(-dsum, -dsum);
+    const float2 c2 = make_float2(a.scale_log2, a.scale_log2), nl2 = make_float2(nlse, nlse);
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
+    float dsum = 0.f;
+    if (n > 1) {
+      dsum = sD[r];
+    } else {
+      // D_i = sum of p dP over the row, of 32-bit weights: those that o was summed with are rounded, which is as much as
+      // the rounding of ds where a row has few keys (gradients of sequences of 20 rows off by 2.4e-3 instead of 2.6e-3 of their
+      // size).  dO's tile is free: its product is done.  (Within the loop below long sequences' dQ took 6 % longer.)
+      float* part = reinterpret_cast<float*>(sG);        // [4][128]
+      ok = mbar_wait_warp(s_full, 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE) && mbar_wait_warp(dp_full, 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
+      if (ok) {
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = cb; c < cb + 32; c += 16) {
+          uint32_t x[16], y[16];
+          __syncwarp();
+          tmem_ld_32x32b_x16(tS + lane_off + c, x);
+          tmem_ld_32x32b_x16(tP + lane_off + c, y);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float w = ex2_approx(fmaf(__uint_as_float(x[e]), a.scale_log2, nlse));
+            if (c + e <= r) dsum = fmaf(w, __uint_as_float(y[e]), dsum);
+          }
+        }
+        part[quarter * 128 + r] = dsum;
+        warp_arrive(part_full);
+        ok = mbar_wait_warp(part_full, 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
+        dsum = (part[r] + part[128 + r]) + (part[256 + r] + part[384 + r]);
+      }
+    }
+    if (mine && quarter == 0) a.dvec[at] = dsum;
+    const float2 nd2 = make_float2(-dsum, -dsum);
+    for (int j = 0; j < n && ok; ++j) {
       const bool diag = j == n - 1;
       if (!mbar_wait_warp(s_full, j & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
       tc_fence_after();
