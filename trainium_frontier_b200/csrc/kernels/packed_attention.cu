@@ -29,10 +29,13 @@
 // dV, four).  Scores are formed twice, seven products instead of the five of a single pass, but that
 // pass would add every dQ tile into 32-bit memory (an accumulator written, added to, read and rounded, in an
 // order that changes from run to run).  Here each gradient is a sum in TMEM, in order, and rounded once.
-// D of the rounded output would be the largest error of short sequences' gradients (a first row's ds, which is 0, would be
-// D's error): 3.4e-3 of their size.  So a forward that a backward follows writes the rest of the output too, 2 bytes an entry
-// (4 to 7 % of the time for documents of 340 tokens, 2 % for long ones): 2.6e-3.  A sequence's first 128 rows, whose weights
-// are all in one tile, take D from those in 32 bits: 2.4e-3, of which 1.7e-3 is the rounding of the result.
+// A sequence's first token sees itself alone: its weight is 1 and its ds 0 whatever the score is, but a weight formed again from a
+// rounded lse is off by some 2^-24 of it, and ds with it.  So that ds is chosen to be 0, as masked ones are (what is no number
+// stays).  Where all sequences are one token, dQ and dK are zeros, not rounding errors.
+// D of the rounded output would be the largest error of short sequences' gradients: 3.4e-3 of their size.  So a forward that
+// a backward follows writes the rest of the output too, 2 bytes an entry (4 to 7 % of the time for documents of 340 tokens,
+// 2 % for long ones): 2.6e-3.  A sequence's first 128 rows, whose weights are all in one tile, take D from those in 32 bits:
+// 2.4e-3, of which 1.7e-3 is the rounding of the result.
 //
 // Measured on a B200, head_dim 128 (counters: profiles/packed_attention.md).  Forward: 16 sequences of 4096 .. 8191 rows, 32 / 8
 // heads, 5.2 ms = 0.98 PFLOP/s, power capped (floor 3.1 at the burst rate of a library product, 3.7 at the sustained one);
@@ -738,6 +741,7 @@ __global__ void __launch_bounds__(608, 1)
     const int r = q4 * 32 + lane, row = row0 + r;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
     const bool mine = row < un.len;
+    const bool first = row == 0 && quarter == 0;         // holds the ds that is 0 by definition
     const long long at = (long long)h * a.pc.M + un.begin + row;
     // D_i = dO_i . o_i, kept for the other kernel: eight rows a warp, 16-byte loads of whole rows.  (A row a thread took 9000
     // cycles, longer than three tiles of keys.)  A sequence's first 128 rows take it from their one tile of weights, below.
@@ -845,6 +849,7 @@ __global__ void __launch_bounds__(608, 1)
         if (diag) {
           if (cb + e > r) y.x = 0.f;
           if (cb + e + 1 > r) y.y = 0.f;
+          if (e == 0 && first) y.x *= 0.f;
         }
         pk[e >> 1] = pack_bf16x2(y.x, y.y);
       }
@@ -1068,6 +1073,7 @@ __global__ void __launch_bounds__(576, 1)
     const int r = q4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
     const float2 c2 = make_float2(a.scale_log2, a.scale_log2);
+    const bool first = row0 + r == 0 && quarter == 0;    // holds the ds that is 0 by definition, in the diagonal tiles
     const bool reads = quarter < 2;      // the first 256 threads: a query's lse (quarter 0) or D
     const float* stats = quarter == 0 ? a.lse : a.dvec;
     int qi = kt, h = hk * a.G;
@@ -1151,6 +1157,7 @@ __global__ void __launch_bounds__(576, 1)
             if (cc + 1 < lo || cc + 1 >= lim) da.y = 0.f;
             if (cc + 2 < lo || cc + 2 >= lim) db.x = 0.f;
             if (cc + 3 < lo || cc + 3 >= lim) db.y = 0.f;
+            if (e == 0 && first && diag) da.x *= 0.f;
           }
           pk[e >> 1] = pack_bf16x2(da.x, da.y);
           pk[(e >> 1) + 1] = pack_bf16x2(db.x, db.y);
