@@ -277,7 +277,7 @@ SHAPE_CRITICAL_TOGGLES = (
 ARCH_TOGGLE_NAMES = SHAPE_CRITICAL_TOGGLES + (
     "rope_base", "logit_softcap", "ve_gate_channels", "qk_shift_beta", "qk_shift_freeze",
     "head_gate_norm", "head_gate_channels", "head_gate_bias", "head_gate_mul",
-    "mlp_sandwich_norm", "relu2_tau", "doc_mask", "window_pattern", "short_window_frac",
+    "mlp_sandwich_norm", "relu2_tau", "doc_mask", "doc_mask_packed", "window_pattern", "short_window_frac",
     "out_bigram_gate_bias", "out_bigram_bf16",
 )
 
