@@ -899,7 +899,8 @@ __global__ void __launch_bounds__(192, 1)
 // D = 128.  One CTA per (batch*head, 128-key tile), transposed frame as above, but:
 //   * Q_i / LSE_i / Dvec_i are double-buffered (tile i+1 loads during tile i); dO_i is
 //     single-buffered and reloaded as soon as the dV MMA of tile i has read it;
-//   * P^T and dS^T share one shared-memory tile (dS is written once the dV MMA has read P);
+//   * P^T goes back into TMEM over S^T, each warp's over columns that it alone has read; dS^T
+//     has the shared-memory tile;
 //   * TMEM: R0 = S^T, R1 = dP^T then dQ, dV, dK.  S^T(i+1) is issued right after dV(i),
 //     before the wait for dS(i); dQ(i) lands in R1 once dP^T(i) has been read;
 //   * four dedicated warps drain dQ: 32-column slices are staged (scaled, 128-byte swizzle)
@@ -932,7 +933,7 @@ __global__ void __launch_bounds__(448, 1)
   uint8_t* sV = sK + TILE;
   uint8_t* sQ = sV + TILE;          // [2]
   uint8_t* sDO = sQ + 2 * TILE;     // [1]
-  uint8_t* sPD = sDO + TILE;        // P^T, then dS^T
+  uint8_t* sPD = sDO + TILE;        // dS^T
   uint8_t* sDQ = sPD + TILE;        // [2] dQ staging slices
   float* sLse = reinterpret_cast<float*>(sDQ + 2 * STG);  // [2][128]
   float* sDv = sLse + 256;                                // [2][128]
@@ -1099,8 +1100,8 @@ __global__ void __launch_bounds__(448, 1)
         fa_stamp(a.trace, 0, it, 1);
         tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)  // dV += P^T dO, P^T from TMEM (over S^T's first 64 columns)
-          umma_bf16_tmem_a(tDV, tR0 + kk * 8, desc_mnmajor(do_addr, kk), IDESC_KV, (it > 0 || kk > 0) ? 1u : 0u);
+        for (int kk = 0; kk < 8; ++kk)  // dV += P^T dO, P^T from TMEM (each half's 32 columns over its own of S^T)
+          umma_bf16_tmem_a(tDV, tR0 + (kk >> 2) * 64 + (kk & 3) * 8, desc_mnmajor(do_addr, kk), IDESC_KV, (it > 0 || kk > 0) ? 1u : 0u);
         umma_commit(dv_done);
         umma_commit(do_empty);  // dO read by dP^T and dV
         if (it + 1 < n_it && !issue_s(it + 1)) { ok = false; break; }
@@ -1193,11 +1194,12 @@ __global__ void __launch_bounds__(448, 1)
           pk[(e >> 1) + 1] = pack_bf16x2(p1.x, p1.y);
         }
       }
-      // P^T back into TMEM over the first 64 columns of S^T (this thread's 64 queries as 32
-      // packed columns): the dV MMA reads it as its A operand, and S^T(i+1) is issued only
-      // after that MMA (one thread's tcgen05 MMAs run in issue order)
+      // P^T back into TMEM over the first 32 of this warp's own 64 columns of S^T (64 queries
+      // as 32 packed columns; the other half's warp may still be reading its own): the dV MMA
+      // reads it as its A operand, and S^T(i+1) is issued only after that MMA (one thread's
+      // tcgen05 MMAs run in issue order)
       __syncwarp();
-      tmem_st_32x32b_x32(tR0 + lane_off + half * 32, pk);
+      tmem_st_32x32b_x32(tR0 + lane_off + cb, pk);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(s_free);
