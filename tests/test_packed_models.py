@@ -2,8 +2,9 @@
 import pytest
 import torch
 
-from test_paged_generator import DEVICES, make_model
+from test_paged_generator import DEVICES, make_model, make_prompts
 from trainium_frontier_b200 import checkpoint as ckpt
+from trainium_frontier_b200.inference.paged import PagedGenerator
 
 
 @torch.no_grad()
@@ -37,3 +38,33 @@ def test_warm_start_says_that_documents_are_masked_in_another_way(tmp_path, caps
     assert "doc_mask_packed mismatch" in capsys.readouterr().out
     ckpt.warm_start_from(str(path), make_model("cpu", doc_mask=True, doc_mask_packed=True))
     assert "mismatch" not in capsys.readouterr().out
+
+
+# ------------------------------------------------------------------------------- sampling
+@pytest.mark.parametrize("temperature", [1e-300, 1e-46, 1e-39, 1e-30, 1e-6])
+def test_temperatures_near_zero_are_greedy(temperature):
+    """However small the temperature: the likeliest token (on the CPU; logits over it would be infinite)."""
+    m = make_model("cpu")
+    g = PagedGenerator(m, 2, 64)
+    prompts = make_prompts([9, 30])
+    got = g.generate(prompts, 8, temperature, generator=torch.Generator().manual_seed(1))
+    want = g.generate(prompts, 8)
+    assert torch.equal(got.tokens, want.tokens) and torch.equal(got.logprobs, want.logprobs)
+
+
+@pytest.mark.parametrize("temperature", [1e30, 1e300, float("inf")])
+def test_any_token_at_great_temperatures(temperature):
+    m = make_model("cpu")
+    got = PagedGenerator(m, 2, 64).generate(make_prompts([9, 30]), 30, temperature, generator=torch.Generator().manual_seed(1))
+    assert int(got.tokens.min()) >= 0 and int(got.tokens.max()) < 300 and torch.isfinite(got.logprobs).all()
+    assert got.tokens.unique().numel() > 40      # 60 draws out of 300 alike: 54 different ones are expected
+
+
+def test_a_model_of_nan_is_sampled_without_a_fault():
+    """Weights that are no number: some token of the vocabulary, its log probability NaN (on the CPU; a draw from
+    probabilities of NaN would be a device-side assertion)."""
+    m = make_model("cpu")
+    m.lm_head.weight.data[7] = float("nan")
+    for temperature in (0.0, 0.7):
+        got = PagedGenerator(m, 2, 64).generate(make_prompts([3, 5]), 4, temperature, generator=torch.Generator().manual_seed(1))
+        assert int(got.tokens.min()) >= 0 and int(got.tokens.max()) < 300 and torch.isnan(got.logprobs).all()

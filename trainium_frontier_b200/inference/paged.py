@@ -80,7 +80,11 @@ class PagedGenerator:
         if temperature == 0.0:
             tok = z.argmax(-1)
         else:
-            tok = torch.multinomial(torch.softmax(z / temperature, -1), 1, generator=generator)[:, 0]
+            # Relative to the row's maximum, so that no temperature makes an infinity of a logit (the least one: a normal number
+            # of float32).  A row with a NaN has none but NaN probabilities, which a draw answers with a device-side
+            # assertion: its token is drawn from all alike, and its log probability says NaN.
+            p = torch.softmax((z - z.amax(-1, keepdim=True)) / max(temperature, 2.0 ** -126), -1)
+            tok = torch.multinomial(p.masked_fill(torch.isnan(p), 1.0), 1, generator=generator)[:, 0]
         return (tok, *ops.token_logprobs(z, tok, top))
 
     # ------------------------------------------------------------------ generation
@@ -88,7 +92,8 @@ class PagedGenerator:
     def generate(self, prompts, max_new_tokens: int, temperature: float = 0.0, top: int = 0,
                  generator: torch.Generator | None = None) -> Generation:
         """``prompts``: a list of 1-D tensors of tokens.  ``temperature`` 0 is greedy; otherwise the softcapped
-        logits over it are sampled with ``generator``'s numbers.  Log probabilities are those of temperature 1."""
+        logits over it are sampled with ``generator``'s numbers.  Log probabilities are those of temperature 1; where a
+        model's logits hold a NaN they are NaN, and the token is any."""
         prompts = [torch.as_tensor(p) for p in prompts]
         lens = [int(p.numel()) for p in prompts]
         if not 1 <= len(prompts) <= self.B:
