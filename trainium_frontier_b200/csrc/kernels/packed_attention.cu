@@ -10,7 +10,10 @@
 // tile that reaches past its sequence holds rows of the next one.  Those keys lie behind every
 // query of the sequence, so the causal mask hides them, and what they hold never enters a product: score
 // and weight are chosen, not multiplied by 0, and rows of an operand that the tensor core would multiply by
-// a weight of 0 are cleared in shared memory first.
+// a weight of 0 are cleared in shared memory first.  In the forward's diagonal tiles the infinities and NaN of a
+// sequence's own values are taken out too, by the producer warp when it has nothing left to load, and the
+// queries that see them get them back at the end.  (Such rows used to be computed again one by one, over all of their
+// keys: by count of operations 0.1 s in place of 0.5 ms for a sequence of 16384 whose values are all NaN.)
 //
 // Which rows a CTA has follows from cu_seqlens alone (packed.cuh): no plan, no launch before the kernel, nothing
 // kept between calls, and rows outside all sequences get zeros.
@@ -19,7 +22,7 @@
 // tile's softmax runs, the other's products do.  The tiles are two query heads of one key/value head
 // where there are an even number of them (both see the same keys: no tile waits for the other's end, and
 // short sequences fill both), else neighbouring rows of one head.
-//   warp 0      TMA: Q tiles, then K_0, V_0, K_1, .. through a ring
+//   warp 0      TMA: Q tiles, then K_0, V_0, K_1, .. through a ring; looks over the last V
 //   warp 1      MMA: per step P0 V, S0(next), P1 V, S1(next); P from TMEM, over its own scores
 //   warps 2-9   softmax of tile 0 / 1, a row a thread
 // The running maximum moves only when it grows by more than 8 (in log2), so outputs are rarely rescaled.
@@ -99,6 +102,11 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uin
     umma_bf16_tmem_a(d, a + (kk >> 1) * GAP + (kk & 1) * 8, mnmajor_at(b, kk), idesc, kk > 0 ? 1u : add ? 1u : 0u);
 }
 
+// Of 8 bf16: which are infinities or NaN (all bits of their halves, else none).
+__device__ __forceinline__ uint4 not_finite8(const uint4& u) {
+  auto of = [](uint32_t w) { return __vcmpeq2(w & 0x7f807f80u, 0x7f807f80u); };
+  return make_uint4(of(u.x), of(u.y), of(u.z), of(u.w));
+}
 // Row `row` of a tile of D columns (swizzled panels of 64): whether it holds an infinity or a NaN.
 template <int D>
 __device__ __forceinline__ bool tile_row_bad(const uint8_t* tile, int row) {
@@ -113,6 +121,16 @@ __device__ __forceinline__ bool tile_row_bad(const uint8_t* tile, int row) {
     }
   }
   return bad != 0;
+}
+// Zeros in their places.  (In line: as a function of its own the forward of 16 x 8191 rows took 4 % longer, for want of registers.)
+template <int D>
+__device__ __forceinline__ void tile_row_mend(uint8_t* tile, int row) {
+#pragma unroll 1
+  for (int c = 0; c < D / 8; ++c) {
+    uint4* at = reinterpret_cast<uint4*>(tile + (c >> 3) * kPanel + sw128_chunk_offset(row, c & 7));
+    const uint4 u = *at, m = not_finite8(u);
+    *at = make_uint4(u.x & ~m.x, u.y & ~m.y, u.z & ~m.z, u.w & ~m.w);
+  }
 }
 template <int D>
 __device__ __forceinline__ void tile_row_clear(uint8_t* tile, int row) {
@@ -181,29 +199,56 @@ __device__ __forceinline__ void store_rows(uint32_t from, float by, uint8_t* sta
   }
 }
 
-// A row's output by itself, keys one after another in 32 bits: for the rows of a diagonal tile whose masked
-// values hold an infinity or a NaN, which the tensor core would multiply by 0.
+// Infinities and NaN of values were taken out of the tile of V before its product; a query row (a lane each, whose output of D
+// columns is at `out` in TMEM) gets those of the rows that it sees, j <= seen of the tile.  `rows`: a bit for each of them;
+// v: the tile's first row.  All of them NaN: 128 rows of loads that the warp shares.
 template <int D>
-__device__ __noinline__ void packed_row(const PkArgs& a, int begin, int i, int h, float lse2, __nv_bfloat16* dst) {
-  const __nv_bfloat16* q = a.q + (long long)(begin + i) * a.qr + h * a.qh;
-  const int hk = h / a.G;
+__device__ __noinline__ void add_not_finite(uint32_t out, const uint32_t* rows, const __nv_bfloat16* v, long long vr, int seen) {
+  if (!(rows[0] | rows[1] | rows[2] | rows[3])) return;
 #pragma unroll 1
   for (int d0 = 0; d0 < D; d0 += 32) {
-    float o[32];
-#pragma unroll
-    for (int d = 0; d < 32; ++d) o[d] = 0.f;
+    uint32_t o[32];
+    __syncwarp();
+    tmem_ld_32x32b_x32(out + d0, o);
+    tmem_ld_wait();
 #pragma unroll 1
-    for (int j = 0; j <= i; ++j) {
-      const __nv_bfloat16* k = a.k + (long long)(begin + j) * a.kr + hk * a.kh;
-      const __nv_bfloat16* v = a.v + (long long)(begin + j) * a.vr + hk * a.vh + d0;
-      float s = 0.f;
+    for (int w = 0; w < 4; ++w) {
 #pragma unroll 1
-      for (int d = 0; d < D; ++d) s += __bfloat162float(q[d]) * __bfloat162float(k[d]);
-      const float p = ex2_approx(s * a.scale_log2 - lse2);
+      for (uint32_t left = rows[w]; left; left &= left - 1) {
+        const int j = w * 32 + __ffs(left) - 1;
 #pragma unroll
-      for (int d = 0; d < 32; ++d) o[d] += p * __bfloat162float(v[d]);
+        for (int c = 0; c < 4; ++c) {
+          const uint4 u = *reinterpret_cast<const uint4*>(v + j * vr + d0 + 8 * c), m = not_finite8(u);
+          const uint32_t x[4] = {u.x & m.x, u.y & m.y, u.z & m.z, u.w & m.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (j <= seen) {
+              o[8 * c + 2 * i] = __float_as_uint(__uint_as_float(o[8 * c + 2 * i]) + __uint_as_float(x[i] << 16));
+              o[8 * c + 2 * i + 1] = __float_as_uint(__uint_as_float(o[8 * c + 2 * i + 1]) + __uint_as_float(x[i] & 0xffff0000u));
+            }
+        }
+      }
     }
-    store_row_bf16_global(dst + d0, o, 32);
+    __syncwarp();
+    tmem_st_32x32b_x32(out + d0, o);
+    tmem_st_wait();
+  }
+}
+
+// The same for tile t of a CTA of the forward, `out` being the warp's lanes of it.  All is found again from the unit, so that the
+// loop over the keys keeps no registers for it.
+template <int D, int TILES>
+__device__ __noinline__ void give_back(uint32_t out, const uint32_t* bad, int t, const PieceUnit& un, int by_heads, int Hq, int G,
+                                       const __nv_bfloat16* v, long long vr, long long vh) {
+  const bool pair = TILES == 2 && by_heads;
+  const int nh = pair ? Hq / 2 : Hq, hk = (int)(blockIdx.x % nh) * (pair ? 2 : 1) / G;
+  const int r = (threadIdx.x >> 5 & 3) * 32 + (threadIdx.x & 31), r0 = un.unit * (TILES == 1 || pair ? 128 : 256);
+  const __nv_bfloat16* first = v + (long long)(un.begin + r0) * vr + hk * vh;
+  if (pair || t == 0) {
+    add_not_finite<D>(out, bad + 4 * t, first, vr, r);
+  } else {                               // of neighbouring tiles the second sees all rows of the first one's last V
+    add_not_finite<D>(out, bad, first, vr, 127);
+    add_not_finite<D>(out, bad + 4, first + 128 * vr, vr, r);
   }
 }
 
@@ -216,6 +261,9 @@ struct PkFwd {
   static constexpr uint32_t COLUMNS = 256 * TILES;     // of TMEM: S and O of each tile
 };
 static_assert(2 * PkFwd<128, 1>::SMEM <= 227 * 1024 && PkFwd<128, 2>::SMEM <= 227 * 1024, "shared memory");
+// The producer looks over the last V of each tile when all loads are issued, so none of them may wait for a product with it:
+// the last load waits for the slot NS items before, and behind tile 0's last V come at most two items.
+static_assert(PkFwd<128, 1>::NS >= 2 && PkFwd<64, 1>::NS >= 2 && PkFwd<128, 2>::NS >= 4 && PkFwd<64, 2>::NS >= 4, "K / V ring");
 
 template <int D, int TILES>
 __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
@@ -238,12 +286,13 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
   uint64_t* s_full = bars + 1 + 2 * NS;  // [2]
   uint64_t* p_full = s_full + 2;         // [2]
   uint64_t* o_done = p_full + 2;         // [2]
-  uint64_t* looked = o_done + 2;         // [2] by_row is what it will be
+  uint64_t* looked = o_done + 2;         // [2] the tile's last V holds finite numbers alone, bad_rows says whether it did before
   uint64_t* drain = looked + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* by_row = abort_flag + 1;               // [2] the tile's rows are computed one by one
   PieceUnit* s_unit = reinterpret_cast<PieceUnit*>(tmem_slot + 4);
+  uint32_t* bad_rows = tmem_slot + 8;    // [2][4] the rows of the tiles' last V that held an infinity or a NaN, a bit each
+  volatile uint32_t* any_bad = tmem_slot + 2;          // whether one of them did
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nh = TILES == 2 && a.by_heads ? a.Hq / 2 : a.Hq;
@@ -265,11 +314,11 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
-      mbar_init(&looked[t], 4);
-      by_row[t] = 0;
+      mbar_init(&looked[t], 1);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
+    *any_bad = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
@@ -296,8 +345,8 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
     if (un.unit >= 0) clear_rows<D>(a.out, a.Hq, h0, pair ? 2 : 1, un.begin + r0, min(U, un.len - r0));
   } else if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
+    bool ok = true;
     if (lane == 0) {
-      bool ok = true;
       uint32_t out_valid = 0, out_parity = 0;
       mbar_arrive_expect_tx(bar_q, (n1 ? 2 : 1) * TILE);
 #pragma unroll
@@ -332,6 +381,38 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
           if (globaltimer_ns() - t0 > 100000000ull) break;
       }
     }
+    // The last V of a tile has rows that some of its queries do not see, but the tensor core multiplies by their weights of 0: no
+    // infinity or NaN may be among them.  They are looked over and taken out under the tile's softmax; who sees them gets them back
+    // at the end.
+    ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    for (int t = 0; t < TILES && ok; ++t) {
+      const int j = (t == 0 ? n0 : n1) - 1, i = 2 * j + 1;
+      if (j < 0) break;
+      if (pair && t == 1) {              // the same V
+        __syncwarp();
+        if (lane < 4) bad_rows[4 + lane] = bad_rows[lane];
+        warp_arrive(&looked[1]);
+        break;
+      }
+      ok = mbar_wait_warp(&kv_full[i % NS], (i / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_PRODUCER);
+      if (!ok) break;
+      uint8_t* tile = sKV + (i % NS) * TILE;
+      bool any = false;
+#pragma unroll 1
+      for (int w = 0; w < 4; ++w) {
+        const int r = w * 32 + lane;
+        const bool bad = j * 128 + r < un.len && tile_row_bad<D>(tile, r);
+        if (bad) tile_row_mend<D>(tile, r);
+        any |= bad;
+        const uint32_t rows = __ballot_sync(0xffffffffu, bad);
+        if (lane == 0) {
+          bad_rows[4 * t + w] = rows;
+          if (rows) *any_bad = 1;
+        }
+      }
+      if (any) fence_proxy_async_smem();
+      warp_arrive(&looked[t]);
+    }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     // The warp runs as one, so that operands stay in uniform registers; one lane issues.
@@ -352,6 +433,7 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
       __syncwarp();
     };
     auto issue_pv = [&](int t, int j) -> bool {
+      if (j == (t == 0 ? n0 : n1) - 1 && !mbar_wait_warp(&looked[t], 0, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
       if (!mbar_wait_warp(&p_full[t], j & 1, abort_flag, a.err, ERR_TIMEOUT_MMA)) return false;
       tc_fence_after();
       if (leader) mma_tmem<16>(tmem + OAT + t * 128, tmem + t * 128, vd + vs * STEP, IDESC_O, j > 0);
@@ -499,30 +581,18 @@ __global__ void __launch_bounds__(64 + 128 * TILES, 3 - TILES)
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&p_full[t]);
-      // its own rows of V that some queries do not see are looked over, while the product runs (nothing is loaded over a
-      // tile's last V)
-      if (diag && j * 128 + r < un.len) {
-        mbar_wait(&kv_full[(2 * j + 1) % NS], ((2 * j + 1) / NS) & 1, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE);
-        if (tile_row_bad<D>(sKV + ((2 * j + 1) % NS) * TILE, r)) by_row[t] = 1;
-      }
-      if (diag) warp_arrive(&looked[t]);
     }
     if (n_t > 0 && ok && mbar_wait_warp(&o_done[t], 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE) &&
         mbar_wait_warp(&looked[t], 0, abort_flag, a.err, ERR_TIMEOUT_EPILOGUE)) {
       tc_fence_after();
-      const float inv_l = 1.f / l, lse2 = m_run + log2f(l);
-      const bool mine = row < un.len, alone = by_row[t] != 0;
+      const bool mine = row < un.len;
       const int first = row - lane;      // the warp's first row; Q's tile is free: all products of it are done
+      // no weight at all (every visible score is -inf): NaN, an infinity of v's among them
+      const float inv_l = l == 0.f ? NAN : 1.f / l, lse2 = m_run + log2f(l);
+      if (*any_bad) give_back<D, TILES>(tO + lane_off, bad_rows, t, *s_unit, a.by_heads, a.Hq, a.G, a.v, a.vr, a.vh);
       __nv_bfloat16* dst = a.out + ((long long)(un.begin + first) * a.Hq + head) * D;
-      if (!alone)
-        store_rows<D / 8, D / 16>(tO + lane_off, inv_l, sQ + t * TILE + q4 * (32 * D * 2), dst, a.low ? a.low + (dst - a.out) : nullptr,
-                                  (long long)a.Hq * D, un.len - first);
-      dst += (long long)lane * a.Hq * D;
-      if (mine && alone) {
-        packed_row<D>(a, un.begin, row, head, lse2, dst);
-        if (a.low)
-          for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(a.low + (dst - a.out))[i] = make_uint4(0, 0, 0, 0);
-      }
+      store_rows<D / 8, D / 16>(tO + lane_off, inv_l, sQ + t * TILE + q4 * (32 * D * 2), dst, a.low ? a.low + (dst - a.out) : nullptr,
+                                (long long)a.Hq * D, un.len - first);
       if (mine && a.lse) a.lse[(long long)head * a.pc.M + un.begin + row] = lse2 * kLn2;
     }
   }
