@@ -1,4 +1,4 @@
-"""Packed attention at the ends of what it takes: first tokens, values that are no number."""
+"""Packed attention at the ends of what it takes: first tokens, values that are no number; what its gradients' D is summed from."""
 import math
 
 import pytest
@@ -120,3 +120,59 @@ def test_values_of_nan_cost_no_more_than_a_few_numbers(heads):
     nan = torch.full_like(v, math.nan)
     assert us(nan) < 4 * us(v)
     assert torch.isnan(ops.packed_attention(q, k, nan, cu)).all()
+
+
+# ------------------------------------------------------------------------------- what D is summed from
+# The gradients' D_i = dO_i . o_i is not taken of the rounded output: in a sequence's first 128 rows it is the sum of the 32-bit
+# weights times dP, and behind them the output's product with its rest, to 16 bits.  (The bounds of packed64's gradients are
+# wider: they would admit a D of the rounded output.)  Values of 16 +- 1 show it: dP - D is of size sqrt(128) = 11.3 (64: 8), and so
+# are sums of dO.  A rounding of o to steps of 2^-3 is off by 0.036 (rms), independently in each dimension: D by 0.036 * 11.3, ds
+# and with it dq and dk by 3.6e-2 of their size.  Weights rounded to bf16 (1.66e-3 rms) move all dimensions of o
+# by 16 * 1.66e-3 sqrt(sum p^2), D by 11.3 times that, ds by 2.7e-2 sqrt(sum p^2); sum p^2 is some e / n among n keys: 1e-2 for
+# n = 20, 2.7e-3 for n = 256.  The rounding of ds and that of the result are 1.66e-3 each: 2.4e-3 in all.
+def offset_values(lens, heads, device, seed):
+    q, k, v, cu, do = pack(lens, *heads, device, seed=seed)
+    return q, k, (16 + v.float()).to(v.dtype), cu, do
+
+
+def rel(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("heads", [(4, 2, 128), (3, 1, 64)], ids=str)
+def test_gradients_of_short_sequences_take_d_from_their_weights(heads, device):
+    """Nearer than weights or an output of 8 bits allow: 5e-3 lies between the 2.4e-3 of the two last roundings and 1e-2."""
+    q, k, v, cu, do = offset_values([20, 3, 128, 9, 2, 60, 14, 31] * 4, heads, device, 27)
+    _, dq, dk, _ = forward_backward(q, k, v, cu, do)
+    want = packed64(q, k, v, cu, heads[2] ** -0.5, do)
+    few = torch.cat([torch.arange(a, b) for a, b in zip(cu.tolist()[:-1], cu.tolist()[1:]) if b - a <= 20]).to(device)
+    for got, name in ((dq, "dq"), (dk, "dk")):
+        assert rel(got, want[name][0]) < 5e-3, name
+        assert rel(got[few], want[name][0][few]) < 5e-3, name + " of up to 20 rows"
+
+
+@pytest.mark.parametrize("device,n", [("cpu", 400), pytest.param("cuda", 1500, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("heads", [(4, 2, 128), (3, 1, 64)], ids=str)
+def test_gradients_of_long_sequences_take_d_from_the_output_and_its_rest(heads, device, n):
+    """8e-3: above the 2.4e-3 and 2.7e-3 of all that is rounded to 8 bits, below the 3.6e-2 of a rounded output."""
+    q, k, v, cu, do = offset_values([n, 256], heads, device, 28)
+    _, dq, dk, _ = forward_backward(q, k, v, cu, do)
+    want = packed64(q, k, v, cu, heads[2] ** -0.5, do)
+    for a, b in ((128, n), (n + 128, n + 256)):
+        assert rel(dq[a:b], want["dq"][0][a:b]) < 8e-3
+    assert rel(dk, want["dk"][0]) < 8e-3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(4, 2, 128), (3, 1, 64)], ids=str)
+def test_the_rest_of_the_output(heads):
+    """The output with its rest is off by what rounded weights cost (2.7e-3 and less from 256 keys on), the output alone by 0.036."""
+    from trainium_frontier_b200.ops._ext import C, err_word
+    q, k, v, cu, _ = offset_values([1200, 700], heads, "cuda", 29)
+    out, _, low = C().packed_attention_fwd(q, k, v, cu, heads[2] ** -0.5, True, err_word(q.device))
+    want = packed64(q, k, v, cu, heads[2] ** -0.5)["o"][0]
+    for a, b in ((256, 1200), (1456, 1900)):
+        alone = float((out.double() - want)[a:b].square().mean().sqrt())
+        both = float((out.double() + low.double() - want)[a:b].square().mean().sqrt())
+        assert both < 6e-3 and 0.02 < alone
