@@ -68,3 +68,17 @@ def test_a_model_of_nan_is_sampled_without_a_fault():
     for temperature in (0.0, 0.7):
         got = PagedGenerator(m, 2, 64).generate(make_prompts([3, 5]), 4, temperature, generator=torch.Generator().manual_seed(1))
         assert int(got.tokens.min()) >= 0 and int(got.tokens.max()) < 300 and torch.isnan(got.logprobs).all()
+
+
+@pytest.mark.parametrize("prompt", [torch.tensor([1.5, 2.0]), torch.tensor([True, False]), [3.0, 4.0]], ids=["float", "bool", "list"])
+def test_prompts_are_integers(prompt):
+    with pytest.raises(ValueError):
+        PagedGenerator(make_model("cpu"), 2, 64).generate([prompt], 2)
+
+
+def test_prompts_of_any_integers():
+    m = make_model("cpu")
+    p = make_prompts([5])[0]
+    want = PagedGenerator(m, 2, 64).generate([p], 4)
+    for q in (p.tolist(), p.int(), p.short(), p.numpy()):
+        assert torch.equal(PagedGenerator(m, 2, 64).generate([q], 4).tokens, want.tokens)

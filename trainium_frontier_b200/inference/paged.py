@@ -100,6 +100,8 @@ class PagedGenerator:
             raise ValueError(f"1 .. {self.B} prompts")
         if min(lens) < 1 or max_new_tokens < 1 or max(lens) + max_new_tokens > self.max_len or any(p.dim() != 1 for p in prompts):
             raise ValueError(f"prompts: 1-D, not empty, and with the new tokens at most {self.max_len} tokens")
+        if any(p.is_floating_point() or p.is_complex() or p.dtype == torch.bool for p in prompts):
+            raise ValueError("prompts: tokens are integers")
         if not 0 <= top <= min(32, self.V):
             raise ValueError("top: 0 .. 32 alternatives, at most the vocabulary")
         if not temperature >= 0:
