@@ -12,8 +12,8 @@
 // and weight are chosen, not multiplied by 0, and rows of an operand that the tensor core would multiply by
 // a weight of 0 are cleared in shared memory first.  In the forward's diagonal tiles the infinities and NaN of a
 // sequence's own values are taken out too, by the producer warp when it has nothing left to load, and the
-// queries that see them get them back at the end.  (Such rows used to be computed again one by one, over all of their
-// keys: by count of operations 0.1 s in place of 0.5 ms for a sequence of 16384 whose values are all NaN.)
+// queries that see them get them back at the end: 0.49 ms instead of 0.24 for a sequence of 16384 whose values are all NaN (2 / 1
+// heads).  (Computing such rows again one by one, over all of their keys, would take some 0.1 s by count of operations.)
 //
 // Which rows a CTA has follows from cu_seqlens alone (packed.cuh): no plan, no launch before the kernel, nothing
 // kept between calls, and rows outside all sequences get zeros.
@@ -36,17 +36,18 @@
 // rounded lse is off by some 2^-24 of it, and ds with it.  So that ds is chosen to be 0, as masked ones are (what is no number
 // stays).  Where all sequences are one token, dQ and dK are zeros, not rounding errors.
 // D of the rounded output would be the largest error of short sequences' gradients: 3.4e-3 of their size.  So a forward that
-// a backward follows writes the rest of the output too, 2 bytes an entry (4 to 7 % of the time for documents of 340 tokens,
-// 2 % for long ones): 2.6e-3.  A sequence's first 128 rows, whose weights are all in one tile, take D from those in 32 bits:
+// a backward follows writes the rest of the output too, 2 bytes an entry (2 to 4 % of the forward's
+// time): 2.6e-3.  A sequence's first 128 rows, whose weights are all in one tile, take D from those in 32 bits:
 // 2.4e-3, of which 1.7e-3 is the rounding of the result.
 //
 // Measured on a B200, head_dim 128 (counters: profiles/packed_attention.md).  Forward: 16 sequences of 4096 .. 8191 rows, 32 / 8
 // heads, 5.2 ms = 0.98 PFLOP/s, power capped (floor 3.1 at the burst rate of a library product, 3.7 at the sustained one);
 // a step of two 128 x 128 tiles takes 3700 cycles of which the tensor core's products are 2048: a tile's
 // softmax (2150) and its own two products follow one another, and only the other tile's lie under them.  192 documents of
-// 340 rows on average, 10 heads: 0.37 ms with what a backward needs (0.34 without), starts and ends of 4200 CTAs.
+// 340 rows on average, 10 heads: 0.35 ms with what a backward needs (0.34 without), starts and ends of 4200 CTAs.
 // Backward: 4 sequences of 4096 .. 8192, 32 / 8 heads, 4.4 ms (dQ 1.9, dK and dV 2.6) = 0.74 PFLOP/s of the formula's five
-// products, 1.04 of the seven; the documents 0.96 ms.
+// products, 1.04 of the seven; the documents 0.95 ms.  With one key/value head dK and dV have few CTAs: one sequence of 4096 rows, 8 / 1
+// heads, 0.54 ms where the products would take 0.05 spread evenly.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/ops/clone.h>
@@ -1363,7 +1364,9 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> pac
   };
   // One tile a CTA, two CTAs an SM, where a tile has few keys and no second head shares them: one's start and end lie under the
   // other's products (10 heads, 65536 rows: 236 instead of 256 us for sequences of 512, 379 instead of 588 for 64; from 1024 on
-  // two tiles that share their keys are as fast or faster).
+  // two tiles that share their keys are as fast or faster).  The lengths are in device memory, so the mean over all entries of
+  // cu_seqlens has to do: where most of them are empty, long sequences get the one-tile form too, at 10971 instead of 9648 us for one of
+  // 65535 rows, 1524 instead of 1392 for eight of 8192 (10 heads).
   const bool one = !a.by_heads && c.M < 1024 * (int64_t)a.pc.S;
   if (one) {
     const int64_t slots = piece_slots(c.M, a.pc.S, 128);

@@ -7,7 +7,7 @@
 // A warp finds its first row's sequence with 32 probes a step and its further rows' by walking on.
 //
 // Measured on a B200 (calls replayed from a graph): 16 prompts of 2048 .. 4096 rows of 8 heads of 128, bf16, pages of 16: 71 us
-// of 61 (87 % of the copy rate); one row for 32 sequences of 10 heads, e4m3: 2.9 us (a launch and three dependent loads).
+// of 61 (87 % of the copy rate), e4m3 102 us of 46 (not looked into yet); one row for 32 sequences of 10 heads, e4m3: 2.9 us (a launch and three dependent loads).
 #include "kv_cache.cuh"
 #include "packed.cuh"
 

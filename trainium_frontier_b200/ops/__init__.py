@@ -307,7 +307,11 @@ def packed_attention(q, k, v, cu_seqlens, scale: float | None = None):
     reaches nothing.  An infinity or a NaN of a token reaches the outputs of the tokens that see it, and no
     other; in the backward pass it may also reach gradients of tokens of its own sequence that lie in
     the same 128 rows of it.  CUDA: bfloat16, head_dim 64 / 128; inputs are read in place (slices of
-    a projection's rows, say) where rows are 16-byte aligned, else copied."""
+    a projection's rows, say) where rows are 16-byte aligned, else copied.  Scores, sums and gradients' sums are
+    32-bit; weights and, in the backward pass, the scores' gradients are rounded to bfloat16 for their products.
+    ``cu_seqlens`` may be longer than the batch (ends that repeat): a captured call then takes other batches.  With an odd
+    number of query heads a key/value head the kernel is chosen by the mean length over all entries, so long
+    sequences among many empty ones run some 5 to 14 % longer."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if _cuda(q):
@@ -339,8 +343,11 @@ def paged_attention(q, k_pages, v_pages, page_table, lens, scale: float | None =
     Rows of table entries that are no page, and those behind the table's last page, are not seen; a sequence
     that sees no row gets zeros.  An
     infinity or a NaN in a seen row (in e4m3: a NaN code, or the scale NaN) reaches its sequence's output
-    and what other rows hold reaches nothing; where all scores are -inf the output is NaN.  Weights are
-    rounded as in ``tree_attention``.  No gradient."""
+    and what other rows hold reaches nothing; where all scores are -inf the output is NaN.  Sums are 32-bit.  For
+    the product with the values weights are rounded to bfloat16, or, over quantised pages, to float16 relative to the
+    largest weight times scale: a row below 2^-25 of that may count nothing there, and still counts in the weights'
+    sum.  Over quantised pages queries are float16 relative to their head's largest entry, below 2^-31 of which an
+    entry loses bits.  No gradient."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if _cuda(k_pages):
