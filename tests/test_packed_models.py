@@ -1,10 +1,11 @@
-"""Models over packed attention and the paged decoder: what is saved comes back, and what the decoder samples."""
+"""Models over packed attention and the paged decoder: what is saved comes back, and what the decoders sample."""
 import pytest
 import torch
 
 from test_paged_generator import DEVICES, make_model, make_prompts
 from trainium_frontier_b200 import checkpoint as ckpt
 from trainium_frontier_b200.inference.paged import PagedGenerator
+from trainium_frontier_b200.inference.speculative import SpeculativeGenerator
 
 
 @torch.no_grad()
@@ -82,3 +83,11 @@ def test_prompts_of_any_integers():
     want = PagedGenerator(m, 2, 64).generate([p], 4)
     for q in (p.tolist(), p.int(), p.short(), p.numpy()):
         assert torch.equal(PagedGenerator(m, 2, 64).generate([q], 4).tokens, want.tokens)
+
+
+@pytest.mark.parametrize("temperature", [1e-300, 1e-46, 1e-39, 1e-6])
+def test_speculative_decoding_near_temperature_zero_is_greedy(temperature):
+    """The other decoder that samples: logits over such a temperature were infinite, and every token 0."""
+    g = SpeculativeGenerator(make_model("cpu"), 2, 64)
+    p = torch.stack([x[:9] for x in make_prompts([9, 30])]).int()
+    assert torch.equal(g.generate(p, 8, temperature, generator=torch.Generator().manual_seed(1)), g.generate(p, 8))

@@ -106,7 +106,8 @@ class SpeculativeGenerator:
         z = ops.softcap_logits(hidden, self.m.lm_head.weight, self.m.rc.logit_softcap, self.V)
         if temperature == 0.0:   # greedy: all mass on the largest logit
             return torch.zeros_like(z).scatter_(-1, z.argmax(-1, keepdim=True), 1.0)
-        return torch.softmax(z / temperature, -1)
+        # relative to the row's maximum, so that no temperature makes an infinity of a logit (the least one: a normal number)
+        return torch.softmax((z - z.amax(-1, keepdim=True)) / max(temperature, 2.0 ** -126), -1)
 
     # ------------------------------------------------------------------ generation
     @torch.no_grad()
