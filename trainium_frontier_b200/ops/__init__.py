@@ -305,8 +305,9 @@ def packed_attention(q, k, v, cu_seqlens, scale: float | None = None):
     Differentiable in q, k and v (a backward pass can be captured in a CUDA graph while no graph recorded before
     the capture still holds its leaves); rows outside all sequences get zero gradients, and what they hold
     reaches nothing.  An infinity or a NaN of a token reaches the outputs of the tokens that see it, and no
-    other (an infinite value under a weight that is too small for float32 or bfloat16 may come out as NaN); in the backward pass it may also reach gradients of tokens of its own sequence that lie in
-    the same 128 rows of it.  CUDA: bfloat16, head_dim 64 / 128; inputs are read in place (slices of
+    other (an infinite value under a weight that is too small for float32 or bfloat16 may come out as NaN); in
+    the backward pass it may also reach gradients of tokens of its own sequence that lie in the same 128 rows
+    of it.  CUDA: bfloat16, head_dim 64 / 128; inputs are read in place (slices of
     a projection's rows, say) where rows are 16-byte aligned, else copied.  Scores, sums and gradients' sums are
     32-bit; weights and, in the backward pass, the scores' gradients are rounded to bfloat16 for their products.
     ``cu_seqlens`` may be longer than the batch (ends that repeat): a captured call then takes other batches.  With an odd
